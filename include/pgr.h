@@ -36,7 +36,7 @@ extern "C" {
 
 /* ---- library ------------------------------------------------------------------------- */
 
-/* ABI version of this header (increments when an entry point is added or changed); 12. */
+/* ABI version of this header (increments when an entry point is added or changed); 13. */
 int pgr_abi_version(void);
 /* Message of the last failing call on this thread ("" if none). */
 const char* pgr_last_error(void);
@@ -157,6 +157,85 @@ int pgr_attn_state_init(float* m, float* l, float* acc, int64_t rows, int64_t he
  * Replaces streaming_attention_finalize, pager_hf/streaming_attention.py:668-670. */
 int pgr_attn_finalize(const float* acc, const float* l, void* out, int64_t rows, int64_t head_dim, int dtype,
                       void* stream);
+
+/* ---- rotary positions and the bounded cache ------------------------------------------
+ * No counterpart in the reference, whose operators take q and k after the rotary embedding and
+ * whose store places blocks but drops none. A bounded cache holds up to `capacity` tokens per row
+ * (batch row x KV head), each in a slot of its own, and keeps the tokens that attention has given
+ * the most weight. Strides are in elements; a tensor's last dimension (head_dim) is contiguous,
+ * and tensors other than the cache's buffers need the alignment of their elements only.
+ */
+
+/* Rotary position embedding: of each head of q [B, Hq, T, D] and k [B, Hk, T, D] (strides: batch,
+ * head, token) the first rotary_dim dims are turned by position * inv_freq[i] (the angle in 64
+ * bits), the rest is copied: (x, y) -> factor * (x cos - y sin, x sin + y cos) for the pairs
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0. inverse != 0 turns by the negative
+ * angle: the transposed map, which takes gradients back. positions [B, T] int32 or int64 with
+ * strides (batch, token); inv_freq [rotary_dim / 2]. Outputs [B, H, T, D] contiguous, not
+ * overlapping the inputs. k_heads (or q_heads) may be 0. dtype fp16, bf16 or fp32; any head_dim. */
+int pgr_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_heads, const void* k,
+               const int64_t* k_strides, void* k_out, int64_t k_heads, const void* positions, int positions_64bit,
+               const int64_t* position_strides, const float* inv_freq, int64_t rotary_dim, int64_t batch,
+               int64_t tokens, int64_t head_dim, int dtype, int interleaved, float factor, int inverse,
+               void* stream);
+
+/* The caller's buffers of a bounded cache, all on the device and contiguous; keys, values, weights
+ * and order 16-byte aligned. fp16 or bf16; head_dim 16, 32, 64, 128 or 256; up to 16 query heads
+ * per KV head; batch * kv_heads <= 65535. lengths[row] slots of a row hold tokens; a token's
+ * `order` counts the row's tokens from 0, and seen[row] is the next one's. Calls on one cache are
+ * ordered by the caller (one stream, or events). */
+typedef struct pgr_hh_cache_s {
+  void* keys;       /* [batch, kv_heads, capacity, head_dim] */
+  void* values;     /* [batch, kv_heads, capacity, head_dim] */
+  float* weights;   /* [batch, kv_heads, capacity]: attention weight accumulated per slot */
+  int32_t* order;   /* [batch, kv_heads, capacity] */
+  int32_t* lengths; /* [batch, kv_heads] */
+  int32_t* seen;    /* [batch, kv_heads] */
+  int64_t batch, query_heads, kv_heads, capacity, head_dim;
+  int dtype;
+  int32_t keep_first;  /* tokens of lower order are kept (>= 0) */
+  int32_t keep_recent; /* so are the last keep_recent tokens (>= 1); the sum is at most capacity */
+} pgr_hh_cache_t;
+
+/* One new token per batch row: k, v [B, Hkv, D] (strides: batch, head) go into the row's next free
+ * slot or, where the row is full, into the slot of the token with the least weight that is neither
+ * among the first keep_first nor among the last keep_recent tokens, the new one counted (ties: the
+ * lowest slot; NaN is the heaviest). Its weight starts at 0. With inv_freq, k and q [B, Hq, D] are
+ * turned first (pgr_rotary's forms) at positions[b], or at the row's `seen` with positions NULL;
+ * q_out [B, Hq, D] contiguous receives q, turned or copied (NULL: q is not read). */
+int pgr_hh_append(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_strides, const void* k,
+                  const int64_t* k_strides, const void* v, const int64_t* v_strides, void* q_out,
+                  const void* positions, int positions_64bit, const float* inv_freq, int64_t rotary_dim,
+                  int interleaved, float factor, void* stream);
+
+/* out [B, Hq, D] contiguous = softmax(scale * q . K^T, softcapped with softcap > 0) V over the row's
+ * slots, and weights[slot] += the probabilities, summed over the KV head's query heads. q strides:
+ * batch, head. A row of length 0 gives zeros. */
+size_t pgr_hh_attend_workspace_bytes(const pgr_hh_cache_t* cache);
+int pgr_hh_attend(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_strides, void* out, float scale,
+                  float softcap, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The attention weight that each token of a prompt gets from its last `window` queries: q [B, Hq,
+ * window, D], k [B, Hkv, tokens, D] (strides: batch, head, token), weights [B, Hkv, tokens] written,
+ * summed over the queries and over each KV head's query heads; causal. lo [B] (NULL: 0): the row's
+ * first valid column (left padding): columns before it get 0, queries before it give nothing, and
+ * what q and k hold there does not matter. */
+size_t pgr_hh_prompt_weights_workspace_bytes(int64_t batch, int64_t num_query_heads, int64_t num_kv_heads,
+                                             int64_t tokens, int64_t window, int64_t head_dim);
+int pgr_hh_prompt_weights(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          const int32_t* lo, float* weights, int64_t batch, int64_t num_query_heads,
+                          int64_t num_kv_heads, int64_t tokens, int64_t window, int64_t head_dim, int dtype,
+                          float scale, float softcap, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Starts every row of the cache over with a prompt's tokens [lo, tokens): all of them where they
+ * fit, else the first keep_first, the last keep_recent and the heaviest of those between (ties: the
+ * lowest column; NaN is the heaviest), in the order of their columns. k, v [B, Hkv, tokens, D]
+ * (strides: batch, head, token), weights [B, Hkv, tokens] contiguous. Slots past the new length are
+ * left as they were. */
+size_t pgr_hh_load_prompt_workspace_bytes(const pgr_hh_cache_t* cache);
+int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t* k_strides, const void* v,
+                       const int64_t* v_strides, const float* weights, const int32_t* lo, int64_t tokens,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- placement policy ----------------------------------------------------------------
  * Restatement of the Rust pager. Handles are opaque; not thread-safe per handle. */

@@ -36,7 +36,7 @@ STREAM_DIRECT = 0
 STREAM_STAGED = 1
 STREAM_MIRROR = 2
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 c_i32, c_i64, c_u8, c_u32, c_u64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint8, ctypes.c_uint32, ctypes.c_uint64
 c_f32, c_f64, c_size, c_vp = ctypes.c_float, ctypes.c_double, ctypes.c_size_t, ctypes.c_void_p
@@ -102,6 +102,27 @@ class KVStepStats(ctypes.Structure):
     ]
 
 
+class HHCache(ctypes.Structure):
+    """pgr_hh_cache_t: the buffers of a bounded cache."""
+
+    _fields_ = [
+        ("keys", c_vp),
+        ("values", c_vp),
+        ("weights", c_vp),
+        ("order", c_vp),
+        ("lengths", c_vp),
+        ("seen", c_vp),
+        ("batch", c_i64),
+        ("query_heads", c_i64),
+        ("kv_heads", c_i64),
+        ("capacity", c_i64),
+        ("head_dim", c_i64),
+        ("dtype", ctypes.c_int),
+        ("keep_first", c_i32),
+        ("keep_recent", c_i32),
+    ]
+
+
 # name -> (restype, argtypes). Every symbol declared in include/pgr.h.
 SIGNATURES: dict[str, tuple] = {
     "pgr_abi_version": (ctypes.c_int, []),
@@ -131,6 +152,29 @@ SIGNATURES: dict[str, tuple] = {
         ctypes.c_int,
         [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, c_f32, c_f32,
          c_vp, c_size, c_vp],
+    ),
+    "pgr_rotary": (
+        ctypes.c_int,
+        [c_vp, P(c_i64), c_vp, c_i64, c_vp, P(c_i64), c_vp, c_i64, c_vp, ctypes.c_int, P(c_i64), c_vp, c_i64, c_i64,
+         c_i64, c_i64, ctypes.c_int, ctypes.c_int, c_f32, ctypes.c_int, c_vp],
+    ),
+    "pgr_hh_append": (
+        ctypes.c_int,
+        [P(HHCache), c_vp, P(c_i64), c_vp, P(c_i64), c_vp, P(c_i64), c_vp, c_vp, ctypes.c_int, c_vp, c_i64,
+         ctypes.c_int, c_f32, c_vp],
+    ),
+    "pgr_hh_attend_workspace_bytes": (c_size, [P(HHCache)]),
+    "pgr_hh_attend": (ctypes.c_int, [P(HHCache), c_vp, P(c_i64), c_vp, c_f32, c_f32, c_vp, c_size, c_vp]),
+    "pgr_hh_prompt_weights_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "pgr_hh_prompt_weights": (
+        ctypes.c_int,
+        [c_vp, P(c_i64), c_vp, P(c_i64), c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, c_f32,
+         c_f32, c_vp, c_size, c_vp],
+    ),
+    "pgr_hh_load_prompt_workspace_bytes": (c_size, [P(HHCache)]),
+    "pgr_hh_load_prompt": (
+        ctypes.c_int,
+        [P(HHCache), c_vp, P(c_i64), c_vp, P(c_i64), c_vp, c_vp, c_i64, c_vp, c_size, c_vp],
     ),
     "pgr_bench_stream_read": (ctypes.c_int, [P(c_vp), c_i32, c_i64, c_i32, c_i32, P(c_f64), c_vp]),
     "pgr_bench_stream_read_back_to_back": (ctypes.c_int, [P(c_vp), c_i32, c_i64, c_i32, c_i32, P(c_f64), c_vp]),

@@ -31,6 +31,9 @@ DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-m
 SOURCES = [
     ("attn_kernels.hip", "hip", []),
     ("kv_kernels.hip", "hip", []),
+    ("rotary_kernels.hip", "hip", []),
+    ("cache_kernels.hip", "hip", []),
+    ("prompt_weight_kernels.hip", "hip", []),
     ("paged_kv.cpp", "hip", []),
     ("capi.cpp", "hip", []),
     # Host-only placement policy: no fused multiply-add, so f32 rounds like the reference.

@@ -10,6 +10,7 @@
 #include <string>
 #include <vector>
 
+#include "cache_kernels.h"
 #include "paged_kv.h"
 #include "pager_core.h"
 #include "pgr_common.h"
@@ -249,6 +250,139 @@ int exception_status() noexcept {
   return code;
 }
 
+// ---- rotary positions and the bounded cache ----------------------------------------------
+pgr::Strides strides_of(const int64_t* s, int n) {
+  pgr::Strides r;
+  r.b = s[0];
+  r.h = s[1];
+  if (n == 3) r.t = s[2];
+  return r;
+}
+
+int check_rotary(const float* inv_freq, int64_t rotary_dim, int64_t head_dim, float factor) {
+  if (inv_freq == nullptr && rotary_dim != 0) return set_err(pgr::kErrInvalid, "rotary_dim without inv_freq");
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2 != 0)
+    return set_err(pgr::kErrInvalid, "rotary_dim must be even and in [0, head_dim]");
+  if (!std::isfinite(factor)) return set_err(pgr::kErrInvalid, "factor must be finite");
+  return pgr::kOk;
+}
+
+pgr::RotaryForm rotary_form(const float* inv_freq, int64_t rotary_dim, int interleaved, float factor, int inverse) {
+  pgr::RotaryForm f;
+  f.inv_freq = rotary_dim > 0 ? inv_freq : nullptr;
+  f.half = (int)(rotary_dim / 2);
+  f.interleaved = interleaved != 0;
+  f.factor = factor;
+  f.sign = inverse ? -1.f : 1.f;
+  return f;
+}
+
+int check_scores(float scale, float softcap) {
+  if (!(scale > 0.f) || !std::isfinite(scale)) return set_err(pgr::kErrInvalid, "scale must be positive and finite");
+  if (!std::isfinite(softcap)) return set_err(pgr::kErrInvalid, "softcap must be finite");
+  return pgr::kOk;
+}
+
+int check_heads(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int dtype) {
+  if (batch < 0 || hq <= 0 || hkv <= 0 || d <= 0) return set_err(pgr::kErrInvalid, "negative or zero dimension");
+  if (hq % hkv != 0) return set_err(pgr::kErrInvalid, "num_query_heads must be a multiple of num_kv_heads");
+  if (hq / hkv > pgr::kMaxRep)
+    return set_err(pgr::kErrUnsupported, "query heads per KV head are supported up to 16");
+  if (!pgr::hh_head_dim_supported(d)) return set_err(pgr::kErrUnsupported, "head_dim must be 16, 32, 64, 128 or 256");
+  if (dtype != pgr::kF16 && dtype != pgr::kBF16) return set_err(pgr::kErrUnsupported, "dtype must be fp16 or bf16");
+  if (hkv > 65535 || batch > 65535 || batch * hkv > 65535)
+    return set_err(pgr::kErrInvalid, "batch * num_kv_heads must not exceed 65535");
+  return pgr::kOk;
+}
+
+int check_cache(const pgr_hh_cache_t* c) {
+  if (c == nullptr) return set_err(pgr::kErrInvalid, "null cache");
+  int rc = check_heads(c->batch, c->query_heads, c->kv_heads, c->head_dim, c->dtype);
+  if (rc != pgr::kOk) return rc;
+  if (c->capacity <= 0 || c->capacity > ((int64_t)1 << 30))
+    return set_err(pgr::kErrInvalid, "capacity must be in [1, 2^30]");
+  if (c->keep_first < 0 || c->keep_recent < 1 || (int64_t)c->keep_first + c->keep_recent > c->capacity)
+    return set_err(pgr::kErrInvalid, "need keep_first >= 0, keep_recent >= 1 and their sum within the capacity");
+  if (c->batch > 0 && (!c->keys || !c->values || !c->weights || !c->order || !c->lengths || !c->seen))
+    return set_err(pgr::kErrInvalid, "null cache buffer");
+  if (((uintptr_t)c->keys | (uintptr_t)c->values | (uintptr_t)c->weights | (uintptr_t)c->order) % 16 != 0)
+    return set_err(pgr::kErrInvalid, "cache buffers must be 16-byte aligned");
+  return pgr::kOk;
+}
+
+pgr::HHCache cache_of(const pgr_hh_cache_t* c) {
+  pgr::HHCache r;
+  r.keys = c->keys;
+  r.values = c->values;
+  r.weights = c->weights;
+  r.order = c->order;
+  r.lengths = c->lengths;
+  r.seen = c->seen;
+  r.batch = (int)c->batch;
+  r.hq = (int)c->query_heads;
+  r.hkv = (int)c->kv_heads;
+  r.capacity = (int)c->capacity;
+  r.d = (int)c->head_dim;
+  r.keep_first = c->keep_first;
+  r.keep_recent = c->keep_recent;
+  return r;
+}
+
+// Offsets into a workspace, each part on a 256-byte border.
+struct Parts {
+  size_t bytes = 0;
+  size_t take(size_t n) {
+    const size_t at = bytes;
+    bytes = pgr::align_up(bytes + n, 256);
+    return at;
+  }
+};
+
+struct AttendPlan {
+  int n_split = 1;
+  size_t o_logits = 0, o_pm = 0, o_pl = 0, o_pacc = 0, bytes = 0;
+};
+
+AttendPlan plan_attend(const pgr_hh_cache_t* c) {
+  AttendPlan p;
+  p.n_split = pgr::hh_attend_splits((int)c->batch, (int)c->kv_heads, (int)c->capacity);
+  const size_t heads = (size_t)(c->batch * c->query_heads), slots = heads * p.n_split;
+  Parts w;
+  p.o_logits = w.take(heads * (size_t)pgr::hh_attend_stride((int)c->capacity) * sizeof(float));
+  p.o_pm = w.take(slots * sizeof(float));
+  p.o_pl = w.take(slots * sizeof(float));
+  p.o_pacc = w.take(slots * (size_t)c->head_dim * sizeof(float));
+  p.bytes = w.bytes;
+  return p;
+}
+
+struct PromptPlan {
+  pgr::PromptWeightPlan k;
+  size_t o_stats = 0, o_norm = 0, o_partial = 0, bytes = 0;
+};
+
+int check_prompt(int64_t batch, int64_t hq, int64_t hkv, int64_t tokens, int64_t window, int64_t d, int dtype) {
+  int rc = check_heads(batch, hq, hkv, d, dtype);
+  if (rc != pgr::kOk) return rc;
+  if (tokens < 0 || tokens > ((int64_t)1 << 30)) return set_err(pgr::kErrInvalid, "tokens must be in [0, 2^30]");
+  if (window < 0 || window > tokens) return set_err(pgr::kErrInvalid, "the window must be in [0, tokens]");
+  if (window * (hq / hkv) > ((int64_t)1 << 30))
+    return set_err(pgr::kErrInvalid, "window * queries per KV head must not exceed 2^30");
+  return pgr::kOk;
+}
+
+PromptPlan plan_prompt(int64_t batch, int64_t hq, int64_t hkv, int64_t tokens, int64_t window, int64_t d) {
+  PromptPlan p;
+  p.k = pgr::prompt_weight_plan((int)batch, (int)hq, (int)hkv, (int)tokens, (int)window, (int)d);
+  const size_t rows = (size_t)(batch * hq * window);
+  Parts w;
+  p.o_stats = w.take(rows * p.k.key_splits * 2 * sizeof(float));
+  p.o_norm = w.take(rows * sizeof(float));
+  p.o_partial = w.take(p.k.row_splits > 1 ? (size_t)(batch * hkv * tokens) * p.k.row_splits * sizeof(float) : 0);
+  p.bytes = w.bytes;
+  return p;
+}
+
 pgr::PagedKV* kv_of(void* h) { return static_cast<pgr::PagedKV*>(h); }
 
 int kv_rc(pgr::PagedKV* kv, int rc) {
@@ -260,7 +394,7 @@ int kv_rc(pgr::PagedKV* kv, int rc) {
 
 extern "C" {
 
-int pgr_abi_version(void) { return 12; }
+int pgr_abi_version(void) { return 13; }
 
 const char* pgr_last_error(void) { return g_last_error.c_str(); }
 
@@ -1043,6 +1177,228 @@ int pgr_kv_sync(void* kv) {
   try {
     if (!kv) return set_err(pgr::kErrInvalid, "null store");
     return kv_rc(kv_of(kv), kv_of(kv)->sync());
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+// ---- rotary positions and the bounded cache ----------------------------------------------
+int pgr_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_heads, const void* k,
+               const int64_t* k_strides, void* k_out, int64_t k_heads, const void* positions, int positions_64bit,
+               const int64_t* position_strides, const float* inv_freq, int64_t rotary_dim, int64_t batch,
+               int64_t tokens, int64_t head_dim, int dtype, int interleaved, float factor, int inverse,
+               void* stream) {
+  try {
+    if (q_heads < 0 || k_heads < 0 || batch < 0 || tokens < 0 || head_dim <= 0)
+      return set_err(pgr::kErrInvalid, "negative or zero dimension");
+    if (dtype != pgr::kF16 && dtype != pgr::kBF16 && dtype != pgr::kF32)
+      return set_err(pgr::kErrInvalid, "dtype must be fp16, bf16 or fp32");
+    int rc = check_rotary(inv_freq, rotary_dim, head_dim, factor);
+    if (rc != pgr::kOk) return rc;
+    if (q_heads > 65535 || k_heads > 65535 || batch > ((int64_t)1 << 30) || tokens > ((int64_t)1 << 30) ||
+        head_dim > 65536 || (batch > 0 && tokens > 0 && batch * tokens > ((int64_t)1 << 38) / head_dim))
+      return set_err(pgr::kErrInvalid, "shape exceeds the launch limits");
+    if (batch == 0 || tokens == 0 || q_heads + k_heads == 0) return pgr::kOk;
+    if ((q_heads > 0 && (!q || !q_out || !q_strides)) || (k_heads > 0 && (!k || !k_out || !k_strides)))
+      return set_err(pgr::kErrInvalid, "null tensor pointer");
+    if (rotary_dim > 0 && (!positions || !position_strides)) return set_err(pgr::kErrInvalid, "null positions");
+    pgr::RotaryLaunch L;
+    L.x[0] = q;
+    L.x[1] = k;
+    L.y[0] = q_out;
+    L.y[1] = k_out;
+    if (q_heads > 0) L.xs[0] = strides_of(q_strides, 3);
+    if (k_heads > 0) L.xs[1] = strides_of(k_strides, 3);
+    L.heads[0] = (int)q_heads;
+    L.heads[1] = (int)k_heads;
+    L.positions = positions;
+    L.positions64 = positions_64bit != 0;
+    if (position_strides != nullptr) {
+      L.pos_b = position_strides[0];
+      L.pos_t = position_strides[1];
+    }
+    L.form = rotary_form(inv_freq, rotary_dim, interleaved, factor, inverse);
+    L.batch = (int)batch;
+    L.tokens = (int)tokens;
+    L.d = (int)head_dim;
+    const hipError_t e = pgr::launch_rotary(dtype, L, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "rotary launch");
+    return pgr::kOk;
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+int pgr_hh_append(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_strides, const void* k,
+                  const int64_t* k_strides, const void* v, const int64_t* v_strides, void* q_out,
+                  const void* positions, int positions_64bit, const float* inv_freq, int64_t rotary_dim,
+                  int interleaved, float factor, void* stream) {
+  try {
+    int rc = check_cache(cache);
+    if (rc != pgr::kOk) return rc;
+    rc = check_rotary(inv_freq, rotary_dim, cache->head_dim, factor);
+    if (rc != pgr::kOk) return rc;
+    if (cache->batch == 0) return pgr::kOk;
+    if (!k || !v || !k_strides || !v_strides || (q_out && (!q || !q_strides)))
+      return set_err(pgr::kErrInvalid, "null tensor pointer");
+    pgr::HHAppendLaunch L;
+    L.c = cache_of(cache);
+    L.k = k;
+    L.v = v;
+    L.ks = strides_of(k_strides, 2);
+    L.vs = strides_of(v_strides, 2);
+    if (q_out != nullptr) {
+      L.q = q;
+      L.qs = strides_of(q_strides, 2);
+      L.q_out = q_out;
+    }
+    L.positions = positions;
+    L.positions64 = positions_64bit != 0;
+    L.form = rotary_form(inv_freq, rotary_dim, interleaved, factor, 0);
+    const hipError_t e = pgr::launch_hh_append(cache->dtype, L, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "append launch");
+    return pgr::kOk;
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+size_t pgr_hh_attend_workspace_bytes(const pgr_hh_cache_t* cache) {
+  try {
+    if (check_cache(cache) != pgr::kOk || cache->batch == 0) return 0;
+    return plan_attend(cache).bytes;
+  } catch (...) {
+    exception_status();
+    return 0;
+  }
+}
+
+int pgr_hh_attend(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_strides, void* out, float scale,
+                  float softcap, void* workspace, size_t workspace_bytes, void* stream) {
+  try {
+    int rc = check_cache(cache);
+    if (rc != pgr::kOk) return rc;
+    rc = check_scores(scale, softcap);
+    if (rc != pgr::kOk) return rc;
+    if (cache->batch == 0) return pgr::kOk;
+    if (!q || !q_strides || !out) return set_err(pgr::kErrInvalid, "null tensor pointer");
+    const AttendPlan p = plan_attend(cache);
+    if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < p.bytes))
+      return set_err(pgr::kErrCapacity, "workspace too small");
+    if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");
+    char* w = static_cast<char*>(workspace);
+    pgr::HHAttendLaunch L;
+    L.c = cache_of(cache);
+    L.q = q;
+    L.qs = strides_of(q_strides, 2);
+    L.out = out;
+    L.scale = scale;
+    L.softcap = softcap;
+    L.n_split = p.n_split;
+    L.logits = reinterpret_cast<float*>(w + p.o_logits);
+    L.pm = reinterpret_cast<float*>(w + p.o_pm);
+    L.pl = reinterpret_cast<float*>(w + p.o_pl);
+    L.pacc = reinterpret_cast<float*>(w + p.o_pacc);
+    const hipError_t e = pgr::launch_hh_attend(cache->dtype, L, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "attend launch");
+    return pgr::kOk;
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+size_t pgr_hh_prompt_weights_workspace_bytes(int64_t batch, int64_t num_query_heads, int64_t num_kv_heads,
+                                             int64_t tokens, int64_t window, int64_t head_dim) {
+  try {
+    if (check_prompt(batch, num_query_heads, num_kv_heads, tokens, window, head_dim, pgr::kF16) != pgr::kOk) return 0;
+    if (batch == 0 || window == 0) return 0;
+    return plan_prompt(batch, num_query_heads, num_kv_heads, tokens, window, head_dim).bytes;
+  } catch (...) {
+    exception_status();
+    return 0;
+  }
+}
+
+int pgr_hh_prompt_weights(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          const int32_t* lo, float* weights, int64_t batch, int64_t num_query_heads,
+                          int64_t num_kv_heads, int64_t tokens, int64_t window, int64_t head_dim, int dtype,
+                          float scale, float softcap, void* workspace, size_t workspace_bytes, void* stream) {
+  try {
+    int rc = check_prompt(batch, num_query_heads, num_kv_heads, tokens, window, head_dim, dtype);
+    if (rc != pgr::kOk) return rc;
+    rc = check_scores(scale, softcap);
+    if (rc != pgr::kOk) return rc;
+    if (batch == 0 || tokens == 0) return pgr::kOk;
+    if (window == 0) return set_err(pgr::kErrInvalid, "the window must hold a query");
+    if (!q || !q_strides || !k || !k_strides || !weights) return set_err(pgr::kErrInvalid, "null tensor pointer");
+    const PromptPlan p = plan_prompt(batch, num_query_heads, num_kv_heads, tokens, window, head_dim);
+    if (workspace == nullptr || workspace_bytes < p.bytes) return set_err(pgr::kErrCapacity, "workspace too small");
+    if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");
+    char* w = static_cast<char*>(workspace);
+    pgr::PromptWeightLaunch L;
+    L.q = q;
+    L.k = k;
+    L.qs = strides_of(q_strides, 3);
+    L.ks = strides_of(k_strides, 3);
+    L.lo = lo;
+    L.out = weights;
+    L.batch = (int)batch;
+    L.hq = (int)num_query_heads;
+    L.hkv = (int)num_kv_heads;
+    L.tokens = (int)tokens;
+    L.window = (int)window;
+    L.d = (int)head_dim;
+    L.scale = scale;
+    L.softcap = softcap;
+    L.plan = p.k;
+    L.stats = reinterpret_cast<float2*>(w + p.o_stats);
+    L.norm = reinterpret_cast<float*>(w + p.o_norm);
+    L.partial = reinterpret_cast<float*>(w + p.o_partial);
+    const hipError_t e = pgr::launch_prompt_weights(dtype, L, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "prompt weights launch");
+    return pgr::kOk;
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+size_t pgr_hh_load_prompt_workspace_bytes(const pgr_hh_cache_t* cache) {
+  try {
+    if (check_cache(cache) != pgr::kOk) return 0;
+    return pgr::align_up((size_t)(cache->batch * cache->kv_heads) * cache->capacity * sizeof(int32_t), 256);
+  } catch (...) {
+    exception_status();
+    return 0;
+  }
+}
+
+int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t* k_strides, const void* v,
+                       const int64_t* v_strides, const float* weights, const int32_t* lo, int64_t tokens,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  try {
+    int rc = check_cache(cache);
+    if (rc != pgr::kOk) return rc;
+    if (tokens < 0 || tokens > ((int64_t)1 << 30)) return set_err(pgr::kErrInvalid, "tokens must be in [0, 2^30]");
+    if (cache->batch == 0) return pgr::kOk;
+    if (tokens > 0 && (!k || !k_strides || !v || !v_strides || !weights))
+      return set_err(pgr::kErrInvalid, "null tensor pointer");
+    if (workspace == nullptr || workspace_bytes < pgr_hh_load_prompt_workspace_bytes(cache))
+      return set_err(pgr::kErrCapacity, "workspace too small");
+    pgr::HHLoadLaunch L;
+    L.c = cache_of(cache);
+    L.k = k;
+    L.v = v;
+    if (tokens > 0) {
+      L.ks = strides_of(k_strides, 3);
+      L.vs = strides_of(v_strides, 3);
+    }
+    L.weights = weights;
+    L.lo = lo;
+    L.tokens = (int)tokens;
+    L.kept = static_cast<int32_t*>(workspace);
+    const hipError_t e = pgr::launch_hh_load(L, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "load prompt launch");
+    return pgr::kOk;
   } catch (...) {
     return exception_status();
   }

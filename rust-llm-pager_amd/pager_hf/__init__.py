@@ -4,11 +4,12 @@ Exports follow pager_hf/__init__.py:1-4 of the reference where the path is built
 ``PagedModel`` (the HuggingFace wrapper), ``KVBlockStore`` (reference API over the native
 slot pools) and the fused multi-session decoder ``PagedDecoder``. Operator functions live in ``pager_hf.streaming_attention``.
 """
+from .heavy_hitter_cache import HeavyHitterCache
 from .kv_block_store import KVBlockStore, KVBlockStoreStats
 from .kv_pool import NativeKVPool
 from .paged_decode import PagedDecoder
 
-__all__ = ["GenerationStats", "KVBlockStore", "KVBlockStoreStats", "NativeKVPool", "PagedDecoder", "PagedModel"]
+__all__ = ["GenerationStats", "HeavyHitterCache", "KVBlockStore", "KVBlockStoreStats", "NativeKVPool", "PagedDecoder", "PagedModel"]
 
 
 def __getattr__(name):

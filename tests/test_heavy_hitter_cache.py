@@ -1,0 +1,141 @@
+"""The bounded cache's refusals and its oracle (CPU)."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import _pgr_native as nat
+from oracle import bounded_cache as O
+from pager_hf.heavy_hitter_cache import HeavyHitterCache, prompt_attention_weights
+
+
+def _cache(**over):
+    fields = dict(keys=256, values=256, weights=256, order=256, lengths=256, seen=256, batch=1, query_heads=4, kv_heads=2,
+                  capacity=64, head_dim=32, dtype=0, keep_first=4, keep_recent=8)
+    return nat.HHCache(**{**fields, **over})
+
+
+BAD_CACHES = [
+    (dict(batch=-1), nat.PGR_ERR_INVALID), (dict(query_heads=3), nat.PGR_ERR_INVALID),
+    (dict(query_heads=34), nat.PGR_ERR_UNSUPPORTED), (dict(head_dim=48), nat.PGR_ERR_UNSUPPORTED),
+    (dict(dtype=2), nat.PGR_ERR_UNSUPPORTED), (dict(capacity=0), nat.PGR_ERR_INVALID),
+    (dict(capacity=(1 << 30) + 1), nat.PGR_ERR_INVALID), (dict(keep_first=-1), nat.PGR_ERR_INVALID),
+    (dict(keep_recent=0), nat.PGR_ERR_INVALID), (dict(keep_first=60, keep_recent=5), nat.PGR_ERR_INVALID),
+    (dict(seen=0), nat.PGR_ERR_INVALID), (dict(keys=264), nat.PGR_ERR_INVALID),
+    (dict(batch=65536), nat.PGR_ERR_INVALID),
+]
+
+
+@pytest.mark.parametrize("over,code", BAD_CACHES)
+def test_c_entries_refuse_a_bad_cache(over, code):
+    lib, c = nat.load(), _cache(**over)
+    s = (ctypes.c_int64 * 3)(1, 1, 1)
+    assert lib.pgr_hh_append(c, 16, s, 16, s, 16, s, 16, None, 0, None, 0, 0, 1.0, None) == code
+    assert lib.pgr_hh_attend(c, 16, s, 16, 1.0, 0.0, 256, 1 << 30, None) == code
+    assert lib.pgr_hh_load_prompt(c, 16, s, 16, s, 16, None, 4, 256, 1 << 30, None) == code
+    assert lib.pgr_hh_attend_workspace_bytes(c) == 0 and lib.pgr_hh_load_prompt_workspace_bytes(c) == 0
+
+
+def test_c_entries_refuse_bad_arguments():
+    lib, c = nat.load(), _cache()
+    s = (ctypes.c_int64 * 3)(1, 1, 1)
+    inv, cap = nat.PGR_ERR_INVALID, nat.PGR_ERR_CAPACITY
+    assert lib.pgr_hh_append(None, 16, s, 16, s, 16, s, 16, None, 0, None, 0, 0, 1.0, None) == inv
+    assert lib.pgr_hh_append(c, 16, s, None, s, 16, s, 16, None, 0, None, 0, 0, 1.0, None) == inv
+    assert lib.pgr_hh_append(c, None, s, 16, s, 16, s, 16, None, 0, None, 0, 0, 1.0, None) == inv
+    assert lib.pgr_hh_append(c, 16, s, 16, s, 16, s, 16, None, 0, None, 2, 0, 1.0, None) == inv  # no inv_freq
+    assert lib.pgr_hh_append(c, 16, s, 16, s, 16, s, 16, None, 0, 16, 34, 0, 1.0, None) == inv   # past the head
+    assert lib.pgr_hh_append(c, 16, s, 16, s, 16, s, 16, None, 0, 16, 3, 0, 1.0, None) == inv    # odd
+    need = lib.pgr_hh_attend_workspace_bytes(c)
+    assert need > 0
+    assert lib.pgr_hh_attend(c, 16, s, 16, 1.0, 0.0, 256, need - 1, None) == cap
+    assert lib.pgr_hh_attend(c, 16, s, 16, 1.0, 0.0, None, need, None) == cap
+    assert lib.pgr_hh_attend(c, 16, s, None, 1.0, 0.0, 256, need, None) == inv
+    assert lib.pgr_hh_attend(c, 16, s, 16, 0.0, 0.0, 256, need, None) == inv
+    assert lib.pgr_hh_attend(c, 16, s, 16, 1.0, float("nan"), 256, need, None) == inv
+    need = lib.pgr_hh_load_prompt_workspace_bytes(c)
+    assert need >= 2 * 64 * 4
+    assert lib.pgr_hh_load_prompt(c, 16, s, 16, s, 16, None, -1, 256, need, None) == inv
+    assert lib.pgr_hh_load_prompt(c, 16, s, 16, s, None, None, 4, 256, need, None) == inv
+    assert lib.pgr_hh_load_prompt(c, 16, s, 16, s, 16, None, 4, 256, need - 1, None) == cap
+    bytes_of = lib.pgr_hh_prompt_weights_workspace_bytes
+    assert bytes_of(1, 4, 2, 100, 10, 32) > 0
+    for bad in ((1, 4, 2, 100, 101, 32), (1, 4, 2, 100, -1, 32), (1, 3, 2, 100, 10, 32), (1, 4, 2, 100, 10, 40),
+                (1, 34, 2, 100, 10, 32)):
+        assert bytes_of(*bad) == 0
+    run = lib.pgr_hh_prompt_weights
+    assert run(16, s, 16, s, None, 16, 1, 4, 2, 100, 101, 32, 0, 1.0, 0.0, 256, 1 << 30, None) == inv
+    assert run(16, s, 16, s, None, 16, 1, 4, 2, 100, 0, 32, 0, 1.0, 0.0, 256, 1 << 30, None) == inv
+    assert run(16, s, 16, s, None, 16, 1, 4, 2, 100, 10, 32, 2, 1.0, 0.0, 256, 1 << 30, None) == nat.PGR_ERR_UNSUPPORTED
+    assert run(16, s, 16, s, None, 16, 1, 4, 2, 100, 10, 32, 0, -1.0, 0.0, 256, 1 << 30, None) == inv
+    assert run(16, s, 16, s, None, 16, 1, 4, 2, 100, 10, 32, 0, 1.0, 0.0, 256, 16, None) == cap
+    assert run(None, s, 16, s, None, 16, 1, 4, 2, 100, 10, 32, 0, 1.0, 0.0, 256, 1 << 30, None) == inv
+    assert run(16, s, 16, s, None, 16, 1, 4, 2, 0, 0, 32, 0, 1.0, 0.0, None, 0, None) == 0  # nothing to do
+
+
+def test_python_refusals_need_no_gpu():
+    def make(**over):
+        a = dict(batch=1, num_query_heads=4, num_kv_heads=2, capacity=64, head_dim=32, dtype=torch.float16, device="cuda")
+        return HeavyHitterCache(**{**a, **over})
+
+    with pytest.raises(ValueError, match="CUDA"):
+        make(device="cpu")
+    with pytest.raises(NotImplementedError, match="float32"):
+        make(dtype=torch.float32)
+    with pytest.raises(NotImplementedError, match="head_dim"):
+        make(head_dim=80)
+    with pytest.raises(NotImplementedError, match="16"):
+        make(num_query_heads=34)
+    with pytest.raises(ValueError, match="multiple"):
+        make(num_query_heads=5)
+    with pytest.raises(ValueError, match="keep_recent"):
+        make(keep_recent=0)
+    with pytest.raises(ValueError, match="capacity"):
+        make(keep_first=40, keep_recent=25)
+    with pytest.raises(ValueError, match="dimension"):
+        make(capacity=0)
+    q, k = torch.zeros(1, 4, 8, 32).half(), torch.zeros(1, 2, 16, 32).half()
+    with pytest.raises(ValueError, match="CUDA"):
+        prompt_attention_weights(q, k)
+    with pytest.raises(NotImplementedError, match="float32"):
+        prompt_attention_weights(q.float(), k.float())
+    with pytest.raises(TypeError, match="one dtype"):
+        prompt_attention_weights(q, k.bfloat16())
+    with pytest.raises(ValueError, match="does not match"):
+        prompt_attention_weights(q, k[..., :16])
+    with pytest.raises(RuntimeError, match="gradient"):
+        prompt_attention_weights(q, k.requires_grad_())
+
+
+# ---- the oracle itself ---------------------------------------------------------------------------
+def test_oracle_keeps_what_the_rule_says():
+    w = np.array([0.0, 5.0, 1.0, 3.0, 3.0, np.nan, 0.5, 3.0, 9.0, 0.1])
+    assert O.kept_columns(w, 0, 10, 1, 1).tolist() == list(range(10))
+    assert O.kept_columns(w, 4, 6, 1, 1).tolist() == [4, 5, 6, 7, 8, 9]
+    # first 1, last 2; then NaN, 5, and the first of the threes
+    assert O.kept_columns(w, 0, 6, 1, 2).tolist() == [0, 1, 3, 5, 8, 9]
+    assert O.kept_columns(w, 0, 7, 1, 2).tolist() == [0, 1, 3, 4, 5, 8, 9]
+    assert O.kept_columns(w, 0, 3, 1, 2).tolist() == [0, 8, 9]
+
+
+def test_oracle_slot_of_an_append():
+    w = np.array([0.0, 2.0, -0.0, np.nan, 2.0, 0.0])
+    order = np.array([0, 1, 7, 3, 9, 5])
+    assert O.append_slot(4, 10, w, order, 6, 1, 2) == 4       # room left
+    assert O.append_slot(6, 10, w, order, 6, 1, 2) == 2       # order 0 and 9 stay; -0 equals 0: the lower slot
+    assert O.append_slot(6, 10, w, order, 6, 1, 4) == 5       # 7 and 9 are recent
+    assert O.append_slot(6, 10, w, order, 6, 0, 1) == 0
+
+
+def test_oracle_prompt_weights_sum_to_the_queries():
+    rng = np.random.default_rng(0)
+    q, k = rng.standard_normal((3, 5, 16)), rng.standard_normal((9, 16))
+    w, _ = O.prompt_weights(q, k, 2, 0.25, 0.0)
+    assert abs(w.sum() - 15) < 1e-12 and not w[:2].any()
+    w, _ = O.prompt_weights(q, k, 6, 0.25, 30.0)  # queries at columns 4, 5 are padding
+    assert abs(w.sum() - 9) < 1e-12 and not w[:6].any()
+    w, _ = O.prompt_weights(q, k, 9, 0.25, 0.0)
+    assert not w.any()

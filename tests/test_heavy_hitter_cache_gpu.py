@@ -1,0 +1,452 @@
+"""The bounded cache on the GPU against the 64-bit oracle, operator by operator and as a run."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import bounded_cache as O
+from pager_hf.heavy_hitter_cache import HeavyHitterCache, prompt_attention_weights
+from pager_hf.rotary import rotary_embedding, rotary_frequencies
+
+pytestmark = pytest.mark.gpu
+STEP = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
+STATE = ("keys", "values", "weights", "order", "lengths", "seen")
+
+
+def _np(t):
+    return t.detach().cpu().double().numpy()
+
+
+def _within(got, ref, bound, what):
+    got = _np(got) if isinstance(got, torch.Tensor) else got
+    err = np.abs(got - ref)
+    assert np.all(err <= bound), f"{what}: off by {np.nanmax(err)}, {np.nanmax(err / np.maximum(bound, 1e-300)):.3g} x bound"
+
+
+def _state(cache):
+    return {n: getattr(cache, n).clone() for n in STATE}
+
+
+def _same(cache, state, *names):
+    for n in names or STATE:
+        a, b = getattr(cache, n), state[n]
+        assert torch.equal(a.view(torch.int16) if a.dtype in STEP else a.view(torch.int32) if a.is_floating_point() else a,
+                           b.view(torch.int16) if b.dtype in STEP else b.view(torch.int32) if b.is_floating_point() else b), n
+
+
+def _filled(b, hq, hkv, c, d, dtype, lengths, seed, garbage=False, **keep):
+    """A cache of random tokens; garbage: NaN in the slots that hold nothing."""
+    g = torch.Generator().manual_seed(seed)
+    cache = HeavyHitterCache(b, hq, hkv, c, d, dtype, "cuda", **keep)
+    cache.keys.copy_(torch.randn(b, hkv, c, d, generator=g))
+    cache.values.copy_(torch.randn(b, hkv, c, d, generator=g))
+    cache.weights.copy_(torch.rand(b, hkv, c, generator=g) * 4)
+    cache.lengths.copy_(torch.tensor(lengths, dtype=torch.int32)[:, None].expand(b, hkv))
+    cache.seen.copy_(cache.lengths)
+    cache.order.copy_(torch.arange(c).expand(b, hkv, c))
+    if garbage:
+        free = torch.arange(c, device="cuda") >= cache.lengths[..., None]
+        for t in (cache.keys, cache.values):
+            t.masked_fill_(free[..., None], float("nan"))
+        cache.weights.masked_fill_(free, float("nan"))
+    return cache, g
+
+
+# ---- attend --------------------------------------------------------------------------------------
+ATTEND = [
+    # batch, query heads, kv heads, head dim, capacity, lengths
+    (1, 14, 2, 64, 256, [256]),
+    (4, 4, 2, 16, 65, [0, 1, 64, 65]),
+    (5, 12, 2, 128, 333, [0, 15, 16, 17, 333]),
+    (3, 16, 1, 32, 1000, [63, 640, 999]),
+    (2, 8, 1, 256, 203, [203, 70]),
+    (2, 16, 16, 64, 130, [129, 3]),
+    (1, 1, 1, 128, 1, [1]),
+    (2, 28, 4, 128, 4133, [4133, 1025]),
+    (1, 16, 1, 64, 16387, [16387]),
+    (40, 16, 8, 64, 70, [i * 70 // 39 for i in range(40)]),
+]
+
+
+@pytest.mark.parametrize("dtype", list(STEP))
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+@pytest.mark.parametrize("case", ATTEND, ids=[str(c[:5]) for c in ATTEND])
+def test_attend(case, dtype, softcap):
+    b, hq, hkv, d, c, lengths = case
+    cache, g = _filled(b, hq, hkv, c, d, dtype, lengths, 11, garbage=True, keep_first=0, keep_recent=1)
+    before = _state(cache)
+    # Queries as views into a larger tensor.
+    q = (torch.randn(b, hq + 2, d + 8, generator=g) * 2).to(dtype).cuda()[:, 1:-1, :d]
+    out = cache.attend(q, softcap=softcap)
+    _same(cache, before, "keys", "values", "order", "lengths", "seen")
+    rep, scale = hq // hkv, 1.0 / d**0.5
+    k, v, w, qn = _np(cache.keys), _np(cache.values), _np(before["weights"]), _np(q)
+    for i in range(b):
+        n = lengths[i]
+        for h in range(hkv):
+            heads = slice(h * rep, (h + 1) * rep)
+            ref, bound, new, new_bound = O.attend(qn[i, heads], k[i, h, :n], v[i, h, :n], w[i, h, :n], scale, softcap,
+                                                  STEP[dtype])
+            _within(out[i, heads], ref, bound, f"out row {i} head {h}")
+            _within(cache.weights[i, h, :n], new, new_bound, f"weights row {i} head {h}")
+            assert torch.isnan(cache.weights[i, h, n:]).all()
+
+
+def test_attend_with_a_few_heavy_and_far_scores():
+    """Scores spread over hundreds: the running maximum moves, most weights underflow."""
+    cache, g = _filled(1, 4, 1, 700, 64, torch.float16, [700], 3, keep_first=0, keep_recent=1)
+    cache.keys.mul_(6)
+    w = _np(cache.weights)
+    q = (torch.randn(1, 4, 64, generator=g) * 8).half().cuda()
+    out = cache.attend(q, scale=0.5)
+    ref, bound, new, nb = O.attend(_np(q)[0], _np(cache.keys)[0, 0], _np(cache.values)[0, 0], w[0, 0], 0.5, 0.0,
+                                   STEP[torch.float16])
+    _within(out[0], ref, bound, "out")
+    _within(cache.weights[0, 0], new, nb, "weights")
+
+
+def test_attend_is_the_same_every_time():
+    cache, g = _filled(2, 8, 2, 3000, 128, torch.bfloat16, [3000, 1234], 4)
+    q = torch.randn(2, 8, 128, generator=g).bfloat16().cuda()
+    before = cache.weights.clone()
+    first, w = cache.attend(q), cache.weights.clone()
+    for _ in range(5):
+        cache.weights.copy_(before)
+        assert torch.equal(cache.attend(q), first) and torch.equal(cache.weights, w)
+
+
+def test_offsets_past_32_bits():
+    """The last rows of a cache of more than 2^32 bytes and 2^31 elements of keys."""
+    b, hkv, c, d = 9, 1, 1 << 20, 256
+    cache = HeavyHitterCache(b, 2, hkv, c, d, torch.float16, "cuda", keep_first=0, keep_recent=1)
+    assert cache.keys.numel() > 1 << 31
+    g = torch.Generator().manual_seed(1)
+    n = 50
+    cache.keys[-1, 0, :n] = torch.randn(n, d, generator=g).half().cuda()
+    cache.values[-1, 0, :n] = torch.randn(n, d, generator=g).half().cuda()
+    cache.lengths[-1] = n
+    q = torch.randn(b, 2, d, generator=g).half().cuda()
+    out = cache.attend(q)
+    ref, bound, new, nb = O.attend(_np(q[-1]), _np(cache.keys[-1, 0, :n]), _np(cache.values[-1, 0, :n]), np.zeros(n),
+                                   1 / 16, 0.0, STEP[torch.float16])
+    _within(out[-1], ref, bound, "out")
+    _within(cache.weights[-1, 0, :n], new, nb, "weights")
+    assert not out[:-1].any()
+    cache.lengths[-1] = c  # full: the lightest slot is the first of the untouched ones
+    cache.seen[-1] = c
+    k = torch.randn(b, 1, d, generator=g).half().cuda()
+    cache.append(q, k, k)
+    assert torch.equal(cache.keys[-1, 0, n], k[-1, 0]) and cache.order[-1, 0, n] == c
+    assert torch.equal(cache.keys[0, 0, 0], k[0, 0]) and cache.lengths[0, 0] == 1
+
+
+# ---- append --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(STEP))
+@pytest.mark.parametrize("case", [(1, 14, 2, 64, 256, 64), (3, 4, 2, 16, 20, 8), (4, 12, 2, 128, 1031, 128),
+                                  (2, 8, 1, 256, 4099, 128), (2, 16, 16, 64, 33, 62), (2, 16, 1, 32, 6, 32)],
+                         ids=str)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append(case, dtype, interleaved):
+    b, hq, hkv, d, c, r = case
+    lengths = [c] * b
+    if b > 2:
+        lengths[1] = c - 2
+    cache, g = _filled(b, hq, hkv, c, d, dtype, lengths, 21, keep_first=2, keep_recent=4)
+    # Full rows have seen more than they hold, out of order, with weights that tie and a few NaN.
+    for i in range(b):
+        if lengths[i] == c:
+            for h in range(hkv):
+                cache.order[i, h] = torch.randperm(2 * c, generator=g)[:c].int()
+            cache.seen[i] = 2 * c
+    cache.weights.copy_((cache.weights * 2).round() / 2)
+    cache.weights[:, :, 3] = float("nan")
+    inv, factor = rotary_frequencies(r, device="cuda")
+    for step in range(4):
+        before = _state(cache)
+        # Views of one projection, as a fused q/k/v product gives them.
+        x = torch.randn(b, (hq + 2 * hkv) * d, generator=g).to(dtype).cuda()
+        q, k, v = (t.view(b, -1, d) for t in x.split([hq * d, hkv * d, hkv * d], dim=1))
+        positions = None if step % 2 == 0 else torch.randint(0, 1 << 18, (b,), generator=g).cuda()
+        got = cache.append(q, k, v, inv, positions=positions, interleaved=interleaved, factor=1.5)
+        pos = before["seen"][:, 0] if positions is None else positions
+        want_q, want_k = rotary_embedding(q, k, pos, inv, interleaved=interleaved, factor=1.5)
+        assert torch.equal(got, want_q)
+        for i in range(b):
+            for h in range(hkv):
+                slot = O.append_slot(int(before["lengths"][i, h]), int(before["seen"][i, h]),
+                                     _np(before["weights"][i, h]), _np(before["order"][i, h]), c, 2, 4)
+                before["keys"][i, h, slot], before["values"][i, h, slot] = want_k[i, h], v[i, h]
+                before["weights"][i, h, slot], before["order"][i, h, slot] = 0.0, before["seen"][i, h]
+        before["lengths"].add_(1).clamp_(max=c)
+        before["seen"].add_(1)
+        _same(cache, before)
+
+
+def test_append_without_rotation_returns_the_queries():
+    cache, g = _filled(2, 4, 2, 8, 32, torch.float16, [0, 8], 5, keep_first=1, keep_recent=2)
+    q, k, v = (torch.randn(2, h, 32, generator=g).half().cuda() for h in (4, 2, 2))
+    assert cache.append(q, k, v) is q
+    assert torch.equal(cache.keys[0, :, 0], k[0]) and torch.equal(cache.values[0, :, 0], v[0])
+    assert cache.lengths.tolist() == [[1, 1], [8, 8]] and cache.seen.tolist() == [[1, 1], [9, 9]]
+    strided = torch.randn(2, 32, 4, generator=g).half().cuda().transpose(1, 2)  # head_dim not contiguous
+    assert torch.equal(cache.append(strided, k, v), strided)
+
+
+def test_a_cache_of_one_slot():
+    cache = HeavyHitterCache(1, 1, 1, 1, 16, torch.float16, "cuda", keep_first=0, keep_recent=1)
+    for n in range(3):
+        k = torch.full((1, 1, 16), n + 1.0, dtype=torch.float16, device="cuda")
+        cache.append(k, k, k)
+        assert torch.equal(cache.attend(k), k)
+        assert (int(cache.lengths), int(cache.seen), int(cache.order), float(cache.weights)) == (1, n + 1, n, 1.0)
+
+
+# ---- prompt weights ------------------------------------------------------------------------------
+PROMPT = [
+    # batch, query heads, kv heads, head dim, tokens, window, lo
+    (1, 4, 2, 64, 1, 1, None),
+    (2, 14, 2, 64, 77, 5, [0, 30]),
+    (3, 4, 2, 16, 130, 130, [0, 129, 130]),
+    (1, 12, 2, 128, 515, 64, None),
+    (2, 8, 1, 256, 300, 33, [299, 1]),
+    (1, 16, 1, 32, 1000, 17, None),
+    (1, 16, 16, 64, 257, 257, None),
+    (2, 28, 4, 128, 384, 200, [128, 200]),
+    (1, 8, 1, 256, 260, 260, [100]),
+    (1, 1, 1, 128, 2500, 1, None),
+]
+
+
+@pytest.mark.parametrize("dtype", list(STEP))
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+@pytest.mark.parametrize("case", PROMPT, ids=[str(c[:6]) for c in PROMPT])
+def test_prompt_weights(case, dtype, softcap):
+    b, hq, hkv, d, t, w, lo = case
+    g = torch.Generator().manual_seed(31)
+    # [B, T, H, D] seen as [B, H, T, D]; the window is a slice of all queries.
+    q = (torch.randn(b, t, hq, d, generator=g) * 2).to(dtype).cuda().transpose(1, 2)[:, :, t - w:]
+    k = torch.randn(b, t, hkv, d, generator=g).to(dtype).cuda().transpose(1, 2)
+    if lo is not None:  # what the padding holds does not matter
+        for i in range(b):
+            k[i, :, : lo[i]] = float("nan")
+            q[i, :, : max(0, lo[i] - (t - w))] = float("nan")
+    forms = [lo] if lo is None else [lo, torch.tensor(lo, device="cuda")]
+    for form in forms:
+        got = prompt_attention_weights(q, k, lo=form, softcap=softcap)
+        assert got.dtype == torch.float32 and got.is_contiguous()
+        for i in range(b):
+            for h in range(hkv):
+                qn = _np(q[i, h * (hq // hkv):(h + 1) * (hq // hkv)])
+                ref, bound = O.prompt_weights(qn, _np(k[i, h]), lo[i] if lo else 0, 1.0 / d**0.5, softcap)
+                _within(got[i, h], ref, bound, f"row {i} head {h}")
+
+
+def test_prompt_weights_are_the_same_every_time():
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(1, 8, 700, 64, generator=g).half().cuda()
+    k = torch.randn(1, 2, 3000, 64, generator=g).half().cuda()
+    first = prompt_attention_weights(q, k)
+    for _ in range(4):
+        assert torch.equal(prompt_attention_weights(q, k), first)
+    assert abs(first.double().sum().item() - 8 * 700) < 8 * 700 * 1e-5
+
+
+def test_prompt_weights_refusals():
+    q, k = torch.zeros(1, 4, 9, 32, device="cuda").half(), torch.zeros(1, 2, 8, 32, device="cuda").half()
+    with pytest.raises(ValueError, match="window"):
+        prompt_attention_weights(q, k)
+    with pytest.raises(ValueError, match="window"):
+        prompt_attention_weights(q[:, :, :0], k)
+    with pytest.raises(NotImplementedError, match="head_dim"):
+        prompt_attention_weights(q[:, :, :8, :24], k[..., :24])
+    with pytest.raises(ValueError, match="scale"):
+        prompt_attention_weights(q[:, :, :8], k, scale=-1.0)
+    with pytest.raises(ValueError, match="lo"):
+        prompt_attention_weights(q[:, :, :8], k, lo=[0, 0])
+    with pytest.raises(TypeError, match="lo"):
+        prompt_attention_weights(q[:, :, :8], k, lo=torch.zeros(1, device="cuda"))
+    assert prompt_attention_weights(q[:, :, :0], k[:, :, :0]).shape == (1, 2, 0)
+
+
+# ---- prompt selection ----------------------------------------------------------------------------
+LOAD = [
+    # batch, kv heads, head dim, tokens, capacity, keep_first, keep_recent, lo
+    (2, 2, 64, 300, 100, 4, 32, [0, 210]),
+    (1, 2, 16, 1, 40, 4, 32, None),
+    (3, 1, 32, 65, 64, 0, 1, [0, 1, 65]),
+    (1, 8, 128, 5000, 1031, 4, 100, None),
+    (2, 1, 256, 1025, 36, 4, 32, [0, 989]),
+    (1, 1, 64, 70000, 4096, 4, 256, None),
+    (1, 2, 64, 0, 40, 4, 32, None),
+]
+
+
+@pytest.mark.parametrize("dtype", list(STEP))
+@pytest.mark.parametrize("kind", ["plain", "ties", "odd"])
+@pytest.mark.parametrize("case", LOAD, ids=[str(c[:7]) for c in LOAD])
+def test_load_prompt(case, kind, dtype):
+    b, hkv, d, t, c, first, recent, lo = case
+    g = torch.Generator().manual_seed(41)
+    cache, _ = _filled(b, 2 * hkv, hkv, c, d, dtype, [c] * b, 42, keep_first=first, keep_recent=recent)
+    k = torch.randn(b, t, hkv, d, generator=g).to(dtype).cuda().transpose(1, 2)
+    v = torch.randn(b, hkv, t, d + 8, generator=g).to(dtype).cuda()[..., :d]
+    w = torch.rand(b, hkv, t, generator=g)
+    if kind == "ties":
+        w = (w * 6).floor() - 1  # six values, one of them negative
+    elif kind == "odd":
+        w = torch.where(w < 0.2, torch.tensor(float("nan")), torch.where(w < 0.4, torch.tensor(float("inf")), w - 0.7))
+        w = torch.where(w > 0.2, torch.tensor(-0.0), w)
+        w[..., ::7] = 0.0
+    before = _state(cache)
+    cache.load_prompt(k, v, w.cuda(), lo=lo)
+    for i in range(b):
+        at0 = lo[i] if lo else 0
+        for h in range(hkv):
+            kept = torch.from_numpy(O.kept_columns(w[i, h].double().numpy(), at0, c, first, recent))
+            m = len(kept)
+            before["keys"][i, h, :m], before["values"][i, h, :m] = k[i, h, kept], v[i, h, kept]
+            before["weights"][i, h, :m] = w[i, h, kept].cuda()
+            before["order"][i, h, :m] = (kept - at0).int().cuda()
+            before["lengths"][i, h], before["seen"][i, h] = m, t - at0
+    _same(cache, before)
+
+
+def test_load_prompt_refusals():
+    cache = HeavyHitterCache(1, 4, 2, 64, 32, torch.float16, "cuda")
+    k = torch.zeros(1, 2, 10, 32, device="cuda").half()
+    w = torch.zeros(1, 2, 10, device="cuda")
+    for bad, err in ((lambda: cache.load_prompt(k[..., :16], k, w), ValueError),
+                     (lambda: cache.load_prompt(k, k[:, :, :9], w), ValueError),
+                     (lambda: cache.load_prompt(k.bfloat16(), k.bfloat16(), w), TypeError),
+                     (lambda: cache.load_prompt(k, k, w.half()), TypeError),
+                     (lambda: cache.load_prompt(k, k, w[..., :9]), ValueError),
+                     (lambda: cache.load_prompt(k, k, w.cpu()), ValueError),
+                     (lambda: cache.load_prompt(k, k, w, lo=[0, 0]), ValueError),
+                     (lambda: cache.append(k[:, 0, :1], k[:, :, 0], k[:, :, 0]), ValueError),
+                     (lambda: cache.append(torch.zeros(1, 4, 32, device="cuda"), k[:, :, 0], k[:, :, 0]), TypeError),
+                     (lambda: cache.append(torch.zeros(1, 4, 32).half(), k[:, :, 0], k[:, :, 0]), ValueError),
+                     (lambda: cache.attend(torch.zeros(1, 2, 32, device="cuda").half()), ValueError),
+                     (lambda: cache.attend(torch.zeros(1, 4, 32, device="cuda").half(), scale=0.0), ValueError)):
+        with pytest.raises(err):
+            bad()
+
+
+# ---- a run of them -------------------------------------------------------------------------------
+def test_prompt_then_decode():
+    """A padded batch's prompt into the cache, then decode steps past its capacity: each operator
+    against the oracle on the state before it, and the masses that must add up."""
+    b, hq, hkv, d, t, c, steps = 2, 6, 2, 64, 150, 64, 40
+    dtype, lo = torch.bfloat16, [0, 100]
+    g = torch.Generator().manual_seed(77)
+    inv, factor = rotary_frequencies(d, device="cuda")
+    cache = HeavyHitterCache(b, hq, hkv, c, d, dtype, "cuda", keep_first=4, keep_recent=16)
+    q, k, v = (torch.randn(b, h, t, d, generator=g).to(dtype).cuda() for h in (hq, hkv, hkv))
+    pos = (torch.arange(t)[None] - torch.tensor(lo)[:, None]).clamp(min=0).cuda()
+    q, k = rotary_embedding(q, k, pos, inv, factor=factor)
+    w = prompt_attention_weights(q[:, :, -32:], k, lo=lo)
+    cache.load_prompt(k, v, w, lo=lo)
+    assert cache.lengths.tolist() == [[64, 64], [50, 50]] and cache.seen.tolist() == [[150, 150], [50, 50]]
+    for step in range(steps):
+        before = _state(cache)
+        q, k, v = ((torch.randn(b, h, d, generator=g) * 2).to(dtype).cuda() for h in (hq, hkv, hkv))
+        turned = cache.append(q, k, v, inv, factor=factor)
+        want_q, want_k = rotary_embedding(q, k, before["seen"][:, 0], inv, factor=factor)
+        assert torch.equal(turned, want_q)
+        for i in range(b):
+            for h in range(hkv):
+                slot = O.append_slot(int(before["lengths"][i, h]), int(before["seen"][i, h]),
+                                     _np(before["weights"][i, h]), _np(before["order"][i, h]), c, 4, 16)
+                assert torch.equal(cache.keys[i, h, slot], want_k[i, h]) and int(cache.order[i, h, slot]) == 150 + step - lo[i]
+        after = _state(cache)
+        out = cache.attend(turned)
+        for i in range(b):
+            n = int(after["lengths"][i, 0])
+            for h in range(hkv):
+                ref, bound, new, nb = O.attend(_np(turned[i, 3 * h:3 * h + 3]), _np(after["keys"][i, h, :n]),
+                                               _np(after["values"][i, h, :n]), _np(after["weights"][i, h, :n]), 1 / 8, 0.0,
+                                               STEP[dtype])
+                _within(out[i, 3 * h:3 * h + 3], ref, bound, f"step {step}")
+                _within(cache.weights[i, h, :n], new, nb, f"step {step} weights")
+    # Row 1 filled up after 14 steps; the sinks and the last 16 tokens are still there in both.
+    for i in range(b):
+        for h in range(hkv):
+            held = set(cache.order[i, h].tolist())
+            assert len(held) == c and set(range(4)) <= held
+            assert set(range(int(cache.seen[i, h]) - 16, int(cache.seen[i, h]))) <= held
+    cache.reset()
+    assert not cache.lengths.any() and not cache.attend(turned).any()
+
+
+def test_captured_steps_replay():
+    """append and attend captured once and replayed, with eager work between, equal eager steps."""
+    b, hq, hkv, d, c = 3, 8, 2, 128, 300
+    inv, _ = rotary_frequencies(d, device="cuda")
+    caches = [_filled(b, hq, hkv, c, d, torch.float16, [0, 297, 300], 9, keep_first=2, keep_recent=8)[0] for _ in range(2)]
+    g = torch.Generator().manual_seed(10)
+    q, k, v = (torch.randn(b, h, d, generator=g).half().cuda() for h in (hq, hkv, hkv))
+    warm, _ = _filled(b, hq, hkv, c, d, torch.float16, [1, 2, 3], 9, keep_first=2, keep_recent=8)
+    warm.attend(warm.append(q, k, v, inv))
+    start = _state(caches[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = caches[0].attend(caches[0].append(q, k, v, inv))
+    _same(caches[0], start)
+    for _ in range(6):
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g))
+        graph.replay()
+        want = caches[1].attend(caches[1].append(q, k, v, inv))
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        _same(caches[0], _state(caches[1]))
+
+
+def test_captured_prompt_replays():
+    g = torch.Generator().manual_seed(12)
+    cache = HeavyHitterCache(2, 4, 2, 64, 64, torch.float16, "cuda")
+    other = HeavyHitterCache(2, 4, 2, 64, 64, torch.float16, "cuda")
+    q = torch.randn(2, 4, 40, 64, generator=g).half().cuda()
+    k, v = (torch.randn(2, 2, 500, 64, generator=g).half().cuda() for _ in range(2))
+    lo = torch.tensor([0, 450], dtype=torch.int32, device="cuda")
+    other.load_prompt(k, v, prompt_attention_weights(q, k, lo=lo), lo=lo)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w = prompt_attention_weights(q, k, lo=lo)
+        cache.load_prompt(k, v, w, lo=lo)
+    for n in range(4):
+        k.copy_(torch.randn(k.shape, generator=g))
+        lo.copy_(torch.tensor([n, 500 - 30 * n], dtype=torch.int32))
+        graph.replay()
+        other.reset()
+        other.load_prompt(k, v, prompt_attention_weights(q, k, lo=lo), lo=lo)
+        torch.cuda.synchronize()
+        m = other.lengths.clone()
+        assert torch.equal(cache.lengths, m) and torch.equal(cache.seen, other.seen)
+        for i in range(2):
+            n_i = int(m[i, 0])
+            for name in ("keys", "values", "weights", "order"):
+                assert torch.equal(getattr(cache, name)[i, :, :n_i], getattr(other, name)[i, :, :n_i])
+
+
+def test_two_caches_on_two_streams():
+    """Calls on different caches from two streams at once: nothing is shared between them."""
+    inv, _ = rotary_frequencies(64, device="cuda")
+    g = torch.Generator().manual_seed(14)
+    runs = []
+    for seed in (1, 2):
+        pair = [_filled(2, 8, 2, 500, 64, torch.bfloat16, [500, 100], seed)[0] for _ in range(2)]
+        x = [torch.randn(2, h, 64, generator=g).bfloat16().cuda() for h in (8, 2, 2)]
+        runs.append((pair, x, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(5):
+        for (a, _), x, stream in runs:
+            with torch.cuda.stream(stream):
+                outs.append(a.attend(a.append(*x, inv)))
+    torch.cuda.synchronize()
+    want = [c.attend(c.append(*x, inv)) for _ in range(5) for (_, c), x, _ in runs]
+    for a, b in zip(outs, want):
+        assert torch.equal(a, b)
+    for (a, c), _, _ in runs:
+        _same(a, _state(c))
