@@ -89,6 +89,8 @@ hipError_t launch_hh_load(const HHLoadLaunch& p, hipStream_t stream);
 
 // Geometry of a prompt_weights call.
 struct PromptWeightPlan {
+  int groups = 1;      // groups of 32 rows (statistics) or keys (sums) that a wave holds
+  int row_waves = 4;   // waves of a statistics workgroup with rows of their own (1 or 4)
   int key_splits = 1;  // statistics pass: parts of the prompt per block of queries
   int row_splits = 1;  // sums pass: parts of the queries per block of keys
 };

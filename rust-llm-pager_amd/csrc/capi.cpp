@@ -364,10 +364,12 @@ struct PromptPlan {
 int check_prompt(int64_t batch, int64_t hq, int64_t hkv, int64_t tokens, int64_t window, int64_t d, int dtype) {
   int rc = check_heads(batch, hq, hkv, d, dtype);
   if (rc != pgr::kOk) return rc;
-  if (tokens < 0 || tokens > ((int64_t)1 << 30)) return set_err(pgr::kErrInvalid, "tokens must be in [0, 2^30]");
+  // (A launch's third grid dimension ends at 65535 blocks of 128 keys or rows.)
+  if (tokens < 0 || tokens > (int64_t)65535 * 128)
+    return set_err(pgr::kErrInvalid, "tokens must be in [0, 8388480]");
   if (window < 0 || window > tokens) return set_err(pgr::kErrInvalid, "the window must be in [0, tokens]");
-  if (window * (hq / hkv) > ((int64_t)1 << 30))
-    return set_err(pgr::kErrInvalid, "window * queries per KV head must not exceed 2^30");
+  if (window * (hq / hkv) > (int64_t)65535 * 32)
+    return set_err(pgr::kErrInvalid, "window * query heads per KV head must not exceed 2097120");
   return pgr::kOk;
 }
 
@@ -1331,6 +1333,9 @@ int pgr_hh_prompt_weights(const void* q, const int64_t* q_strides, const void* k
     if (batch == 0 || tokens == 0) return pgr::kOk;
     if (window == 0) return set_err(pgr::kErrInvalid, "the window must hold a query");
     if (!q || !q_strides || !k || !k_strides || !weights) return set_err(pgr::kErrInvalid, "null tensor pointer");
+    for (int i = 1; i < 3; ++i)
+      if (q_strides[i] < 0 || k_strides[i] < 0 || q_strides[i] >> 31 != 0 || k_strides[i] >> 31 != 0)
+        return set_err(pgr::kErrInvalid, "head and token strides must be in [0, 2^31)");
     const PromptPlan p = plan_prompt(batch, num_query_heads, num_kv_heads, tokens, window, head_dim);
     if (workspace == nullptr || workspace_bytes < p.bytes) return set_err(pgr::kErrCapacity, "workspace too small");
     if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");

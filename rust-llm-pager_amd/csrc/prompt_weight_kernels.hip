@@ -13,6 +13,8 @@
 // Nothing is added by atomics: the same inputs give the same sums.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "cache_device.h"
 
 namespace pgr {
@@ -20,17 +22,19 @@ namespace {
 
 constexpr int kTile = 128;  // keys (statistics) or rows (sums) in LDS
 
-// Groups of 32 rows (statistics) or keys (sums) that a wave holds in registers.
-template <int D>
-constexpr int groups() {
-  return D <= 128 ? 2 : 1;
-}
-
 struct ScoreScale {
   float c;          // log2 units per unit of the (softcapped) score
   float cap_scale;  // softcap: scale / cap, else 0
-  float cap;
 };
+
+// x / n_rep for 0 <= x < 2^32 / 16: exact with magic = floor(2^32 / n_rep) + 1 (0: n_rep is 1). An
+// ordinary division is some thirty instructions, and a tile's rows take one per 16-byte piece.
+__device__ __forceinline__ int div_rep(int x, uint32_t magic) {
+  return magic == 0 ? x : (int)__umulhi((uint32_t)x, magic);
+}
+__device__ __forceinline__ uint32_t rep_magic(int n_rep) {
+  return n_rep == 1 ? 0u : 0xffffffffu / (uint32_t)n_rep + 1u;
+}
 
 // The (softcapped) score in units of `c`.
 template <bool kCap>
@@ -38,26 +42,48 @@ __device__ __forceinline__ float raw_score(float s, const ScoreScale& sc) {
   return kCap ? tanhf(s * sc.cap_scale) : s;
 }
 
-// kTile rows of D elements into LDS, `row_ptr(i)` giving row i's address (null: zeros).
-template <int D, class F>
-__device__ __forceinline__ void stage(uint16_t* lds, F row_ptr) {
-  constexpr int kStride = D + 8, kPieces = D / 8;
+// One tile of rows on its way to LDS: 16-byte pieces in registers, so that a later tile's loads run
+// under the current one's products.
+template <int D>
+struct Stage {
+  static constexpr int kStride = D + 8, kPieces = D / 8, kPer = kTile * kPieces / 256;
+  u32x4 v[kPer];
+
+  // offset(i): element offset of row i from `base`; rows from `valid` on are zeros.
+  template <class F>
+  __device__ __forceinline__ void fetch(const uint16_t* base, int valid, F offset) {
 #pragma unroll
-  for (int x = 0; x < kTile * kPieces / 256; ++x) {
-    const int id = x * 256 + (int)threadIdx.x, i = id / kPieces, e = (id - i * kPieces) * 8;
-    const uint16_t* p = row_ptr(i);
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (p != nullptr) v = *reinterpret_cast<const u32x4_e*>(p + e);
-    *reinterpret_cast<u32x4*>(lds + i * kStride + e) = v;
+    for (int x = 0; x < kPer; ++x) {
+      const int id = x * 256 + (int)threadIdx.x, i = id / kPieces, e = (id - i * kPieces) * 8;
+      v[x] = u32x4{0u, 0u, 0u, 0u};
+      if (valid >= kTile || i < valid) v[x] = *reinterpret_cast<const u32x4_e*>(base + offset(i) + e);
+    }
   }
+  __device__ __forceinline__ void put(uint16_t* lds) const {
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+      const int id = x * 256 + (int)threadIdx.x, i = id / kPieces, e = (id - i * kPieces) * 8;
+      *reinterpret_cast<u32x4*>(lds + i * kStride + e) = v[x];
+    }
+  }
+};
+
+// The lane's part of 32 LDS rows: the first operand of a step's products. All of it is asked for at
+// once, and a step ahead: the products then wait for nothing.
+template <int D>
+__device__ __forceinline__ void read_rows(u32x4 (&r)[D / 16], const uint16_t* lds_row) {
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c) r[c] = *reinterpret_cast<const u32x4*>(lds_row + 16 * c);
 }
 
-template <class Ty, int D>
-__device__ __forceinline__ f32x16 product(const uint16_t* lds_row, const u32x4 (&own)[D / 16]) {
-  f32x16 s = {};
+template <class Ty, int D, int kN>
+__device__ __forceinline__ void product(f32x16 (&s)[kN], const u32x4 (&rows)[D / 16], const u32x4 (&own)[kN][D / 16]) {
 #pragma unroll
-  for (int c = 0; c < D / 16; ++c) s = Ty::mma32(*reinterpret_cast<const u32x4*>(lds_row + 16 * c), own[c], s);
-  return s;
+  for (int g = 0; g < kN; ++g) s[g] = f32x16{};
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+    for (int g = 0; g < kN; ++g) s[g] = Ty::mma32(rows[c], own[g][c], s[g]);
 }
 
 template <int D>
@@ -69,36 +95,63 @@ __device__ __forceinline__ void load_own(u32x4 (&r)[D / 16], const uint16_t* row
   }
 }
 
+// The sum of 16 values, as four chains: one chain would wait for each addition.
+__device__ __forceinline__ float sum16(const float (&p)[16]) {
+  float t[4] = {p[0], p[1], p[2], p[3]};
+#pragma unroll
+  for (int x = 4; x < 16; ++x) t[x & 3] += p[x];
+  return (t[0] + t[1]) + (t[2] + t[3]);
+}
+
+// p[x] = exp2(s[x] * c - ref(x)). The steps are kept apart: left to itself the compiler makes one
+// value after the other in one register, and each waits for the exponential before it.
+template <class F>
+__device__ __forceinline__ void exp_all(float (&p)[16], const f32x16& s, float c, F ref) {
+#pragma unroll
+  for (int x = 0; x < 16; ++x) p[x] = fmaf(s[x], c, -ref(x));
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(p[x]);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+
 // kRowWaves 4: the waves hold rows of their own and all take every key; 1: they hold the same rows
-// and take a quarter of the keys each.
-template <class Ty, int D, int kRowWaves, bool kCap>
+// and take a quarter of the keys each. Grid (batch x KV heads, key splits, row blocks): the KV head
+// varies fastest, so that workgroups of one head tend to share an XCD's L2, and the blocks of the
+// last rows, which attend to most, start first.
+template <class Ty, int D, int kN, int kRowWaves, bool kCap>
 __global__ __launch_bounds__(256) void prompt_stats_kernel(PromptWeightLaunch a, ScoreScale sc) {
-  constexpr int kN = groups<D>();
-  constexpr int kStride = D + 8;
-  __shared__ __align__(16) uint16_t lds[kTile * kStride];
+  typedef Stage<D> S;
+  constexpr int kSubs = kRowWaves == 4 ? kTile / 32 : 1;  // steps of a wave per tile
+  __shared__ __align__(16) uint16_t lds[2][kTile * S::kStride];
+  __shared__ float2 part[4][kN * 32];
   const int n_rep = a.hq / a.hkv, rows = a.window * n_rep;
-  const int bh = blockIdx.z, b = bh / a.hkv, h = bh - b * a.hkv;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5, j = lane & 31;
+  const uint32_t magic = rep_magic(n_rep), q_h = (uint32_t)a.qs.h, q_t = (uint32_t)a.qs.t, k_t = (uint32_t)a.ks.t;
+  const int bh = blockIdx.x, b = bh / a.hkv, h = bh - b * a.hkv;
+  const int wave = wave_index(), lane = threadIdx.x & 63, half = lane >> 5, j = lane & 31;
   const int lo = a.lo != nullptr ? min(max(a.lo[b], 0), a.tokens) : 0;
   const uint16_t* qb = static_cast<const uint16_t*>(a.q) + b * a.qs.b + (int64_t)h * n_rep * a.qs.h;
   const uint16_t* kb = static_cast<const uint16_t*>(a.k) + b * a.ks.b + h * a.ks.h;
 
-  const int wg_row = blockIdx.x * kRowWaves * kN * 32;
+  const int wg_row = (int)(gridDim.z - 1 - blockIdx.z) * kRowWaves * kN * 32;
   const int wave_row = wg_row + (kRowWaves == 4 ? wave * kN * 32 : 0);
   u32x4 own[kN][D / 16];
   int last[kN];  // the last column that the lane's row attends to (-1: no such row)
 #pragma unroll
   for (int g = 0; g < kN; ++g) {
-    const int r = wave_row + g * 32 + j, i = r / n_rep;
+    const int r = wave_row + g * 32 + j, i = div_rep(r, magic);
     last[g] = r < rows ? a.tokens - a.window + i : -1;
-    load_own<D>(own[g], r < rows ? qb + (r - i * n_rep) * a.qs.h + i * a.qs.t : nullptr, half);
+    load_own<D>(own[g], r < rows ? qb + (uint64_t)(r - i * n_rep) * q_h + (uint64_t)i * q_t : nullptr, half);
   }
-  // Keys that any row of the workgroup, and every row of the wave, attends to.
-  const int wg_last = a.tokens - a.window + min(wg_row + kRowWaves * kN * 32, rows) / n_rep;
-  const int every = a.tokens - a.window + wave_row / n_rep;
+  // The last keys that any row of the workgroup, any row of the wave, and every row of the wave attends to.
+  auto last_of = [&](int r) { return a.tokens - a.window + div_rep(min(r, rows - 1), magic); };
+  const int wg_last = last_of(wg_row + kRowWaves * kN * 32 - 1);
+  const int any = last_of(wave_row + kN * 32 - 1), every = a.tokens - a.window + div_rep(wave_row, magic);
 
   // This split's tiles of [lo, wg_last].
-  const int t_lo = lo / kTile, t_hi = min(wg_last, a.tokens - 1) / kTile + 1;
+  const int t_lo = lo / kTile, t_hi = wg_last / kTile + 1;
   const int per = (max(t_hi - t_lo, 0) + a.plan.key_splits - 1) / a.plan.key_splits;
   const int t_begin = t_lo + (int)blockIdx.y * per, t_end = min(t_begin + per, t_hi);
 
@@ -108,39 +161,72 @@ __global__ __launch_bounds__(256) void prompt_stats_kernel(PromptWeightLaunch a,
     m[g] = kMinusInf;
     l[g] = 0.f;
   }
-  for (int tile = t_begin; tile < t_end; ++tile) {
-    const int key0 = tile * kTile;
-    __syncthreads();
-    stage<D>(lds, [&](int i) { return key0 + i < a.tokens ? kb + (key0 + i) * a.ks.t : nullptr; });
-    __syncthreads();
-    for (int sub = kRowWaves == 4 ? 0 : wave; sub < kTile / 32; sub += kRowWaves == 4 ? 1 : 4) {
-      const int k0 = key0 + sub * 32;
-      const bool edge = k0 < lo || k0 + 31 > every;
+  S st;
+  auto fetch = [&](int tile) {
+    st.fetch(kb + (int64_t)tile * kTile * a.ks.t, a.tokens - tile * kTile, [&](int i) { return (uint64_t)i * k_t; });
+  };
+  // Folds the scores of 32 keys into the rows' statistics; masked: some row does not attend to some key.
+  auto fold = [&](f32x16 (&s)[kN], int k0, auto masked) {
 #pragma unroll
-      for (int g = 0; g < kN; ++g) {
-        f32x16 s = product<Ty, D>(lds + (sub * 32 + j) * kStride + 8 * half, own[g]);
-        float top = kMinusInf;
+    for (int g = 0; g < kN; ++g) {
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          s[x] = raw_score<kCap>(s[x], sc);
-          if (edge) {
-            const int key = k0 + 8 * (x / 4) + 4 * half + (x & 3);
-            if (key < lo || key > last[g]) s[x] = kMinusInf;
-          }
-          top = fmaxf(top, s[x]);
+      for (int x = 0; x < 16; ++x) {
+        s[g][x] = raw_score<kCap>(s[g][x], sc);
+        if constexpr (decltype(masked)::value) {
+          const int key = k0 + 8 * (x / 4) + 4 * half + (x & 3);
+          s[g][x] = key < lo || key > last[g] ? kMinusInf : s[g][x];
         }
-        const float m_new = fmaxf(m[g], top);
-        const float ref = m_new == kMinusInf ? 0.f : m_new * sc.c;
-        float sum = 0.f;
+      }
+      float top = m[g], top2 = s[g][15];
 #pragma unroll
-        for (int x = 0; x < 16; ++x) sum += __builtin_amdgcn_exp2f(fmaf(s[x], sc.c, -ref));
-        l[g] = l[g] * __builtin_amdgcn_exp2f(fmaf(m[g], sc.c, -ref)) + sum;
-        m[g] = m_new;
+      for (int x = 0; x < 14; x += 4) {
+        top = fmaxf(fmaxf(top, s[g][x]), s[g][x + 1]);
+        if (x + 3 < 15) top2 = fmaxf(fmaxf(top2, s[g][x + 2]), s[g][x + 3]);
+      }
+      top = fmaxf(fmaxf(top, top2), s[g][14]);
+      const float ref = decltype(masked)::value && top == kMinusInf ? 0.f : top * sc.c;
+      float p[16];
+      exp_all(p, s[g], sc.c, [&](int) { return ref; });
+      l[g] = fmaf(l[g], __builtin_amdgcn_exp2f(fmaf(m[g], sc.c, -ref)), sum16(p));
+      m[g] = top;
+    }
+  };
+  u32x4 keys[D / 16];
+  const int sub0 = kRowWaves == 4 ? 0 : wave, at = j * S::kStride + 8 * half;
+  if (t_begin < t_end) {
+    fetch(t_begin);
+    st.put(lds[0]);
+    if (t_begin + 1 < t_end) fetch(t_begin + 1);
+    __syncthreads();
+    read_rows<D>(keys, lds[0] + sub0 * 32 * S::kStride + at);
+  }
+  for (int tile = t_begin; tile < t_end; ++tile) {
+    uint16_t* const here = lds[(tile - t_begin) & 1];
+    uint16_t* const there = lds[(tile - t_begin + 1) & 1];
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub) {
+      const int k0 = tile * kTile + (sub0 + sub) * 32;
+      const bool some = k0 <= any;  // otherwise no row of the wave attends to these keys
+      f32x16 s[kN];
+      if (some) product<Ty, D, kN>(s, keys, own);
+      __builtin_amdgcn_sched_barrier(0);
+      if (sub + 1 < kSubs) {
+        read_rows<D>(keys, here + (sub + 1) * 32 * S::kStride + at);
+      } else if (tile + 1 < t_end) {
+        st.put(there);
+        if (tile + 2 < t_end) fetch(tile + 2);
+        __syncthreads();
+        read_rows<D>(keys, there + sub0 * 32 * S::kStride + at);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (k0 < lo || k0 + 31 > every) {
+        if (some) fold(s, k0, std::true_type{});
+      } else {
+        fold(s, k0, std::false_type{});
       }
     }
   }
   // The halves of the wave hold other keys of the same rows; so do the waves where they share rows.
-  __shared__ float2 part[4][kN * 32];
 #pragma unroll
   for (int g = 0; g < kN; ++g) {
     const float m2 = __shfl_xor(m[g], 32), l2 = __shfl_xor(l[g], 32);
@@ -166,80 +252,141 @@ __global__ __launch_bounds__(256) void prompt_stats_kernel(PromptWeightLaunch a,
   }
 }
 
-// norm = m + log2(l) over the splits of each row; +inf for a row that attends to nothing.
+// norm = m + log2(l) over the splits of each row; +inf for a row that attends to nothing. 64 rows a
+// workgroup, each wave a quarter of the splits, eight loads in flight.
 __global__ __launch_bounds__(256) void prompt_norm_kernel(PromptWeightLaunch a, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float m = kMinusInf;
-  for (int s = 0; s < a.plan.key_splits; ++s) m = fmaxf(m, a.stats[s * n + i].x);
-  const float ref = m == kMinusInf ? 0.f : m;
-  float l = 0.f;
-  for (int s = 0; s < a.plan.key_splits; ++s) {
-    const float2 p = a.stats[s * n + i];
-    l += p.y * __builtin_amdgcn_exp2f(p.x - ref);
+  __shared__ float2 part[4][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 64 + lane, at = i < n ? i : n - 1;
+  float m = kMinusInf, l = 0.f;
+  for (int s0 = wave; s0 < a.plan.key_splits; s0 += 32) {
+    float2 p[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int s = s0 + 4 * x;
+      p[x] = a.stats[(s < a.plan.key_splits ? s : s0) * n + at];
+      if (s >= a.plan.key_splits) p[x] = float2{kMinusInf, 0.f};
+    }
+    float top = m;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) top = fmaxf(top, p[x].x);
+    const float ref = top == kMinusInf ? 0.f : top;
+    l *= __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) l += p[x].y * __builtin_amdgcn_exp2f(p[x].x - ref);
+    m = top;
   }
+  part[wave][lane] = float2{m, l};
+  __syncthreads();
+  if (wave != 0 || i >= n) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) m = fmaxf(m, part[w][lane].x);
+  const float ref = m == kMinusInf ? 0.f : m;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) l += part[w][lane].y * __builtin_amdgcn_exp2f(part[w][lane].x - ref);
   a.norm[i] = l == 0.f ? -kMinusInf : ref + __builtin_amdgcn_logf(l);
 }
 
-template <class Ty, int D, bool kCap>
+// Grid (batch x KV heads, row splits, key blocks): as above; the first keys, which most rows attend
+// to, start first.
+template <class Ty, int D, int kN, bool kCap>
 __global__ __launch_bounds__(256) void prompt_sums_kernel(PromptWeightLaunch a, ScoreScale sc) {
-  constexpr int kN = groups<D>();
-  constexpr int kStride = D + 8;
-  __shared__ __align__(16) uint16_t lds[kTile * kStride];
-  __shared__ __align__(16) float norm_s[kTile];
-  const int n_rep = a.hq / a.hkv, rows = a.window * n_rep;
-  const int bh = blockIdx.z, b = bh / a.hkv, h = bh - b * a.hkv;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5, j = lane & 31;
+  typedef Stage<D> S;
+  constexpr int kSubs = kTile / 32, kNever = 0x7fffffff;
+  __shared__ __align__(16) uint16_t lds[2][kTile * S::kStride];
+  __shared__ __align__(16) float norm_s[2][kTile];
+  const int n_rep = a.hq / a.hkv, rows = a.window * n_rep, before = a.tokens - a.window;
+  const uint32_t magic = rep_magic(n_rep), q_h = (uint32_t)a.qs.h, q_t = (uint32_t)a.qs.t;
+  const int bh = blockIdx.x, b = bh / a.hkv, h = bh - b * a.hkv;
+  const int wave = wave_index(), lane = threadIdx.x & 63, half = lane >> 5, j = lane & 31;
   const int lo = a.lo != nullptr ? min(max(a.lo[b], 0), a.tokens) : 0;
   const uint16_t* qb = static_cast<const uint16_t*>(a.q) + b * a.qs.b + (int64_t)h * n_rep * a.qs.h;
   const uint16_t* kb = static_cast<const uint16_t*>(a.k) + b * a.ks.b + h * a.ks.h;
   const float* norm = a.norm + (int64_t)bh * rows;
 
-  const int wg_key = blockIdx.x * 4 * kN * 32, wave_key = wg_key + wave * kN * 32;
+  const int wg_key = (int)blockIdx.z * 4 * kN * 32, wave_key = wg_key + wave * kN * 32;
   u32x4 own[kN][D / 16];
   float sum[kN];
+  int from[kN];  // the first row that attends to the lane's key (padding: none, whatever the key holds)
 #pragma unroll
   for (int g = 0; g < kN; ++g) {
     const int key = wave_key + g * 32 + j;
     load_own<D>(own[g], key < a.tokens ? kb + key * a.ks.t : nullptr, half);
     sum[g] = 0.f;
+    from[g] = key < lo || key >= a.tokens ? kNever : max(key - before, 0) * n_rep;
   }
-  // The first row that attends to the workgroup's first key, and this split's tiles from there on.
-  const int first = max(wg_key - (a.tokens - a.window), 0) * n_rep;
+  // The first rows that attend to the workgroup's first key, to the wave's first and to all of the wave's.
+  const int first = max(wg_key - before, 0) * n_rep, any = max(wave_key - before, 0) * n_rep;
+  const int every = wave_key < lo ? kNever : max(wave_key + kN * 32 - 1 - before, 0) * n_rep;
   const int t_lo = first / kTile, t_hi = (rows + kTile - 1) / kTile;
   const int per = (max(t_hi - t_lo, 0) + a.plan.row_splits - 1) / a.plan.row_splits;
   const int t_begin = t_lo + (int)blockIdx.y * per, t_end = min(t_begin + per, t_hi);
-  for (int tile = t_begin; tile < t_end; ++tile) {
+
+  S st;
+  float nm_next = 0.f;
+  auto fetch = [&](int tile) {
     const int row0 = tile * kTile;
-    __syncthreads();
-    stage<D>(lds, [&](int i) {
-      const int r = row0 + i, qi = r / n_rep;
-      return r < rows ? qb + (r - qi * n_rep) * a.qs.h + qi * a.qs.t : nullptr;
+    st.fetch(qb, rows - row0, [&](int i) {
+      const int qi = div_rep(row0 + i, magic);
+      return (uint64_t)(uint32_t)(row0 + i - qi * n_rep) * q_h + (uint64_t)(uint32_t)qi * q_t;
     });
-    if (threadIdx.x < kTile)
-      norm_s[threadIdx.x] = row0 + (int)threadIdx.x < rows ? norm[row0 + threadIdx.x] : -kMinusInf;
+    if (threadIdx.x < kTile) nm_next = row0 + (int)threadIdx.x < rows ? norm[row0 + threadIdx.x] : -kMinusInf;
+  };
+  auto put = [&](int buffer) {
+    st.put(lds[buffer]);
+    if (threadIdx.x < kTile) norm_s[buffer][threadIdx.x] = nm_next;
+  };
+  // Adds the probabilities of 32 rows up; masked: some row does not attend to some key.
+  auto fold = [&](const f32x16 (&s)[kN], const f32x4 (&nm)[4], int r0, auto masked) {
+#pragma unroll
+    for (int g = 0; g < kN; ++g) {
+      float p[16];
+      f32x16 x16;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) x16[x] = raw_score<kCap>(s[g][x], sc);
+      exp_all(p, x16, sc.c, [&](int x) { return nm[x / 4][x & 3]; });
+      if constexpr (decltype(masked)::value) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) p[x] = r0 + 8 * (x / 4) + 4 * half + (x & 3) < from[g] ? 0.f : p[x];
+      }
+      sum[g] += sum16(p);  // 16 rows at a time, so that long sums of small terms lose less
+    }
+  };
+  u32x4 q[D / 16];
+  const int at = j * S::kStride + 8 * half;
+  if (t_begin < t_end) {
+    fetch(t_begin);
+    put(0);
+    if (t_begin + 1 < t_end) fetch(t_begin + 1);
     __syncthreads();
-    for (int sub = 0; sub < kTile / 32; ++sub) {
-      const int r0 = row0 + sub * 32;
-      // Rows that do not attend to every key of the wave.
-      const bool edge = wave_key < lo || wave_key + kN * 32 - 1 > a.tokens - a.window + r0 / n_rep;
+    read_rows<D>(q, lds[0] + at);
+  }
+  for (int tile = t_begin; tile < t_end; ++tile) {
+    const int here = (tile - t_begin) & 1, there = here ^ 1;
 #pragma unroll
-      for (int g = 0; g < kN; ++g) {
-        const f32x16 s = product<Ty, D>(lds + (sub * 32 + j) * kStride + 8 * half, own[g]);
-        const int key = wave_key + g * 32 + j;
+    for (int sub = 0; sub < kSubs; ++sub) {
+      const int r0 = tile * kTile + sub * 32;
+      const bool some = r0 + 31 >= any;  // otherwise none of these rows attends to a key of the wave
+      f32x16 s[kN];
+      f32x4 nm[4];
 #pragma unroll
-        for (int x = 0; x < 16; x += 4) {
-          const f32x4 nm = *reinterpret_cast<const f32x4*>(norm_s + sub * 32 + 2 * x + 4 * half);
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            float p = __builtin_amdgcn_exp2f(fmaf(raw_score<kCap>(s[x + y], sc), sc.c, -nm[y]));
-            if (edge) {
-              const int r = r0 + 2 * x + 4 * half + y;
-              if (key < lo || key > a.tokens - a.window + r / n_rep) p = 0.f;
-            }
-            sum[g] += p;
-          }
-        }
+      for (int x = 0; x < 4; ++x) nm[x] = *reinterpret_cast<const f32x4*>(norm_s[here] + sub * 32 + 8 * x + 4 * half);
+      if (some) product<Ty, D, kN>(s, q, own);
+      __builtin_amdgcn_sched_barrier(0);
+      if (sub + 1 < kSubs) {
+        read_rows<D>(q, lds[here] + (sub + 1) * 32 * S::kStride + at);
+      } else if (tile + 1 < t_end) {
+        put(there);
+        if (tile + 2 < t_end) fetch(tile + 2);
+        __syncthreads();
+        read_rows<D>(q, lds[there] + at);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (r0 < every) {
+        if (some) fold(s, nm, r0, std::true_type{});
+      } else {
+        fold(s, nm, r0, std::false_type{});
       }
     }
   }
@@ -256,31 +403,30 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptWeightLaunch a, 
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   float x = 0.f;
+#pragma unroll 8
   for (int s = 0; s < a.plan.row_splits; ++s) x += a.partial[s * n + i];
   a.out[i] = x;
 }
 
-bool shared_rows(int rows) { return rows <= 128; }
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-template <class Ty, int D, bool kCap>
+template <class Ty, int D, int kN, bool kCap>
 hipError_t run(const PromptWeightLaunch& p, const ScoreScale& sc, hipStream_t stream) {
-  const int rows = p.window * (p.hq / p.hkv), own = groups<D>() * 32;
+  const int rows = p.window * (p.hq / p.hkv), own = kN * 32;
   const unsigned bh = (unsigned)(p.batch * p.hkv);
-  if (shared_rows(rows)) {
-    const dim3 grid((unsigned)((rows + own - 1) / own), (unsigned)p.plan.key_splits, bh);
-    prompt_stats_kernel<Ty, D, 1, kCap><<<grid, 256, 0, stream>>>(p, sc);
-  } else {
-    const dim3 grid((unsigned)((rows + 4 * own - 1) / (4 * own)), (unsigned)p.plan.key_splits, bh);
-    prompt_stats_kernel<Ty, D, 4, kCap><<<grid, 256, 0, stream>>>(p, sc);
-  }
+  const dim3 stats(bh, (unsigned)p.plan.key_splits, (unsigned)ceil_div(rows, p.plan.row_waves * own));
+  if (p.plan.row_waves == 1)
+    prompt_stats_kernel<Ty, D, kN, 1, kCap><<<stats, 256, 0, stream>>>(p, sc);
+  else
+    prompt_stats_kernel<Ty, D, kN, 4, kCap><<<stats, 256, 0, stream>>>(p, sc);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t n = (int64_t)bh * rows;
-  prompt_norm_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(p, n);
+  prompt_norm_kernel<<<(unsigned)((n + 63) / 64), 256, 0, stream>>>(p, n);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const dim3 grid((unsigned)((p.tokens + 4 * own - 1) / (4 * own)), (unsigned)p.plan.row_splits, bh);
-  prompt_sums_kernel<Ty, D, kCap><<<grid, 256, 0, stream>>>(p, sc);
+  const dim3 sums(bh, (unsigned)p.plan.row_splits, (unsigned)ceil_div(p.tokens, 4 * own));
+  prompt_sums_kernel<Ty, D, kN, kCap><<<sums, 256, 0, stream>>>(p, sc);
   e = hipGetLastError();
   if (e != hipSuccess || p.plan.row_splits == 1) return e;
   const int64_t m = (int64_t)bh * p.tokens;
@@ -290,13 +436,12 @@ hipError_t run(const PromptWeightLaunch& p, const ScoreScale& sc, hipStream_t st
 
 template <class Ty, int D>
 hipError_t run_cap(const PromptWeightLaunch& p, hipStream_t stream) {
-  ScoreScale sc;
-  if (p.softcap > 0.f) {
-    sc = {p.softcap * kLog2e, p.scale / p.softcap, p.softcap};
-    return run<Ty, D, true>(p, sc, stream);
+  const bool cap = p.softcap > 0.f;
+  const ScoreScale sc = cap ? ScoreScale{p.softcap * kLog2e, p.scale / p.softcap} : ScoreScale{p.scale * kLog2e, 0.f};
+  if constexpr (D == 128) {
+    if (p.plan.groups == 2) return cap ? run<Ty, D, 2, true>(p, sc, stream) : run<Ty, D, 2, false>(p, sc, stream);
   }
-  sc = {p.scale * kLog2e, 0.f, 0.f};
-  return run<Ty, D, false>(p, sc, stream);
+  return cap ? run<Ty, D, 1, true>(p, sc, stream) : run<Ty, D, 1, false>(p, sc, stream);
 }
 
 template <class Ty>
@@ -314,16 +459,23 @@ hipError_t run_dim(const PromptWeightLaunch& p, hipStream_t stream) {
 
 PromptWeightPlan prompt_weight_plan(int batch, int hq, int hkv, int tokens, int window, int d) {
   PromptWeightPlan plan;
-  const int64_t rows = (int64_t)window * (hq / hkv), own = d <= 128 ? 64 : 32, bh = (int64_t)batch * hkv;
-  const int64_t row_blocks = shared_rows((int)rows) ? (rows + own - 1) / own : (rows + 4 * own - 1) / (4 * own);
-  auto parts = [](int64_t workgroups, int64_t tiles) {  // about 1024 workgroups, two tiles each
-    int64_t n = (1024 + workgroups - 1) / workgroups;
+  const int64_t rows = (int64_t)window * (hq / hkv), bh = (int64_t)batch * hkv;
+  // Two groups of 32 per wave at head dim 128 where that still leaves two workgroups for every CU:
+  // each operand read from LDS then feeds two products (8192 tokens and queries, 32/8 heads: 341 + 356
+  // us against 402 + 427 with one group; two batch rows of 4133 tokens and 32 queries, 28/4 heads, where
+  // it does not: 12.1 + 12.3 against 10.4 + 11.1). At head dim 64 one group is as fast (35 + 36 against
+  // 42 + 35 us at 65536 tokens and 64 queries, 32/4 heads).
+  plan.groups = d == 128 && ceil_div(rows, 256) * bh * ceil_div(tokens, 2048) >= 512 ? 2 : 1;
+  const int64_t own = 32 * plan.groups;
+  plan.row_waves = rows <= 2 * own ? 1 : 4;
+  auto parts = [](int64_t workgroups, int64_t tiles) {  // about 1536 workgroups, of two tiles or more
+    int64_t n = (1536 + workgroups - 1) / workgroups;
     const int64_t most = (tiles + 1) / 2;
     if (n > most) n = most;
     return (int)(n < 1 ? 1 : n);
   };
-  plan.key_splits = parts(row_blocks * bh, (tokens + kTile - 1) / kTile);
-  plan.row_splits = parts((tokens + 4 * own - 1) / (4 * own) * bh, (rows + kTile - 1) / kTile);
+  plan.key_splits = parts(ceil_div(rows, plan.row_waves * own) * bh, ceil_div(tokens, kTile));
+  plan.row_splits = parts(ceil_div(tokens, 4 * own) * bh, ceil_div(rows, kTile));
   return plan;
 }
 

@@ -215,6 +215,7 @@ PROMPT = [
     (2, 28, 4, 128, 384, 200, [128, 200]),
     (1, 8, 1, 256, 260, 260, [100]),
     (1, 1, 1, 128, 2500, 1, None),
+    (8, 128, 8, 128, 300, 128, [0, 0, 5, 40, 171, 200, 299, 300]),  # two groups of rows and keys per wave
 ]
 
 
