@@ -232,7 +232,7 @@ int pgr_hh_prompt_weights(const void* q, const int64_t* q_strides, const void* k
  * lowest column; NaN is the heaviest), in the order of their columns. k, v [B, Hkv, tokens, D]
  * (strides: batch, head, token), weights [B, Hkv, tokens] contiguous. Slots past the new length are
  * left as they were. */
-size_t pgr_hh_load_prompt_workspace_bytes(const pgr_hh_cache_t* cache);
+size_t pgr_hh_load_prompt_workspace_bytes(const pgr_hh_cache_t* cache, int64_t tokens);
 int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t* k_strides, const void* v,
                        const int64_t* v_strides, const float* weights, const int32_t* lo, int64_t tokens,
                        void* workspace, size_t workspace_bytes, void* stream);

@@ -171,7 +171,7 @@ SIGNATURES: dict[str, tuple] = {
         [c_vp, P(c_i64), c_vp, P(c_i64), c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, c_f32,
          c_f32, c_vp, c_size, c_vp],
     ),
-    "pgr_hh_load_prompt_workspace_bytes": (c_size, [P(HHCache)]),
+    "pgr_hh_load_prompt_workspace_bytes": (c_size, [P(HHCache), c_i64]),
     "pgr_hh_load_prompt": (
         ctypes.c_int,
         [P(HHCache), c_vp, P(c_i64), c_vp, P(c_i64), c_vp, c_vp, c_i64, c_vp, c_size, c_vp],

@@ -76,6 +76,12 @@ struct HHAttendLaunch {
 };
 hipError_t launch_hh_attend(int dtype, const HHAttendLaunch& p, hipStream_t stream);
 
+// What the launches of a long row's selection tell each other.
+struct HHSelectRow {
+  uint32_t cls, need, whole;  // the last taken token's class, how many of it are taken, whether all are
+  uint32_t listed;            // its members
+};
+
 struct HHLoadLaunch {
   HHCache c;
   const void *k = nullptr, *v = nullptr;
@@ -84,7 +90,14 @@ struct HHLoadLaunch {
   const int32_t* lo = nullptr;
   int tokens = 0;
   int32_t* kept = nullptr;  // [batch, hkv, capacity]
+  // Long rows, dealt out in parts:
+  uint16_t* part_counts = nullptr;  // [batch, hkv, parts, 2048]: tokens of each class
+  uint32_t* part_above = nullptr;   // [batch, hkv, parts]: tokens of classes above the last one
+  uint32_t* listed = nullptr;       // [batch, hkv, parts * hh_select_part_tokens()] (key, part)
+  HHSelectRow* rows = nullptr;      // [batch, hkv]
 };
+int hh_select_parts(int tokens);
+size_t hh_select_part_tokens();
 hipError_t launch_hh_load(const HHLoadLaunch& p, hipStream_t stream);
 
 // Geometry of a prompt_weights call.

@@ -12,9 +12,9 @@ namespace {
 
 // ---------------------------------------------------------------------------------------
 // Weights in their order as unsigned numbers: a heavier token has the larger key, -0 and 0 are
-// equal, and NaN (one key for all of them) is the heaviest.
+// equal, and NaN (one key for all of them) is the heaviest. 0 and 0xffffffff are no weight's key.
 __device__ __forceinline__ uint32_t weight_key(float w) {
-  if (w != w) return 0xffffffffu;
+  if (w != w) return 0xfffffffeu;
   const uint32_t u = __builtin_bit_cast(uint32_t, w == 0.f ? 0.f : w);
   return (u >> 31) ? ~u : u | 0x80000000u;
 }
@@ -333,120 +333,360 @@ __global__ __launch_bounds__(256) void hh_attend_merge_kernel(HHAttendLaunch a) 
 }
 
 // ---------------------------------------------------------------------------------------
-// Which of a prompt's tokens stay. One workgroup per row. More tokens than slots: the first
-// keep_first and the last keep_recent, and of those between the capacity's remainder by weight,
-// the lowest column first among equals. The weight of the last one taken is found byte by byte
-// from the top (four counts of 256 classes), then one pass writes the kept columns in order.
-constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
+// Which of a prompt's tokens stay, where a row has more than slots: the `capacity` heaviest, the
+// lowest column first among equals, where the first keep_first and the last keep_recent tokens count as
+// heavier than any other. The key of the last one taken (`last`; of those equal to it the first `need`
+// are taken) is found from its top 11 bits down: 11, 11, 10, a count per class, then a scan over the
+// classes from the heaviest. Then every token above it, and every equal one of low enough rank, has
+// its slot from the counts before it.
+//
+// Latency-bound: the weights are few bytes (256 KB a row at 65536 tokens), the passes and their barriers
+// many. Up to kSelShort tokens one workgroup per row does it all, its keys in registers. Longer rows are
+// dealt out in parts of kSelPart tokens over three launches: the parts' counts of the top 11 bits; from
+// all of a row's counts the class of the last token, whose members go to the row's list; and from that
+// list (a hundredth of the tokens, if weights differ) the last key and each part's slots. 16 rows of
+// 65536 tokens: 4.8 + 7.0 + 9.0 us; one workgroup per row took 71 us (129 with 8-bit classes and without
+// registers), the fetching of its unrolled code included, on 16 of the 256 CUs. 8 rows of 1023 tokens in
+// one launch: 9.2 us (31.8).
+//
+// Counts of one class are added one after the other; where all of a wave's tokens are of one class
+// (equal weights), one lane adds them up.
+constexpr int kSelThreads = 1024, kSelShort = 8192;
+constexpr int kPartThreads = 512, kSelPart = 4096, kPartKeys = kSelPart / kPartThreads;
 
-__global__ __launch_bounds__(kSelThreads) void hh_select_kernel(HHLoadLaunch a) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t picked[2];  // class taken in this round, tokens still to take in it
-  __shared__ int base_s[kSelWaves][2];
-  const HHCache& c = a.c;
-  const int64_t row = blockIdx.x;
-  const int b = (int)(row / c.hkv), tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int lo = a.lo != nullptr ? min(max(a.lo[b], 0), a.tokens) : 0;
-  const int n = a.tokens - lo;
-  const float* w = a.weights + row * a.tokens + lo;
-  int32_t* kept = a.kept + row * c.capacity;
-  float* wo = c.weights + row * c.capacity;
-  int32_t* order = c.order + row * c.capacity;
-  if (tid == 0) {
-    c.lengths[row] = min(n, c.capacity);
-    c.seen[row] = n;
+// The sum of x over the threads before this one; *all: over the workgroup. `part`: a value per wave.
+template <int kWaveCount>
+__device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* part, uint32_t* all) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  uint32_t incl = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t y = __shfl_up(incl, d);
+    if (lane >= d) incl += y;
   }
-  if (n <= c.capacity) {
-    for (int i = tid; i < n; i += kSelThreads) {
-      kept[i] = lo + i;
-      wo[i] = w[i];
-      order[i] = i;
-    }
-    return;
-  }
-  const int mid0 = c.keep_first, mid1 = n - c.keep_recent;  // mid1 - mid0 > need, since n > capacity
-  uint32_t need = (uint32_t)(c.capacity - c.keep_first - c.keep_recent);
-  uint32_t prefix = 0, mask = 0;  // of the last taken token's key
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = mid0 + tid; i < mid1; i += kSelThreads) {
-        const uint32_t key = weight_key(w[i]);
-        if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        uint32_t left = need;
-        int cls = 255;
-        while (hist[cls] < left) left -= hist[cls--];
-        picked[0] = (uint32_t)cls;
-        picked[1] = left;
-      }
-      __syncthreads();
-      prefix |= picked[0] << shift;
-      mask |= 255u << shift;
-      need = picked[1];
-    }
-  }
-  // `need` tokens of key == prefix are taken, and every one above it. Each wave takes a stretch of
-  // columns, 64 at a time; its first slot and first equal token come from the waves before it.
-  const bool none = c.capacity == c.keep_first + c.keep_recent;
-  const int chunk = ((n + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
-  const int from = min(wave * chunk, n), to = min(from + chunk, n);
-  int above = 0, equal = 0;
-  for (int i0 = from; i0 < to; i0 += 64) {
-    const int i = i0 + lane;
-    bool up = false, eq = false;
-    if (i < to) {
-      if (i < mid0 || i >= mid1) {
-        up = true;
-      } else if (!none) {
-        const uint32_t key = weight_key(w[i]);
-        up = key > prefix;
-        eq = key == prefix;
-      }
-    }
-    above += __popcll(__ballot(up));
-    equal += __popcll(__ballot(eq));
-  }
-  if (lane == 0) {
-    base_s[wave][0] = above;
-    base_s[wave][1] = equal;
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();
+  uint32_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaveCount; ++w) {
+    const uint32_t y = part[w];
+    before += w < wave ? y : 0u;
+    total += y;
   }
   __syncthreads();
-  int slot = 0, rank = 0;
-  for (int v = 0; v < wave; ++v) {
-    slot += base_s[v][0];
-    rank += base_s[v][1];
+  *all = total;
+  return before + incl - x;
+}
+
+// Adds 1 to hist[digit] for the calling lanes.
+__device__ __forceinline__ void count_class(uint32_t* hist, uint32_t digit) {
+  const uint32_t first = __builtin_amdgcn_readfirstlane(digit);
+  const uint64_t here = __ballot(true), same = __ballot(digit == first);
+  if (same == here) {
+    if (__builtin_ctzll(here) == (int)(threadIdx.x & 63)) atomicAdd(&hist[digit], (uint32_t)__popcll(here));
+  } else {
+    atomicAdd(&hist[digit], 1u);
   }
-  slot += min(rank, (int)need);
-  for (int i0 = from; i0 < to; i0 += 64) {
-    const int i = i0 + lane;
-    bool up = false, eq = false;
-    float x = 0.f;
-    if (i < to) {
-      x = w[i];
-      if (i < mid0 || i >= mid1) {
-        up = true;
-      } else if (!none) {
-        const uint32_t key = weight_key(x);
-        up = key > prefix;
-        eq = key == prefix;
+}
+
+// The class that holds the need-th heaviest of 2048 counted classes: thread t holds the counts of the
+// kN classes from 2047 - kN * t down. out: class, how many of its members are taken, whether all are.
+// The caller synchronizes before it reads out.
+template <int kN, int kWaveCount>
+__device__ __forceinline__ void pick_class(const uint32_t (&count)[kN], uint32_t need, uint32_t* part, uint32_t* out) {
+  uint32_t mine = 0, total;
+#pragma unroll
+  for (int x = 0; x < kN; ++x) mine += count[x];
+  uint32_t before = scan_before<kWaveCount>(mine, part, &total);
+  if (before < need && need <= before + mine) {
+#pragma unroll
+    for (int x = 0; x < kN; ++x) {
+      if (before < need && need <= before + count[x]) {
+        out[0] = 2047 - kN * threadIdx.x - x;
+        out[1] = need - before;
+        out[2] = need - before == count[x];
       }
+      before += count[x];
     }
-    const uint64_t below = (1ull << lane) - 1;
-    const uint64_t eqs = __ballot(eq);
-    const bool take = up || (eq && rank + __popcll(eqs & below) < (int)need);
-    const uint64_t takes = __ballot(take);
-    const int at = slot + __popcll(takes & below);
-    if (take && at < c.capacity) {
-      kept[at] = lo + i;
-      wo[at] = x;
-      order[at] = i;
+  }
+}
+
+struct SelectRow {
+  int lo, n, mid0, mid1;
+  const float* w;
+  __device__ __forceinline__ SelectRow(const HHLoadLaunch& a, int64_t row) {
+    const int b = (int)(row / a.c.hkv);
+    lo = a.lo != nullptr ? min(max(a.lo[b], 0), a.tokens) : 0;
+    n = a.tokens - lo;
+    mid0 = a.c.keep_first;
+    mid1 = n - a.c.keep_recent;
+    w = a.weights + row * a.tokens + lo;
+  }
+  // Token i's key: 0xffffffff for one that is kept in any case, 0 past the row's end.
+  __device__ __forceinline__ uint32_t key(int i) const {
+    const uint32_t k = weight_key(w[min(i, n - 1)]);
+    return i >= n ? 0u : i < mid0 || i >= mid1 ? 0xffffffffu : k;
+  }
+};
+
+__device__ __forceinline__ void keep_token(const HHLoadLaunch& a, const SelectRow& r, int64_t row, uint32_t at, int i) {
+  if (at >= (uint32_t)a.c.capacity) return;
+  const int64_t to = row * a.c.capacity + at;
+  a.kept[to] = r.lo + i;
+  a.c.weights[to] = r.w[i];
+  a.c.order[to] = i;
+}
+
+// A row that fits: every token stays. Also sets the row's length.
+__device__ __forceinline__ bool keep_all(const HHLoadLaunch& a, const SelectRow& r, int64_t row, int part, int parts) {
+  if (part == 0 && threadIdx.x == 0) {
+    a.c.lengths[row] = min(r.n, a.c.capacity);
+    a.c.seen[row] = r.n;
+  }
+  if (r.n > a.c.capacity) return false;
+  for (int i = part * (int)blockDim.x + threadIdx.x; i < r.n; i += parts * (int)blockDim.x)
+    keep_token(a, r, row, (uint32_t)i, i);
+  return true;
+}
+
+__global__ __launch_bounds__(kSelThreads) void hh_select_kernel(HHLoadLaunch a) {
+  constexpr int kPer = kSelShort / kSelThreads, kWaveCount = kSelThreads / 64, kGroups = kPer * kWaveCount;
+  __shared__ uint32_t hist[2048];
+  __shared__ uint32_t ups[kGroups], eqs[kGroups];  // per group of 64: tokens above the key, equal to it
+  __shared__ uint32_t part[kWaveCount], picked[3];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const SelectRow r(a, row);
+  if (keep_all(a, r, row, 0, 1)) return;
+  uint32_t keys[kPer];
+#pragma unroll
+  for (int y = 0; y < kPer; ++y) keys[y] = r.key(y * kSelThreads + tid);
+
+  uint32_t need = (uint32_t)a.c.capacity, last = 0;
+#pragma unroll 1
+  for (int shift = 21, above = 32; above > 0; above = shift, shift = shift == 21 ? 10 : 0) {
+    hist[tid] = 0;
+    hist[tid + 1024] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int y = 0; y < kPer; ++y)
+      if (((uint64_t)(keys[y] ^ last) >> above) == 0) count_class(hist, keys[y] >> shift & (above == 10 ? 1023u : 2047u));
+    __syncthreads();
+    const uint32_t counts[2] = {hist[2047 - 2 * tid], hist[2046 - 2 * tid]};
+    pick_class<2, kWaveCount>(counts, need, part, picked);
+    __syncthreads();
+    last |= picked[0] << shift;
+    need = picked[1];
+    if (picked[2] != 0) {  // the whole class is taken: all above its lowest key less one (no class holds key 0)
+      last -= 1;
+      need = 0;
+      break;
     }
-    rank += __popcll(eqs);
-    slot += __popcll(takes);
+  }
+
+#pragma unroll
+  for (int y = 0; y < kPer; ++y) {
+    const uint32_t u = (uint32_t)__popcll(__ballot(keys[y] > last)), e = (uint32_t)__popcll(__ballot(keys[y] == last));
+    if (lane == 0) {
+      ups[y * kWaveCount + wave] = u;  // the columns' order
+      eqs[y * kWaveCount + wave] = e;
+    }
+  }
+  __syncthreads();
+  // (At most 8192 of either: both in one scan.)
+  uint32_t all;
+  const uint32_t ue = scan_before<kWaveCount>(tid < kGroups ? ups[tid] << 16 | eqs[tid] : 0u, part, &all);
+  if (tid < kGroups) {
+    ups[tid] = ue >> 16;
+    eqs[tid] = ue & 0xffffu;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int y = 0; y < kPer; ++y) {
+    const uint64_t um = __ballot(keys[y] > last), em = __ballot(keys[y] == last), below = (1ull << lane) - 1;
+    const uint32_t rank = eqs[y * kWaveCount + wave] + (uint32_t)__popcll(em & below);
+    if (keys[y] > last || (keys[y] == last && rank < need))
+      keep_token(a, r, row, ups[y * kWaveCount + wave] + (uint32_t)__popcll(um & below) + min(rank, need),
+                 y * kSelThreads + tid);
+  }
+}
+
+// A thread's keys of a part, all asked for at once: kPartKeys groups of 64 tokens a wave, in order.
+__device__ __forceinline__ int part_column(int part, int y) {
+  return part * kSelPart + ((int)threadIdx.x >> 6) * (64 * kPartKeys) + 64 * y + ((int)threadIdx.x & 63);
+}
+__device__ __forceinline__ void part_keys(uint32_t (&keys)[kPartKeys], const SelectRow& r, int part) {
+#pragma unroll
+  for (int y = 0; y < kPartKeys; ++y) keys[y] = r.key(part_column(part, y));
+}
+
+// Long rows, first launch: the counts of the top 11 bits of each part's keys.
+__global__ __launch_bounds__(kPartThreads) void hh_part_count_kernel(HHLoadLaunch a) {
+  __shared__ uint32_t hist[2048];
+  const int64_t row = blockIdx.y;
+  const int part = blockIdx.x, tid = threadIdx.x;
+  const SelectRow r(a, row);
+  if (keep_all(a, r, row, part, gridDim.x)) return;
+  uint32_t keys[kPartKeys];
+  part_keys(keys, r, part);
+  for (int x = tid; x < 2048; x += kPartThreads) hist[x] = 0;
+  if (part == 0 && tid == 0) a.rows[row].listed = 0;
+  __syncthreads();
+#pragma unroll
+  for (int y = 0; y < kPartKeys; ++y) count_class(hist, keys[y] >> 21);
+  __syncthreads();
+  uint32_t* out = reinterpret_cast<uint32_t*>(a.part_counts) + (row * gridDim.x + part) * 1024;  // 16 bits a class
+  for (int x = tid; x < 1024; x += kPartThreads) out[x] = hist[2 * x] | hist[2 * x + 1] << 16;
+}
+
+// Second launch: the class of the last taken token, from the counts of all parts of the row (every
+// workgroup finds it for itself). Its members go to the row's list, in any order, each with its part; the
+// part's tokens above it are counted.
+__global__ __launch_bounds__(kPartThreads) void hh_part_list_kernel(HHLoadLaunch a) {
+  constexpr int kWaveCount = kPartThreads / 64, kWords = 1024 / kPartThreads;
+  __shared__ uint32_t wave_part[kWaveCount], wave_mine[kWaveCount], picked[3], higher, first;
+  const int64_t row = blockIdx.y;
+  const int part = blockIdx.x, parts = gridDim.x, tid = threadIdx.x, lane = tid & 63;
+  const SelectRow r(a, row);
+  if (r.n <= a.c.capacity) return;
+  uint32_t keys[kPartKeys];
+  part_keys(keys, r, part);
+  uint32_t counts[2 * kWords] = {};
+  const uint32_t* in = reinterpret_cast<const uint32_t*>(a.part_counts) + row * parts * 1024 + 1024 - kWords * (tid + 1);
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) {
+#pragma unroll
+    for (int y = 0; y < kWords; ++y) {
+      const uint32_t x = in[p * 1024 + kWords - 1 - y];
+      counts[2 * y] += x >> 16;
+      counts[2 * y + 1] += x & 0xffffu;
+    }
+  }
+  if (tid == 0) higher = 0;
+  pick_class<2 * kWords, kWaveCount>(counts, (uint32_t)a.c.capacity, wave_part, picked);
+  __syncthreads();
+  const uint32_t cls = picked[0];
+  if (part == 0 && tid == 0) {
+    a.rows[row].cls = cls;
+    a.rows[row].need = picked[1];
+    a.rows[row].whole = picked[2];
+  }
+  u32x2* list = reinterpret_cast<u32x2*>(a.listed) + row * parts * kSelPart;
+  uint32_t above = 0, mine = 0;
+#pragma unroll
+  for (int y = 0; y < kPartKeys; ++y) {
+    above += (uint32_t)__popcll(__ballot(keys[y] >> 21 > cls));
+    mine += (uint32_t)__popcll(__ballot(keys[y] >> 21 == cls));
+  }
+  if (lane == 0) {
+    wave_mine[tid >> 6] = mine;
+    if (above != 0) atomicAdd(&higher, above);
+  }
+  __syncthreads();
+  if (tid == 0) {  // (one addition per workgroup: the row's 16 parts wait for each other)
+    uint32_t sum = 0;
+#pragma unroll
+    for (int v = 0; v < kWaveCount; ++v) {
+      const uint32_t x = wave_mine[v];
+      wave_mine[v] = sum;
+      sum += x;
+    }
+    first = sum != 0 ? atomicAdd(&a.rows[row].listed, sum) : 0u;
+    a.part_above[row * parts + part] = higher;
+  }
+  __syncthreads();
+  uint32_t base = first + wave_mine[tid >> 6];
+#pragma unroll
+  for (int y = 0; y < kPartKeys; ++y) {
+    const bool in_class = keys[y] >> 21 == cls;
+    const uint64_t mask = __ballot(in_class);
+    if (in_class) list[base + (uint32_t)__popcll(mask & ((1ull << lane) - 1))] = u32x2{keys[y], (uint32_t)part};
+    base += (uint32_t)__popcll(mask);
+  }
+}
+
+// Third launch: the last key from the row's list, the part's first slot, its tokens' slots.
+__global__ __launch_bounds__(kPartThreads) void hh_part_keep_kernel(HHLoadLaunch a) {
+  constexpr int kWaveCount = kPartThreads / 64, kPer = 2048 / kPartThreads;
+  __shared__ uint32_t hist[2048];
+  __shared__ uint32_t wave_part[kWaveCount], picked[3], base_u, base_e, wave_u[kWaveCount], wave_e[kWaveCount];
+  const int64_t row = blockIdx.y;
+  const int part = blockIdx.x, parts = gridDim.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const SelectRow r(a, row);
+  if (r.n <= a.c.capacity) return;
+  uint32_t keys[kPartKeys];
+  part_keys(keys, r, part);
+  const HHSelectRow info = a.rows[row];
+  const u32x2* list = reinterpret_cast<const u32x2*>(a.listed) + row * parts * kSelPart;
+  const int m = (int)info.listed;
+  uint32_t last = info.cls << 21, need = info.need;
+  bool whole = info.whole != 0;
+  uint32_t u = 0, e = 0;  // tokens of the parts before this one above the key, and equal to it
+  for (int p = tid; p < part; p += kPartThreads) u += a.part_above[row * parts + p];
+  if (tid == 0) base_u = base_e = 0;
+#pragma unroll 1
+  for (int shift = 10, above = 21; above > 0 && !whole; above = shift, shift = 0) {
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) hist[tid + x * kPartThreads] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < m; i += kPartThreads) {
+      const uint32_t key = list[i].x;
+      if ((key ^ last) >> above == 0) count_class(hist, key >> shift & (above == 10 ? 1023u : 2047u));
+    }
+    __syncthreads();
+    uint32_t counts[kPer];
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) counts[x] = hist[2047 - kPer * tid - x];
+    pick_class<kPer, kWaveCount>(counts, need, wave_part, picked);
+    __syncthreads();
+    last |= picked[0] << shift;
+    need = picked[1];
+    whole = picked[2] != 0;
+  }
+  if (whole) {  // the whole class is taken: all above its lowest key less one (no class holds key 0)
+    last -= 1;
+    need = 0;
+  }
+#pragma unroll 4
+  for (int i = tid; i < m; i += kPartThreads) {
+    const u32x2 x = list[i];
+    if ((int)x.y < part) {
+      u += x.x > last;
+      e += x.x == last;
+    }
+  }
+  __syncthreads();
+  if (u != 0) atomicAdd(&base_u, u);
+  if (e != 0) atomicAdd(&base_e, e);
+  u = e = 0;
+#pragma unroll
+  for (int y = 0; y < kPartKeys; ++y) {
+    u += (uint32_t)__popcll(__ballot(keys[y] > last));
+    e += (uint32_t)__popcll(__ballot(keys[y] == last));
+  }
+  if (lane == 0) {
+    wave_u[wave] = u;
+    wave_e[wave] = e;
+  }
+  __syncthreads();
+  u = base_u;
+  e = base_e;
+  for (int v = 0; v < wave; ++v) {
+    u += wave_u[v];
+    e += wave_e[v];
+  }
+#pragma unroll
+  for (int y = 0; y < kPartKeys; ++y) {
+    const uint64_t um = __ballot(keys[y] > last), em = __ballot(keys[y] == last), below = (1ull << lane) - 1;
+    const uint32_t rank = e + (uint32_t)__popcll(em & below);
+    // Before this token: those above the key, and of the equal ones as many as are taken.
+    if (keys[y] > last || (keys[y] == last && rank < need))
+      keep_token(a, r, row, u + (uint32_t)__popcll(um & below) + min(rank, need), part_column(part, y));
+    u += (uint32_t)__popcll(um);
+    e += (uint32_t)__popcll(em);
   }
 }
 
@@ -516,10 +756,26 @@ hipError_t launch_hh_attend(int dtype, const HHAttendLaunch& p, hipStream_t stre
   return dtype == kF16 ? attend<HalfT>(p, sc, stream) : attend<Bf16T>(p, sc, stream);
 }
 
+int hh_select_parts(int tokens) { return (tokens + kSelPart - 1) / kSelPart; }
+size_t hh_select_part_tokens() { return kSelPart; }
+
 hipError_t launch_hh_load(const HHLoadLaunch& p, hipStream_t stream) {
   const unsigned rows = (unsigned)(p.c.batch * p.c.hkv);
-  hh_select_kernel<<<rows, kSelThreads, 0, stream>>>(p);
-  hipError_t e = hipGetLastError();
+  hipError_t e = hipSuccess;
+  if (p.tokens <= kSelShort || p.tokens <= p.c.capacity) {
+    hh_select_kernel<<<rows, kSelThreads, 0, stream>>>(p);
+    e = hipGetLastError();
+  } else {
+    const dim3 grid((unsigned)hh_select_parts(p.tokens), rows);
+    hh_part_count_kernel<<<grid, kPartThreads, 0, stream>>>(p);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hh_part_list_kernel<<<grid, kPartThreads, 0, stream>>>(p);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hh_part_keep_kernel<<<grid, kPartThreads, 0, stream>>>(p);
+    e = hipGetLastError();
+  }
   if (e != hipSuccess) return e;
   const int most = p.tokens < p.c.capacity ? p.tokens : p.c.capacity;
   const int64_t pieces = (int64_t)most * (p.c.d / 8);

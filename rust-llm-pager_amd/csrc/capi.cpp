@@ -356,6 +356,23 @@ AttendPlan plan_attend(const pgr_hh_cache_t* c) {
   return p;
 }
 
+struct LoadPlan {
+  size_t o_kept = 0, o_counts = 0, o_above = 0, o_listed = 0, o_rows = 0, bytes = 0;
+};
+
+LoadPlan plan_load(const pgr_hh_cache_t* c, int64_t tokens) {
+  LoadPlan p;
+  const size_t rows = (size_t)(c->batch * c->kv_heads), parts = rows * (size_t)pgr::hh_select_parts((int)tokens);
+  Parts w;
+  p.o_kept = w.take(rows * (size_t)c->capacity * sizeof(int32_t));
+  p.o_counts = w.take(parts * 2048 * sizeof(uint16_t));
+  p.o_above = w.take(parts * sizeof(uint32_t));
+  p.o_listed = w.take(parts * pgr::hh_select_part_tokens() * 2 * sizeof(uint32_t));
+  p.o_rows = w.take(rows * sizeof(pgr::HHSelectRow));
+  p.bytes = w.bytes;
+  return p;
+}
+
 struct PromptPlan {
   pgr::PromptWeightPlan k;
   size_t o_stats = 0, o_norm = 0, o_partial = 0, bytes = 0;
@@ -1367,10 +1384,10 @@ int pgr_hh_prompt_weights(const void* q, const int64_t* q_strides, const void* k
   }
 }
 
-size_t pgr_hh_load_prompt_workspace_bytes(const pgr_hh_cache_t* cache) {
+size_t pgr_hh_load_prompt_workspace_bytes(const pgr_hh_cache_t* cache, int64_t tokens) {
   try {
-    if (check_cache(cache) != pgr::kOk) return 0;
-    return pgr::align_up((size_t)(cache->batch * cache->kv_heads) * cache->capacity * sizeof(int32_t), 256);
+    if (check_cache(cache) != pgr::kOk || tokens < 0 || tokens > ((int64_t)1 << 30)) return 0;
+    return plan_load(cache, tokens).bytes;
   } catch (...) {
     exception_status();
     return 0;
@@ -1387,8 +1404,10 @@ int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t
     if (cache->batch == 0) return pgr::kOk;
     if (tokens > 0 && (!k || !k_strides || !v || !v_strides || !weights))
       return set_err(pgr::kErrInvalid, "null tensor pointer");
-    if (workspace == nullptr || workspace_bytes < pgr_hh_load_prompt_workspace_bytes(cache))
-      return set_err(pgr::kErrCapacity, "workspace too small");
+    const LoadPlan p = plan_load(cache, tokens);
+    if (workspace == nullptr || workspace_bytes < p.bytes) return set_err(pgr::kErrCapacity, "workspace too small");
+    if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");
+    char* w = static_cast<char*>(workspace);
     pgr::HHLoadLaunch L;
     L.c = cache_of(cache);
     L.k = k;
@@ -1400,7 +1419,11 @@ int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t
     L.weights = weights;
     L.lo = lo;
     L.tokens = (int)tokens;
-    L.kept = static_cast<int32_t*>(workspace);
+    L.kept = reinterpret_cast<int32_t*>(w + p.o_kept);
+    L.part_counts = reinterpret_cast<uint16_t*>(w + p.o_counts);
+    L.listed = reinterpret_cast<uint32_t*>(w + p.o_listed);
+    L.part_above = reinterpret_cast<uint32_t*>(w + p.o_above);
+    L.rows = reinterpret_cast<pgr::HHSelectRow*>(w + p.o_rows);
     const hipError_t e = pgr::launch_hh_load(L, as_stream(stream));
     if (e != hipSuccess) return hip_err(e, "load prompt launch");
     return pgr::kOk;

@@ -144,7 +144,6 @@ class HeavyHitterCache:
         )
         self._ref = ctypes.byref(self._c)
         self._attend_bytes = N.lib().pgr_hh_attend_workspace_bytes(self._ref)
-        self._load_bytes = N.lib().pgr_hh_load_prompt_workspace_bytes(self._ref)
 
     # The kernels hold the buffers' addresses: they can be written to, not replaced.
     keys = property(lambda self: self._keys)
@@ -192,11 +191,12 @@ class HeavyHitterCache:
                 raise ValueError(f"tensors on different devices: {self.device} and {x.device}")
         lo = _first_columns(lo, self.batch, self.device)
         k, v, weights = _dense_last(k), _dense_last(v), weights.contiguous()
-        ws = torch.empty(self._load_bytes, dtype=torch.uint8, device=self.device)
+        nbytes = N.lib().pgr_hh_load_prompt_workspace_bytes(self._ref, t)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         with _on(self.device):
             N.nat.check(
                 N.lib().pgr_hh_load_prompt(self._ref, k.data_ptr(), _strides(k, 3), v.data_ptr(), _strides(v, 3),
-                                           weights.data_ptr(), N.ptr(lo), t, ws.data_ptr(), self._load_bytes,
+                                           weights.data_ptr(), N.ptr(lo), t, ws.data_ptr(), nbytes,
                                            N.stream_of(self.device)),
                 "HeavyHitterCache.load_prompt",
             )

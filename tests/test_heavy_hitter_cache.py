@@ -36,7 +36,7 @@ def test_c_entries_refuse_a_bad_cache(over, code):
     assert lib.pgr_hh_append(c, 16, s, 16, s, 16, s, 16, None, 0, None, 0, 0, 1.0, None) == code
     assert lib.pgr_hh_attend(c, 16, s, 16, 1.0, 0.0, 256, 1 << 30, None) == code
     assert lib.pgr_hh_load_prompt(c, 16, s, 16, s, 16, None, 4, 256, 1 << 30, None) == code
-    assert lib.pgr_hh_attend_workspace_bytes(c) == 0 and lib.pgr_hh_load_prompt_workspace_bytes(c) == 0
+    assert lib.pgr_hh_attend_workspace_bytes(c) == 0 and lib.pgr_hh_load_prompt_workspace_bytes(c, 4) == 0
 
 
 def test_c_entries_refuse_bad_arguments():
@@ -56,7 +56,8 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.pgr_hh_attend(c, 16, s, None, 1.0, 0.0, 256, need, None) == inv
     assert lib.pgr_hh_attend(c, 16, s, 16, 0.0, 0.0, 256, need, None) == inv
     assert lib.pgr_hh_attend(c, 16, s, 16, 1.0, float("nan"), 256, need, None) == inv
-    need = lib.pgr_hh_load_prompt_workspace_bytes(c)
+    need = lib.pgr_hh_load_prompt_workspace_bytes(c, 4)
+    assert lib.pgr_hh_load_prompt_workspace_bytes(c, -1) == 0
     assert need >= 2 * 64 * 4
     assert lib.pgr_hh_load_prompt(c, 16, s, 16, s, 16, None, -1, 256, need, None) == inv
     assert lib.pgr_hh_load_prompt(c, 16, s, 16, s, None, None, 4, 256, need, None) == inv

@@ -280,6 +280,9 @@ LOAD = [
     (2, 1, 256, 1025, 36, 4, 32, [0, 989]),
     (1, 1, 64, 70000, 4096, 4, 256, None),
     (1, 2, 64, 0, 40, 4, 32, None),
+    (4, 2, 16, 9001, 36, 4, 32, [0, 4500, 8970, 9001]),
+    (1, 2, 16, 20001, 12000, 5000, 1, [3]),
+    (2, 1, 16, 8193, 8192, 0, 1, [0, 1]),
 ]
 
 
