@@ -58,9 +58,10 @@ struct HHAppendLaunch {
 };
 hipError_t launch_hh_append(int dtype, const HHAppendLaunch& p, hipStream_t stream);
 
-// Splits of a cache row that an attend call makes, and the tokens of a row's logits (padded).
+// Splits of a cache row that an attend call makes (0: one workgroup per row, no merge launch), and the
+// tokens of a row's scores (padded to whole tiles).
 int hh_attend_splits(int batch, int hkv, int capacity);
-__host__ __device__ inline int64_t hh_attend_stride(int capacity) { return ((int64_t)capacity + 15) / 16 * 16; }
+__host__ __device__ inline int64_t hh_attend_stride(int capacity) { return ((int64_t)capacity + 31) / 32 * 32; }
 
 struct HHAttendLaunch {
   HHCache c;

@@ -104,40 +104,67 @@ __global__ __launch_bounds__(256) void hh_append_kernel(HHAppendLaunch a) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Attention of one new token. MFMA tiles as in the decode kernels: a 16-token tile is
-//     S^T[16 tok x 16 heads] = K . Q^T,   O^T[D x 16 heads] += V^T . P^T
-// lane (g, n) holding tokens 4g..4g+3 of query head n, so the softmax state is a per-lane scalar.
+// Attention of one new token. Each wave folds tiles of 32 tokens, two halves of 16, on
+// v_mfma_f32_16x16x32:
+//     S^T[16 tok x 16 heads] = K . Q^T,   O^T[D x 16 heads] += V^T[D x 32 tok] . P^T[32 tok x 16 heads]
+// Lane (g, n) holds tokens 4g..4g+3 of each half for query head n, which is the P^T operand as it
+// stands (contraction slot 8g + e: token 4g + e of the first half, 4g + e - 4 of the second), and every
+// O^T value of a lane belongs to head n as well: the softmax state is a scalar of the lane.
+// A lane reads 16-byte pieces 4c + g of K row n, so that an instruction covers 64 bytes of each of
+// 16 rows, and of V the D/16 elements n of its eight rows, transposed in registers (v_perm_b32).
+//
+// Bound by HBM. The next tile's K is loaded as soon as the scores of this one are taken, its V after
+// P.V, without a second set of registers. The scores go to memory once (4 bytes a head and token,
+// beside 4 D of K and V), since the weights need each head's final maximum and sum: the merge launch adds
+// them up. 32 full rows x 8192 tokens, 32/8 heads, D 128: 206 + 13 us for 1.08 GB (5.2 TB/s in the first
+// launch; a copy reaches 5.1, a plain read in this order 6.25, this launch without its stores 5.8). Tiles
+// of 16 tokens, one load after the other: 221 us; 256 to 8192 workgroups, non-temporal loads or not: 205-212.
 template <int D>
 struct KVTile {
-  static constexpr int KD = D / 8;                     // dwords: D/4 elements of K row n
-  static constexpr int VD = D >= 32 ? D / 32 : 1;      // dwords: D/16 elements of each of 4 V rows
-  uint32_t k[KD];
-  uint32_t v[4][VD];
+  static constexpr int KP = D >= 32 ? D / 32 : 1;  // 16-byte pieces of a K row (D 16: one of 8 bytes)
+  static constexpr int VD = D >= 32 ? D / 32 : 1;  // dwords of each V row (D 16: half of one)
+  u32x4 k[2][KP];
+  uint32_t v[2][4][VD];
 };
 
-template <int N>
-__device__ __forceinline__ void load_dwords(uint32_t (&r)[N], const uint16_t* src) {
-  if constexpr (N % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const u32x4 x = *reinterpret_cast<const u32x4_e*>(src + 8 * i);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) r[4 * i + c] = x[c];
-    }
+typedef uint32_t u32x2_e __attribute__((ext_vector_type(2), aligned(2)));
+
+// The lane's pieces of a K row (or of a query).
+template <int D>
+__device__ __forceinline__ void load_pieces(u32x4 (&r)[KVTile<D>::KP], const uint16_t* row, int g) {
+  if constexpr (D == 16) {
+    const u32x2 x = *reinterpret_cast<const u32x2_e*>(row + 4 * g);
+    r[0] = u32x4{x.x, x.y, 0u, 0u};
   } else {
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) r[c] = *reinterpret_cast<const u32x4_e*>(row + 32 * c + 8 * g);
+  }
+}
+
+// Elements (D/16) n.. of a V row.
+template <int D>
+__device__ __forceinline__ void load_v(uint32_t (&r)[KVTile<D>::VD], const uint16_t* row, int n) {
+  const uint16_t* p = row + (D / 16) * n;
+  if constexpr (D == 16) {
+    r[0] = *p;
+  } else if constexpr (D == 32) {
     typedef uint32_t u32_e __attribute__((aligned(2)));
-    typedef uint32_t u32x2_e __attribute__((ext_vector_type(2), aligned(2)));
-    if constexpr (N == 2) {
-      const u32x2 x = *reinterpret_cast<const u32x2_e*>(src);
-      r[0] = x.x;
-      r[1] = x.y;
-    } else {
-      static_assert(N == 1, "1, 2 or a multiple of 4 dwords");
-      r[0] = *reinterpret_cast<const u32_e*>(src);
+    r[0] = *reinterpret_cast<const u32_e*>(p);
+  } else if constexpr (D == 64) {
+    const u32x2 x = *reinterpret_cast<const u32x2_e*>(p);
+    r[0] = x.x;
+    r[1] = x.y;
+  } else {
+#pragma unroll
+    for (int c = 0; c < D / 128; ++c) {
+      const u32x4 x = *reinterpret_cast<const u32x4_e*>(p + 8 * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[4 * c + i] = x[i];
     }
   }
 }
 
+// Max and sum over the four lane groups g.
 __device__ __forceinline__ float max_g(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
@@ -148,105 +175,159 @@ __device__ __forceinline__ float sum_g(float x) {
 }
 
 // Scores in log2 units: scale_log2 = scale * log2(e), or with a softcap cap * log2(e).
-__device__ __forceinline__ float log2_score(float s, float scale_log2, float cap_scale, float cap_log2) {
-  return cap_log2 > 0.f ? cap_log2 * tanhf(s * cap_scale) : s * scale_log2;
-}
-
 struct AttendScale {
   float scale_log2, cap_scale, cap_log2;
 };
 
-// Tokens [begin, end) of a row of `length` that split `split` of n_split takes: whole 16-token
+// Tokens [begin, end) of a row of `length` that split `split` of n_split takes: whole 32-token
 // tiles, evenly.
-__device__ __forceinline__ void split_range(int length, int split, int n_split, int& begin, int& end) {
-  const int tiles = (length + 15) / 16, per = (tiles + n_split - 1) / n_split;
-  begin = min(split * per, tiles) * 16;
-  end = min(min((split + 1) * per, tiles) * 16, length);
+constexpr int kTileTokens = 32;
+__device__ __forceinline__ int split_tiles(int length, int n_split) {
+  const int tiles = (length + kTileTokens - 1) / kTileTokens;
+  return (tiles + n_split - 1) / n_split;
 }
 
-template <class Ty, int D>
-__global__ __launch_bounds__(256) void hh_attend_kernel(HHAttendLaunch a, AttendScale sc) {
+// Rows of up to kOneTokens slots: the workgroup holds the whole row, its scores in LDS, and finishes
+// it without a merge launch (256 tokens, 28/4 heads, D 128: 7.0 us instead of 5.1 + 4.8).
+constexpr int kOneTokens = 512;
+constexpr int kMostSplits = 1024;
+
+template <class Ty, int D, int kW, bool kOne>
+__global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, AttendScale sc) {
   typedef KVTile<D> T;
-  constexpr int kRep = kMaxRep;
-  __shared__ float sm_m[kWaves][kRep], sm_l[kWaves][kRep];
-  __shared__ float sm_acc[kWaves][kRep][D + 1];
+  constexpr int kThreads = 64 * kW;
+  __shared__ float sm_m[kW][kMaxRep], sm_l[kW][kMaxRep];
+  __shared__ float sm_acc[kW][kMaxRep][D + 1];
+  __shared__ __align__(16) float sm_logits[kOne ? kMaxRep * kOneTokens : 1];
+  __shared__ float norm_s[kMaxRep];
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const HHCache& c = a.c;
   const int n_rep = c.hq / c.hkv;
   const int64_t row = (int64_t)b * c.hkv + h;
   const int length = min(max(c.lengths[row], 0), c.capacity);
-  int begin, end;
-  split_range(length, split, a.n_split, begin, end);
-  if (begin >= end) return;  // uniform; the merge reads the splits that hold tokens
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int per = kOne ? length : split_tiles(length, a.n_split) * kTileTokens;
+  const int begin = min(split * per, length), end = min(begin + per, length);
+  // Uniform: nothing to fold. (The merge reads only the splits that hold tokens; a row that is
+  // finished here and holds none still has its zeros to write.)
+  if (!kOne && begin >= end) return;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
   const bool real = n < n_rep;
-  const uint16_t* kp = static_cast<const uint16_t*>(c.keys) + row * c.capacity * D;
-  const uint16_t* vp = static_cast<const uint16_t*>(c.values) + row * c.capacity * D;
-  const int tiles = (end - begin + 15) / 16;
+  const uint16_t* kp = static_cast<const uint16_t*>(c.keys) + (row * c.capacity + begin) * D;
+  const uint16_t* vp = static_cast<const uint16_t*>(c.values) + (row * c.capacity + begin) * D;
+  const int tokens = end - begin, tiles = (tokens + kTileTokens - 1) / kTileTokens;
 
-  auto fetch = [&](T& t, int ti) {
-    const int t0 = begin + ti * 16;
-    load_dwords(t.k, kp + (int64_t)min(t0 + n, end - 1) * D + (D / 4) * g);
+  T t;
+  // Rows past the split's end read its last row; what they hold is masked.
+  auto fetch_k = [&](int ti) {
+    const int most = tokens - 1 - ti * kTileTokens;
+    const uint16_t* p = kp + (int64_t)ti * kTileTokens * D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint16_t* p = vp + (int64_t)min(t0 + 4 * g + i, end - 1) * D + (D / 16) * n;
-      if constexpr (D < 32)
-        t.v[i][0] = *p;
-      else
-        load_dwords(t.v[i], p);
-    }
+    for (int x = 0; x < 2; ++x) load_pieces<D>(t.k[x], p + min(16 * x + n, most) * D, g);
   };
-
-  uint32_t q[T::KD];
+  auto fetch_v = [&](int ti) {
+    const int most = tokens - 1 - ti * kTileTokens;
+    const uint16_t* p = vp + (int64_t)ti * kTileTokens * D;
 #pragma unroll
-  for (int i = 0; i < T::KD; ++i) q[i] = 0u;
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load_v<D>(t.v[x][i], p + min(16 * x + 4 * g + i, most) * D, n);
+  };
+  if (wave < tiles) {
+    fetch_k(wave);
+    fetch_v(wave);
+  }
+
+  u32x4 q[T::KP];
+#pragma unroll
+  for (int i = 0; i < T::KP; ++i) q[i] = u32x4{0u, 0u, 0u, 0u};
   if (real)
-    load_dwords(q, static_cast<const uint16_t*>(a.q) + b * a.qs.b + ((int64_t)h * n_rep + n) * a.qs.h + (D / 4) * g);
+    load_pieces<D>(q, static_cast<const uint16_t*>(a.q) + b * a.qs.b + ((int64_t)h * n_rep + n) * a.qs.h, g);
 
   float m_run = kMinusInf, l_run = 0.f;
   f32x4 acc[D / 16];
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int64_t stride = hh_attend_stride(c.capacity);
-  float* lg = a.logits + ((int64_t)b * c.hq + (int64_t)h * n_rep + n) * stride;
+  // Scores of a tile lie together, head by head (32 tokens: 128 bytes): whole lines, one after the other.
+  float* lg = kOne ? sm_logits : a.logits + (row * hh_attend_stride(c.capacity) + begin) * n_rep;
+  lg += n * kTileTokens + 4 * g;
 
-  for (int ti = wave; ti < tiles; ti += kWaves) {
-    T t;
-    fetch(t, ti);
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  auto scores = [&](f32x4 (&s)[2]) {
 #pragma unroll
-    for (int i = 0; i < T::KD; i += 2) s = Ty::mma16(u32x2{t.k[i], t.k[i + 1]}, u32x2{q[i], q[i + 1]}, s);
-    const int tok = begin + ti * 16 + 4 * g;
-    f32x4 x;
+    for (int x = 0; x < 2; ++x) {
+      s[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (D == 16) {
+        s[x] = Ty::mma16(u32x2{t.k[x][0].x, t.k[x][0].y}, u32x2{q[0].x, q[0].y}, s[x]);
+      } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool ok = tok + i < end;
-      x[i] = ok ? log2_score(s[i], sc.scale_log2, sc.cap_scale, sc.cap_log2) : kMinusInf;
-      if (!ok) {
-#pragma unroll
-        for (int j = 0; j < T::VD; ++j) t.v[i][j] = 0u;
+        for (int i = 0; i < T::KP; ++i) s[x] = Ty::mma16x32(t.k[x][i], q[i], s[x]);
       }
     }
-    if (real) *reinterpret_cast<f32x4*>(lg + tok) = x;
-    const float m_new = fmaxf(m_run, max_g(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))));
-    const bool none = m_new == kMinusInf;
-    const float alpha = none ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
-    float p[4];
+  };
+  auto fold = [&](f32x4 (&s)[2], int ti) {
+    float p[8], top = kMinusInf;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = none ? 0.f : __builtin_amdgcn_exp2f(x[i] - m_new);
-    l_run = l_run * alpha + ((p[0] + p[1]) + (p[2] + p[3]));
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool ok = ti * kTileTokens + 16 * x + 4 * g + i < tokens;
+        const float y = sc.cap_log2 > 0.f ? sc.cap_log2 * tanhf(s[x][i] * sc.cap_scale) : s[x][i] * sc.scale_log2;
+        s[x][i] = ok ? y : kMinusInf;
+        if (!ok) {
+#pragma unroll
+          for (int j = 0; j < T::VD; ++j) t.v[x][i][j] = 0u;
+        }
+        top = fmaxf(top, s[x][i]);
+      }
+    const float m_new = fmaxf(m_run, max_g(top));
+    const bool none = m_new == kMinusInf;
+    if (__any(m_new > m_run)) {  // (otherwise the factor is 1)
+      const float alpha = none ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) acc[j] *= alpha;
+      m_run = m_new;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = none ? 0.f : __builtin_amdgcn_exp2f(s[i / 4][i & 3] - m_new);
+    l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
     // P is rounded to the K/V type for the matrix cores, as in the framework's other decode kernels.
-    const u32x2 pb = {Ty::pack(p[0], p[1]), Ty::pack(p[2], p[3])};
+    const u32x4 pb = {Ty::pack(p[0], p[1]), Ty::pack(p[2], p[3]), Ty::pack(p[4], p[5]), Ty::pack(p[6], p[7])};
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
       const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
       const int e = j >> 1;
-      const u32x2 vt = {__builtin_amdgcn_perm(t.v[1][e], t.v[0][e], sel),
-                        __builtin_amdgcn_perm(t.v[3][e], t.v[2][e], sel)};
-      acc[j] = Ty::mma16(vt, pb, acc[j] * alpha);
+      u32x4 vt;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        vt[2 * x] = __builtin_amdgcn_perm(t.v[x][1][e], t.v[x][0][e], sel);
+        vt[2 * x + 1] = __builtin_amdgcn_perm(t.v[x][3][e], t.v[x][2][e], sel);
+      }
+      acc[j] = Ty::mma16x32(vt, pb, acc[j]);
     }
-    m_run = m_new;
+  };
+  // After the next tile's loads, which are waited for in the order of all memory operations.
+  auto store = [&](const f32x4 (&s)[2], int ti) {
+    if (real) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) *reinterpret_cast<f32x4*>(lg + (int64_t)ti * kTileTokens * n_rep + 16 * x) = s[x];
+    }
+  };
+  int ti = wave;
+  for (; ti + kW < tiles; ti += kW) {
+    f32x4 s[2];
+    scores(s);
+    fetch_k(ti + kW);
+    fold(s, ti);
+    fetch_v(ti + kW);
+    __builtin_amdgcn_sched_barrier(0);
+    store(s, ti);
+  }
+  if (ti < tiles) {
+    f32x4 s[2];
+    scores(s);
+    fold(s, ti);
+    store(s, ti);
   }
 
   const float l_wave = sum_g(l_run);
@@ -260,75 +341,124 @@ __global__ __launch_bounds__(256) void hh_attend_kernel(HHAttendLaunch a, Attend
     for (int i = 0; i < 4; ++i) sm_acc[wave][n][(D / 4) * g + (D / 16) * i + j] = acc[j][i];
   __syncthreads();
   const int64_t part = (row * a.n_split + split) * n_rep;
-  for (int i = threadIdx.x; i < n_rep * D; i += 256) {
+  for (int i = threadIdx.x; i < n_rep * D; i += kThreads) {
     const int r = i / D, e = i - r * D;
     float m = kMinusInf;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sm_m[w][r]);
+    for (int w = 0; w < kW; ++w) m = fmaxf(m, sm_m[w][r]);
     float x = 0.f, l = 0.f;
     if (m != kMinusInf) {
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < kW; ++w) {
         const float f = __builtin_amdgcn_exp2f(sm_m[w][r] - m);
         x += sm_acc[w][r][e] * f;
         l += sm_l[w][r] * f;
       }
     }
-    a.pacc[part * D + i] = x;
-    if (e == 0) {
-      a.pm[part + r] = m;
-      a.pl[part + r] = l;
+    if constexpr (kOne) {
+      static_cast<uint16_t*>(a.out)[(row * n_rep + r) * D + e] = Ty::cvt(length > 0 ? x / l : 0.f);
+      if (e == 0) norm_s[r] = m + __builtin_amdgcn_logf(l);
+    } else {
+      a.pacc[part * D + i] = x;
+      if (e == 0) {
+        a.pm[part + r] = m;
+        a.pl[part + r] = l;
+      }
+    }
+  }
+  if constexpr (kOne) {
+    __syncthreads();
+    float* w = c.weights + row * c.capacity;
+    for (int i = threadIdx.x; i < length; i += kThreads) {
+      float sum = 0.f;
+      const float* y = sm_logits + i / kTileTokens * kTileTokens * n_rep + i % kTileTokens;
+      for (int r = 0; r < n_rep; ++r) sum += __builtin_amdgcn_exp2f(y[r * kTileTokens] - norm_s[r]);
+      w[i] += sum;
     }
   }
 }
 
+typedef float f32x4_e __attribute__((ext_vector_type(4), aligned(4)));
+
 // Joins the splits. Workgroups x < n_rep of a row write the output of query head x; the others add
 // the probabilities of 1024 tokens each, summed over the row's heads in their order, to the weights.
+// The splits' maxima and sums are read by a wave at once, the splits' outputs by groups of d / 4 threads
+// (32 splits of 32 rows: 5.6 us; 21.1 with a thread's loop over the splits).
 template <class Ty>
 __global__ __launch_bounds__(256) void hh_attend_merge_kernel(HHAttendLaunch a) {
-  typedef typename Ty::Raw Raw;
-  __shared__ float norm_s[kMaxRep];
+  __shared__ float norm_s[kMaxRep], f_s[kMostSplits];
+  __shared__ __align__(16) float sum_s[256 * 4];
   const HHCache& c = a.c;
-  const int n_rep = c.hq / c.hkv, d = c.d, tid = threadIdx.x;
+  const int n_rep = c.hq / c.hkv, d = c.d, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.y;
-  const int b = (int)(row / c.hkv), h = (int)(row - (int64_t)b * c.hkv);
   const int length = min(max(c.lengths[row], 0), c.capacity);
-  const int tiles = (length + 15) / 16, per = (tiles + a.n_split - 1) / a.n_split;
+  const int tiles = (length + kTileTokens - 1) / kTileTokens, per = split_tiles(length, a.n_split);
   const int used = per > 0 ? (tiles + per - 1) / per : 0;
   const float* pm = a.pm + row * a.n_split * n_rep;
   const float* pl = a.pl + row * a.n_split * n_rep;
+  // (m, l) of head r over the splits, in every lane of the calling wave.
+  auto head_stats = [&](int r, float& m, float& l) {
+    m = kMinusInf;
+    l = 0.f;
+    for (int s = lane; s < used; s += 64) {
+      const float ms = pm[s * n_rep + r], ls = pl[s * n_rep + r], top = fmaxf(m, ms);
+      if (top != kMinusInf) l = l * __builtin_amdgcn_exp2f(m - top) + ls * __builtin_amdgcn_exp2f(ms - top);
+      else l += ls;
+      m = top;
+    }
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) {
+      const float m2 = __shfl_xor(m, x), l2 = __shfl_xor(l, x), top = fmaxf(m, m2);
+      if (top != kMinusInf) l = l * __builtin_amdgcn_exp2f(m - top) + l2 * __builtin_amdgcn_exp2f(m2 - top);
+      else l += l2;
+      m = top;
+    }
+  };
   const int x = blockIdx.x;
   if (x < n_rep) {
-    float m = kMinusInf;
-    for (int s = 0; s < used; ++s) m = fmaxf(m, pm[s * n_rep + x]);
-    float l = 0.f;
-    for (int s = 0; s < used; ++s) l += m == kMinusInf ? 0.f : pl[s * n_rep + x] * __builtin_amdgcn_exp2f(pm[s * n_rep + x] - m);
-    const float* pacc = a.pacc + (row * a.n_split * n_rep + x) * d;
-    Raw* out = static_cast<Raw*>(a.out) + ((int64_t)b * c.hq + (int64_t)h * n_rep + x) * d;
-    for (int e = tid; e < d; e += 256) {
-      float o = 0.f;
-      for (int s = 0; s < used; ++s)
-        o += m == kMinusInf ? 0.f : pacc[(int64_t)s * n_rep * d + e] * __builtin_amdgcn_exp2f(pm[s * n_rep + x] - m);
-      out[e] = Ty::cvt(used > 0 ? o / l : 0.f);
+    float m, l;
+    head_stats(x, m, l);
+    for (int s = tid; s < used; s += 256) f_s[s] = m == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(pm[s * n_rep + x] - m);
+    __syncthreads();
+    const int cols = d / 4, groups = 256 / cols, g = tid / cols, e = (tid - g * cols) * 4;
+    const float* pacc = a.pacc + (row * a.n_split * n_rep + x) * d + e;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = g; s < used; s += groups) o += *reinterpret_cast<const f32x4*>(pacc + (int64_t)s * n_rep * d) * f_s[s];
+    *reinterpret_cast<f32x4*>(sum_s + 4 * tid) = o;
+    __syncthreads();
+    if (tid < d) {
+      float y = 0.f;
+      for (int k = 0; k < min(groups, used); ++k) y += sum_s[k * d + tid];
+      static_cast<uint16_t*>(a.out)[(row * n_rep + x) * d + tid] = Ty::cvt(used > 0 ? y / l : 0.f);
     }
     return;
   }
   const int first = (x - n_rep) * 1024;
   if (first >= length) return;
-  if (tid < n_rep) {
-    float m = kMinusInf;
-    for (int s = 0; s < used; ++s) m = fmaxf(m, pm[s * n_rep + tid]);
-    float l = 0.f;
-    for (int s = 0; s < used; ++s) l += m == kMinusInf ? 0.f : pl[s * n_rep + tid] * __builtin_amdgcn_exp2f(pm[s * n_rep + tid] - m);
-    norm_s[tid] = m + __builtin_amdgcn_logf(l);  // log2
+  for (int r = wave; r < n_rep; r += 4) {
+    float m, l;
+    head_stats(r, m, l);
+    if (lane == 0) norm_s[r] = m + __builtin_amdgcn_logf(l);  // log2
   }
+  const int t = first + 4 * tid;
+  float* w = c.weights + row * c.capacity + t;
+  const float* lg = a.logits + (row * hh_attend_stride(c.capacity) + t / kTileTokens * kTileTokens) * n_rep +
+                    t % kTileTokens;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   __syncthreads();
-  const int64_t stride = hh_attend_stride(c.capacity);
-  const float* lg = a.logits + ((int64_t)b * c.hq + (int64_t)h * n_rep) * stride;
-  for (int t = first + tid; t < min(first + 1024, length); t += 256) {
-    float sum = 0.f;
-    for (int r = 0; r < n_rep; ++r) sum += __builtin_amdgcn_exp2f(lg[r * stride + t] - norm_s[r]);
-    c.weights[row * c.capacity + t] += sum;
+  if (t >= length) return;
+#pragma unroll 4
+  for (int r = 0; r < n_rep; ++r) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(lg + r * kTileTokens);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(y[i] - norm_s[r]);
+  }
+  if (t + 3 < length) {
+    f32x4_e* to = reinterpret_cast<f32x4_e*>(w);
+    *to = *to + sum;
+  } else {  // slots from the length on stay as they are
+    for (int i = 0; i < length - t; ++i) w[i] += sum[i];
   }
 }
 
@@ -711,23 +841,32 @@ __global__ __launch_bounds__(256) void hh_gather_kernel(HHLoadLaunch a) {
   *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(c.values) + to) = y;
 }
 
-template <class Ty>
-hipError_t attend(const HHAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
+template <class Ty, int D>
+hipError_t attend_dim(const HHAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
   const HHCache& c = p.c;
   const dim3 grid((unsigned)p.n_split, (unsigned)c.hkv, (unsigned)c.batch);
-  switch (c.d) {
-    case 16: hh_attend_kernel<Ty, 16><<<grid, 256, 0, stream>>>(p, sc); break;
-    case 32: hh_attend_kernel<Ty, 32><<<grid, 256, 0, stream>>>(p, sc); break;
-    case 64: hh_attend_kernel<Ty, 64><<<grid, 256, 0, stream>>>(p, sc); break;
-    case 128: hh_attend_kernel<Ty, 128><<<grid, 256, 0, stream>>>(p, sc); break;
-    default: hh_attend_kernel<Ty, 256><<<grid, 256, 0, stream>>>(p, sc); break;
+  if (p.n_split == 0) {  // one workgroup finishes a row
+    constexpr int kW = D == 256 ? 4 : 8;
+    hh_attend_kernel<Ty, D, kW, true><<<dim3(1, grid.y, grid.z), 64 * kW, 0, stream>>>(p, sc);
+    return hipGetLastError();
   }
+  hh_attend_kernel<Ty, D, 4, false><<<grid, 256, 0, stream>>>(p, sc);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int n_rep = c.hq / c.hkv;
-  const dim3 merge((unsigned)(n_rep + (c.capacity + 1023) / 1024), (unsigned)(c.batch * c.hkv));
+  const dim3 merge((unsigned)(c.hq / c.hkv + (c.capacity + 1023) / 1024), (unsigned)(c.batch * c.hkv));
   hh_attend_merge_kernel<Ty><<<merge, 256, 0, stream>>>(p);
   return hipGetLastError();
+}
+
+template <class Ty>
+hipError_t attend(const HHAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
+  switch (p.c.d) {
+    case 16: return attend_dim<Ty, 16>(p, sc, stream);
+    case 32: return attend_dim<Ty, 32>(p, sc, stream);
+    case 64: return attend_dim<Ty, 64>(p, sc, stream);
+    case 128: return attend_dim<Ty, 128>(p, sc, stream);
+    default: return attend_dim<Ty, 256>(p, sc, stream);
+  }
 }
 
 }  // namespace
@@ -742,10 +881,12 @@ hipError_t launch_hh_append(int dtype, const HHAppendLaunch& p, hipStream_t stre
 }
 
 int hh_attend_splits(int batch, int hkv, int capacity) {
-  const int most = (capacity + 63) / 64;  // a tile for each wave
-  const int want = (1024 + batch * hkv - 1) / (batch * hkv);
-  const int n = most < want ? most : want;
-  return n < 1 ? 1 : n;
+  const int rows = batch * hkv;
+  if (capacity <= kOneTokens && rows <= 512) return 0;
+  const int most = (capacity + 4 * kTileTokens - 1) / (4 * kTileTokens);  // a tile for each wave
+  int n = (2048 + rows - 1) / rows;
+  if (n > most) n = most;
+  return n < 1 ? 1 : n > kMostSplits ? kMostSplits : n;
 }
 
 hipError_t launch_hh_attend(int dtype, const HHAttendLaunch& p, hipStream_t stream) {

@@ -243,12 +243,12 @@ class HeavyHitterCache:
         _inference_only(q)
         q = self._token(q, self.num_query_heads, "q")
         out = torch.empty((self.batch, self.num_query_heads, self.head_dim), dtype=self.dtype, device=self.device)
-        ws = torch.empty(self._attend_bytes, dtype=torch.uint8, device=self.device)
+        ws = torch.empty(self._attend_bytes, dtype=torch.uint8, device=self.device) if self._attend_bytes else None
         with _on(self.device):
             N.nat.check(
                 N.lib().pgr_hh_attend(
                     self._ref, q.data_ptr(), _strides(q, 2), out.data_ptr(),
-                    1.0 / self.head_dim**0.5 if scale is None else float(scale), float(softcap or 0.0), ws.data_ptr(),
+                    1.0 / self.head_dim**0.5 if scale is None else float(scale), float(softcap or 0.0), N.ptr(ws),
                     self._attend_bytes, N.stream_of(self.device),
                 ),
                 "HeavyHitterCache.attend",

@@ -49,10 +49,12 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.pgr_hh_append(c, 16, s, 16, s, 16, s, 16, None, 0, None, 2, 0, 1.0, None) == inv  # no inv_freq
     assert lib.pgr_hh_append(c, 16, s, 16, s, 16, s, 16, None, 0, 16, 34, 0, 1.0, None) == inv   # past the head
     assert lib.pgr_hh_append(c, 16, s, 16, s, 16, s, 16, None, 0, 16, 3, 0, 1.0, None) == inv    # odd
-    need = lib.pgr_hh_attend_workspace_bytes(c)
+    assert lib.pgr_hh_attend_workspace_bytes(c) == 0  # a short row needs none
+    long = _cache(capacity=4096)
+    need = lib.pgr_hh_attend_workspace_bytes(long)
     assert need > 0
-    assert lib.pgr_hh_attend(c, 16, s, 16, 1.0, 0.0, 256, need - 1, None) == cap
-    assert lib.pgr_hh_attend(c, 16, s, 16, 1.0, 0.0, None, need, None) == cap
+    assert lib.pgr_hh_attend(long, 16, s, 16, 1.0, 0.0, 256, need - 1, None) == cap
+    assert lib.pgr_hh_attend(long, 16, s, 16, 1.0, 0.0, None, need, None) == cap
     assert lib.pgr_hh_attend(c, 16, s, None, 1.0, 0.0, 256, need, None) == inv
     assert lib.pgr_hh_attend(c, 16, s, 16, 0.0, 0.0, 256, need, None) == inv
     assert lib.pgr_hh_attend(c, 16, s, 16, 1.0, float("nan"), 256, need, None) == inv
