@@ -1,24 +1,30 @@
 // Call path of the operator API for plain tensors: the Python functions of
-// pager_hf/streaming_attention.py hand their arguments to these before anything else.
+// pager_hf/streaming_attention.py, pager_hf/rotary.py and pager_hf/heavy_hitter_cache.py hand their
+// arguments to these before anything else.
 //
 // Each function checks that its arguments are what the kernels take as they are (exact
 // torch.Tensor objects without functorch, functionalization or lazy-bit keys, one GPU, one
-// dtype, contiguous, matching shapes), allocates the workspace or outputs from torch's current
+// dtype, contiguous (rotary and cache operands: head_dim contiguous), matching shapes), allocates the workspace or outputs from torch's current
 // allocator, and calls the C entry point of libpgr.so. It returns the entry point's status, or
 // None where any check fails: the caller then runs its general Python path, which converts,
 // copies or refuses as it always has. So this file decides nothing but speed: checks in Python,
 // one attribute object at a time, and a ctypes call of 19 arguments held the GPU up. A call of one
 // query (init, fold, finalize; 28/4 heads, D 128, fp16, 64 tokens) 30.6 -> 16.8 us, 4133 tokens
 // the same; the two-pass run of 12 calls (32/4, D 64, batch 4, 8209 tokens) 151 -> 84.6 us.
+// q and k of one token turned (14/2 heads, D 64) 17.9 -> @ROT@ us, an append to a full cache of 256 tokens 13.4
+// -> @APP@ us, attention over 256 tokens (28/4, D 128) 10.8 -> @ATT@ us.
 //
 // libpgr.so's entry points come as addresses (bind), so that the library the Python package has
 // loaded is the one called.
 #include <Python.h>
 
+#include "../../include/pgr.h"
+
 #include <ATen/ATen.h>
 #include <ATen/detail/CUDAHooksInterface.h>
 #include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <torch/csrc/Device.h>
@@ -45,6 +51,13 @@ int (*g_fold_fixed)(const void*, const void*, const void*, const int32_t*, const
                     int64_t, int64_t, int64_t, int64_t, int, float, float, void*, size_t, void*);
 int (*g_state_init)(float*, float*, float*, int64_t, int64_t, void*);
 int (*g_finalize)(const float*, const float*, void*, int64_t, int64_t, int, void*);
+decltype(&pgr_rotary) g_rotary;
+decltype(&pgr_hh_append) g_append;
+decltype(&pgr_hh_attend) g_attend;
+decltype(&pgr_hh_prompt_weights) g_prompt_weights;
+decltype(&pgr_hh_prompt_weights_workspace_bytes) g_prompt_weights_bytes;
+decltype(&pgr_hh_load_prompt) g_load_prompt;
+decltype(&pgr_hh_load_prompt_workspace_bytes) g_load_prompt_bytes;
 PyObject* g_raw_stream;     // torch._C._cuda_getCurrentRawStream
 PyObject* g_out_of_memory;  // torch.OutOfMemoryError
 
@@ -354,6 +367,277 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+// ---- rotary positions and the bounded cache --------------------------------------------
+// An operand whose last dimension is contiguous, the others strided at will. Null: not plain, or its
+// gradient is being recorded (the general path refuses it).
+const Tensor* viewed(PyObject* o, int64_t dims) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || !t.is_cuda() || !plain_keys(t) || !t.has_storage() || t.dim() != dims) return nullptr;
+  if (t.stride(-1) != 1 && t.size(-1) != 1) return nullptr;
+  return t.requires_grad() && c10::GradMode::is_enabled() ? nullptr : &t;
+}
+
+bool shaped(const Tensor* t, const Tensor* like, at::IntArrayRef shape) {
+  return t && t->scalar_type() == like->scalar_type() && t->device() == like->device() && t->sizes() == shape;
+}
+
+bool truth(PyObject* o, int* out) {
+  if (!PyBool_Check(o)) return false;
+  *out = o == Py_True;
+  return true;
+}
+
+// inv_freq: None, or the frequencies of at most head_dim / 2 pairs.
+bool frequencies(PyObject* o, const c10::Device& dev, int64_t head_dim, const float** data, int64_t* rotary) {
+  *data = nullptr;
+  *rotary = 0;
+  if (o == Py_None) return true;
+  const Tensor* t = plain(o);
+  if (!t || t->scalar_type() != at::kFloat || t->device() != dev || t->dim() != 1 || 2 * t->size(0) > head_dim ||
+      (t->requires_grad() && c10::GradMode::is_enabled()))
+    return false;
+  *data = t->const_data_ptr<float>();
+  *rotary = 2 * t->size(0);
+  return true;
+}
+
+bool whole_numbers(const Tensor* t, const c10::Device& dev) {
+  return t && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && t->device() == dev;
+}
+
+// rotary(q, k or None, positions, inv_freq, interleaved, factor, inverse) -> (status, q', k') or None
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 7)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    if (modes_active() || !THPVariable_CheckExact(a[0])) Py_RETURN_NONE;
+    const int64_t dims = THPVariable_Unpack(a[0]).dim();
+    if (dims != 3 && dims != 4) Py_RETURN_NONE;
+    const Tensor *q = viewed(a[0], dims), *k = a[1] == Py_None ? nullptr : viewed(a[1], dims);
+    if (!q || (a[1] != Py_None && !k) || !THPVariable_CheckExact(a[2])) Py_RETURN_NONE;
+    const c10::Device dev = q->device();
+    const Tensor* pos = &THPVariable_Unpack(a[2]);
+    if (!pos->defined() || !pos->is_cuda() || !plain_keys(*pos) || !whole_numbers(pos, dev)) Py_RETURN_NONE;
+    // [B, H, D] is [B, H, 1, D], its positions [B] are [B, 1].
+    const int64_t b = q->size(0), hq = q->size(1), t = dims == 4 ? q->size(2) : 1, d = q->size(-1);
+    const int code = dtype_code(q->scalar_type());
+    if (code < 0 || b == 0 || t == 0 || hq == 0 || d == 0 || pos->dim() != dims - 2) Py_RETURN_NONE;
+    if (dims == 4 ? (pos->size(0) != b && pos->size(0) != 1) || pos->size(1) != t : pos->size(0) != b) Py_RETURN_NONE;
+    const int64_t hk = k ? k->size(1) : 0;
+    if (k && (k->scalar_type() != q->scalar_type() || k->device() != dev || k->size(0) != b ||
+              (dims == 4 && k->size(2) != t) || k->size(-1) != d))
+      Py_RETURN_NONE;
+    const float* freq = nullptr;
+    int64_t turning = 0;
+    int interleaved = 0, inverse = 0;
+    double factor = 0.0;
+    if (a[3] == Py_None || !frequencies(a[3], dev, d, &freq, &turning) || !truth(a[4], &interleaved) ||
+        !PyFloat_CheckExact(a[5]) || !number(a[5], 1.0, &factor) || !truth(a[6], &inverse))
+      Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    const auto opt = at::TensorOptions().dtype(q->scalar_type()).device(dev);
+    Tensor qo = at::empty(q->sizes(), opt), ko;
+    if (k) ko = at::empty(k->sizes(), opt);
+    if (!plain_keys(qo)) Py_RETURN_NONE;
+    const int64_t qs[3] = {q->stride(0), q->stride(1), dims == 4 ? q->stride(2) : 0};
+    const int64_t ks[3] = {k ? k->stride(0) : 0, k ? k->stride(1) : 0, k && dims == 4 ? k->stride(2) : 0};
+    const int64_t ps[2] = {dims == 4 && pos->size(0) == 1 ? 0 : pos->stride(0), dims == 4 ? pos->stride(1) : 0};
+    const void *pq = q->const_data_ptr(), *pk = k ? k->const_data_ptr() : nullptr, *pp = pos->const_data_ptr();
+    void *pqo = qo.mutable_data_ptr(), *pko = k ? ko.mutable_data_ptr() : nullptr;
+    const int long_pos = pos->scalar_type() == at::kLong;
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_rotary(pq, qs, pqo, hq, pk, ks, pko, hk, pp, long_pos, ps, freq, turning, b, t, d, code, interleaved,
+                  (float)factor, inverse, stream);
+    Py_END_ALLOW_THREADS;
+    if (!k) return Py_BuildValue("(iNO)", rc, THPVariable_Wrap(qo), Py_None);
+    return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(qo), THPVariable_Wrap(ko));
+  });
+}
+
+// The cache of a call: the address of its pgr_hh_cache_t, which the Python object holds.
+const pgr_hh_cache_t* cache_at(PyObject* o) {
+  return PyLong_CheckExact(o) ? static_cast<const pgr_hh_cache_t*>(PyLong_AsVoidPtr(o)) : nullptr;
+}
+
+// t is a [batch, heads, head_dim] token operand of the cache on device `index`.
+bool token(const Tensor* t, const pgr_hh_cache_t* c, int64_t heads, int64_t index) {
+  return t && dtype_code(t->scalar_type()) == c->dtype && t->device().index() == index &&
+         t->sizes() == at::IntArrayRef({c->batch, heads, c->head_dim});
+}
+
+// append(cache, device index, q, k, v, inv_freq or None, positions or None, interleaved, factor) -> (status, q')
+// or None
+PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 9)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const pgr_hh_cache_t* c = cache_at(a[0]);
+    int64_t index = 0;
+    if (modes_active() || !c || !integer(a[1], &index)) Py_RETURN_NONE;
+    const Tensor *q = viewed(a[2], 3), *k = viewed(a[3], 3), *v = viewed(a[4], 3);
+    if (!token(q, c, c->query_heads, index) || !token(k, c, c->kv_heads, index) || !token(v, c, c->kv_heads, index))
+      Py_RETURN_NONE;
+    const c10::Device dev = q->device();
+    const float* freq = nullptr;
+    int64_t turning = 0;
+    int interleaved = 0;
+    double factor = 0.0;
+    if (!frequencies(a[5], dev, c->head_dim, &freq, &turning) || !truth(a[7], &interleaved) ||
+        !PyFloat_CheckExact(a[8]) || !number(a[8], 1.0, &factor))
+      Py_RETURN_NONE;
+    const void* positions = nullptr;
+    int long_pos = 0;
+    if (a[6] != Py_None) {
+      const Tensor* pos = plain(a[6]);
+      if (!whole_numbers(pos, dev) || pos->sizes() != at::IntArrayRef({c->batch})) Py_RETURN_NONE;
+      positions = pos->const_data_ptr();
+      long_pos = pos->scalar_type() == at::kLong;
+    }
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    Tensor qo;
+    void* pqo = nullptr;
+    if (a[5] != Py_None) {
+      qo = at::empty(q->sizes(), at::TensorOptions().dtype(q->scalar_type()).device(dev));
+      if (!plain_keys(qo)) Py_RETURN_NONE;
+      pqo = qo.mutable_data_ptr();
+    }
+    const int64_t qs[2] = {q->stride(0), q->stride(1)}, ks[2] = {k->stride(0), k->stride(1)},
+                  vs[2] = {v->stride(0), v->stride(1)};
+    const void *pq = q->const_data_ptr(), *pk = k->const_data_ptr(), *pv = v->const_data_ptr();
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_append(c, pq, qs, pk, ks, pv, vs, pqo, positions, long_pos, freq, turning, interleaved, (float)factor,
+                  stream);
+    Py_END_ALLOW_THREADS;
+    if (!pqo) return Py_BuildValue("(iO)", rc, a[2]);
+    return Py_BuildValue("(iN)", rc, THPVariable_Wrap(qo));
+  });
+}
+
+// attend(cache, device index, workspace bytes, q, scale, softcap) -> (status, out) or None
+PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 6)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const pgr_hh_cache_t* c = cache_at(a[0]);
+    int64_t index = 0, bytes = 0;
+    if (modes_active() || !c || !integer(a[1], &index) || !integer(a[2], &bytes)) Py_RETURN_NONE;
+    const Tensor* q = viewed(a[3], 3);
+    double scale = 0.0, softcap = 0.0;
+    if (!token(q, c, c->query_heads, index) || !number(a[4], 1.0 / std::pow((double)c->head_dim, 0.5), &scale) ||
+        !number(a[5], 0.0, &softcap))
+      Py_RETURN_NONE;
+    const c10::Device dev = q->device();
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    Tensor out = at::empty(q->sizes(), at::TensorOptions().dtype(q->scalar_type()).device(dev));
+    if (!plain_keys(out)) Py_RETURN_NONE;
+    c10::DataPtr ws;
+    if (bytes > 0) ws = at::detail::getCUDAHooks().getCUDADeviceAllocator()->allocate((size_t)bytes);
+    const int64_t qs[2] = {q->stride(0), q->stride(1)};
+    const void* pq = q->const_data_ptr();
+    void* po = out.mutable_data_ptr();
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_attend(c, pq, qs, po, (float)scale, (float)softcap, ws.get(), (size_t)bytes, stream);
+    Py_END_ALLOW_THREADS;
+    return Py_BuildValue("(iN)", rc, THPVariable_Wrap(out));
+  });
+}
+
+// lo: None, or int32 [batch].
+bool first_columns(PyObject* o, const c10::Device& dev, int64_t batch, const int32_t** out) {
+  return mask(o, dev, {batch}, out);
+}
+
+// prompt_weights(q, k, lo or None, scale, softcap) -> (status, weights) or None
+PyObject* py_prompt_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 5)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    if (modes_active()) Py_RETURN_NONE;
+    const Tensor *q = viewed(a[0], 4), *k = viewed(a[1], 4);
+    if (!q || !k) Py_RETURN_NONE;
+    const c10::Device dev = q->device();
+    const int64_t b = q->size(0), hq = q->size(1), w = q->size(2), d = q->size(3), hkv = k->size(1), t = k->size(2);
+    const int code = dtype_code(q->scalar_type());
+    const int32_t* lo = nullptr;
+    double scale = 0.0, softcap = 0.0;
+    if (!shaped(k, q, {b, hkv, t, d}) || code < 0 || code == 2 || b == 0 || t == 0 ||
+        !first_columns(a[2], dev, b, &lo) || !number(a[3], 1.0 / std::pow((double)d, 0.5), &scale) ||
+        !number(a[4], 0.0, &softcap))
+      Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    const size_t bytes = g_prompt_weights_bytes(b, hq, hkv, t, w, d);
+    if (bytes == 0) Py_RETURN_NONE;  // refused: the general path says why
+    Tensor out = at::empty({b, hkv, t}, at::TensorOptions().dtype(at::kFloat).device(dev));
+    if (!plain_keys(out)) Py_RETURN_NONE;
+    const c10::DataPtr ws = at::detail::getCUDAHooks().getCUDADeviceAllocator()->allocate(bytes);
+    const int64_t qs[3] = {q->stride(0), q->stride(1), q->stride(2)}, ks[3] = {k->stride(0), k->stride(1), k->stride(2)};
+    const void *pq = q->const_data_ptr(), *pk = k->const_data_ptr();
+    float* po = f32(&out);
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_prompt_weights(pq, qs, pk, ks, lo, po, b, hq, hkv, t, w, d, code, (float)scale, (float)softcap, ws.get(),
+                          bytes, stream);
+    Py_END_ALLOW_THREADS;
+    return Py_BuildValue("(iN)", rc, THPVariable_Wrap(out));
+  });
+}
+
+// load_prompt(cache, device index, k, v, weights, lo or None) -> status or None
+PyObject* py_load_prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 6)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const pgr_hh_cache_t* c = cache_at(a[0]);
+    int64_t index = 0;
+    if (modes_active() || !c || !integer(a[1], &index)) Py_RETURN_NONE;
+    const Tensor *k = viewed(a[2], 4), *v = viewed(a[3], 4), *w = plain(a[4]);
+    if (!k || !v || dtype_code(k->scalar_type()) != c->dtype || k->device().index() != index) Py_RETURN_NONE;
+    const c10::Device dev = k->device();
+    const int64_t t = k->size(2);
+    const int32_t* lo = nullptr;
+    if (t == 0 || k->sizes() != at::IntArrayRef({c->batch, c->kv_heads, t, c->head_dim}) || !shaped(v, k, k->sizes()) ||
+        !is_f32(w, dev, {c->batch, c->kv_heads, t}) || (w->requires_grad() && c10::GradMode::is_enabled()) ||
+        !first_columns(a[5], dev, c->batch, &lo))
+      Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    const size_t bytes = g_load_prompt_bytes(c, t);
+    if (bytes == 0) Py_RETURN_NONE;
+    const c10::DataPtr ws = at::detail::getCUDAHooks().getCUDADeviceAllocator()->allocate(bytes);
+    const int64_t ks[3] = {k->stride(0), k->stride(1), k->stride(2)}, vs[3] = {v->stride(0), v->stride(1), v->stride(2)};
+    const void *pk = k->const_data_ptr(), *pv = v->const_data_ptr();
+    const float* pw = w->const_data_ptr<float>();
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_load_prompt(c, pk, ks, pv, vs, pw, lo, t, ws.get(), bytes, stream);
+    Py_END_ALLOW_THREADS;
+    return PyLong_FromLong(rc);
+  });
+}
+
+// bind_cache(rotary, append, attend, prompt_weights, its workspace size, load_prompt, its workspace size: addresses)
+PyObject* py_bind_cache(PyObject*, PyObject* args) {
+  unsigned long long p[7];
+  if (!PyArg_ParseTuple(args, "KKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6])) return nullptr;
+  auto set = [](auto& fn, unsigned long long addr) { fn = reinterpret_cast<std::decay_t<decltype(fn)>>(addr); };
+  set(g_rotary, p[0]);
+  set(g_append, p[1]);
+  set(g_attend, p[2]);
+  set(g_prompt_weights, p[3]);
+  set(g_prompt_weights_bytes, p[4]);
+  set(g_load_prompt, p[5]);
+  set(g_load_prompt_bytes, p[6]);
+  Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, nullptr},
     {"step", (PyCFunction)(void (*)(void))py_step, METH_FASTCALL, nullptr},
@@ -362,6 +646,12 @@ PyMethodDef methods[] = {
     {"fold_fixed_step", (PyCFunction)(void (*)(void))py_fold_fixed, METH_FASTCALL, nullptr},
     {"state_init", (PyCFunction)(void (*)(void))py_state_init, METH_FASTCALL, nullptr},
     {"finalize", (PyCFunction)(void (*)(void))py_finalize, METH_FASTCALL, nullptr},
+    {"bind_cache", py_bind_cache, METH_VARARGS, nullptr},
+    {"rotary", (PyCFunction)(void (*)(void))py_rotary, METH_FASTCALL, nullptr},
+    {"append", (PyCFunction)(void (*)(void))py_append, METH_FASTCALL, nullptr},
+    {"attend", (PyCFunction)(void (*)(void))py_attend, METH_FASTCALL, nullptr},
+    {"prompt_weights", (PyCFunction)(void (*)(void))py_prompt_weights, METH_FASTCALL, nullptr},
+    {"load_prompt", (PyCFunction)(void (*)(void))py_load_prompt, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -55,7 +55,21 @@ def bind_ops():
     names = ("workspace_bytes", "step", "stats_step", "accumulate_step", "fold_fixed_step", "state_init", "finalize")
     _pgr_ops.bind(*(ctypes.cast(getattr(lib(), "pgr_attn_" + n), ctypes.c_void_p).value for n in names), raw,
                   torch.OutOfMemoryError)
+    names = ("rotary", "hh_append", "hh_attend", "hh_prompt_weights", "hh_prompt_weights_workspace_bytes",
+             "hh_load_prompt", "hh_load_prompt_workspace_bytes")
+    _pgr_ops.bind_cache(*(ctypes.cast(getattr(lib(), "pgr_" + n), ctypes.c_void_p).value for n in names))
     return _pgr_ops
+
+
+_ops = None
+
+
+def ops():
+    """bind_ops() on the first call: for modules that are imported where _pgr_ops.so may be absent."""
+    global _ops
+    if _ops is None:
+        _ops = bind_ops()
+    return _ops
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

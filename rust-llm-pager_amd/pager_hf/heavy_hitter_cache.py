@@ -69,6 +69,10 @@ def prompt_attention_weights(
     strides, after the rotary embedding; causal. ``lo`` [B]: each row's first valid column (left
     padding); padded columns get 0 and padded queries give nothing. scale defaults to
     1/sqrt(head_dim); softcap None or 0.0 disables c*tanh(s/c)."""
+    done = N.ops().prompt_weights(q, k, lo, scale, softcap)
+    if done is not None:
+        N.nat.check(done[0], "prompt_attention_weights")
+        return done[1]
     _inference_only(q, k)
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"q and k must be [B, H, tokens, D], got {tuple(q.shape)} and {tuple(k.shape)}")
@@ -143,6 +147,7 @@ class HeavyHitterCache:
             code, keep_first, keep_recent,
         )
         self._ref = ctypes.byref(self._c)
+        self._address, self._index, self._ops = ctypes.addressof(self._c), device.index, N.ops()
         self._attend_bytes = N.lib().pgr_hh_attend_workspace_bytes(self._ref)
 
     # The kernels hold the buffers' addresses: they can be written to, not replaced.
@@ -173,6 +178,10 @@ class HeavyHitterCache:
         float32 (prompt_attention_weights). Row b's tokens are the columns from lo[b] on: all of them
         where they fit, else the first keep_first, the last keep_recent and the heaviest of the rest (the
         lowest column first among equals; NaN is the heaviest), in the order of their columns."""
+        done = self._ops.load_prompt(self._address, self._index, k, v, weights, lo)
+        if done is not None:
+            N.nat.check(done, "HeavyHitterCache.load_prompt")
+            return
         _inference_only(k, v, weights)
         if k.dim() != 4 or k.shape[0] != self.batch or k.shape[1] != self.num_kv_heads or k.shape[3] != self.head_dim:
             raise ValueError(f"k must have shape ({self.batch}, {self.num_kv_heads}, T, {self.head_dim}), got "
@@ -210,6 +219,10 @@ class HeavyHitterCache:
         ``inv_freq`` (rotary.rotary_frequencies) q [B, Hq, D] and k are turned as rotary_embedding turns them,
         at the row's number of tokens seen so far or at positions[b]; without it both are taken as they
         are and q is returned itself."""
+        done = self._ops.append(self._address, self._index, q, k, v, inv_freq, positions, interleaved, factor)
+        if done is not None:
+            N.nat.check(done[0], "HeavyHitterCache.append")
+            return done[1]
         _inference_only(q, k, v)
         q = self._token(q, self.num_query_heads, "q")
         k = self._token(k, self.num_kv_heads, "k")
@@ -240,6 +253,10 @@ class HeavyHitterCache:
         """Attention of q [B, Hq, D] over each row's tokens; their probabilities, summed over each KV
         head's query heads, are added to ``weights``. Returns [B, Hq, D]; zeros for an empty row. scale
         defaults to 1/sqrt(head_dim); softcap None or 0.0 disables c*tanh(s/c)."""
+        done = self._ops.attend(self._address, self._index, self._attend_bytes, q, scale, softcap)
+        if done is not None:
+            N.nat.check(done[0], "HeavyHitterCache.attend")
+            return done[1]
         _inference_only(q)
         q = self._token(q, self.num_query_heads, "q")
         out = torch.empty((self.batch, self.num_query_heads, self.head_dim), dtype=self.dtype, device=self.device)

@@ -151,6 +151,10 @@ def rotary_embedding(
     positions [B, T] or [1, T]; or, one token per row, q [B, Hq, D], k [B, Hk, D] and positions [B].
     The pairs are (i, i + len(inv_freq)), or (2i, 2i + 1) with ``interleaved``; ``factor`` scales the
     turned dims (rotary_frequencies' second result). New contiguous tensors are returned."""
+    done = N.ops().rotary(q, k, positions, inv_freq, interleaved, factor, inverse)
+    if done is not None:
+        N.nat.check(done[0], "rotary_embedding")
+        return done[1], done[2]
     single = q.dim() == 3
     if q.dim() not in (3, 4):
         raise ValueError(f"q must be [B, H, T, D] or [B, H, D], got {tuple(q.shape)}")

@@ -457,3 +457,94 @@ def test_two_caches_on_two_streams():
         assert torch.equal(a, b)
     for (a, c), _, _ in runs:
         _same(a, _state(c))
+
+
+# ---- the two call paths ----------------------------------------------------------------------------
+class _General:
+    """_pgr_ops that hands every call to the general path."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def _forms():
+    g = torch.Generator().manual_seed(60)
+    b, hq, hkv, d, t = 3, 6, 2, 64, 90
+    a = dict(q4=torch.randn(b, hq, t, d, generator=g).half().cuda(), k4=torch.randn(b, hkv, t, d, generator=g).half().cuda(),
+             v4=torch.randn(b, hkv, t, d, generator=g).half().cuda(), q=torch.randn(b, hq, d, generator=g).half().cuda(),
+             k=torch.randn(b, hkv, d, generator=g).half().cuda(), v=torch.randn(b, hkv, d, generator=g).half().cuda(),
+             pos=torch.arange(t).repeat(b, 1).cuda(), one=torch.tensor([3, 900, 41]).cuda(), lo=None, scale=None, softcap=None,
+             factor=1.0, interleaved=False)
+    yield "plain", a, 9
+    yield "masked, softcapped", dict(a, lo=torch.tensor([0, 5, 60], dtype=torch.int32).cuda(), softcap=9.0, scale=0.2), 9
+    yield "interleaved, int32 positions", dict(a, interleaved=True, factor=1.5, pos=a["pos"].int(), one=a["one"].int()), 9
+    yield "shared positions, none for the step", dict(a, pos=a["pos"][:1], one=None), 9
+    yield "transposed", dict(a, **{n: a[n].transpose(1, 2).contiguous().transpose(1, 2) for n in ("q4", "k4", "v4")}), 9
+    yield "lists and integers", dict(a, lo=[0, 5, 60], scale=1, softcap=30, factor=2), None
+    yield "strided head_dim", dict(a, **{n: a[n].transpose(-1, -2).contiguous().transpose(-1, -2) for n in ("q4", "k", "q")}), None
+    yield "64-bit lo", dict(a, lo=torch.tensor([0, 5, 60]).cuda()), None
+    yield "parameters", dict(a, q=torch.nn.Parameter(a["q"].clone()), k4=torch.nn.Parameter(a["k4"].clone())), None
+
+
+def test_both_call_paths_agree(monkeypatch):
+    from pager_hf import _native as N
+
+    inv, _ = rotary_frequencies(32, device="cuda")
+
+    class Counting:
+        def __init__(self):
+            self.taken = 0
+
+        def __getattr__(self, name):
+            def call(*args):
+                got = getattr(ops, name)(*args)
+                self.taken += got is not None
+                return got
+            return call
+
+    ops = N.ops()
+    for name, a, taken in _forms():
+        print(f"call path: {name}", flush=True)
+        got = []
+        count = Counting()
+        for path in (count, _General()):
+            monkeypatch.setattr(N, "_ops", path)
+            with torch.no_grad():
+                cache = HeavyHitterCache(3, 6, 2, 48, 64, torch.float16, "cuda", keep_recent=8)
+                out = list(rotary_embedding(a["q4"], a["k4"], a["pos"], inv, interleaved=a["interleaved"], factor=a["factor"],
+                                            inverse=True))
+                out += rotary_embedding(a["q"], a["k"], a["one"] if a["one"] is not None else a["pos"][0, :3], inv)
+                w = prompt_attention_weights(a["q4"][:, :, -7:], a["k4"], lo=a["lo"], scale=a["scale"], softcap=a["softcap"])
+                cache.load_prompt(a["k4"], a["v4"], w, lo=a["lo"])
+                turned = cache.append(a["q"], a["k"], a["v"], inv, positions=a["one"], interleaved=a["interleaved"],
+                                      factor=a["factor"])
+                out += [w, turned, cache.attend(turned, scale=a["scale"], softcap=a["softcap"])]
+                same = cache.append(a["q"], a["k"], a["v"])
+                assert same is a["q"] or torch.equal(same, a["q"])
+                out.append(cache.attend(a["q"]))
+                rotary_embedding(a["q"], None, a["pos"][0, :3], inv)
+            got.append(out + [getattr(cache, n) for n in STATE])
+        for x, y in zip(*got):
+            assert x.dtype == y.dtype and torch.equal(x, y), name
+        # the calls above: three of rotary_embedding, two appends, two attends, weights, load
+        assert taken is None or count.taken == taken, (name, count.taken)
+
+
+def test_gradients_are_refused():
+    from pager_hf import _native as N
+
+    assert N.ops() is not None
+    cache = HeavyHitterCache(1, 2, 1, 48, 32, torch.float16, "cuda")
+    q, k = torch.zeros(1, 2, 32, device="cuda").half(), torch.zeros(1, 1, 32, device="cuda").half()
+    w = torch.zeros(1, 1, 5, device="cuda", requires_grad=True)
+    k4 = torch.zeros(1, 1, 5, 32, device="cuda").half()
+    inv, _ = rotary_frequencies(32, device="cuda")
+    for bad in (lambda: cache.attend(q.clone().requires_grad_()), lambda: cache.append(q, k.clone().requires_grad_(), k),
+                lambda: cache.load_prompt(k4, k4, w), lambda: prompt_attention_weights(k4.clone().requires_grad_(), k4),
+                lambda: rotary_embedding(q, None, torch.zeros(1, dtype=torch.int64, device="cuda"), inv.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="gradient"):
+            bad()
+    assert not cache.seen.any()
+    with torch.inference_mode():
+        cache.attend(cache.append(q, k, k, inv))
+    assert int(cache.seen) == 1
