@@ -26,29 +26,35 @@ __device__ __forceinline__ uint64_t shuffle_xor(uint64_t x, int mask) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// Element i of a head's rotary part (or of its copied part) after the turn.
+// Element i of a head after the turn; cs, sn: the pairs' cosines and sines.
 template <class Ty>
-__device__ __forceinline__ float turned(const typename Ty::Raw* x, int i, const RotaryForm& f, int64_t pos) {
-  const float own = Ty::to_f(x[i]);
-  if (i >= 2 * f.half) return own;
+__device__ __forceinline__ typename Ty::Raw turned(const typename Ty::Raw* x, int i, const RotaryForm& f,
+                                                   const float* cs, const float* sn) {
+  if (i >= 2 * f.half) return x[i];
   const bool first = f.interleaved ? (i & 1) == 0 : i < f.half;
   const int pair = f.interleaved ? i >> 1 : (first ? i : i - f.half);
   const int mate = f.interleaved ? i ^ 1 : (first ? i + f.half : i - f.half);
-  float cs, sn;
-  turn(pos, f.inv_freq[pair], cs, sn);
-  cs *= f.factor;
-  sn *= f.factor * f.sign;
-  const float other = Ty::to_f(x[mate]);
-  return first ? turned_x(own, other, cs, sn) : turned_y(other, own, cs, sn);
+  const float own = Ty::to_f(x[i]), other = Ty::to_f(x[mate]);
+  return Ty::cvt(first ? turned_x(own, other, cs[pair], sn[pair]) : turned_y(other, own, cs[pair], sn[pair]));
 }
+
+typedef float f32x4_e __attribute__((ext_vector_type(4), aligned(4)));
+typedef int32_t i32x4_e __attribute__((ext_vector_type(4), aligned(4)));
 
 // One workgroup per row: the new token's slot (the next free one, or in a full row the lightest
 // token's that is neither among the first keep_first nor among the last keep_recent, the new one
 // counted), its turned key, its value, and the turned queries of the row's heads.
+//
+// Latency-bound: a full row's weights and orders are 8 bytes a slot. The first 4096 slots' are asked for
+// 16 bytes at a time before anything else, and the angles and queries are done under them. 512 rows
+// (64 x 8 KV heads, 32 heads, D 128), three quarters of them full with 4096 slots: 8.9 us (11.7 with one
+// slot a thread at a time and an angle per element); one row of 256 slots: 4.7 us, a launch.
 template <class Ty>
 __global__ __launch_bounds__(256) void hh_append_kernel(HHAppendLaunch a) {
   typedef typename Ty::Raw Raw;
+  constexpr int kAhead = 4;  // times 4 slots a thread
   __shared__ uint64_t best_s[4];
+  __shared__ float cs[128], sn[128];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const HHCache& c = a.c;
   const int64_t row = (int64_t)b * c.hkv + h;
@@ -58,15 +64,67 @@ __global__ __launch_bounds__(256) void hh_append_kernel(HHAppendLaunch a) {
   float* w = c.weights + row * c.capacity;
   int32_t* order = c.order + row * c.capacity;
 
+  // (A row of less than four slots is read one by one.)
+  const int groups = full ? c.capacity / 4 : 0;
+  f32x4_e wa[kAhead];
+  i32x4_e oa[kAhead];
+#pragma unroll
+  for (int x = 0; x < kAhead; ++x) {
+    const int i = 4 * min(tid + x * 256, groups - 1);
+    if (groups > 0) {
+      wa[x] = *reinterpret_cast<const f32x4_e*>(w + i);
+      oa[x] = *reinterpret_cast<const i32x4_e*>(order + i);
+    }
+  }
+
+  const int d = c.d, n_rep = c.hq / c.hkv;
+  const Raw* k = static_cast<const Raw*>(a.k) + b * a.ks.b + h * a.ks.h;
+  const Raw* v = static_cast<const Raw*>(a.v) + b * a.vs.b + h * a.vs.h;
+  if (tid < a.form.half) {
+    const int64_t pos = a.positions != nullptr ? load_position(a.positions, a.positions64, b) : (int64_t)seen;
+    float x, y;
+    turn(pos, a.form.inv_freq[tid], x, y);
+    cs[tid] = x * a.form.factor;
+    sn[tid] = y * (a.form.factor * a.form.sign);
+  }
+  __syncthreads();  // (also: every thread has read the row's length and number)
+  Raw k_new{}, v_new{};
+  if (tid < d) {
+    k_new = turned<Ty>(k, tid, a.form, cs, sn);
+    v_new = v[tid];
+  }
+  if (a.q_out != nullptr) {
+    Raw* qo = static_cast<Raw*>(a.q_out) + ((int64_t)b * c.hq + (int64_t)h * n_rep) * d;
+    const Raw* q = static_cast<const Raw*>(a.q) + b * a.qs.b + (int64_t)h * n_rep * a.qs.h;
+    for (int i = tid; i < n_rep * d; i += 256) {
+      const int r = i / d;
+      qo[i] = turned<Ty>(q + r * a.qs.h, i - r * d, a.form, cs, sn);
+    }
+  }
+
   int slot = length;
   if (full) {
-    uint64_t best = ~0ull;
     const int64_t recent = (int64_t)seen + 1 - c.keep_recent;
-    for (int i = tid; i < c.capacity; i += 256) {
-      const int32_t o = order[i];
+    uint64_t best = ~0ull;
+    auto look = [&](int i, float x, int32_t o) {
       const uint64_t held = o < c.keep_first || o >= recent;
-      best = min_u64(best, held << 63 | (uint64_t)weight_key(w[i]) << 31 | (uint64_t)i);
+      best = min_u64(best, held << 63 | (uint64_t)weight_key(x) << 31 | (uint64_t)i);
+    };
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+      if (tid + x * 256 >= groups) continue;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) look(4 * (tid + x * 256) + y, wa[x][y], oa[x][y]);
     }
+#pragma unroll 2
+    for (int g = tid + kAhead * 256; g < groups; g += 256) {
+      const f32x4_e x = *reinterpret_cast<const f32x4_e*>(w + 4 * g);
+      const i32x4_e o = *reinterpret_cast<const i32x4_e*>(order + 4 * g);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) look(4 * g + y, x[y], o[y]);
+    }
+    const int i = 4 * groups + tid;
+    if (i < c.capacity) look(i, w[i], order[i]);
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) best = min_u64(best, shuffle_xor(best, m));
     if ((tid & 63) == 0) best_s[tid >> 6] = best;
@@ -75,27 +133,12 @@ __global__ __launch_bounds__(256) void hh_append_kernel(HHAppendLaunch a) {
     slot = (int)(best & 0x7fffffffu);
   }
 
-  const int64_t pos =
-      a.positions != nullptr ? load_position(a.positions, a.positions64, b) : (int64_t)seen;
-  const int d = c.d, n_rep = c.hq / c.hkv;
-  const Raw* k = static_cast<const Raw*>(a.k) + b * a.ks.b + h * a.ks.h;
-  const Raw* v = static_cast<const Raw*>(a.v) + b * a.vs.b + h * a.vs.h;
-  Raw* ko = static_cast<Raw*>(c.keys) + (row * c.capacity + slot) * d;
-  Raw* vo = static_cast<Raw*>(c.values) + (row * c.capacity + slot) * d;
-  for (int i = tid; i < d; i += 256) {
-    ko[i] = a.form.inv_freq != nullptr ? Ty::cvt(turned<Ty>(k, i, a.form, pos)) : k[i];
-    vo[i] = v[i];
+  const int64_t to = (row * c.capacity + slot) * d;
+  if (tid < d) {
+    static_cast<Raw*>(c.keys)[to + tid] = k_new;
+    static_cast<Raw*>(c.values)[to + tid] = v_new;
   }
-  if (a.q_out != nullptr) {
-    Raw* qo = static_cast<Raw*>(a.q_out) + ((int64_t)b * c.hq + (int64_t)h * n_rep) * d;
-    for (int i = tid; i < n_rep * d; i += 256) {
-      const int r = i / d, e = i - r * d;
-      const Raw* q = static_cast<const Raw*>(a.q) + b * a.qs.b + ((int64_t)h * n_rep + r) * a.qs.h;
-      qo[i] = a.form.inv_freq != nullptr ? Ty::cvt(turned<Ty>(q, e, a.form, pos)) : q[e];
-    }
-  }
-  __syncthreads();  // every thread has read the row's state
-  if (tid == 0) {
+  if (tid == 0) {  // (in a full row every thread is past its reads: the barrier above)
     w[slot] = 0.f;
     order[slot] = seen;
     c.seen[row] = seen + 1;
@@ -377,8 +420,6 @@ __global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, At
     }
   }
 }
-
-typedef float f32x4_e __attribute__((ext_vector_type(4), aligned(4)));
 
 // Joins the splits. Workgroups x < n_rep of a row write the output of query head x; the others add
 // the probabilities of 1024 tokens each, summed over the row's heads in their order, to the weights.
