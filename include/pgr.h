@@ -172,7 +172,8 @@ int pgr_attn_finalize(const float* acc, const float* l, void* out, int64_t rows,
  * (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0. inverse != 0 turns by the negative
  * angle: the transposed map, which takes gradients back. positions [B, T] int32 or int64 with
  * strides (batch, token); inv_freq [rotary_dim / 2]. Outputs [B, H, T, D] contiguous, not
- * overlapping the inputs. k_heads (or q_heads) may be 0. dtype fp16, bf16 or fp32; any head_dim. */
+ * overlapping the inputs. k_heads (or q_heads) may be 0. dtype fp16, bf16 or fp32; any head_dim;
+ * batch * tokens * head_dim below 2^32. */
 int pgr_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_heads, const void* k,
                const int64_t* k_strides, void* k_out, int64_t k_heads, const void* positions, int positions_64bit,
                const int64_t* position_strides, const float* inv_freq, int64_t rotary_dim, int64_t batch,
@@ -181,7 +182,7 @@ int pgr_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_h
 
 /* The caller's buffers of a bounded cache, all on the device and contiguous; keys, values, weights
  * and order 16-byte aligned. fp16 or bf16; head_dim 16, 32, 64, 128 or 256; up to 16 query heads
- * per KV head; batch * kv_heads <= 65535. lengths[row] slots of a row hold tokens; a token's
+ * per KV head; batch * kv_heads <= 65535; capacity <= 2^26. lengths[row] slots of a row hold tokens; a token's
  * `order` counts the row's tokens from 0, and seen[row] is the next one's. Calls on one cache are
  * ordered by the caller (one stream, or events). */
 typedef struct pgr_hh_cache_s {
@@ -219,7 +220,8 @@ int pgr_hh_attend(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
  * window, D], k [B, Hkv, tokens, D] (strides: batch, head, token), weights [B, Hkv, tokens] written,
  * summed over the queries and over each KV head's query heads; causal. lo [B] (NULL: 0): the row's
  * first valid column (left padding): columns before it get 0, queries before it give nothing, and
- * what q and k hold there does not matter. */
+ * what q and k hold there does not matter. tokens <= 8388480, window * num_query_heads /
+ * num_kv_heads <= 2097120, batch * heads * tokens <= 2^31; head and token strides below 2^31. */
 size_t pgr_hh_prompt_weights_workspace_bytes(int64_t batch, int64_t num_query_heads, int64_t num_kv_heads,
                                              int64_t tokens, int64_t window, int64_t head_dim);
 int pgr_hh_prompt_weights(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -230,8 +232,8 @@ int pgr_hh_prompt_weights(const void* q, const int64_t* q_strides, const void* k
 /* Starts every row of the cache over with a prompt's tokens [lo, tokens): all of them where they
  * fit, else the first keep_first, the last keep_recent and the heaviest of those between (ties: the
  * lowest column; NaN is the heaviest), in the order of their columns. k, v [B, Hkv, tokens, D]
- * (strides: batch, head, token), weights [B, Hkv, tokens] contiguous. Slots past the new length are
- * left as they were. */
+ * (strides: batch, head, token), weights [B, Hkv, tokens] contiguous, tokens <= 2^26. Slots past the new
+ * length are left as they were. */
 size_t pgr_hh_load_prompt_workspace_bytes(const pgr_hh_cache_t* cache, int64_t tokens);
 int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t* k_strides, const void* v,
                        const int64_t* v_strides, const float* weights, const int32_t* lo, int64_t tokens,

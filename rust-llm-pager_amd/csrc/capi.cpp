@@ -299,8 +299,8 @@ int check_cache(const pgr_hh_cache_t* c) {
   if (c == nullptr) return set_err(pgr::kErrInvalid, "null cache");
   int rc = check_heads(c->batch, c->query_heads, c->kv_heads, c->head_dim, c->dtype);
   if (rc != pgr::kOk) return rc;
-  if (c->capacity <= 0 || c->capacity > ((int64_t)1 << 30))
-    return set_err(pgr::kErrInvalid, "capacity must be in [1, 2^30]");
+  if (c->capacity <= 0 || c->capacity > ((int64_t)1 << 26))
+    return set_err(pgr::kErrInvalid, "capacity must be in [1, 2^26]");
   if (c->keep_first < 0 || c->keep_recent < 1 || (int64_t)c->keep_first + c->keep_recent > c->capacity)
     return set_err(pgr::kErrInvalid, "need keep_first >= 0, keep_recent >= 1 and their sum within the capacity");
   if (c->batch > 0 && (!c->keys || !c->values || !c->weights || !c->order || !c->lengths || !c->seen))
@@ -388,6 +388,8 @@ int check_prompt(int64_t batch, int64_t hq, int64_t hkv, int64_t tokens, int64_t
   if (window < 0 || window > tokens) return set_err(pgr::kErrInvalid, "the window must be in [0, tokens]");
   if (window * (hq / hkv) > (int64_t)65535 * 32)
     return set_err(pgr::kErrInvalid, "window * query heads per KV head must not exceed 2097120");
+  if (batch > 0 && (batch * hkv * tokens > ((int64_t)1 << 31) || batch * hq * window > ((int64_t)1 << 31)))
+    return set_err(pgr::kErrInvalid, "batch * heads * tokens must not exceed 2^31");
   return pgr::kOk;
 }
 
@@ -1216,8 +1218,8 @@ int pgr_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_h
     int rc = check_rotary(inv_freq, rotary_dim, head_dim, factor);
     if (rc != pgr::kOk) return rc;
     if (q_heads > 65535 || k_heads > 65535 || batch > ((int64_t)1 << 30) || tokens > ((int64_t)1 << 30) ||
-        head_dim > 65536 || (batch > 0 && tokens > 0 && batch * tokens > ((int64_t)1 << 38) / head_dim))
-      return set_err(pgr::kErrInvalid, "shape exceeds the launch limits");
+        head_dim > 65536 || (batch > 0 && tokens > 0 && batch * tokens >= ((int64_t)1 << 32) / head_dim))
+      return set_err(pgr::kErrInvalid, "shape exceeds the launch limits (batch * tokens * head_dim below 2^32)");
     if (batch == 0 || tokens == 0 || q_heads + k_heads == 0) return pgr::kOk;
     if ((q_heads > 0 && (!q || !q_out || !q_strides)) || (k_heads > 0 && (!k || !k_out || !k_strides)))
       return set_err(pgr::kErrInvalid, "null tensor pointer");
@@ -1387,7 +1389,7 @@ int pgr_hh_prompt_weights(const void* q, const int64_t* q_strides, const void* k
 
 size_t pgr_hh_load_prompt_workspace_bytes(const pgr_hh_cache_t* cache, int64_t tokens) {
   try {
-    if (check_cache(cache) != pgr::kOk || tokens < 0 || tokens > ((int64_t)1 << 30)) return 0;
+    if (check_cache(cache) != pgr::kOk || tokens < 0 || tokens > ((int64_t)1 << 26)) return 0;
     return plan_load(cache, tokens).bytes;
   } catch (...) {
     exception_status();
@@ -1401,7 +1403,7 @@ int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t
   try {
     int rc = check_cache(cache);
     if (rc != pgr::kOk) return rc;
-    if (tokens < 0 || tokens > ((int64_t)1 << 30)) return set_err(pgr::kErrInvalid, "tokens must be in [0, 2^30]");
+    if (tokens < 0 || tokens > ((int64_t)1 << 26)) return set_err(pgr::kErrInvalid, "tokens must be in [0, 2^26]");
     if (cache->batch == 0) return pgr::kOk;
     if (tokens > 0 && (!k || !k_strides || !v || !v_strides || !weights))
       return set_err(pgr::kErrInvalid, "null tensor pointer");

@@ -107,7 +107,7 @@ class HeavyHitterCache:
     The buffers can be read (and written, by a program that knows what it does) as ``keys`` and
     ``values`` [B, Hkv, capacity, D], ``weights`` [B, Hkv, capacity] float32, ``order`` [B, Hkv, capacity]
     int32 (a slot's token, counted from the row's first valid one), ``lengths`` and ``seen`` [B, Hkv] int32
-    (slots in use, tokens seen so far). Slots from lengths on hold nothing."""
+    (slots in use, tokens seen so far). Slots from lengths on hold nothing (zeros at first)."""
 
     def __init__(self, batch: int, num_query_heads: int, num_kv_heads: int, capacity: int, head_dim: int,
                  dtype: torch.dtype, device: torch.device | str, *, keep_first: int = 4, keep_recent: int = 32):
@@ -127,13 +127,11 @@ class HeavyHitterCache:
             raise ValueError("batch * num_kv_heads must not exceed 65535")
         if keep_first < 0 or keep_recent < 1 or keep_first + keep_recent > capacity:
             raise ValueError("need keep_first >= 0, keep_recent >= 1 and their sum within the capacity")
-        if capacity > 1 << 30:
-            raise ValueError("capacity must not exceed 2^30")
+        if capacity > 1 << 26:
+            raise ValueError("capacity must not exceed 2^26")
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        self.batch, self.num_query_heads, self.num_kv_heads = batch, num_query_heads, num_kv_heads
-        self.capacity, self.head_dim, self.dtype, self.device = capacity, head_dim, dtype, device
-        self.keep_first, self.keep_recent = keep_first, keep_recent
+        self._dtype, self._device = dtype, device
         rows = (batch, num_kv_heads)
         self._keys = torch.zeros((*rows, capacity, head_dim), dtype=dtype, device=device)
         self._values = torch.zeros((*rows, capacity, head_dim), dtype=dtype, device=device)
@@ -150,7 +148,16 @@ class HeavyHitterCache:
         self._address, self._index, self._ops = ctypes.addressof(self._c), device.index, N.ops()
         self._attend_bytes = N.lib().pgr_hh_attend_workspace_bytes(self._ref)
 
-    # The kernels hold the buffers' addresses: they can be written to, not replaced.
+    # What the kernels go by is fixed with the cache: the buffers can be written to, not replaced.
+    batch = property(lambda self: self._c.batch)
+    num_query_heads = property(lambda self: self._c.query_heads)
+    num_kv_heads = property(lambda self: self._c.kv_heads)
+    capacity = property(lambda self: self._c.capacity)
+    head_dim = property(lambda self: self._c.head_dim)
+    keep_first = property(lambda self: self._c.keep_first)
+    keep_recent = property(lambda self: self._c.keep_recent)
+    dtype = property(lambda self: self._dtype)
+    device = property(lambda self: self._device)
     keys = property(lambda self: self._keys)
     values = property(lambda self: self._values)
     weights = property(lambda self: self._weights)

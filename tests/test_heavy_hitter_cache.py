@@ -22,7 +22,7 @@ BAD_CACHES = [
     (dict(batch=-1), nat.PGR_ERR_INVALID), (dict(query_heads=3), nat.PGR_ERR_INVALID),
     (dict(query_heads=34), nat.PGR_ERR_UNSUPPORTED), (dict(head_dim=48), nat.PGR_ERR_UNSUPPORTED),
     (dict(dtype=2), nat.PGR_ERR_UNSUPPORTED), (dict(capacity=0), nat.PGR_ERR_INVALID),
-    (dict(capacity=(1 << 30) + 1), nat.PGR_ERR_INVALID), (dict(keep_first=-1), nat.PGR_ERR_INVALID),
+    (dict(capacity=(1 << 26) + 1), nat.PGR_ERR_INVALID), (dict(keep_first=-1), nat.PGR_ERR_INVALID),
     (dict(keep_recent=0), nat.PGR_ERR_INVALID), (dict(keep_first=60, keep_recent=5), nat.PGR_ERR_INVALID),
     (dict(seen=0), nat.PGR_ERR_INVALID), (dict(keys=264), nat.PGR_ERR_INVALID),
     (dict(batch=65536), nat.PGR_ERR_INVALID),
@@ -66,7 +66,8 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.pgr_hh_load_prompt(c, 16, s, 16, s, 16, None, 4, 256, need - 1, None) == cap
     bytes_of = lib.pgr_hh_prompt_weights_workspace_bytes
     assert bytes_of(1, 4, 2, 100, 10, 32) > 0
-    for bad in ((1, 4, 2, 100, 101, 32), (1, 4, 2, 100, -1, 32), (1, 3, 2, 100, 10, 32), (1, 4, 2, 100, 10, 40),
+    for bad in ((1, 4, 2, 8388481, 1, 32), (1, 32, 2, 200000, 131071, 32), (300, 32, 8, 1000000, 1, 32),
+                (1, 4, 2, 100, 101, 32), (1, 4, 2, 100, -1, 32), (1, 3, 2, 100, 10, 32), (1, 4, 2, 100, 10, 40),
                 (1, 34, 2, 100, 10, 32)):
         assert bytes_of(*bad) == 0
     run = lib.pgr_hh_prompt_weights
@@ -75,6 +76,8 @@ def test_c_entries_refuse_bad_arguments():
     assert run(16, s, 16, s, None, 16, 1, 4, 2, 100, 10, 32, 2, 1.0, 0.0, 256, 1 << 30, None) == nat.PGR_ERR_UNSUPPORTED
     assert run(16, s, 16, s, None, 16, 1, 4, 2, 100, 10, 32, 0, -1.0, 0.0, 256, 1 << 30, None) == inv
     assert run(16, s, 16, s, None, 16, 1, 4, 2, 100, 10, 32, 0, 1.0, 0.0, 256, 16, None) == cap
+    wide = (ctypes.c_int64 * 3)(1, 1 << 31, 1)
+    assert run(16, wide, 16, s, None, 16, 1, 4, 2, 100, 10, 32, 0, 1.0, 0.0, 256, 1 << 30, None) == inv
     assert run(None, s, 16, s, None, 16, 1, 4, 2, 100, 10, 32, 0, 1.0, 0.0, 256, 1 << 30, None) == inv
     assert run(16, s, 16, s, None, 16, 1, 4, 2, 0, 0, 32, 0, 1.0, 0.0, None, 0, None) == 0  # nothing to do
 

@@ -196,6 +196,19 @@ def test_append_without_rotation_returns_the_queries():
     assert torch.equal(cache.append(strided, k, v), strided)
 
 
+def test_what_the_kernels_go_by_is_fixed():
+    import copy
+
+    cache = HeavyHitterCache(2, 4, 2, 64, 32, torch.float16, "cuda", keep_first=3, keep_recent=5)
+    assert (cache.batch, cache.num_query_heads, cache.num_kv_heads, cache.capacity, cache.head_dim) == (2, 4, 2, 64, 32)
+    assert (cache.keep_first, cache.keep_recent, cache.dtype, cache.device) == (3, 5, torch.float16, torch.device("cuda", 0))
+    for name in ("batch", "capacity", "dtype", "device", *STATE):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name))
+    with pytest.raises((ValueError, TypeError)):  # a copy would hold the original's addresses
+        copy.deepcopy(cache)
+
+
 def test_a_cache_of_one_slot():
     cache = HeavyHitterCache(1, 1, 1, 1, 16, torch.float16, "cuda", keep_first=0, keep_recent=1)
     for n in range(3):
