@@ -89,6 +89,14 @@ __device__ __forceinline__ void turn(int64_t position, float inv_freq, float& cs
   sincospif(2.f * part, &sn, &cs);
 }
 
+// Registers loaded before a loop, complete here: otherwise the compiler, which counts outstanding loads
+// in their order, waits in the loop for whatever was asked for after them.
+template <int N>
+__device__ __forceinline__ void arrived(u32x4 (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(r[i]));
+}
+
 // The pair (x, y) turned, as fused multiply-adds with a float32 result of their own (the empty
 // statement keeps the conversion to fp16 from being fused into them, which rounds once instead of
 // twice): every kernel gets the same bits.

@@ -276,16 +276,16 @@ __global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, At
 #pragma unroll
       for (int i = 0; i < 4; ++i) load_v<D>(t.v[x][i], p + min(16 * x + 4 * g + i, most) * D, n);
   };
-  if (wave < tiles) {
-    fetch_k(wave);
-    fetch_v(wave);
-  }
-
   u32x4 q[T::KP];
 #pragma unroll
   for (int i = 0; i < T::KP; ++i) q[i] = u32x4{0u, 0u, 0u, 0u};
   if (real)
     load_pieces<D>(q, static_cast<const uint16_t*>(a.q) + b * a.qs.b + ((int64_t)h * n_rep + n) * a.qs.h, g);
+  if (wave < tiles) {
+    fetch_k(wave);
+    fetch_v(wave);
+  }
+  arrived(q);
 
   float m_run = kMinusInf, l_run = 0.f;
   f32x4 acc[D / 16];
@@ -309,19 +309,26 @@ __global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, At
   };
   auto fold = [&](f32x4 (&s)[2], int ti) {
     float p[8], top = kMinusInf;
+    if (sc.cap_log2 > 0.f) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+      for (int i = 0; i < 8; ++i) s[i / 4][i & 3] = sc.cap_log2 * tanhf(s[i / 4][i & 3] * sc.cap_scale);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool ok = ti * kTileTokens + 16 * x + 4 * g + i < tokens;
-        const float y = sc.cap_log2 > 0.f ? sc.cap_log2 * tanhf(s[x][i] * sc.cap_scale) : s[x][i] * sc.scale_log2;
-        s[x][i] = ok ? y : kMinusInf;
-        if (!ok) {
+      for (int x = 0; x < 2; ++x) s[x] *= sc.scale_log2;
+    }
+    if ((ti + 1) * kTileTokens > tokens) {  // uniform: the last tile, ragged
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (ti * kTileTokens + 16 * x + 4 * g + i < tokens) continue;
+          s[x][i] = kMinusInf;
 #pragma unroll
           for (int j = 0; j < T::VD; ++j) t.v[x][i][j] = 0u;
         }
-        top = fmaxf(top, s[x][i]);
-      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i / 4][i & 3]);
     const float m_new = fmaxf(m_run, max_g(top));
     const bool none = m_new == kMinusInf;
     if (__any(m_new > m_run)) {  // (otherwise the factor is 1)

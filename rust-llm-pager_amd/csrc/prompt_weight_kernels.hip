@@ -49,14 +49,14 @@ struct Stage {
   static constexpr int kStride = D + 8, kPieces = D / 8, kPer = kTile * kPieces / 256;
   u32x4 v[kPer];
 
-  // offset(i): element offset of row i from `base`; rows from `valid` on are zeros.
+  // offset(i): element offset of row i from `base`; rows from `valid` on repeat the last one (what they
+  // give is masked, or weighs nothing, or is not stored).
   template <class F>
   __device__ __forceinline__ void fetch(const uint16_t* base, int valid, F offset) {
 #pragma unroll
     for (int x = 0; x < kPer; ++x) {
       const int id = x * 256 + (int)threadIdx.x, i = id / kPieces, e = (id - i * kPieces) * 8;
-      v[x] = u32x4{0u, 0u, 0u, 0u};
-      if (valid >= kTile || i < valid) v[x] = *reinterpret_cast<const u32x4_e*>(base + offset(i) + e);
+      v[x] = *reinterpret_cast<const u32x4_e*>(base + offset(min(i, valid - 1)) + e);
     }
   }
   __device__ __forceinline__ void put(uint16_t* lds) const {
@@ -89,10 +89,7 @@ __device__ __forceinline__ void product(f32x16 (&s)[kN], const u32x4 (&rows)[D /
 template <int D>
 __device__ __forceinline__ void load_own(u32x4 (&r)[D / 16], const uint16_t* row, int half) {
 #pragma unroll
-  for (int c = 0; c < D / 16; ++c) {
-    r[c] = u32x4{0u, 0u, 0u, 0u};
-    if (row != nullptr) r[c] = *reinterpret_cast<const u32x4_e*>(row + 16 * c + 8 * half);
-  }
+  for (int c = 0; c < D / 16; ++c) r[c] = *reinterpret_cast<const u32x4_e*>(row + 16 * c + 8 * half);
 }
 
 // The sum of 16 values, as four chains: one chain would wait for each addition.
@@ -138,17 +135,17 @@ __global__ __launch_bounds__(256) void prompt_stats_kernel(PromptWeightLaunch a,
   const int wg_row = (int)(gridDim.z - 1 - blockIdx.z) * kRowWaves * kN * 32;
   const int wave_row = wg_row + (kRowWaves == 4 ? wave * kN * 32 : 0);
   u32x4 own[kN][D / 16];
-  int last[kN];  // the last column that the lane's row attends to (-1: no such row)
+  int last[kN];  // the last column that the lane's row attends to (past the last row: that one again)
 #pragma unroll
   for (int g = 0; g < kN; ++g) {
-    const int r = wave_row + g * 32 + j, i = div_rep(r, magic);
-    last[g] = r < rows ? a.tokens - a.window + i : -1;
-    load_own<D>(own[g], r < rows ? qb + (uint64_t)(r - i * n_rep) * q_h + (uint64_t)i * q_t : nullptr, half);
+    const int r = min(wave_row + g * 32 + j, rows - 1), i = div_rep(r, magic);
+    last[g] = a.tokens - a.window + i;
+    load_own<D>(own[g], qb + (uint64_t)(uint32_t)(r - i * n_rep) * q_h + (uint64_t)(uint32_t)i * q_t, half);
   }
   // The last keys that any row of the workgroup, any row of the wave, and every row of the wave attends to.
   auto last_of = [&](int r) { return a.tokens - a.window + div_rep(min(r, rows - 1), magic); };
   const int wg_last = last_of(wg_row + kRowWaves * kN * 32 - 1);
-  const int any = last_of(wave_row + kN * 32 - 1), every = a.tokens - a.window + div_rep(wave_row, magic);
+  const int any = last_of(wave_row + kN * 32 - 1), every = last_of(wave_row);
 
   // This split's tiles of [lo, wg_last].
   const int t_lo = lo / kTile, t_hi = wg_last / kTile + 1;
@@ -193,8 +190,10 @@ __global__ __launch_bounds__(256) void prompt_stats_kernel(PromptWeightLaunch a,
   };
   u32x4 keys[D / 16];
   const int sub0 = kRowWaves == 4 ? 0 : wave, at = j * S::kStride + 8 * half;
+  if (t_begin < t_end) fetch(t_begin);
+#pragma unroll
+  for (int g = 0; g < kN; ++g) arrived(own[g]);
   if (t_begin < t_end) {
-    fetch(t_begin);
     st.put(lds[0]);
     if (t_begin + 1 < t_end) fetch(t_begin + 1);
     __syncthreads();
@@ -312,7 +311,7 @@ __global__ __launch_bounds__(256) void prompt_sums_kernel(PromptWeightLaunch a, 
 #pragma unroll
   for (int g = 0; g < kN; ++g) {
     const int key = wave_key + g * 32 + j;
-    load_own<D>(own[g], key < a.tokens ? kb + key * a.ks.t : nullptr, half);
+    load_own<D>(own[g], kb + min(key, a.tokens - 1) * a.ks.t, half);
     sum[g] = 0.f;
     from[g] = key < lo || key >= a.tokens ? kNever : max(key - before, 0) * n_rep;
   }
@@ -355,8 +354,10 @@ __global__ __launch_bounds__(256) void prompt_sums_kernel(PromptWeightLaunch a, 
   };
   u32x4 q[D / 16];
   const int at = j * S::kStride + 8 * half;
+  if (t_begin < t_end) fetch(t_begin);
+#pragma unroll
+  for (int g = 0; g < kN; ++g) arrived(own[g]);
   if (t_begin < t_end) {
-    fetch(t_begin);
     put(0);
     if (t_begin + 1 < t_end) fetch(t_begin + 1);
     __syncthreads();
