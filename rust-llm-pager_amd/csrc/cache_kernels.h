@@ -60,7 +60,7 @@ hipError_t launch_hh_append(int dtype, const HHAppendLaunch& p, hipStream_t stre
 
 // Splits of a cache row that an attend call makes (0: one workgroup per row, no merge launch), and the
 // tokens of a row's scores (padded to whole tiles).
-int hh_attend_splits(int batch, int hkv, int capacity);
+int hh_attend_splits(int batch, int hkv, int capacity, int d);
 __host__ __device__ inline int64_t hh_attend_stride(int capacity) { return ((int64_t)capacity + 31) / 32 * 32; }
 
 struct HHAttendLaunch {

@@ -230,8 +230,10 @@ __device__ __forceinline__ int split_tiles(int length, int n_split) {
   return (tiles + n_split - 1) / n_split;
 }
 
-// Rows of up to kOneTokens slots: the workgroup holds the whole row, its scores in LDS, and finishes
-// it without a merge launch (256 tokens, 28/4 heads, D 128: 7.0 us instead of 5.1 + 4.8).
+// Rows of up to kOneTokens slots (half of that at head dim 256): the workgroup holds the whole row, its
+// scores in LDS, and finishes it without a merge launch. 28/4 heads, D 128, one row of 64 / 256 / 512
+// tokens: 4.8 / 6.6 / 8.4 us against 9.2 / 9.8 / 10.0 split; 32/8 heads, 64 and 128 rows of 512: 28.8 and
+// 55.3 against 37.7 and 65.4; at head dim 256 (8/1, 8 rows of 512) 14.7 against 12.1.
 constexpr int kOneTokens = 512;
 constexpr int kMostSplits = 1024;
 
@@ -519,7 +521,9 @@ __global__ __launch_bounds__(256) void hh_attend_merge_kernel(HHAttendLaunch a) 
 // its slot from the counts before it.
 //
 // Latency-bound: the weights are few bytes (256 KB a row at 65536 tokens), the passes and their barriers
-// many. Up to kSelShort tokens one workgroup per row does it all, its keys in registers. Longer rows are
+// many. Up to kSelShort tokens one workgroup per row does it all, its keys in registers (2 / 32 / 512 rows
+// of 8192 tokens, the copy of short records included: 11.4 / 12.9 / 31.7 us against 16.5 / 18.2 / 41.5 in
+// parts). Longer rows are
 // dealt out in parts of kSelPart tokens over three launches: the parts' counts of the top 11 bits; from
 // all of a row's counts the class of the last token, whose members go to the row's list; and from that
 // list (a hundredth of the tokens, if weights differ) the last key and each part's slots. 16 rows of
@@ -928,9 +932,9 @@ hipError_t launch_hh_append(int dtype, const HHAppendLaunch& p, hipStream_t stre
   return hipGetLastError();
 }
 
-int hh_attend_splits(int batch, int hkv, int capacity) {
+int hh_attend_splits(int batch, int hkv, int capacity, int d) {
   const int rows = batch * hkv;
-  if (capacity <= kOneTokens && rows <= 512) return 0;
+  if (capacity <= (d == 256 ? kOneTokens / 2 : kOneTokens)) return 0;
   const int most = (capacity + 4 * kTileTokens - 1) / (4 * kTileTokens);  // a tile for each wave
   int n = (2048 + rows - 1) / rows;
   if (n > most) n = most;

@@ -345,7 +345,7 @@ struct AttendPlan {
 
 AttendPlan plan_attend(const pgr_hh_cache_t* c) {
   AttendPlan p;
-  p.n_split = pgr::hh_attend_splits((int)c->batch, (int)c->kv_heads, (int)c->capacity);
+  p.n_split = pgr::hh_attend_splits((int)c->batch, (int)c->kv_heads, (int)c->capacity, (int)c->head_dim);
   if (p.n_split == 0) return p;  // no workspace
   const size_t heads = (size_t)(c->batch * c->query_heads), slots = heads * p.n_split;
   Parts w;

@@ -11,6 +11,18 @@
 //   sums        S[32 rows x 32 keys] = Q . K^T, the keys in registers, the rows through LDS: a lane
 //               holds 16 rows of one key and adds exp2(s - norm[row]) up, norm = m + log2(l).
 // Nothing is added by atomics: the same inputs give the same sums.
+//
+// Bound by the matrix cores, the vector unit and LDS together: a score costs 2 D flops, one exponential
+// (v_exp_f32, 8 cycles a wave) and two or three plain operations (4 cycles each), 544 and 590 cycles
+// a wave and 2048 scores at head dim 128, and 8 KB of operands from LDS, which two waves per SIMD only
+// partly overlap. 8192 tokens, all of them queries, 32/8 heads, D 128 (275 GF a sweep): 585 us a call,
+// 0.94 PFLOP/s over both sweeps where a large matrix product of the library reaches 1.27 (the first form of
+// these kernels: 2333 us). With parts taken out of the two sweeps (284 and 296 us then): no LDS operands 189
+// and 197, no products 213 and 221, no exponentials 268 and 280, no staging 255 and 243.
+// Where a step waits matters most: the operands of the next 32 rows are read under the fold of the last,
+// the next tile goes to the other LDS buffer under the last step, and the exponentials come 16 at a time
+// (one after the other each waited for its own). A window of few queries has few steps a workgroup and is
+// bound by latency: two rows of 4133 tokens and 32 queries, 28/4 heads, D 128: 9.6 + 2.3 + 10.1 us.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -468,7 +480,10 @@ PromptWeightPlan prompt_weight_plan(int batch, int hq, int hkv, int tokens, int 
   // 42 + 35 us at 65536 tokens and 64 queries, 32/4 heads).
   plan.groups = d == 128 && ceil_div(rows, 256) * bh * ceil_div(tokens, 2048) >= 512 ? 2 : 1;
   const int64_t own = 32 * plan.groups;
-  plan.row_waves = rows <= 2 * own ? 1 : 4;
+  // Rows that one wave holds are shared by the four, a quarter of the keys each: 4 rows a KV head, 4096
+  // tokens (32/8, D 128) 11.4 us against 13.1, 32768 tokens 41.1 against 44.6; 64 rows, two blocks so,
+  // 50.2 against 44.3.
+  plan.row_waves = rows <= own ? 1 : 4;
   auto parts = [](int64_t workgroups, int64_t tiles) {  // about 1536 workgroups, of two tiles or more
     int64_t n = (1536 + workgroups - 1) / workgroups;
     const int64_t most = (tiles + 1) / 2;

@@ -66,8 +66,9 @@ ATTEND = [
     (2, 28, 4, 128, 4133, [4133, 1025]),
     (1, 16, 1, 64, 16387, [16387]),
     (40, 16, 8, 64, 70, [i * 70 // 39 for i in range(40)]),
-    (65, 8, 8, 64, 300, [i * 300 // 64 for i in range(65)]),  # short rows, too many for one workgroup each
+    (65, 8, 8, 64, 300, [i * 300 // 64 for i in range(65)]),
     (2, 8, 1, 256, 1025, [1025, 0]),
+    (3, 8, 1, 256, 300, [300, 257, 0]),
     (1, 8, 4, 128, 512, [511]),
 ]
 
