@@ -107,6 +107,7 @@ struct PromptWeightPlan {
   int row_waves = 4;   // waves of a statistics workgroup with rows of their own (1 or 4)
   int key_splits = 1;  // statistics pass: parts of the prompt per block of queries
   int row_splits = 1;  // sums pass: parts of the queries per block of keys
+  bool norm_apart = true;  // the statistics' parts are joined by a launch of their own
 };
 PromptWeightPlan prompt_weight_plan(int batch, int hq, int hkv, int tokens, int window, int d);
 
