@@ -15,8 +15,8 @@
 // Bound by the matrix cores, the vector unit and LDS together: a score costs 2 D flops, one exponential
 // (v_exp_f32, 8 cycles a wave) and two or three plain operations (4 cycles each), 544 and 590 cycles
 // a wave and 2048 scores at head dim 128, and 8 KB of operands from LDS, which two waves per SIMD only
-// partly overlap. 8192 tokens, all of them queries, 32/8 heads, D 128 (275 GF a sweep): 585 us a call,
-// 0.94 PFLOP/s over both sweeps where a large matrix product of the library reaches 1.27 (the first form of
+// partly overlap. 8192 tokens, all of them queries, 32/8 heads, D 128 (275 GF a sweep): 590 us a call,
+// 0.93 PFLOP/s over both sweeps where a large matrix product of the library reaches 1.27 (the first form of
 // these kernels: 2333 us). With parts taken out of the two sweeps (284 and 296 us then): no LDS operands 189
 // and 197, no products 213 and 221, no exponentials 268 and 280, no staging 255 and 243.
 // Where a step waits matters most: the operands of the next 32 rows are read under the fold of the last,
@@ -507,8 +507,9 @@ PromptWeightPlan prompt_weight_plan(int batch, int hq, int hkv, int tokens, int 
   plan.row_splits = parts(ceil_div(tokens, 4 * own) * bh, ceil_div(rows, kTile));
   // Up to 8 parts of a row's statistics are joined by every workgroup of the sums for itself, without a
   // launch: 1000 tokens and 32 queries (32/8, D 128; 4 parts) 12.1 us against 14.3 apart; 17 parts (4133
-  // tokens, 28/4) 20.4 against 20.2, 64 and more (16384 tokens, 32/4, D 64) 22.8 against 17.2.
-  plan.norm_apart = plan.key_splits > 8;
+  // tokens, 28/4) 20.4 against 20.2, 64 and more (16384 tokens, 32/4, D 64) 22.8 against 17.2. Where a
+  // workgroup sums many tiles of rows (8192 queries: 602 us against 591), the launch is the smaller part.
+  plan.norm_apart = plan.key_splits > 8 || rows > 1024;
   return plan;
 }
 
