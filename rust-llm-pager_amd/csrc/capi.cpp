@@ -310,6 +310,16 @@ int check_cache(const pgr_hh_cache_t* c) {
   return pgr::kOk;
 }
 
+// Whether an operand starts inside one of the cache's buffers: the kernels read operands and write the
+// buffers in no order.
+bool in_cache(const pgr_hh_cache_t* c, const void* p) {
+  const size_t slots = (size_t)(c->batch * c->kv_heads) * (size_t)c->capacity, kv = slots * (size_t)c->head_dim * 2;
+  auto within = [p](const void* base, size_t bytes) {
+    return (uintptr_t)p >= (uintptr_t)base && (uintptr_t)p - (uintptr_t)base < bytes;
+  };
+  return p != nullptr && (within(c->keys, kv) || within(c->values, kv) || within(c->weights, slots * sizeof(float)));
+}
+
 pgr::HHCache cache_of(const pgr_hh_cache_t* c) {
   pgr::HHCache r;
   r.keys = c->keys;
@@ -1263,6 +1273,8 @@ int pgr_hh_append(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
     if (cache->batch == 0) return pgr::kOk;
     if (!k || !v || !k_strides || !v_strides || (q_out && (!q || !q_strides)))
       return set_err(pgr::kErrInvalid, "null tensor pointer");
+    if (in_cache(cache, k) || in_cache(cache, v) || (q_out && (in_cache(cache, q) || in_cache(cache, q_out))))
+      return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
     pgr::HHAppendLaunch L;
     L.c = cache_of(cache);
     L.k = k;
@@ -1304,6 +1316,8 @@ int pgr_hh_attend(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
     if (rc != pgr::kOk) return rc;
     if (cache->batch == 0) return pgr::kOk;
     if (!q || !q_strides || !out) return set_err(pgr::kErrInvalid, "null tensor pointer");
+    if (in_cache(cache, q) || in_cache(cache, out))
+      return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
     const AttendPlan p = plan_attend(cache);
     if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < p.bytes))
       return set_err(pgr::kErrCapacity, "workspace too small");
@@ -1407,6 +1421,8 @@ int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t
     if (cache->batch == 0) return pgr::kOk;
     if (tokens > 0 && (!k || !k_strides || !v || !v_strides || !weights))
       return set_err(pgr::kErrInvalid, "null tensor pointer");
+    if (tokens > 0 && (in_cache(cache, k) || in_cache(cache, v) || in_cache(cache, weights)))
+      return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
     const LoadPlan p = plan_load(cache, tokens);
     if (workspace == nullptr || workspace_bytes < p.bytes) return set_err(pgr::kErrCapacity, "workspace too small");
     if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");

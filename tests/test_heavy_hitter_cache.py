@@ -82,6 +82,22 @@ def test_c_entries_refuse_bad_arguments():
     assert run(16, s, 16, s, None, 16, 1, 4, 2, 0, 0, 32, 0, 1.0, 0.0, None, 0, None) == 0  # nothing to do
 
 
+def test_c_entries_refuse_operands_in_the_cache():
+    """keys, values and weights at addresses of their own: 1 x 2 rows of 64 slots, 32 dims."""
+    lib, inv = nat.load(), nat.PGR_ERR_INVALID
+    c = _cache(keys=1 << 20, values=2 << 20, weights=3 << 20, order=4 << 20, lengths=5 << 20, seen=6 << 20)
+    s = (ctypes.c_int64 * 3)(1, 1, 1)
+    kv = 2 * 64 * 32 * 2
+    for at in (1 << 20, (1 << 20) + kv - 2, (2 << 20) + 64, (3 << 20) + 4):
+        assert lib.pgr_hh_append(c, 16, s, at, s, 16, s, None, None, 0, None, 0, 0, 1.0, None) == inv
+        assert lib.pgr_hh_append(c, 16, s, 16, s, at, s, None, None, 0, None, 0, 0, 1.0, None) == inv
+        assert lib.pgr_hh_load_prompt(c, at, s, 16, s, 16, None, 4, 256, 1 << 30, None) == inv
+        assert lib.pgr_hh_load_prompt(c, 16, s, at, s, 16, None, 4, 256, 1 << 30, None) == inv
+        assert lib.pgr_hh_load_prompt(c, 16, s, 16, s, at, None, 4, 256, 1 << 30, None) == inv
+        assert lib.pgr_hh_attend(c, at, s, 16, 1.0, 0.0, None, 0, None) == inv
+        assert "own buffers" in nat.last_error()
+
+
 def test_python_refusals_need_no_gpu():
     def make(**over):
         a = dict(batch=1, num_query_heads=4, num_kv_heads=2, capacity=64, head_dim=32, dtype=torch.float16, device="cuda")

@@ -344,6 +344,9 @@ def test_load_prompt_refusals():
                      (lambda: cache.load_prompt(k, k, w[..., :9]), ValueError),
                      (lambda: cache.load_prompt(k, k, w.cpu()), ValueError),
                      (lambda: cache.load_prompt(k, k, w, lo=[0, 0]), ValueError),
+                     (lambda: cache.load_prompt(cache.keys, cache.values, cache.weights, lo=[3]), ValueError),
+                     (lambda: cache.append(torch.zeros(1, 4, 32, device="cuda").half(), cache.keys[:, :, 3], k[:, :, 0]),
+                      ValueError),
                      (lambda: cache.append(k[:, 0, :1], k[:, :, 0], k[:, :, 0]), ValueError),
                      (lambda: cache.append(torch.zeros(1, 4, 32, device="cuda"), k[:, :, 0], k[:, :, 0]), TypeError),
                      (lambda: cache.append(torch.zeros(1, 4, 32).half(), k[:, :, 0], k[:, :, 0]), ValueError),
