@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256) void prompt_stats_kernel(PromptWeightLaunch a,
         if (x + 3 < 15) top2 = fmaxf(fmaxf(top2, s[g][x + 2]), s[g][x + 3]);
       }
       top = fmaxf(fmaxf(top, top2), s[g][14]);
-      const float ref = decltype(masked)::value && top == kMinusInf ? 0.f : top * sc.c;
+      const float ref = top == kMinusInf ? 0.f : top * sc.c;  // (scores may be -inf without a mask)
       float p[16];
       exp_all(p, s[g], sc.c, [&](int) { return ref; });
       l[g] = fmaf(l[g], __builtin_amdgcn_exp2f(fmaf(m[g], sc.c, -ref)), sum16(p));

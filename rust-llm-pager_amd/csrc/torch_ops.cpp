@@ -5,9 +5,9 @@
 // Each function checks that its arguments are what the kernels take as they are (exact
 // torch.Tensor objects without functorch, functionalization or lazy-bit keys, one GPU, one
 // dtype, contiguous (rotary and cache operands: head_dim contiguous), matching shapes), allocates the
-// workspace or outputs from torch's current allocator, and calls the C entry point of libpgr.so. It returns the entry point's status, or
-// None where any check fails: the caller then runs its general Python path, which converts,
-// copies or refuses as it always has. So this file decides nothing but speed: checks in Python,
+// workspace or outputs from torch's current allocator, and calls the C entry point of libpgr.so. It
+// returns the entry point's status, or None where any check fails: the caller then runs its general
+// Python path, which converts, copies or refuses as it always has. So this file decides nothing but speed: checks in Python,
 // one attribute object at a time, and a ctypes call of 19 arguments held the GPU up. A call of one
 // query (init, fold, finalize; 28/4 heads, D 128, fp16, 64 tokens) 30.6 -> 16.8 us, 4133 tokens
 // the same; the two-pass run of 12 calls (32/4, D 64, batch 4, 8209 tokens) 151 -> 84.6 us.

@@ -167,8 +167,9 @@ class HeavyHitterCache:
 
     def reset(self) -> None:
         """Empties every row."""
-        self._lengths.zero_()
-        self._seen.zero_()
+        with torch.inference_mode():  # (the cache may have been made in it)
+            self._lengths.zero_()
+            self._seen.zero_()
 
     def _token(self, t: torch.Tensor, heads: int, name: str) -> torch.Tensor:
         if tuple(t.shape) != (self.batch, heads, self.head_dim):
@@ -230,7 +231,7 @@ class HeavyHitterCache:
         if done is not None:
             N.nat.check(done[0], "HeavyHitterCache.append")
             return done[1]
-        _inference_only(q, k, v)
+        _inference_only(q, k, v, inv_freq)
         q = self._token(q, self.num_query_heads, "q")
         k = self._token(k, self.num_kv_heads, "k")
         v = self._token(v, self.num_kv_heads, "v")

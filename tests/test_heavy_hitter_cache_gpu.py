@@ -210,6 +210,16 @@ def test_what_the_kernels_go_by_is_fixed():
         copy.deepcopy(cache)
 
 
+def test_a_cache_made_under_inference_mode_can_be_reset_outside():
+    with torch.inference_mode():
+        cache = HeavyHitterCache(1, 2, 1, 48, 32, torch.float16, "cuda")
+        k = torch.ones(1, 1, 32, device="cuda").half()
+        cache.append(torch.ones(1, 2, 32, device="cuda").half(), k, k)
+    assert int(cache.lengths) == 1
+    cache.reset()
+    assert int(cache.lengths) == 0 and int(cache.seen) == 0
+
+
 def test_a_cache_of_one_slot():
     cache = HeavyHitterCache(1, 1, 1, 1, 16, torch.float16, "cuda", keep_first=0, keep_recent=1)
     for n in range(3):
@@ -258,6 +268,30 @@ def test_prompt_weights(case, dtype, softcap):
                 qn = _np(q[i, h * (hq // hkv):(h + 1) * (hq // hkv)])
                 ref, bound = O.prompt_weights(qn, _np(k[i, h]), lo[i] if lo else 0, 1.0 / d**0.5, softcap)
                 _within(got[i, h], ref, bound, f"row {i} head {h}")
+
+
+@pytest.mark.parametrize("d", [16, 128, 256])
+@pytest.mark.parametrize("w", [3, 700])
+def test_prompt_weights_of_scores_of_minus_infinity(d, w):
+    """Keys whose every score is -inf weigh nothing, in whole tiles and beside others; no mask is involved."""
+    g = torch.Generator().manual_seed(12)
+    t, hq, hkv = 1500, 4, 2
+    q = torch.randn(1, hq, w, d, generator=g).to(torch.bfloat16)
+    k = torch.randn(1, hkv, t, d, generator=g).to(torch.bfloat16)
+    q[..., 0] = 1.0
+    gone = torch.zeros(t, dtype=torch.bool)
+    gone[:650], gone[701], gone[1408:1440] = True, True, True
+    k[:, :, gone, 0] = -float("inf")
+    got = prompt_attention_weights(q.cuda(), k.cuda())
+    assert not got[:, :, gone].any()
+    for h in range(hkv):
+        qn, ref, bound = _np(q[0, 2 * h:2 * h + 2]), np.zeros(t), np.zeros(t)
+        for i in range(w):
+            last = t - w + i
+            at = np.flatnonzero(~gone[:last + 1].numpy())
+            r, e = O.prompt_weights(qn[:, i:i + 1], _np(k[0, h])[at], 0, 1.0 / d**0.5, 0.0)
+            ref[at], bound[at] = ref[at] + r, bound[at] + e
+        _within(got[0, h], ref, bound + 2 * w * 2.0**-24 * ref, f"head {h}")  # (the sum over the queries)
 
 
 def test_prompt_weights_are_the_same_every_time():
@@ -557,6 +591,7 @@ def test_gradients_are_refused():
     k4 = torch.zeros(1, 1, 5, 32, device="cuda").half()
     inv, _ = rotary_frequencies(32, device="cuda")
     for bad in (lambda: cache.attend(q.clone().requires_grad_()), lambda: cache.append(q, k.clone().requires_grad_(), k),
+                lambda: cache.append(q, k, k, inv.clone().requires_grad_()),
                 lambda: cache.load_prompt(k4, k4, w), lambda: prompt_attention_weights(k4.clone().requires_grad_(), k4),
                 lambda: rotary_embedding(q, None, torch.zeros(1, dtype=torch.int64, device="cuda"), inv.clone().requires_grad_())):
         with pytest.raises(RuntimeError, match="gradient"):
