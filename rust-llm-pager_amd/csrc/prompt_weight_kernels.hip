@@ -25,6 +25,8 @@
 // bound by latency: two rows of 4133 tokens and 32 queries, 28/4 heads, D 128: 9.6 + 2.3 + 10.1 us.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cstdint>
 #include <type_traits>
 
 #include "cache_device.h"
@@ -59,24 +61,32 @@ __device__ __forceinline__ float raw_score(float s, const ScoreScale& sc) {
 template <int D>
 struct Stage {
   static constexpr int kStride = D + 8, kPieces = D / 8, kPer = kTile * kPieces / 256;
+  static constexpr int kRound = 256 / kPieces;  // rows that the workgroup reads at once
   u32x4 v[kPer];
 
+  __device__ __forceinline__ static int first_row() { return (int)threadIdx.x / kPieces; }
+  __device__ __forceinline__ static int element() { return (int)threadIdx.x % kPieces * 8; }
+
+  // A whole tile whose rounds lie `step` elements apart; own: the thread's piece of the first one. An
+  // addition a round instead of a division and two products a piece, which were a fifth of the vector
+  // instructions of the sums: 302 -> 295 us at 8192 tokens and queries (32/8 heads, D 128), 30.5 -> 29.4 at
+  // 65536 tokens and 64 queries (32/4, D 64). The keys' tiles have less to save: 297 with it and without.
+  __device__ __forceinline__ void fetch_even(const uint16_t* own, uint64_t step) {
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) v[x] = *reinterpret_cast<const u32x4_e*>(own + x * step);
+  }
   // offset(i): element offset of row i from `base`; rows from `valid` on repeat the last one (what they
   // give is masked, or weighs nothing, or is not stored).
   template <class F>
   __device__ __forceinline__ void fetch(const uint16_t* base, int valid, F offset) {
 #pragma unroll
-    for (int x = 0; x < kPer; ++x) {
-      const int id = x * 256 + (int)threadIdx.x, i = id / kPieces, e = (id - i * kPieces) * 8;
-      v[x] = *reinterpret_cast<const u32x4_e*>(base + offset(min(i, valid - 1)) + e);
-    }
+    for (int x = 0; x < kPer; ++x)
+      v[x] = *reinterpret_cast<const u32x4_e*>(base + offset(min(x * kRound + first_row(), valid - 1)) + element());
   }
   __device__ __forceinline__ void put(uint16_t* lds) const {
+    uint16_t* const to = lds + first_row() * kStride + element();
 #pragma unroll
-    for (int x = 0; x < kPer; ++x) {
-      const int id = x * 256 + (int)threadIdx.x, i = id / kPieces, e = (id - i * kPieces) * 8;
-      *reinterpret_cast<u32x4*>(lds + i * kStride + e) = v[x];
-    }
+    for (int x = 0; x < kPer; ++x) *reinterpret_cast<u32x4*>(to + x * kRound * kStride) = v[x];
   }
 };
 
@@ -340,12 +350,22 @@ __global__ __launch_bounds__(256) void prompt_sums_kernel(PromptWeightLaunch a, 
 
   S st;
   float nm_next = 0.f;
+  auto row_offset = [&](int r) {
+    const int i = div_rep(r, magic);
+    return (uint64_t)(uint32_t)(r - i * n_rep) * q_h + (uint64_t)(uint32_t)i * q_t;
+  };
+  // Rounds of whole queries lie evenly: heads that divide a round's rows.
+  const int round_queries = div_rep(S::kRound, magic);
+  const bool even = round_queries * n_rep == S::kRound;
+  const uint16_t* const mine = qb + row_offset(S::first_row()) + S::element();
   auto fetch = [&](int tile) {
     const int row0 = tile * kTile;
-    st.fetch(qb, rows - row0, [&](int i) {
-      const int qi = div_rep(row0 + i, magic);
-      return (uint64_t)(uint32_t)(row0 + i - qi * n_rep) * q_h + (uint64_t)(uint32_t)qi * q_t;
-    });
+    if (even && row0 + kTile <= rows) {
+      const uint64_t step = (uint64_t)(uint32_t)round_queries * q_t;
+      st.fetch_even(mine + (uint64_t)(uint32_t)(tile * S::kPer) * step, step);
+    } else {
+      st.fetch(qb, rows - row0, [&](int i) { return row_offset(row0 + i); });
+    }
     if (threadIdx.x < kTile) {
       const int r = min(row0 + (int)threadIdx.x, rows - 1);
       if (a.plan.norm_apart)
@@ -497,11 +517,24 @@ PromptWeightPlan prompt_weight_plan(int batch, int hq, int hkv, int tokens, int 
   // tokens (32/8, D 128) 11.4 us against 13.1, 32768 tokens 41.1 against 44.6; 64 rows, two blocks so,
   // 50.2 against 44.3.
   plan.row_waves = rows <= own ? 1 : 4;
-  auto parts = [](int64_t workgroups, int64_t tiles) {  // about 1536 workgroups, of two tiles or more
-    int64_t n = (1536 + workgroups - 1) / workgroups;
-    const int64_t most = (tiles + 1) / 2;
-    if (n > most) n = most;
-    return (int)(n < 1 ? 1 : n);
+  // Parts of two tiles or more. Where every part is as long as the others, the choice among whole rounds of
+  // the workgroups that the chip holds (by LDS) with the fewest tiles one after the other, half a tile
+  // for a workgroup's start: 65536 tokens and 64 queries (32/4, D 64), statistics in 32 / 48 / 64 / 96 / 128
+  // parts 36.6 / 33.6 / 31.4 / 33.8 / 31.4 us. Where the window is more than a quarter of the prompt the
+  // causal bound makes them unequal, and about 1536 workgroups, the longest first, fill up evenly.
+  const bool even = (int64_t)window * 4 <= tokens;
+  const int64_t slots = 256 * std::min<int64_t>(6, 160 * 1024 / (2 * kTile * (d + 8) * 2 + 2048));
+  auto parts = [&](int64_t workgroups, int64_t tiles) {
+    const int64_t most = std::max<int64_t>((tiles + 1) / 2, 1);
+    if (!even) return (int)std::min<int64_t>(most, (1536 + workgroups - 1) / workgroups);
+    int64_t best = 1, best_cost = INT64_MAX;
+    for (int64_t rounds = 1; rounds <= 8; ++rounds) {
+      const int64_t n = std::clamp<int64_t>(slots * rounds / workgroups, 1, most);
+      const int64_t per = (tiles + n - 1) / n, used = (tiles + per - 1) / per;
+      const int64_t cost = (workgroups * used + slots - 1) / slots * (2 * per + 1);
+      if (cost < best_cost) best = used, best_cost = cost;
+    }
+    return (int)best;
   };
   plan.key_splits = parts(ceil_div(rows, plan.row_waves * own) * bh, ceil_div(tokens, kTile));
   plan.row_splits = parts(ceil_div(tokens, 4 * own) * bh, ceil_div(rows, kTile));
