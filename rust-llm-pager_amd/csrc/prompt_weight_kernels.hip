@@ -15,8 +15,8 @@
 // Bound by the matrix cores, the vector unit and LDS together: a score costs 2 D flops, one exponential
 // (v_exp_f32, 8 cycles a wave) and two or three plain operations (4 cycles each), 544 and 590 cycles
 // a wave and 2048 scores at head dim 128, and 8 KB of operands from LDS, which two waves per SIMD only
-// partly overlap. 8192 tokens, all of them queries, 32/8 heads, D 128 (275 GF a sweep): 590 us a call,
-// 0.93 PFLOP/s over both sweeps where a large matrix product of the library reaches 1.27 (the first form of
+// partly overlap. 8192 tokens, all of them queries, 32/8 heads, D 128 (275 GF a sweep): 583 us a call,
+// 0.94 PFLOP/s over both sweeps where a large matrix product of the library reaches 1.27 (the first form of
 // these kernels: 2333 us). With parts taken out of the two sweeps (284 and 296 us then): no LDS operands 189
 // and 197, no products 213 and 221, no exponentials 268 and 280, no staging 255 and 243.
 // Where a step waits matters most: the operands of the next 32 rows are read under the fold of the last,
