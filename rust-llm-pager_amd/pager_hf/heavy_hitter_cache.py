@@ -133,12 +133,14 @@ class HeavyHitterCache:
             device = torch.device("cuda", torch.cuda.current_device())
         self._dtype, self._device = dtype, device
         rows = (batch, num_kv_heads)
-        self._keys = torch.zeros((*rows, capacity, head_dim), dtype=dtype, device=device)
-        self._values = torch.zeros((*rows, capacity, head_dim), dtype=dtype, device=device)
-        self._weights = torch.zeros((*rows, capacity), dtype=torch.float32, device=device)
-        self._order = torch.zeros((*rows, capacity), dtype=torch.int32, device=device)
-        self._lengths = torch.zeros(rows, dtype=torch.int32, device=device)
-        self._seen = torch.zeros(rows, dtype=torch.int32, device=device)
+        # Two allocations: what a token holds, and what is kept about it (each part on a 16-byte border).
+        self._keys, self._values = torch.zeros((2, *rows, capacity, head_dim), dtype=dtype, device=device).unbind(0)
+        slots, count = -(-batch * num_kv_heads * capacity // 4) * 4, -(-batch * num_kv_heads // 4) * 4
+        state = torch.zeros(2 * (slots + count), dtype=torch.int32, device=device)
+        weights, order, lengths, seen = state.split([slots, slots, count, count])
+        self._weights = weights.view(torch.float32)[: batch * num_kv_heads * capacity].view(*rows, capacity)
+        self._order = order[: batch * num_kv_heads * capacity].view(*rows, capacity)
+        self._lengths, self._seen = (x[: batch * num_kv_heads].view(rows) for x in (lengths, seen))
         self._c = N.nat.HHCache(
             self._keys.data_ptr(), self._values.data_ptr(), self._weights.data_ptr(), self._order.data_ptr(),
             self._lengths.data_ptr(), self._seen.data_ptr(), batch, num_query_heads, num_kv_heads, capacity, head_dim,
