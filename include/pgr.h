@@ -184,7 +184,8 @@ int pgr_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_h
  * and order 16-byte aligned. fp16 or bf16; head_dim 16, 32, 64, 128 or 256; up to 16 query heads
  * per KV head; batch * kv_heads <= 65535; capacity <= 2^26. lengths[row] slots of a row hold tokens; a token's
  * `order` counts the row's tokens from 0, and seen[row] is the next one's. Calls on one cache are
- * ordered by the caller (one stream, or events). Other operands must not lie in its buffers. */
+ * ordered by the caller (one stream, or events). Other operands must not lie in its buffers, in whole or in
+ * part: such a call is refused. */
 typedef struct pgr_hh_cache_s {
   void* keys;       /* [batch, kv_heads, capacity, head_dim] */
   void* values;     /* [batch, kv_heads, capacity, head_dim] */

@@ -310,14 +310,73 @@ int check_cache(const pgr_hh_cache_t* c) {
   return pgr::kOk;
 }
 
-// Whether an operand starts inside one of the cache's buffers: the kernels read operands and write the
-// buffers in no order.
-bool in_cache(const pgr_hh_cache_t* c, const void* p) {
-  const size_t slots = (size_t)(c->batch * c->kv_heads) * (size_t)c->capacity, kv = slots * (size_t)c->head_dim * 2;
-  auto within = [p](const void* base, size_t bytes) {
-    return (uintptr_t)p >= (uintptr_t)base && (uintptr_t)p - (uintptr_t)base < bytes;
-  };
-  return p != nullptr && (within(c->keys, kv) || within(c->values, kv) || within(c->weights, slots * sizeof(float)));
+// An operand of a cache call: rows of `row` bytes, whose outer dimensions (batch, heads, tokens) have the
+// sizes and the strides, in elements of `elem` bytes, given.
+struct Operand {
+  const void* p = nullptr;
+  int64_t row = 0;
+  int dims = 0;
+  int64_t size[3] = {};
+  const int64_t* stride = nullptr;
+  int64_t elem = 2;
+};
+
+Operand flat(const void* p, int64_t bytes) {
+  Operand x;
+  x.p = p;
+  x.row = bytes;
+  return x;
+}
+
+Operand heads_of(const pgr_hh_cache_t* c, const void* p, const int64_t* stride, int64_t heads, int64_t tokens = 0) {
+  Operand x = flat(p, c->head_dim * 2);
+  x.dims = tokens > 0 ? 3 : 2;
+  x.size[0] = c->batch;
+  x.size[1] = heads;
+  x.size[2] = tokens;
+  x.stride = stride;
+  return x;
+}
+
+// Whether some byte of x's dimensions from `dim` on, the first row at p, lies in [lo, hi). The bytes from the
+// first to the last are looked at first; dimension by dimension only where their gaps span the range.
+bool touches(const Operand& x, int dim, uintptr_t p, uintptr_t lo, uintptr_t hi) {
+  __int128 first = p, last = first + x.row;
+  for (int i = dim; i < x.dims; ++i) {
+    const __int128 span = (__int128)(x.size[i] - 1) * x.stride[i] * x.elem;
+    (span < 0 ? first : last) += span;
+  }
+  if (last <= (__int128)lo || first >= (__int128)hi) return false;
+  if (dim == x.dims) return true;
+  for (int64_t i = 0; i < x.size[dim]; ++i)
+    if (touches(x, dim + 1, p + (uintptr_t)(i * x.stride[dim] * x.elem), lo, hi)) return true;
+  return false;
+}
+
+// Whether an operand lies, in whole or in part, in one of the cache's buffers: the kernels read operands and
+// write the buffers in no order, in one workgroup per row.
+bool in_cache(const pgr_hh_cache_t* c, const Operand& x) {
+  if (x.p == nullptr) return false;
+  const size_t rows = (size_t)(c->batch * c->kv_heads), slots = rows * (size_t)c->capacity;
+  const size_t kv = slots * (size_t)c->head_dim * 2;
+  const struct {
+    const void* p;
+    size_t bytes;
+  } buffers[] = {{c->keys, kv},
+                 {c->values, kv},
+                 {c->weights, slots * sizeof(float)},
+                 {c->order, slots * sizeof(int32_t)},
+                 {c->lengths, rows * sizeof(int32_t)},
+                 {c->seen, rows * sizeof(int32_t)}};
+  for (const auto& b : buffers)
+    if (touches(x, 0, (uintptr_t)x.p, (uintptr_t)b.p, (uintptr_t)b.p + b.bytes)) return true;
+  return false;
+}
+
+template <class... Operands>
+int check_apart(const pgr_hh_cache_t* c, const Operands&... x) {
+  if ((in_cache(c, x) || ...)) return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
+  return pgr::kOk;
 }
 
 pgr::HHCache cache_of(const pgr_hh_cache_t* c) {
@@ -1273,8 +1332,12 @@ int pgr_hh_append(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
     if (cache->batch == 0) return pgr::kOk;
     if (!k || !v || !k_strides || !v_strides || (q_out && (!q || !q_strides)))
       return set_err(pgr::kErrInvalid, "null tensor pointer");
-    if (in_cache(cache, k) || in_cache(cache, v) || (q_out && (in_cache(cache, q) || in_cache(cache, q_out))))
-      return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
+    const int64_t turned = cache->batch * cache->query_heads * cache->head_dim * 2;
+    rc = check_apart(cache, heads_of(cache, k, k_strides, cache->kv_heads), heads_of(cache, v, v_strides, cache->kv_heads),
+                     heads_of(cache, q_out ? q : nullptr, q_strides, cache->query_heads), flat(q_out, turned),
+                     flat(positions, cache->batch * (positions_64bit ? 8 : 4)),
+                     flat(rotary_dim > 0 ? inv_freq : nullptr, rotary_dim / 2 * (int64_t)sizeof(float)));
+    if (rc != pgr::kOk) return rc;
     pgr::HHAppendLaunch L;
     L.c = cache_of(cache);
     L.k = k;
@@ -1316,12 +1379,13 @@ int pgr_hh_attend(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
     if (rc != pgr::kOk) return rc;
     if (cache->batch == 0) return pgr::kOk;
     if (!q || !q_strides || !out) return set_err(pgr::kErrInvalid, "null tensor pointer");
-    if (in_cache(cache, q) || in_cache(cache, out))
-      return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
     const AttendPlan p = plan_attend(cache);
     if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < p.bytes))
       return set_err(pgr::kErrCapacity, "workspace too small");
     if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");
+    rc = check_apart(cache, heads_of(cache, q, q_strides, cache->query_heads),
+                     flat(out, cache->batch * cache->query_heads * cache->head_dim * 2));
+    if (rc != pgr::kOk) return rc;
     char* w = static_cast<char*>(workspace);
     pgr::HHAttendLaunch L;
     L.c = cache_of(cache);
@@ -1421,8 +1485,13 @@ int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t
     if (cache->batch == 0) return pgr::kOk;
     if (tokens > 0 && (!k || !k_strides || !v || !v_strides || !weights))
       return set_err(pgr::kErrInvalid, "null tensor pointer");
-    if (tokens > 0 && (in_cache(cache, k) || in_cache(cache, v) || in_cache(cache, weights)))
-      return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
+    if (tokens > 0) {
+      rc = check_apart(cache, heads_of(cache, k, k_strides, cache->kv_heads, tokens),
+                       heads_of(cache, v, v_strides, cache->kv_heads, tokens),
+                       flat(weights, cache->batch * cache->kv_heads * tokens * (int64_t)sizeof(float)),
+                       flat(lo, cache->batch * (int64_t)sizeof(int32_t)));
+      if (rc != pgr::kOk) return rc;
+    }
     const LoadPlan p = plan_load(cache, tokens);
     if (workspace == nullptr || workspace_bytes < p.bytes) return set_err(pgr::kErrCapacity, "workspace too small");
     if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");

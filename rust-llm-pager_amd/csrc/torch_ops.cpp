@@ -468,6 +468,17 @@ bool token(const Tensor* t, const pgr_hh_cache_t* c, int64_t heads, int64_t inde
          t->sizes() == at::IntArrayRef({c->batch, heads, c->head_dim});
 }
 
+// Whether an index operand views the cache's own state, which a call changes while it reads the operand: the
+// general path copies it.
+bool in_state(const pgr_hh_cache_t* c, const void* p) {
+  const size_t rows = (size_t)(c->batch * c->kv_heads), slots = rows * (size_t)c->capacity;
+  auto within = [p](const void* base, size_t count) {
+    return (uintptr_t)p >= (uintptr_t)base && (uintptr_t)p - (uintptr_t)base < count * 4;
+  };
+  return p != nullptr && (within(c->seen, rows) || within(c->lengths, rows) || within(c->order, slots) ||
+                          within(c->weights, slots));
+}
+
 // append(cache, device index, q, k, v, inv_freq or None, positions or None, interleaved, factor) -> (status, q')
 // or None
 PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -493,6 +504,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const Tensor* pos = plain(a[6]);
       if (!whole_numbers(pos, dev) || pos->sizes() != at::IntArrayRef({c->batch})) Py_RETURN_NONE;
       positions = pos->const_data_ptr();
+      if (in_state(c, positions)) Py_RETURN_NONE;
       long_pos = pos->scalar_type() == at::kLong;
     }
     void* stream = nullptr;
@@ -604,7 +616,7 @@ PyObject* py_load_prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t* lo = nullptr;
     if (t == 0 || k->sizes() != at::IntArrayRef({c->batch, c->kv_heads, t, c->head_dim}) || !shaped(v, k, k->sizes()) ||
         !is_f32(w, dev, {c->batch, c->kv_heads, t}) || (w->requires_grad() && c10::GradMode::is_enabled()) ||
-        !first_columns(a[5], dev, c->batch, &lo))
+        !first_columns(a[5], dev, c->batch, &lo) || in_state(c, lo))
       Py_RETURN_NONE;
     void* stream = nullptr;
     if (!current_stream(dev, &stream)) return nullptr;

@@ -173,6 +173,11 @@ class HeavyHitterCache:
             self._lengths.zero_()
             self._seen.zero_()
 
+    def _apart(self, t: torch.Tensor | None) -> torch.Tensor | None:
+        """t, or a copy where it views the cache's own state, which a call changes while it reads t."""
+        own = t is not None and t.untyped_storage().data_ptr() == self._seen.untyped_storage().data_ptr()
+        return t.clone() if own else t
+
     def _token(self, t: torch.Tensor, heads: int, name: str) -> torch.Tensor:
         if tuple(t.shape) != (self.batch, heads, self.head_dim):
             raise ValueError(f"{name} must have shape {(self.batch, heads, self.head_dim)}, got {tuple(t.shape)}")
@@ -208,7 +213,7 @@ class HeavyHitterCache:
         for x in (k, v, weights):
             if x.device != self.device:
                 raise ValueError(f"tensors on different devices: {self.device} and {x.device}")
-        lo = _first_columns(lo, self.batch, self.device)
+        lo = self._apart(_first_columns(lo, self.batch, self.device))
         k, v, weights = _dense_last(k), _dense_last(v), weights.contiguous()
         nbytes = N.lib().pgr_hh_load_prompt_workspace_bytes(self._ref, t)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -246,7 +251,7 @@ class HeavyHitterCache:
             positions = _positions(positions, self.device)
             if tuple(positions.shape) != (self.batch,):
                 raise ValueError(f"positions must have shape ({self.batch},), got {tuple(positions.shape)}")
-            positions = positions.contiguous()
+            positions = self._apart(positions.contiguous())
         with _on(self.device):
             N.nat.check(
                 N.lib().pgr_hh_append(

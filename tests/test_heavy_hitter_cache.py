@@ -98,6 +98,74 @@ def test_c_entries_refuse_operands_in_the_cache():
         assert "own buffers" in nat.last_error()
 
 
+# The same cache: where each of its buffers begins and how many bytes it has.
+BUFFERS = dict(keys=(1 << 20, 8192), values=(2 << 20, 8192), weights=(3 << 20, 512), order=(4 << 20, 512),
+               lengths=(5 << 20, 8), seen=(6 << 20, 8))
+
+
+@pytest.mark.parametrize("name", list(BUFFERS))
+def test_c_entries_refuse_every_operand_in_every_buffer(name):
+    """Operands that begin in a buffer, end in it, or reach it with one of their rows; the index operands too,
+    which the workgroups of other rows read while a row's own workgroup changes the buffer."""
+    lib, inv = nat.load(), nat.PGR_ERR_INVALID
+    c = _cache(**{n: at for n, (at, _) in BUFFERS.items()})
+    s, far = (ctypes.c_int64 * 3)(1, 1, 1), 1 << 30
+    base, size = BUFFERS[name]
+
+    def append(q=far, k=far, v=far, q_out=far, positions=None, inv_freq=None, long=0, strides=s):
+        return lib.pgr_hh_append(c, q, strides, k, strides, v, strides, q_out, positions, long, inv_freq,
+                                 32 if inv_freq else 0, 0, 1.0, None)
+
+    def load(k=far, v=far, weights=far, lo=None, strides=s):
+        return lib.pgr_hh_load_prompt(c, k, strides, v, strides, weights, lo, 4, 256, 1 << 30, None)
+
+    def attend(q=far, out=far, strides=s):
+        return lib.pgr_hh_attend(c, q, strides, out, 1.0, 0.0, None, 0, None)
+
+    refused = []
+
+    def refuse(rc):
+        refused.append(rc == inv and "own buffers" in nat.last_error())
+
+    for at in (base, base + size - 4, base - 2):  # (every operand has more than two bytes)
+        refuse(append(k=at))
+        refuse(append(v=at))
+        refuse(append(q=at))
+        refuse(append(q_out=at))
+        refuse(append(positions=at))
+        refuse(append(positions=at, long=1))
+        refuse(append(inv_freq=at))
+        refuse(load(k=at))
+        refuse(load(v=at))
+        refuse(load(weights=at))
+        refuse(load(lo=at))
+        refuse(attend(q=at))
+        refuse(attend(out=at))
+    # The second head's row, 4096 elements behind or before the first.
+    for step in (4096, -4096):
+        apart = (ctypes.c_int64 * 3)(1, step, 1)
+        refuse(append(k=base - 2 * step, strides=apart))
+        refuse(load(v=base - 2 * step, strides=apart))
+        refuse(attend(q=base - 2 * step, strides=apart))
+    assert all(refused), refused
+
+
+def test_c_entries_take_operands_around_the_buffers():
+    """Rows whose gaps span the cache, operands that end where a buffer begins: past the checks of the operands,
+    so another error than theirs (no device here), or none."""
+    if torch.cuda.is_available():
+        pytest.skip("addresses without memory behind them: for hosts without a GPU")
+    lib, s = nat.load(), (ctypes.c_int64 * 3)(1, 1, 1)
+    c = _cache(**{n: at for n, (at, _) in BUFFERS.items()})
+    far = 1 << 30
+    spans = (ctypes.c_int64 * 3)(1, 8 << 20, 1)  # rows at 64 KB and, 16 MB on, past every buffer
+    for rc in (lib.pgr_hh_append(c, far, s, 1 << 16, spans, far, s, None, None, 0, None, 0, 0, 1.0, None),
+               lib.pgr_hh_append(c, far, s, far, s, far, s, None, (6 << 20) - 8, 1, None, 0, 0, 1.0, None),
+               lib.pgr_hh_load_prompt(c, 1 << 16, spans, far, s, far, (6 << 20) + 8, 4, 256, 1 << 30, None),
+               lib.pgr_hh_attend(c, far, s, (1 << 20) - 4 * 32 * 2, 1.0, 0.0, None, 0, None)):
+        assert rc not in (0, nat.PGR_ERR_INVALID)
+
+
 def test_python_refusals_need_no_gpu():
     def make(**over):
         a = dict(batch=1, num_query_heads=4, num_kv_heads=2, capacity=64, head_dim=32, dtype=torch.float16, device="cuda")

@@ -390,6 +390,29 @@ def test_load_prompt_refusals():
             bad()
 
 
+@pytest.mark.parametrize("batch", [1, 2])
+def test_index_operands_that_view_the_caches_state(batch):
+    """positions and lo may be the cache's own counters: they are taken as they were before the call."""
+    g = torch.Generator().manual_seed(51)
+    lengths = [5, 40][:batch]
+    inv, _ = rotary_frequencies(64, device="cuda")
+    q, k, v = (torch.randn(batch, h, 64, generator=g).half().cuda() for h in (64, 32, 32))
+    k4, v4 = (torch.randn(batch, 32, 200, 64, generator=g).half().cuda() for _ in range(2))
+    w = torch.rand(batch, 32, 200, generator=g).cuda()
+    got = []
+    for name in ("seen", "lengths", "order"):
+        for own in (True, False):
+            cache, _ = _filled(batch, 64, 32, 48, 64, torch.float16, lengths, 50, keep_recent=8)
+            view = getattr(cache, name).flatten(1)[:, 0]
+            out = [cache.append(q, k, v, inv, positions=view if own else view.clone())]
+            got.append(out + list(_state(cache).values()))
+            cache.load_prompt(k4, v4, w, lo=view if own else view.clone())
+            got[-1] += list(_state(cache).values())
+    for a, b in zip(got[::2], got[1::2]):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
 # ---- a run of them -------------------------------------------------------------------------------
 def test_prompt_then_decode():
     """A padded batch's prompt into the cache, then decode steps past its capacity: each operator
