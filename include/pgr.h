@@ -204,7 +204,8 @@ typedef struct pgr_hh_cache_s {
  * among the first keep_first nor among the last keep_recent tokens, the new one counted (ties: the
  * lowest slot; NaN is the heaviest). Its weight starts at 0. With inv_freq, k and q [B, Hq, D] are
  * turned first (pgr_rotary's forms) at positions[b], or at the row's `seen` with positions NULL;
- * q_out [B, Hq, D] contiguous receives q, turned or copied (NULL: q is not read). */
+ * q_out [B, Hq, D] contiguous receives q, turned or copied (NULL: q is not read); it must not overlap
+ * the other operands. */
 int pgr_hh_append(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_strides, const void* k,
                   const int64_t* k_strides, const void* v, const int64_t* v_strides, void* q_out,
                   const void* positions, int positions_64bit, const float* inv_freq, int64_t rotary_dim,
@@ -212,7 +213,8 @@ int pgr_hh_append(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
 
 /* out [B, Hq, D] contiguous = softmax(scale * q . K^T, softcapped with softcap > 0) V over the row's
  * slots, and weights[slot] += the probabilities, summed over the KV head's query heads. q strides:
- * batch, head. A row of length 0 gives zeros. */
+ * batch, head; out may be q itself where that is contiguous, and must not overlap it otherwise. A row of
+ * length 0 gives zeros. */
 size_t pgr_hh_attend_workspace_bytes(const pgr_hh_cache_t* cache);
 int pgr_hh_attend(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_strides, void* out, float scale,
                   float softcap, void* workspace, size_t workspace_bytes, void* stream);

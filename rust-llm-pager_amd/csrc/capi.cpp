@@ -379,6 +379,11 @@ int check_apart(const pgr_hh_cache_t* c, const Operands&... x) {
   return pgr::kOk;
 }
 
+// Whether x lies, in whole or in part, in an output of `bytes` contiguous bytes.
+bool overlaps(const Operand& x, const void* out, int64_t bytes) {
+  return x.p != nullptr && out != nullptr && touches(x, 0, (uintptr_t)x.p, (uintptr_t)out, (uintptr_t)out + bytes);
+}
+
 pgr::HHCache cache_of(const pgr_hh_cache_t* c) {
   pgr::HHCache r;
   r.keys = c->keys;
@@ -1333,11 +1338,14 @@ int pgr_hh_append(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
     if (!k || !v || !k_strides || !v_strides || (q_out && (!q || !q_strides)))
       return set_err(pgr::kErrInvalid, "null tensor pointer");
     const int64_t turned = cache->batch * cache->query_heads * cache->head_dim * 2;
-    rc = check_apart(cache, heads_of(cache, k, k_strides, cache->kv_heads), heads_of(cache, v, v_strides, cache->kv_heads),
-                     heads_of(cache, q_out ? q : nullptr, q_strides, cache->query_heads), flat(q_out, turned),
-                     flat(positions, cache->batch * (positions_64bit ? 8 : 4)),
-                     flat(rotary_dim > 0 ? inv_freq : nullptr, rotary_dim / 2 * (int64_t)sizeof(float)));
+    const Operand xq = heads_of(cache, q_out ? q : nullptr, q_strides, cache->query_heads),
+                  xk = heads_of(cache, k, k_strides, cache->kv_heads), xv = heads_of(cache, v, v_strides, cache->kv_heads),
+                  xp = flat(positions, cache->batch * (positions_64bit ? 8 : 4)),
+                  xf = flat(rotary_dim > 0 ? inv_freq : nullptr, rotary_dim / 2 * (int64_t)sizeof(float));
+    rc = check_apart(cache, xq, xk, xv, xp, xf, flat(q_out, turned));
     if (rc != pgr::kOk) return rc;
+    for (const Operand* x : {&xq, &xk, &xv, &xp, &xf})
+      if (overlaps(*x, q_out, turned)) return set_err(pgr::kErrInvalid, "q_out must not overlap the other operands");
     pgr::HHAppendLaunch L;
     L.c = cache_of(cache);
     L.k = k;
@@ -1383,9 +1391,14 @@ int pgr_hh_attend(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
     if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < p.bytes))
       return set_err(pgr::kErrCapacity, "workspace too small");
     if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");
-    rc = check_apart(cache, heads_of(cache, q, q_strides, cache->query_heads),
-                     flat(out, cache->batch * cache->query_heads * cache->head_dim * 2));
+    const Operand xq = heads_of(cache, q, q_strides, cache->query_heads);
+    const int64_t out_bytes = cache->batch * cache->query_heads * cache->head_dim * 2;
+    rc = check_apart(cache, xq, flat(out, out_bytes));
     if (rc != pgr::kOk) return rc;
+    const bool in_place = q == out && (cache->query_heads == 1 || q_strides[1] == cache->head_dim) &&
+                          (cache->batch == 1 || q_strides[0] == cache->query_heads * cache->head_dim);
+    if (!in_place && overlaps(xq, out, out_bytes))
+      return set_err(pgr::kErrInvalid, "out must not overlap q, except in place");
     char* w = static_cast<char*>(workspace);
     pgr::HHAttendLaunch L;
     L.c = cache_of(cache);

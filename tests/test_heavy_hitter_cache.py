@@ -166,6 +166,29 @@ def test_c_entries_take_operands_around_the_buffers():
         assert rc not in (0, nat.PGR_ERR_INVALID)
 
 
+def test_c_entries_refuse_outputs_over_their_inputs():
+    """append's threads read the partner of the element they write, and other heads' workgroups the rest; attend
+    in place (the same contiguous layout) reads before it writes."""
+    if torch.cuda.is_available():
+        pytest.skip("addresses without memory behind them: for hosts without a GPU")
+    lib, inv = nat.load(), nat.PGR_ERR_INVALID
+    c = _cache(**{n: at for n, (at, _) in BUFFERS.items()})
+    s, dense = (ctypes.c_int64 * 3)(1, 1, 1), (ctypes.c_int64 * 2)(128, 32)  # 4 query heads of 32
+    far, out = 1 << 30, 1 << 29
+
+    def append(q=far, k=far, v=far, positions=None, inv_freq=None, strides=dense):
+        return lib.pgr_hh_append(c, q, strides, k, s, v, s, out, positions, 0, inv_freq, 32 if inv_freq else 0, 0, 1.0, None)
+
+    for at in (out, out + 254, out - 2):
+        for rc in (append(q=at), append(k=at), append(v=at), append(positions=at), append(inv_freq=at, q=far)):
+            assert rc == inv and "overlap" in nat.last_error(), at
+    assert append(q=out - 256) not in (0, inv) and append(q=out + 256) not in (0, inv)
+    attend = lambda q, strides: lib.pgr_hh_attend(c, q, strides, out, 1.0, 0.0, None, 0, None)
+    for q, strides in ((out + 64, dense), (out - 64, dense), (out, (ctypes.c_int64 * 2)(128, 64))):
+        assert attend(q, strides) == inv and "overlap" in nat.last_error()
+    assert attend(out, dense) not in (0, inv) and attend(out + 256, dense) not in (0, inv)
+
+
 def test_python_refusals_need_no_gpu():
     def make(**over):
         a = dict(batch=1, num_query_heads=4, num_kv_heads=2, capacity=64, head_dim=32, dtype=torch.float16, device="cuda")
