@@ -332,16 +332,16 @@ __global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, At
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i / 4][i & 3]);
     const float m_new = fmaxf(m_run, max_g(top));
-    const bool none = m_new == kMinusInf;
+    const float ref = m_new == kMinusInf ? 0.f : m_new;  // (scores of -inf weigh nothing, those of NaN stay NaN)
     if (__any(m_new > m_run)) {  // (otherwise the factor is 1)
-      const float alpha = none ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - ref);
       l_run *= alpha;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) acc[j] *= alpha;
       m_run = m_new;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = none ? 0.f : __builtin_amdgcn_exp2f(s[i / 4][i & 3] - m_new);
+    for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(s[i / 4][i & 3] - ref);
     l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
     // P is rounded to the K/V type for the matrix cores, as in the framework's other decode kernels.
     const u32x4 pb = {Ty::pack(p[0], p[1]), Ty::pack(p[2], p[3]), Ty::pack(p[4], p[5]), Ty::pack(p[6], p[7])};
@@ -399,13 +399,12 @@ __global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, At
 #pragma unroll
     for (int w = 0; w < kW; ++w) m = fmaxf(m, sm_m[w][r]);
     float x = 0.f, l = 0.f;
-    if (m != kMinusInf) {
+    const float ref = m == kMinusInf ? 0.f : m;
 #pragma unroll
-      for (int w = 0; w < kW; ++w) {
-        const float f = __builtin_amdgcn_exp2f(sm_m[w][r] - m);
-        x += sm_acc[w][r][e] * f;
-        l += sm_l[w][r] * f;
-      }
+    for (int w = 0; w < kW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sm_m[w][r] - ref);
+      x += sm_acc[w][r][e] * f;
+      l += sm_l[w][r] * f;
     }
     if constexpr (kOne) {
       static_cast<uint16_t*>(a.out)[(row * n_rep + r) * D + e] = Ty::cvt(length > 0 ? x / l : 0.f);

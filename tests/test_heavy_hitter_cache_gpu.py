@@ -110,6 +110,24 @@ def test_attend_with_a_few_heavy_and_far_scores():
     _within(cache.weights[0, 0], new, nb, "weights")
 
 
+@pytest.mark.parametrize("d,capacity", [(64, 300), (64, 2000), (256, 200), (256, 900)])
+def test_attend_over_tokens_that_are_nan(d, capacity):
+    """Keys of NaN in a row's tokens make that row NaN, a whole tile of them and nothing else too; others stay."""
+    for first, last in ((64, 96), (0, 150), (37, 38), (0, capacity)):
+        cache, g = _filled(3, 4, 2, capacity, d, torch.bfloat16, [capacity] * 3, 13, keep_first=0, keep_recent=1)
+        before = _state(cache)
+        cache.keys[1, 0, first:last] = float("nan")
+        q = torch.randn(3, 4, d, generator=g).bfloat16().cuda()
+        out, weights = cache.attend(q), cache.weights.clone()
+        assert torch.isnan(out[1, :2]).all() and torch.isnan(weights[1, 0]).all(), (first, last)
+        cache.keys.copy_(before["keys"])
+        cache.weights.copy_(before["weights"])
+        want = cache.attend(q)
+        for i, h in ((0, 0), (0, 1), (1, 1), (2, 0), (2, 1)):
+            assert torch.equal(out[i, 2 * h:2 * h + 2], want[i, 2 * h:2 * h + 2])
+            assert torch.equal(weights[i, h], cache.weights[i, h])
+
+
 def test_attend_is_the_same_every_time():
     cache, g = _filled(2, 8, 2, 3000, 128, torch.bfloat16, [3000, 1234], 4)
     q = torch.randn(2, 8, 128, generator=g).bfloat16().cuda()
