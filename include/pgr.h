@@ -214,7 +214,7 @@ int pgr_hh_append(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
 /* out [B, Hq, D] contiguous = softmax(scale * q . K^T, softcapped with softcap > 0) V over the row's
  * slots, and weights[slot] += the probabilities, summed over the KV head's query heads. q strides:
  * batch, head; out may be q itself where that is contiguous, and must not overlap it otherwise. A row of
- * length 0 gives zeros. */
+ * length 0 gives zeros, as does a head whose scores are all -inf. */
 size_t pgr_hh_attend_workspace_bytes(const pgr_hh_cache_t* cache);
 int pgr_hh_attend(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_strides, void* out, float scale,
                   float softcap, void* workspace, size_t workspace_bytes, void* stream);

@@ -217,6 +217,12 @@ __device__ __forceinline__ float sum_g(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+// What a head's scores are taken against for their probabilities, in log2 units. +inf where nothing has weight
+// (no tokens, or scores of -inf only): the head then gives zeros, and nothing to the weights.
+__device__ __forceinline__ float norm_of(float m, float l) {
+  return l == 0.f ? -kMinusInf : m + __builtin_amdgcn_logf(l);
+}
+
 // Scores in log2 units: scale_log2 = scale * log2(e), or with a softcap cap * log2(e).
 struct AttendScale {
   float scale_log2, cap_scale, cap_log2;
@@ -407,8 +413,8 @@ __global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, At
       l += sm_l[w][r] * f;
     }
     if constexpr (kOne) {
-      static_cast<uint16_t*>(a.out)[(row * n_rep + r) * D + e] = Ty::cvt(length > 0 ? x / l : 0.f);
-      if (e == 0) norm_s[r] = m + __builtin_amdgcn_logf(l);
+      static_cast<uint16_t*>(a.out)[(row * n_rep + r) * D + e] = Ty::cvt(l == 0.f ? 0.f : x / l);
+      if (e == 0) norm_s[r] = norm_of(m, l);
     } else {
       a.pacc[part * D + i] = x;
       if (e == 0) {
@@ -479,7 +485,7 @@ __global__ __launch_bounds__(256) void hh_attend_merge_kernel(HHAttendLaunch a) 
     if (tid < d) {
       float y = 0.f;
       for (int k = 0; k < min(groups, used); ++k) y += sum_s[k * d + tid];
-      static_cast<uint16_t*>(a.out)[(row * n_rep + x) * d + tid] = Ty::cvt(used > 0 ? y / l : 0.f);
+      static_cast<uint16_t*>(a.out)[(row * n_rep + x) * d + tid] = Ty::cvt(l == 0.f ? 0.f : y / l);
     }
     return;
   }
@@ -488,7 +494,7 @@ __global__ __launch_bounds__(256) void hh_attend_merge_kernel(HHAttendLaunch a) 
   for (int r = wave; r < n_rep; r += 4) {
     float m, l;
     head_stats(r, m, l);
-    if (lane == 0) norm_s[r] = m + __builtin_amdgcn_logf(l);  // log2
+    if (lane == 0) norm_s[r] = norm_of(m, l);
   }
   const int t = first + 4 * tid;
   float* w = c.weights + row * c.capacity + t;

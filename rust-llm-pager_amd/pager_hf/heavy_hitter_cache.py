@@ -266,8 +266,9 @@ class HeavyHitterCache:
 
     def attend(self, q: torch.Tensor, *, scale: float | None = None, softcap: float | None = None) -> torch.Tensor:
         """Attention of q [B, Hq, D] over each row's tokens; their probabilities, summed over each KV
-        head's query heads, are added to ``weights``. Returns [B, Hq, D]; zeros for an empty row. scale
-        defaults to 1/sqrt(head_dim); softcap None or 0.0 disables c*tanh(s/c)."""
+        head's query heads, are added to ``weights``. Returns [B, Hq, D]; zeros for an empty row and
+        for a head whose scores are all -inf. scale defaults to 1/sqrt(head_dim); softcap None or 0.0
+        disables c*tanh(s/c)."""
         done = self._ops.attend(self._address, self._index, self._attend_bytes, q, scale, softcap)
         if done is not None:
             N.nat.check(done[0], "HeavyHitterCache.attend")

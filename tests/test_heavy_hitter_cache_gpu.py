@@ -110,6 +110,52 @@ def test_attend_with_a_few_heavy_and_far_scores():
     _within(cache.weights[0, 0], new, nb, "weights")
 
 
+@pytest.mark.parametrize("d,capacity", [(16, 400), (64, 300), (64, 2000), (256, 200), (256, 900)])
+def test_attend_with_scores_of_minus_infinity(d, capacity):
+    """Scores of -inf weigh nothing: a head that has no others gives zeros and no weight to any token, and takes
+    none from the other heads; tokens that have no others weigh nothing, in whole tiles and beside others."""
+    for lone in (True, False):
+        cache, g = _filled(2, 4, 1, capacity, d, torch.bfloat16, [capacity] * 2, 17, keep_first=0, keep_recent=1)
+        q = torch.randn(2, 4, d, generator=g).bfloat16()
+        q[..., 0] = 0.0
+        cache.keys[1, 0, :, 0] = -2.0**120
+        q[1, 1, 0] = 2.0**100  # the products are past float32, the other heads' are 0
+        if not lone:
+            q[1, :, 0] = 2.0**100
+        before = _state(cache)
+        out = cache.attend(q.cuda())
+        _same(cache, before, "keys", "values", "order", "lengths", "seen")
+        assert not out[1, 1].any()
+        if not lone:
+            assert not out[1].any()
+            assert torch.equal(cache.weights[1], before["weights"][1])
+        k, v, w, qn = _np(cache.keys), _np(cache.values), _np(before["weights"]), _np(q)
+        k[..., 0] = 0.0
+        for i, heads in ((0, [0, 1, 2, 3]), (1, [0, 2, 3])):
+            if i == 1 and not lone:
+                continue
+            ref, bound, new, new_bound = O.attend(qn[i, heads], k[i, 0], v[i, 0], w[i, 0], 1.0 / d**0.5, 0.0,
+                                                  STEP[torch.bfloat16])
+            _within(out[i, heads], ref, bound, f"out {i}")
+            _within(cache.weights[i, 0], new, new_bound, f"weights {i}")
+    # Tokens without weight beside others.
+    cache, g = _filled(1, 4, 1, capacity, d, torch.float16, [capacity], 18, keep_first=0, keep_recent=1)
+    q = torch.randn(1, 4, d, generator=g).half()
+    q[..., 0] = 1.0
+    gone = torch.zeros(capacity, dtype=torch.bool)
+    gone[:70], gone[75], gone[128:160] = True, True, True
+    cache.keys[0, 0, gone.cuda(), 0] = -float("inf")
+    w = _np(cache.weights)[0, 0]
+    out = cache.attend(q.cuda())
+    at = (~gone).numpy()
+    ref, bound, new, new_bound = O.attend(_np(q)[0], _np(cache.keys)[0, 0][at], _np(cache.values)[0, 0][at], w[at],
+                                          1.0 / d**0.5, 0.0, STEP[torch.float16])
+    _within(out[0], ref, bound, "out")
+    got = _np(cache.weights)[0, 0]
+    _within(got[at], new, new_bound, "weights")
+    assert np.array_equal(got[~at], w[~at])
+
+
 @pytest.mark.parametrize("d,capacity", [(64, 300), (64, 2000), (256, 200), (256, 900)])
 def test_attend_over_tokens_that_are_nan(d, capacity):
     """Keys of NaN in a row's tokens make that row NaN, a whole tile of them and nothing else too; others stay."""
