@@ -4,7 +4,7 @@ The decode paths here take q and k after the rotary embedding (as the reference'
 hand them over, paged_model.py:926-955). These functions make them from a projection's output, for
 callers that run a model's layers themselves::
 
-    inv_freq, factor = rotary_frequencies(head_dim, base=10000.0, device=device)
+    inv_freq, factor = rotary_frequencies(head_dim, scaling=config.rope_parameters, device=device)
     q, k = rotary_embedding(q, k, positions, inv_freq, factor=factor)
 
 The angle position * inv_freq[i] is taken in 64 bits: in 32 its error grows with the position (2^-7
@@ -25,10 +25,11 @@ from . import _native as N
 _CODES = {torch.float16: N.nat.DTYPE_F16, torch.bfloat16: N.nat.DTYPE_BF16, torch.float32: N.nat.DTYPE_F32}
 
 
-def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None,
+def rotary_frequencies(rotary_dim: int, base: float | None = None, scaling: dict | None = None,
                        device: torch.device | str | None = None) -> tuple[torch.Tensor, float]:
     """(inv_freq float32 [rotary_dim / 2], factor of cos and sin) of a model's rotary settings.
 
+    ``base`` is scaling's "rope_theta" where None, else 10000; both may be given if they agree.
     ``scaling`` (a config's rope_scaling / rope_parameters) is None or a dict whose "rope_type" is
 
     * "default": inv_freq[i] = base^(-2i / rotary_dim);
@@ -44,10 +45,14 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be a positive even number, got {rotary_dim}")
-    if not base > 0 or not math.isfinite(base):
-        raise ValueError(f"base must be positive, got {base}")
     scaling = scaling or {}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    theta = scaling.get("rope_theta")
+    if base is not None and theta is not None and float(base) != float(theta):
+        raise ValueError(f"base {base} differs from the settings' rope_theta {theta}")
+    base = float(base if base is not None else theta if theta is not None else 10000.0)
+    if not base > 0 or not math.isfinite(base):
+        raise ValueError(f"base (rope_theta) must be positive, got {base}")
     attention_factor = 1.0
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
 

@@ -80,6 +80,38 @@ def test_frequencies_match_the_models_own():
         assert abs(factor - got) < 1e-12
 
 
+def test_base_comes_from_the_settings():
+    """A config's rope_parameters hold the base as rope_theta."""
+    llama3 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+              "original_max_position_embeddings": 8192}
+    yarn = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
+    for s in ({"rope_type": "default"}, {"rope_type": "linear", "factor": 2.0}, {"rope_type": "ntk", "factor": 2.0}, llama3,
+              yarn):
+        want = rotary_frequencies(128, 500000.0, s)
+        for got in (rotary_frequencies(128, scaling=dict(s, rope_theta=500000)),
+                    rotary_frequencies(128, 500000.0, dict(s, rope_theta=500000.0))):
+            assert torch.equal(got[0], want[0]) and got[1] == want[1]
+        assert torch.equal(rotary_frequencies(128, scaling=s)[0], rotary_frequencies(128, 10000.0, s)[0])
+        with pytest.raises(ValueError, match="rope_theta"):
+            rotary_frequencies(128, 10000.0, dict(s, rope_theta=500000.0))
+    with pytest.raises(ValueError, match="rope_theta"):
+        rotary_frequencies(128, scaling={"rope_type": "default", "rope_theta": -1.0})
+
+
+def test_base_of_a_models_own_settings():
+    rope = pytest.importorskip("transformers.modeling_rope_utils")
+    from transformers import LlamaConfig
+
+    cfg = LlamaConfig(hidden_size=512, num_attention_heads=8, max_position_embeddings=8192,
+                      rope_parameters={"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+                                       "original_max_position_embeddings": 2048, "rope_theta": 500000.0})
+    want, factor = rope.ROPE_INIT_FUNCTIONS["llama3"](cfg, torch.device("cpu"))
+    inv, got = rotary_frequencies(64, scaling=cfg.rope_parameters)
+    # (the model's are float32 throughout: base, power, quotient and blend, a few roundings each)
+    np.testing.assert_allclose(inv.double().numpy(), want.double().numpy(), rtol=2.0**-19)
+    assert factor == got == 1.0
+
+
 def test_frequency_refusals():
     with pytest.raises(ValueError, match="even"):
         rotary_frequencies(63)
