@@ -39,7 +39,8 @@ def rotary_frequencies(rotary_dim: int, base: float | None = None, scaling: dict
     * "yarn": pairs that turn more than "beta_fast" (32) times within
       "original_max_position_embeddings" stay, those that turn less than "beta_slow" (1) times are
       divided by "factor", linear in the pair's index between; cos and sin are scaled by
-      "attention_factor" (0.1 ln(factor) + 1);
+      "attention_factor" (0.1 ln(factor) + 1, or with "mscale" and "mscale_all_dim" the ratio of
+      0.1 mscale ln(factor) + 1 and 0.1 mscale_all_dim ln(factor) + 1);
     * "llama3": wavelengths below original / "high_freq_factor" stay, those above original /
       "low_freq_factor" are divided by "factor", linear in original / wavelength between.
     """
@@ -87,10 +88,17 @@ def rotary_frequencies(rotary_dim: int, base: float | None = None, scaling: dict
             last += 0.001
         ramp = ((i / 2 - first) / (last - first)).clamp(0, 1)
         freq = freq * (1 - ramp) + freq / factor * ramp
+        scales = [name for name in ("mscale", "mscale_all_dim") if scaling.get(name) is not None]
+
+        def stretch(m):
+            return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+
         if scaling.get("attention_factor") is not None:
             attention_factor = setting("attention_factor")
+        elif len(scales) == 1:
+            raise ValueError(f"{scales[0]} needs the other of mscale and mscale_all_dim")
         else:
-            attention_factor = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+            attention_factor = stretch(setting("mscale")) / stretch(setting("mscale_all_dim")) if scales else stretch(1.0)
     elif kind == "llama3":
         factor, original = setting("factor"), setting("original_max_position_embeddings")
         low, high = setting("low_freq_factor"), setting("high_freq_factor")

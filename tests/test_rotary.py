@@ -112,6 +112,34 @@ def test_base_of_a_models_own_settings():
     assert factor == got == 1.0
 
 
+@pytest.mark.parametrize("mscale,all_dim", [(1.0, 1.0), (0.707, 0.707), (1.0, 0.8), (0.5, 1.25)])
+@pytest.mark.parametrize("factor", [40.0, 4.0, 1.0])
+def test_yarn_factor_of_two_scales(mscale, all_dim, factor):
+    """cos and sin are scaled by (0.1 mscale ln(factor) + 1) / (0.1 mscale_all_dim ln(factor) + 1)."""
+    cfg = {"rope_type": "yarn", "factor": factor, "original_max_position_embeddings": 4096, "mscale": mscale,
+           "mscale_all_dim": all_dim}
+    inv, got = rotary_frequencies(64, 10000.0, cfg)
+    want = (0.1 * mscale * math.log(factor) + 1) / (0.1 * all_dim * math.log(factor) + 1)
+    assert abs(got - want) < 1e-12
+    assert torch.equal(inv, rotary_frequencies(64, 10000.0, {k: v for k, v in cfg.items() if "mscale" not in k})[0])
+    assert rotary_frequencies(64, 10000.0, dict(cfg, attention_factor=1.5))[1] == 1.5
+    rope = pytest.importorskip("transformers.modeling_rope_utils")
+    from transformers import LlamaConfig
+
+    model = LlamaConfig(hidden_size=512, num_attention_heads=8, max_position_embeddings=8192,
+                        rope_parameters=dict(cfg, rope_theta=10000.0))
+    assert abs(rope.ROPE_INIT_FUNCTIONS["yarn"](model, torch.device("cpu"))[1] - got) < 1e-12
+
+
+def test_yarn_scale_refusals():
+    cfg = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096}
+    for name in ("mscale", "mscale_all_dim"):
+        with pytest.raises(ValueError, match="mscale"):
+            rotary_frequencies(64, scaling=dict(cfg, **{name: 0.7}))
+        with pytest.raises(ValueError, match="positive"):
+            rotary_frequencies(64, scaling=dict({**cfg, "mscale": 1.0, "mscale_all_dim": 1.0}, **{name: -1.0}))
+
+
 def test_frequency_refusals():
     with pytest.raises(ValueError, match="even"):
         rotary_frequencies(63)
