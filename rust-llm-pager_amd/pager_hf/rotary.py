@@ -25,6 +25,12 @@ from . import _native as N
 _CODES = {torch.float16: N.nat.DTYPE_F16, torch.bfloat16: N.nat.DTYPE_BF16, torch.float32: N.nat.DTYPE_F32}
 
 
+# What the rope types below read; a type passes over what another one reads.
+_SETTINGS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "factor", "original_max_position_embeddings",
+             "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim", "low_freq_factor",
+             "high_freq_factor"}
+
+
 def rotary_frequencies(rotary_dim: int, base: float | None = None, scaling: dict | None = None,
                        device: torch.device | str | None = None) -> tuple[torch.Tensor, float]:
     """(inv_freq float32 [rotary_dim / 2], factor of cos and sin) of a model's rotary settings.
@@ -43,11 +49,19 @@ def rotary_frequencies(rotary_dim: int, base: float | None = None, scaling: dict
       0.1 mscale ln(factor) + 1 and 0.1 mscale_all_dim ln(factor) + 1);
     * "llama3": wavelengths below original / "high_freq_factor" stay, those above original /
       "low_freq_factor" are divided by "factor", linear in original / wavelength between.
+
+    Entries that none of these reads raise NotImplementedError, and so does a "partial_rotary_factor" other
+    than 1: pass the dims that turn as rotary_dim, and the settings without it.
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be a positive even number, got {rotary_dim}")
     scaling = scaling or {}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    unread = sorted(name for name, value in scaling.items() if value is not None and name not in _SETTINGS)
+    if unread:
+        raise NotImplementedError(f"rope_type {kind!r} with settings that are not supported: {', '.join(unread)}")
+    if scaling.get("partial_rotary_factor") not in (None, 1.0):
+        raise NotImplementedError("partial_rotary_factor: pass the dims that turn as rotary_dim, without this entry")
     theta = scaling.get("rope_theta")
     if base is not None and theta is not None and float(base) != float(theta):
         raise ValueError(f"base {base} differs from the settings' rope_theta {theta}")

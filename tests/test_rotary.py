@@ -140,6 +140,23 @@ def test_yarn_scale_refusals():
             rotary_frequencies(64, scaling=dict({**cfg, "mscale": 1.0, "mscale_all_dim": 1.0}, **{name: -1.0}))
 
 
+def test_settings_that_are_not_read_are_refused():
+    """An entry that would change a model's angles and that no supported rope type reads."""
+    for s in ({"rope_type": "default", "mrope_section": [16, 24, 24]},
+              {"rope_type": "linear", "factor": 2.0, "short_factor": [1.0]},
+              {"full_attention": {"rope_type": "default", "rope_theta": 1e6}, "sliding_attention": {"rope_type": "default"}}):
+        with pytest.raises(NotImplementedError, match="mrope_section|short_factor|full_attention"):
+            rotary_frequencies(128, scaling=s)
+    # rotary_dim is the part that turns: whether the share is in it already cannot be seen here.
+    with pytest.raises(NotImplementedError, match="partial_rotary_factor"):
+        rotary_frequencies(128, scaling={"rope_type": "default", "partial_rotary_factor": 0.5})
+    # Entries that change nothing: absent ones, a whole share, what another rope type reads.
+    want = rotary_frequencies(128, 10000.0)[0]
+    for s in ({"rope_type": "default", "partial_rotary_factor": 1.0, "rope_theta": 10000.0},
+              {"rope_type": "default", "mrope_section": None, "factor": 4.0, "original_max_position_embeddings": 4096}):
+        assert torch.equal(rotary_frequencies(128, scaling=s)[0], want)
+
+
 def test_frequency_refusals():
     with pytest.raises(ValueError, match="even"):
         rotary_frequencies(63)
