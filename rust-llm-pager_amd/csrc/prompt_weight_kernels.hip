@@ -301,11 +301,12 @@ __device__ __forceinline__ float norm_of(float2 p) {
   return p.y == 0.f ? -kMinusInf : (p.x == kMinusInf ? 0.f : p.x) + __builtin_amdgcn_logf(p.y);
 }
 
-// The norms of 64 rows a workgroup, each wave a quarter of the splits.
+// The norms of 64 rows a workgroup, each wave a quarter of the splits. (Two grid dimensions: one ends at 2^32
+// threads, here 2^30 rows, and a launch past it runs too few workgroups without an error.)
 __global__ __launch_bounds__(256) void prompt_norm_kernel(PromptWeightLaunch a, int64_t n) {
   __shared__ float2 part[4][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 64 + lane;
   part[wave][lane] = join_stats(a.stats, n, i < n ? i : n - 1, a.plan.key_splits, wave, 4);
   __syncthreads();
   if (wave != 0 || i >= n) return;
@@ -467,7 +468,9 @@ hipError_t run(const PromptWeightLaunch& p, const ScoreScale& sc, hipStream_t st
   if (e != hipSuccess) return e;
   if (p.plan.norm_apart) {
     const int64_t n = (int64_t)bh * rows;
-    prompt_norm_kernel<<<(unsigned)((n + 63) / 64), 256, 0, stream>>>(p, n);
+    const int64_t blocks = (n + 63) / 64, most = 1 << 20;
+    const dim3 grid((unsigned)std::min(blocks, most), (unsigned)ceil_div(blocks, most));
+    prompt_norm_kernel<<<grid, 256, 0, stream>>>(p, n);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

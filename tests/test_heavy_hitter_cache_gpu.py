@@ -358,6 +358,20 @@ def test_prompt_weights_of_scores_of_minus_infinity(d, w):
         _within(got[0, h], ref, bound + 2 * w * 2.0**-24 * ref, f"head {h}")  # (the sum over the queries)
 
 
+def test_prompt_weights_of_more_than_2_to_the_30_query_rows():
+    """Within the stated limits, and more than one dimension of a launch holds at four threads a row. Every
+    batch row is the same one (expanded, so that the operands stay small)."""
+    b, hq, d, t = 65535, 16, 16, 1025
+    assert b * hq * t > 1 << 30
+    g = torch.Generator().manual_seed(13)
+    q = torch.randn(1, hq, t, d, generator=g).half().cuda()
+    k = torch.randn(1, 1, t, d, generator=g).half().cuda()
+    got = prompt_attention_weights(q.expand(b, hq, t, d), k.expand(b, 1, t, d))
+    ref, bound = O.prompt_weights(_np(q[0]), _np(k[0, 0]), 0, 0.25, 0.0)
+    _within(got[0, 0], ref, bound, "row 0")
+    assert torch.equal(got, got[:1].expand_as(got))
+
+
 def test_prompt_weights_are_the_same_every_time():
     g = torch.Generator().manual_seed(6)
     q = torch.randn(1, 8, 700, 64, generator=g).half().cuda()
