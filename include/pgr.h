@@ -173,7 +173,7 @@ int pgr_attn_finalize(const float* acc, const float* l, void* out, int64_t rows,
  * angle: the transposed map, which takes gradients back. positions [B, T] int32 or int64 with
  * strides (batch, token); inv_freq [rotary_dim / 2]. Outputs [B, H, T, D] contiguous, not
  * overlapping the inputs. k_heads (or q_heads) may be 0. dtype fp16, bf16 or fp32; any head_dim;
- * batch * tokens * head_dim below 2^32. */
+ * batch * tokens * head_dim up to 2^32 - 256. */
 int pgr_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_heads, const void* k,
                const int64_t* k_strides, void* k_out, int64_t k_heads, const void* positions, int positions_64bit,
                const int64_t* position_strides, const float* inv_freq, int64_t rotary_dim, int64_t batch,

@@ -1292,8 +1292,8 @@ int pgr_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_h
     int rc = check_rotary(inv_freq, rotary_dim, head_dim, factor);
     if (rc != pgr::kOk) return rc;
     if (q_heads > 65535 || k_heads > 65535 || batch > ((int64_t)1 << 30) || tokens > ((int64_t)1 << 30) ||
-        head_dim > 65536 || (batch > 0 && tokens > 0 && batch * tokens >= ((int64_t)1 << 32) / head_dim))
-      return set_err(pgr::kErrInvalid, "shape exceeds the launch limits (batch * tokens * head_dim below 2^32)");
+        head_dim > 65536 || (batch > 0 && tokens > 0 && batch * tokens > (((int64_t)1 << 32) - 256) / head_dim))
+      return set_err(pgr::kErrInvalid, "shape exceeds the launch limits (batch * tokens * head_dim up to 2^32 - 256)");
     if (batch == 0 || tokens == 0 || q_heads + k_heads == 0) return pgr::kOk;
     if ((q_heads > 0 && (!q || !q_out || !q_strides)) || (k_heads > 0 && (!k || !k_out || !k_strides)))
       return set_err(pgr::kErrInvalid, "null tensor pointer");

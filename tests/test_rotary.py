@@ -187,6 +187,21 @@ def test_c_entry_refuses_before_any_launch():
         assert call(**bad) == nat.PGR_ERR_INVALID, bad
 
 
+def test_c_entry_refuses_a_grid_that_wraps():
+    """A grid dimension of 2^32 threads runs none without an error: the last sizes below it round up to that."""
+    lib = nat.load()
+
+    def call(tokens, d):
+        rc = lib.pgr_rotary(None, None, None, 1, None, None, None, 0, None, 0, None, None, 0, 1, tokens, d, 0, 0, 1.0, 0, None)
+        assert rc == nat.PGR_ERR_INVALID
+        return "limits" in nat.last_error()
+
+    for d in (4, 12, 65, 100, 4097):
+        most = ((1 << 32) - 256) // d
+        assert call(most + 1, d), d
+        assert not call(most, d), d  # (refused for its null pointers)
+
+
 def test_python_refusals_need_no_gpu():
     q, k = torch.zeros(1, 2, 4, 16), torch.zeros(1, 1, 4, 16)
     pos, inv = torch.zeros(1, 4, dtype=torch.int64), torch.ones(8)
