@@ -368,6 +368,11 @@ PyObject* py_bind(PyObject*, PyObject* args) {
 }
 
 // ---- rotary positions and the bounded cache --------------------------------------------
+// Whether a call would lose a gradient that is being recorded, or a forward-mode tangent.
+bool differentiated(const Tensor& t) {
+  return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(/*level=*/0).defined();
+}
+
 // An operand whose last dimension is contiguous, the others strided at will. Null: not plain, or its
 // gradient is being recorded (the general path refuses it).
 const Tensor* viewed(PyObject* o, int64_t dims) {
@@ -375,7 +380,7 @@ const Tensor* viewed(PyObject* o, int64_t dims) {
   const Tensor& t = THPVariable_Unpack(o);
   if (!t.defined() || !t.is_cuda() || !plain_keys(t) || !t.has_storage() || t.dim() != dims) return nullptr;
   if (t.stride(-1) != 1 && t.size(-1) != 1) return nullptr;
-  return t.requires_grad() && c10::GradMode::is_enabled() ? nullptr : &t;
+  return differentiated(t) ? nullptr : &t;
 }
 
 bool shaped(const Tensor* t, const Tensor* like, at::IntArrayRef shape) {
@@ -395,7 +400,7 @@ bool frequencies(PyObject* o, const c10::Device& dev, int64_t head_dim, const fl
   if (o == Py_None) return true;
   const Tensor* t = plain(o);
   if (!t || t->scalar_type() != at::kFloat || t->device() != dev || t->dim() != 1 || 2 * t->size(0) > head_dim ||
-      (t->requires_grad() && c10::GradMode::is_enabled()))
+      differentiated(*t))
     return false;
   *data = t->const_data_ptr<float>();
   *rotary = 2 * t->size(0);
@@ -615,7 +620,7 @@ PyObject* py_load_prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t t = k->size(2);
     const int32_t* lo = nullptr;
     if (t == 0 || k->sizes() != at::IntArrayRef({c->batch, c->kv_heads, t, c->head_dim}) || !shaped(v, k, k->sizes()) ||
-        !is_f32(w, dev, {c->batch, c->kv_heads, t}) || (w->requires_grad() && c10::GradMode::is_enabled()) ||
+        !is_f32(w, dev, {c->batch, c->kv_heads, t}) || differentiated(*w) ||
         !first_columns(a[5], dev, c->batch, &lo) || in_state(c, lo))
       Py_RETURN_NONE;
     void* stream = nullptr;

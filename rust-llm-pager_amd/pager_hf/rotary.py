@@ -9,7 +9,7 @@ callers that run a model's layers themselves::
 
 The angle position * inv_freq[i] is taken in 64 bits: in 32 its error grows with the position (2^-7
 rad at 131072), which a model's own float32 tables show. Inference only: tensors that require
-gradients are refused while gradients are recorded; ``inverse=True`` is the transposed map, which
+gradients are refused while gradients are recorded, and forward-mode tangents always; ``inverse=True`` is the transposed map, which
 takes a gradient of the outputs back to the inputs.
 """
 from __future__ import annotations
@@ -19,6 +19,7 @@ import math
 from contextlib import nullcontext
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -127,8 +128,11 @@ def rotary_frequencies(rotary_dim: int, base: float | None = None, scaling: dict
 
 
 def _inference_only(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("this operator records no gradient; call it under torch.no_grad() or torch.inference_mode()")
+    recording = torch.is_grad_enabled()
+    if any(t is not None and (recording and t.requires_grad or forward_ad.unpack_dual(t).tangent is not None)
+           for t in tensors):
+        raise RuntimeError("this operator records no gradient and takes no forward-mode tangents; call it under "
+                           "torch.no_grad() (gradients) or torch.inference_mode() (both)")
 
 
 def _on(device: torch.device):

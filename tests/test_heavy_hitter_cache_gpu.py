@@ -701,3 +701,29 @@ def test_gradients_are_refused():
     with torch.inference_mode():
         cache.attend(cache.append(q, k, k, inv))
     assert int(cache.seen) == 1
+
+
+def test_forward_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    cache = HeavyHitterCache(1, 2, 1, 48, 32, torch.float16, "cuda")
+    q, k = torch.zeros(1, 2, 32, device="cuda").half(), torch.zeros(1, 1, 32, device="cuda").half()
+    w, k4 = torch.zeros(1, 1, 5, device="cuda"), torch.zeros(1, 1, 5, 32, device="cuda").half()
+    inv, _ = rotary_frequencies(32, device="cuda")
+    pos = torch.zeros(1, dtype=torch.int64, device="cuda")
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for bad in (lambda: cache.attend(dual(q)), lambda: cache.append(dual(q), k, k), lambda: cache.append(q, dual(k), k),
+                    lambda: cache.append(q, k, dual(k)), lambda: cache.append(q, k, k, dual(inv)),
+                    lambda: cache.load_prompt(dual(k4), k4, w), lambda: cache.load_prompt(k4, dual(k4), w),
+                    lambda: cache.load_prompt(k4, k4, dual(w)), lambda: prompt_attention_weights(dual(k4), k4),
+                    lambda: prompt_attention_weights(k4, dual(k4)), lambda: rotary_embedding(dual(q), None, pos, inv),
+                    lambda: rotary_embedding(q, dual(k), pos, inv), lambda: rotary_embedding(q, None, pos, dual(inv))):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="gradient"):
+                    bad()
+        assert not cache.seen.any()
+        cache.attend(cache.append(q, k, k, inv))
+    assert int(cache.seen) == 1

@@ -219,6 +219,29 @@ def test_python_refusals_need_no_gpu():
         rotary_embedding(q.requires_grad_(), k, pos, inv)
 
 
+def test_forward_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    from pager_hf.heavy_hitter_cache import prompt_attention_weights
+
+    q, k = torch.zeros(1, 2, 4, 16), torch.zeros(1, 1, 4, 16)
+    pos, inv = torch.zeros(1, 4, dtype=torch.int64), torch.ones(8)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                for bad in (lambda: rotary_embedding(dual(q), k, pos, inv), lambda: rotary_embedding(q, dual(k), pos, inv),
+                            lambda: rotary_embedding(q, k, pos, dual(inv)),
+                            lambda: rotary_embedding(dual(q[:, :, 0]), None, pos[:, 0], inv),
+                            lambda: prompt_attention_weights(dual(q.half()), k.half())):
+                    with pytest.raises(RuntimeError, match="gradient"):
+                        bad()
+        with pytest.raises(ValueError, match="CUDA"):
+            rotary_embedding(q, k, pos, inv)
+
+
 # ---- kernel --------------------------------------------------------------------------------------
 def _check(got, x, ref, inv_freq, factor, interleaved):
     """Half a step of the output type, and of the float32 steps before it: cos and sin within 2 steps
