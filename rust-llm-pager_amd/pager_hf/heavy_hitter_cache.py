@@ -239,10 +239,10 @@ class HeavyHitterCache:
             N.nat.check(done[0], "HeavyHitterCache.append")
             return done[1]
         _inference_only(q, k, v, inv_freq)
-        q = self._token(q, self.num_query_heads, "q")
+        q_out, q = q, self._token(q, self.num_query_heads, "q")
         k = self._token(k, self.num_kv_heads, "k")
         v = self._token(v, self.num_kv_heads, "v")
-        q_out, turning = q, 0
+        turning = 0
         if inv_freq is not None:
             inv_freq = _inv_freq(inv_freq, self.head_dim, self.device)
             turning = 2 * inv_freq.numel()

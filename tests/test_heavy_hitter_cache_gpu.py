@@ -261,6 +261,14 @@ def test_append_without_rotation_returns_the_queries():
     assert torch.equal(cache.append(strided, k, v), strided)
 
 
+def test_append_without_rotation_returns_strided_queries_themselves():
+    cache = HeavyHitterCache(2, 4, 2, 48, 32, torch.float16, "cuda")
+    q = torch.randn(2, 32, 4, device="cuda").half().transpose(1, 2)  # head_dim not contiguous
+    k = torch.randn(2, 2, 32, device="cuda").half()
+    assert cache.append(q, k, k) is q
+    assert cache.lengths.tolist() == [[1, 1], [1, 1]]
+
+
 def test_what_the_kernels_go_by_is_fixed():
     import copy
 
