@@ -41,9 +41,11 @@ def scores(q, k, scale, softcap):
     return s, bound
 
 
-def attend(q, keys, values, weights, scale, softcap, step):
+def attend(q, keys, values, weights, scale, softcap, step, p_step=None, p_floor=2.0**-25):
     """One row: q [n_rep, D], keys and values [n, D], weights [n]. Returns (out, out bound, weights, weights
-    bound); `step` is half a step of the K/V and output type."""
+    bound); `step` is half a step of the K/V and output type, p_step (`step`) and p_floor what P may be off by
+    as it enters the product with V: relative, and absolute where its largest value is 1."""
+    p_step = step if p_step is None else p_step
     n_rep, d = q.shape
     n = len(keys)
     if n == 0:
@@ -57,7 +59,7 @@ def attend(q, keys, values, weights, scale, softcap, step):
     out = p @ values
     # P rounded under a maximum of its own: half a step, or half of the smallest fp16 subnormal of weights
     # whose largest is 1; the output's own rounding likewise.
-    out_bound = (p * (step + rel)) @ np.abs(values) + 2.0**-25 * np.abs(values).sum(axis=0)
+    out_bound = (p * (p_step + rel)) @ np.abs(values) + p_floor * np.abs(values).sum(axis=0)
     out_bound = out_bound + step * (np.abs(out) + out_bound) + 2.0**-25
     new = weights + p.sum(axis=0)
     new_bound = (p * rel).sum(axis=0) + (n_rep + 1) * U32 * np.abs(new)

@@ -24,6 +24,13 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 constexpr float kMinusInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Weights w in [0, 1] of a product with V, which the matrix cores take as numbers of the K/V type, go in as two
+// of them, so that what a rounding to one would lose is kept: hi, w lowered by half a step u and cut off, and
+// lo, the rest w - hi (exact in float32, at most 3 u w), rounded: hi + lo is within 3 u^2 w of w (2^-14.4 w in
+// bf16, 2^-20.4 w in fp16). Lowered first, so that neither part of a weight is 0: 0 times an infinite V is NaN.
+// Both are 1 / kUnit times the weight's, which keeps lo above fp16's smallest number down to weights of 2^-39;
+// the caller takes the sum of the products times kUnit.
+
 struct HalfT {
   typedef uint16_t Raw;
   static __device__ __forceinline__ float to_f(Raw x) { return (float)__builtin_bit_cast(_Float16, x); }
@@ -31,6 +38,13 @@ struct HalfT {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     const f16x2 h = {(_Float16)x, (_Float16)y};
     return __builtin_bit_cast(uint32_t, h);
+  }
+  static constexpr float kUnit = 0x1p-14f;
+  static __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    constexpr float kLower = (1.f - 0x1p-11f) / kUnit;
+    const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x * kLower, y * kLower));
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = pack(fmaf(x, 1.f / kUnit, -(float)h.x), fmaf(y, 1.f / kUnit, -(float)h.y));
   }
   static __device__ __forceinline__ f32x4 mma16(u32x2 a, u32x2 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0,
@@ -53,6 +67,13 @@ struct Bf16T {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     const bf16x2 h = {(__bf16)x, (__bf16)y};
     return __builtin_bit_cast(uint32_t, h);
+  }
+  static constexpr float kUnit = 1.f;
+  static __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    constexpr float kLower = 1.f - 0x1p-8f;
+    const uint32_t a = __builtin_bit_cast(uint32_t, x * kLower), b = __builtin_bit_cast(uint32_t, y * kLower);
+    hi = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    lo = pack(x - __builtin_bit_cast(float, a & 0xffff0000u), y - __builtin_bit_cast(float, b & 0xffff0000u));
   }
   static __device__ __forceinline__ f32x4 mma16(u32x2 a, u32x2 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, a), __builtin_bit_cast(i16x4, b), c, 0,

@@ -153,6 +153,9 @@ __global__ __launch_bounds__(256) void hh_append_kernel(HHAppendLaunch a) {
 // Lane (g, n) holds tokens 4g..4g+3 of each half for query head n, which is the P^T operand as it
 // stands (contraction slot 8g + e: token 4g + e of the first half, 4g + e - 4 of the second), and every
 // O^T value of a lane belongs to head n as well: the softmax state is a scalar of the lane.
+// P goes in as two numbers of the K/V type, P.V in two products each: with one, rounded, the output of 24 like
+// tokens was off by up to seven times what its other roundings explain, and the products are free beside the
+// loads (the sizes below take the same time either way).
 // A lane reads 16-byte pieces 4c + g of K row n, so that an instruction covers 64 bytes of each of
 // 16 rows, and of V the D/16 elements n of its eight rows, transposed in registers (v_perm_b32).
 //
@@ -349,8 +352,14 @@ __global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, At
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(s[i / 4][i & 3] - ref);
     l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-    // P is rounded to the K/V type for the matrix cores, as in the framework's other decode kernels.
-    const u32x4 pb = {Ty::pack(p[0], p[1]), Ty::pack(p[2], p[3]), Ty::pack(p[4], p[5]), Ty::pack(p[6], p[7])};
+    u32x4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t x, y;
+      Ty::split(p[2 * i], p[2 * i + 1], x, y);
+      hi[i] = x;
+      lo[i] = y;
+    }
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
       const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
@@ -361,7 +370,8 @@ __global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, At
         vt[2 * x] = __builtin_amdgcn_perm(t.v[x][1][e], t.v[x][0][e], sel);
         vt[2 * x + 1] = __builtin_amdgcn_perm(t.v[x][3][e], t.v[x][2][e], sel);
       }
-      acc[j] = Ty::mma16x32(vt, pb, acc[j]);
+      acc[j] = Ty::mma16x32(vt, lo, acc[j]);
+      acc[j] = Ty::mma16x32(vt, hi, acc[j]);
     }
   };
   // After the next tile's loads, which are waited for in the order of all memory operations.
@@ -396,7 +406,7 @@ __global__ __launch_bounds__(64 * kW) void hh_attend_kernel(HHAttendLaunch a, At
 #pragma unroll
   for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sm_acc[wave][n][(D / 4) * g + (D / 16) * i + j] = acc[j][i];
+    for (int i = 0; i < 4; ++i) sm_acc[wave][n][(D / 4) * g + (D / 16) * i + j] = acc[j][i] * Ty::kUnit;
   __syncthreads();
   const int64_t part = (row * a.n_split + split) * n_rep;
   for (int i = threadIdx.x; i < n_rep * D; i += kThreads) {

@@ -97,6 +97,43 @@ def test_attend(case, dtype, softcap):
             assert torch.isnan(cache.weights[i, h, n:]).all()
 
 
+@pytest.mark.parametrize("dtype", list(STEP))
+@pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("capacity", [200, 2000])
+def test_attend_keeps_more_of_p_than_the_cache_type(d, capacity, dtype):
+    """P enters the product with V as a part cut off after it was lowered by half a step, and the rest, rounded:
+    with half a step u the rest is at most p u + 2 u p, its rounding 3 u^2 p. Under fp16 P's largest value is
+    2^14, so that half of the smallest subnormal is 2^-39 of it. Few tokens of like weights, whose sums all but
+    cancel in some dims: rounding P to the type itself is off by several times the bound."""
+    n, u = 24, STEP[dtype]
+    cache, g = _filled(4, 8, 2, capacity, d, dtype, [n] * 4, 15, keep_first=0, keep_recent=1)
+    q = (torch.randn(4, 8, d, generator=g) / 8).to(dtype).cuda()
+    out = cache.attend(q)
+    for i in range(4):
+        for h in range(2):
+            heads = slice(4 * h, 4 * h + 4)
+            ref, bound, _, _ = O.attend(_np(q[i, heads]), _np(cache.keys[i, h, :n]), _np(cache.values[i, h, :n]),
+                                        np.zeros(n), 1.0 / d**0.5, 0.0, u, p_step=3 * u * u, p_floor=2.0**-39)
+            _within(out[i, heads], ref, bound, f"row {i} head {h}")
+
+
+@pytest.mark.parametrize("dtype", list(STEP))
+@pytest.mark.parametrize("d,capacity", [(16, 90), (64, 300), (64, 2000), (256, 900)])
+def test_attend_over_infinite_values(d, capacity, dtype):
+    """A value of inf or -inf makes its dim that, however small its token's weight or exact in the type."""
+    cache, g = _filled(2, 4, 2, capacity, d, dtype, [capacity, 1], 16, keep_first=0, keep_recent=1)
+    q = torch.randn(2, 4, d, generator=g).to(dtype).cuda()
+    want = cache.attend(q)
+    cache.values[:, :, 0, 3] = float("inf")  # (row 1 holds this token alone: its weight is 1)
+    cache.values[0, :, 77, 5] = -float("inf")
+    out = cache.attend(q)
+    assert torch.equal(out[:, :, 3], torch.full_like(out[:, :, 3], float("inf")))
+    assert torch.equal(out[0, :, 5], torch.full_like(out[0, :, 5], -float("inf")))
+    for i, dims in ((0, (3, 5)), (1, (3,))):
+        rest = [e for e in range(d) if e not in dims]
+        assert torch.equal(out[i][:, rest], want[i][:, rest])
+
+
 def test_attend_with_a_few_heavy_and_far_scores():
     """Scores spread over hundreds: the running maximum moves, most weights underflow."""
     cache, g = _filled(1, 4, 1, 700, 64, torch.float16, [700], 3, keep_first=0, keep_recent=1)
