@@ -221,9 +221,9 @@ int pgr_hh_attend(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
 
 /* The attention weight that each token of a prompt gets from its last `window` queries: q [B, Hq,
  * window, D], k [B, Hkv, tokens, D] (strides: batch, head, token), weights [B, Hkv, tokens] written,
- * summed over the queries and over each KV head's query heads; causal. lo [B] (NULL: 0): the row's
- * first valid column (left padding): columns before it get 0, queries before it give nothing, and
- * what q and k hold there does not matter. tokens <= 8388480, window * num_query_heads /
+ * not over the other operands; summed over the queries and over each KV head's query heads; causal. lo
+ * [B] (NULL: 0): the row's first valid column (left padding): columns before it get 0, queries before it
+ * give nothing, and what q and k hold there does not matter. tokens <= 8388480, window * num_query_heads /
  * num_kv_heads <= 2097120, batch * heads * tokens <= 2^31; head and token strides below 2^31. */
 size_t pgr_hh_prompt_weights_workspace_bytes(int64_t batch, int64_t num_query_heads, int64_t num_kv_heads,
                                              int64_t tokens, int64_t window, int64_t head_dim);

@@ -328,14 +328,19 @@ Operand flat(const void* p, int64_t bytes) {
   return x;
 }
 
-Operand heads_of(const pgr_hh_cache_t* c, const void* p, const int64_t* stride, int64_t heads, int64_t tokens = 0) {
-  Operand x = flat(p, c->head_dim * 2);
+// [batch, heads, tokens, head_dim] of 16-bit elements; tokens 0: [batch, heads, head_dim].
+Operand rows_of(const void* p, const int64_t* stride, int64_t batch, int64_t heads, int64_t tokens, int64_t head_dim) {
+  Operand x = flat(p, head_dim * 2);
   x.dims = tokens > 0 ? 3 : 2;
-  x.size[0] = c->batch;
+  x.size[0] = batch;
   x.size[1] = heads;
   x.size[2] = tokens;
   x.stride = stride;
   return x;
+}
+
+Operand heads_of(const pgr_hh_cache_t* c, const void* p, const int64_t* stride, int64_t heads, int64_t tokens = 0) {
+  return rows_of(p, stride, c->batch, heads, tokens, c->head_dim);
 }
 
 // Whether some byte of x's dimensions from `dim` on, the first row at p, lies in [lo, hi). The bytes from the
@@ -1450,6 +1455,12 @@ int pgr_hh_prompt_weights(const void* q, const int64_t* q_strides, const void* k
     const PromptPlan p = plan_prompt(batch, num_query_heads, num_kv_heads, tokens, window, head_dim);
     if (workspace == nullptr || workspace_bytes < p.bytes) return set_err(pgr::kErrCapacity, "workspace too small");
     if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");
+    const Operand xq = rows_of(q, q_strides, batch, num_query_heads, window, head_dim),
+                  xk = rows_of(k, k_strides, batch, num_kv_heads, tokens, head_dim),
+                  xl = flat(lo, batch * (int64_t)sizeof(int32_t));
+    for (const Operand* x : {&xq, &xk, &xl})
+      if (overlaps(*x, weights, batch * num_kv_heads * tokens * (int64_t)sizeof(float)))
+        return set_err(pgr::kErrInvalid, "weights must not overlap the other operands");
     char* w = static_cast<char*>(workspace);
     pgr::PromptWeightLaunch L;
     L.q = q;

@@ -189,6 +189,23 @@ def test_c_entries_refuse_outputs_over_their_inputs():
     assert attend(out, dense) not in (0, inv) and attend(out + 256, dense) not in (0, inv)
 
 
+def test_prompt_weights_refuse_an_output_over_the_inputs():
+    """Workgroups write their keys' weights while others still read q, k and lo."""
+    if torch.cuda.is_available():
+        pytest.skip("addresses without memory behind them: for hosts without a GPU")
+    lib, inv = nat.load(), nat.PGR_ERR_INVALID
+    s, far, out = (ctypes.c_int64 * 3)(1, 1, 1), 1 << 30, 1 << 29  # out: 2 heads of 100 floats
+
+    def run(q=far, k=far, lo=None):
+        return lib.pgr_hh_prompt_weights(q, s, k, s, lo, out, 1, 4, 2, 100, 10, 32, 0, 1.0, 0.0, 256, 1 << 30, None)
+
+    for at in (out, out + 798, out - 2):
+        assert run(q=at) == inv and "overlap" in nat.last_error()
+        assert run(k=at) == inv and "overlap" in nat.last_error()
+        assert run(lo=at) == inv and "overlap" in nat.last_error()
+    assert run(q=out + 800, k=out - 1024, lo=out - 4) not in (0, inv)
+
+
 def test_python_refusals_need_no_gpu():
     def make(**over):
         a = dict(batch=1, num_query_heads=4, num_kv_heads=2, capacity=64, head_dim=32, dtype=torch.float16, device="cuda")
