@@ -538,13 +538,15 @@ __global__ __launch_bounds__(256) void hh_attend_merge_kernel(HHAttendLaunch a) 
 // Latency-bound: the weights are few bytes (256 KB a row at 65536 tokens), the passes and their barriers
 // many. Up to kSelShort tokens one workgroup per row does it all, its keys in registers (2 / 32 / 512 rows
 // of 8192 tokens, the copy of short records included: 11.4 / 12.9 / 31.7 us against 16.5 / 18.2 / 41.5 in
-// parts). Longer rows are
-// dealt out in parts of kSelPart tokens over three launches: the parts' counts of the top 11 bits; from
-// all of a row's counts the class of the last token, whose members go to the row's list; and from that
-// list (a hundredth of the tokens, if weights differ) the last key and each part's slots. 16 rows of
-// 65536 tokens: 4.8 + 7.0 + 9.0 us; one workgroup per row took 71 us (129 with 8-bit classes and without
-// registers), the fetching of its unrolled code included, on 16 of the 256 CUs. 8 rows of 1023 tokens in
-// one launch: 9.2 us (31.8).
+// parts). Longer rows are dealt out in parts of kSelPart tokens over three launches: the parts' counts of the
+// top 11 bits; from all of a row's counts the class of the last token, whose members go to the row's list; and
+// from that list the last key and each part's slots. 16 rows of 65536 tokens, 4096 kept, weights over many
+// binades (the list is a hundredth of the row): 4.4 + 6.8 + 9.6 us; one workgroup per row took 71 us (129 with
+// 8-bit classes and without registers), the fetching of its unrolled code included, on 16 of the 256 CUs.
+// Every part reads the row's whole list, up to three times, and the list is as long as weights are alike: of a
+// prompt's attention weights (64 queries, D 128) 4% of the row with queries of scale 2, 44-49% at scale 1 and
+// 0.5, where the last launch takes 12 and 42-46 us (at 131072 tokens and 8192 kept 16 and 70-77); 114 us
+// if all weights are equal. 8 rows of 1023 tokens in one launch: 9.3 us (31.8).
 //
 // Counts of one class are added one after the other; where all of a wave's tokens are of one class
 // (equal weights), one lane adds them up.
