@@ -36,7 +36,7 @@ extern "C" {
 
 /* ---- library ------------------------------------------------------------------------- */
 
-/* ABI version of this header (increments when an entry point is added or changed); 13. */
+/* ABI version of this header (increments when an entry point is added or changed); 14. */
 int pgr_abi_version(void);
 /* Message of the last failing call on this thread ("" if none). */
 const char* pgr_last_error(void);
@@ -241,6 +241,83 @@ size_t pgr_hh_load_prompt_workspace_bytes(const pgr_hh_cache_t* cache, int64_t t
 int pgr_hh_load_prompt(const pgr_hh_cache_t* cache, const void* k, const int64_t* k_strides, const void* v,
                        const int64_t* v_strides, const float* weights, const int32_t* lo, int64_t tokens,
                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- drafted tokens over a cache of pages ------------------------------------------------
+ * No counterpart in the reference. */
+
+/* The RMS norm of each head, x / sqrt(mean(x^2) + eps) * weight, and pgr_rotary's turn in one pass:
+ * pgr_rotary's operands and forms (no inverse), with weights [D] of the operands' dtype or, with weights_f32,
+ * float32; computed in fp32, rounded once. batch * tokens <= 2^26 - 4; outputs must not overlap the other
+ * operands. */
+int pgr_norm_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_heads, const void* k,
+                    const int64_t* k_strides, void* k_out, int64_t k_heads, const void* q_weight, const void* k_weight,
+                    int weights_f32, float eps, const void* positions, int positions_64bit,
+                    const int64_t* position_strides, const float* inv_freq, int64_t rotary_dim, int64_t batch,
+                    int64_t tokens, int64_t head_dim, int dtype, int interleaved, float factor, void* stream);
+
+/* A cache of pages (device buffers of the caller): K and V of all layers, whose pages the calls' tables name.
+ * D in {16, 32, 64, 128, 256}; Hq / Hkv <= 16; fp16 or bf16; page_tokens 16, 32, 64, 128 or 256. */
+typedef struct pgr_pt_cache_s {
+  void* keys;   /* [layers, pages, Hkv, page_tokens, D], 16-byte aligned */
+  void* values;
+  int64_t layers;
+  int64_t pages;
+  int64_t query_heads;
+  int64_t kv_heads;
+  int64_t page_tokens;
+  int64_t head_dim;
+  int dtype;
+} pgr_pt_cache_t;
+
+/* What the calls go by: table [batch, width] (rows table_stride entries apart) names each row's pages in order,
+ * lengths [batch] the tokens a row holds, counts [batch] (NULL: `tokens` each) how many of a call's `tokens` columns
+ * are the row's new ones. They are read on the device. New token t is the row's token lengths[b] + t. A table entry
+ * outside [0, pages) stands for a page that is not there: tokens in it are not stored, moved or attended to; nor
+ * are those behind the table's end. width * page_tokens <= 2^30; batch * Hkv <= 65535. */
+typedef struct pgr_pt_rows_s {
+  const int32_t* table;
+  int64_t table_stride;
+  int64_t width;
+  const int32_t* lengths;
+  const int32_t* counts;
+  int64_t batch;
+  int64_t tokens;
+} pgr_pt_rows_t;
+
+/* New tokens into the pages of one layer: k, v [batch, Hkv, tokens, D] and q [batch, Hq, tokens, D] (strides: batch,
+ * head, token); with weights q and k are normed as pgr_norm_rotary norms them, with inv_freq turned, at
+ * positions (strides: batch, token), or, with positions NULL, at lengths[b] plus depths[b, t] (depths NULL: plus t).
+ * q_out [batch, Hq, tokens, D] contiguous receives q, zeros where a token is not new; it must not overlap the other
+ * operands. No operand may lie in the cache. Rows that put a token in one and the same place race for it. */
+int pgr_pt_append(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_t* rows, const void* q,
+                  const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                  const int64_t* v_strides, void* q_out, const void* positions, int positions_64bit,
+                  const int64_t* position_strides, const int32_t* depths, const float* inv_freq, int64_t rotary_dim,
+                  int interleaved, float factor, const void* q_weight, const void* k_weight, int weights_f32, float eps,
+                  void* stream);
+
+/* Attention of each row's new tokens (appended before): out [batch, tokens, Hq, D] contiguous = softmax(scale * q .
+ * K^T, softcapped with softcap > 0) V over the tokens that the row holds and those new ones that token t sees: the
+ * first t + 1, or with masks [batch, tokens] (tokens <= 64) new token j where bit j is set. window > 0: only tokens
+ * whose position is less than `window` before the token's own (positions: held tokens' numbers, lengths[b] + t, with
+ * masks lengths[b] + depths[b, t]). Columns that are not new tokens get zeros, as does a head that sees nothing or
+ * scores of -inf only. What the cache holds behind a row's new tokens and before all of their windows does not
+ * matter; a value that is not finite among those that some token of the call sees may reach all the row's new
+ * tokens. q strides: batch, head, token. tokens * Hq / Hkv <= 2^20. */
+size_t pgr_pt_attend_workspace_bytes(const pgr_pt_cache_t* cache, int64_t batch, int64_t tokens, int64_t width);
+int pgr_pt_attend(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_t* rows, const void* q,
+                  const int64_t* q_strides, void* out, const uint64_t* masks, const int32_t* depths, int64_t window,
+                  float scale, float softcap, void* workspace, size_t workspace_bytes, void* stream);
+
+/* In every layer, keys and values of token lengths[b] + path[b, j] go to token lengths[b] + j, all at once. path
+ * [batch, tokens] contiguous, tokens <= 64; an entry outside [0, 64) leaves token j as it is. counts is not read. */
+int pgr_pt_keep(const pgr_pt_cache_t* cache, const pgr_pt_rows_t* rows, const int32_t* path, void* stream);
+
+/* masks and depths [batch, tokens] (tokens <= 64) of trees of drafted tokens: parents [batch, tokens] contiguous
+ * holds an earlier token, or anything else for a token that follows the held ones. Bit j of a token's mask: token j
+ * is the token itself or an ancestor; depth: its ancestors' number. */
+int pgr_draft_tree(const int32_t* parents, int64_t batch, int64_t tokens, uint64_t* masks, int32_t* depths,
+                   void* stream);
 
 /* ---- placement policy ----------------------------------------------------------------
  * Restatement of the Rust pager. Handles are opaque; not thread-safe per handle. */

@@ -36,7 +36,7 @@ STREAM_DIRECT = 0
 STREAM_STAGED = 1
 STREAM_MIRROR = 2
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 c_i32, c_i64, c_u8, c_u32, c_u64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint8, ctypes.c_uint32, ctypes.c_uint64
 c_f32, c_f64, c_size, c_vp = ctypes.c_float, ctypes.c_double, ctypes.c_size_t, ctypes.c_void_p
@@ -123,6 +123,36 @@ class HHCache(ctypes.Structure):
     ]
 
 
+class PTCache(ctypes.Structure):
+    """pgr_pt_cache_t: the buffers of a cache of pages."""
+
+    _fields_ = [
+        ("keys", c_vp),
+        ("values", c_vp),
+        ("layers", c_i64),
+        ("pages", c_i64),
+        ("query_heads", c_i64),
+        ("kv_heads", c_i64),
+        ("page_tokens", c_i64),
+        ("head_dim", c_i64),
+        ("dtype", ctypes.c_int),
+    ]
+
+
+class PTRows(ctypes.Structure):
+    """pgr_pt_rows_t: the rows of a call on a cache of pages."""
+
+    _fields_ = [
+        ("table", c_vp),
+        ("table_stride", c_i64),
+        ("width", c_i64),
+        ("lengths", c_vp),
+        ("counts", c_vp),
+        ("batch", c_i64),
+        ("tokens", c_i64),
+    ]
+
+
 # name -> (restype, argtypes). Every symbol declared in include/pgr.h.
 SIGNATURES: dict[str, tuple] = {
     "pgr_abi_version": (ctypes.c_int, []),
@@ -158,6 +188,23 @@ SIGNATURES: dict[str, tuple] = {
         [c_vp, P(c_i64), c_vp, c_i64, c_vp, P(c_i64), c_vp, c_i64, c_vp, ctypes.c_int, P(c_i64), c_vp, c_i64, c_i64,
          c_i64, c_i64, ctypes.c_int, ctypes.c_int, c_f32, ctypes.c_int, c_vp],
     ),
+    "pgr_norm_rotary": (
+        ctypes.c_int,
+        [c_vp, P(c_i64), c_vp, c_i64, c_vp, P(c_i64), c_vp, c_i64, c_vp, c_vp, ctypes.c_int, c_f32, c_vp, ctypes.c_int,
+         P(c_i64), c_vp, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, ctypes.c_int, c_f32, c_vp],
+    ),
+    "pgr_pt_append": (
+        ctypes.c_int,
+        [P(PTCache), c_i64, P(PTRows), c_vp, P(c_i64), c_vp, P(c_i64), c_vp, P(c_i64), c_vp, c_vp, ctypes.c_int,
+         P(c_i64), c_vp, c_vp, c_i64, ctypes.c_int, c_f32, c_vp, c_vp, ctypes.c_int, c_f32, c_vp],
+    ),
+    "pgr_pt_attend_workspace_bytes": (c_size, [P(PTCache), c_i64, c_i64, c_i64]),
+    "pgr_pt_attend": (
+        ctypes.c_int,
+        [P(PTCache), c_i64, P(PTRows), c_vp, P(c_i64), c_vp, c_vp, c_vp, c_i64, c_f32, c_f32, c_vp, c_size, c_vp],
+    ),
+    "pgr_pt_keep": (ctypes.c_int, [P(PTCache), P(PTRows), c_vp, c_vp]),
+    "pgr_draft_tree": (ctypes.c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "pgr_hh_append": (
         ctypes.c_int,
         [P(HHCache), c_vp, P(c_i64), c_vp, P(c_i64), c_vp, P(c_i64), c_vp, c_vp, ctypes.c_int, c_vp, c_i64,

@@ -34,6 +34,8 @@ SOURCES = [
     ("rotary_kernels.hip", "hip", []),
     ("cache_kernels.hip", "hip", []),
     ("prompt_weight_kernels.hip", "hip", []),
+    ("norm_rotary_kernels.hip", "hip", []),
+    ("page_table_kernels.hip", "hip", []),
     ("paged_kv.cpp", "hip", []),
     ("capi.cpp", "hip", []),
     # Host-only placement policy: no fused multiply-add, so f32 rounds like the reference.

@@ -165,71 +165,11 @@ __global__ __launch_bounds__(256) void hh_append_kernel(HHAppendLaunch a) {
 // them up. 32 full rows x 8192 tokens, 32/8 heads, D 128: 206 + 13 us for 1.08 GB (5.2 TB/s in the first
 // launch; a copy reaches 5.1, a plain read in this order 6.25, this launch without its stores 5.8). Tiles
 // of 16 tokens, one load after the other: 221 us; 256 to 8192 workgroups, non-temporal loads or not: 205-212.
-template <int D>
-struct KVTile {
-  static constexpr int KP = D >= 32 ? D / 32 : 1;  // 16-byte pieces of a K row (D 16: one of 8 bytes)
-  static constexpr int VD = D >= 32 ? D / 32 : 1;  // dwords of each V row (D 16: half of one)
-  u32x4 k[2][KP];
-  uint32_t v[2][4][VD];
-};
-
-typedef uint32_t u32x2_e __attribute__((ext_vector_type(2), aligned(2)));
-
-// The lane's pieces of a K row (or of a query).
-template <int D>
-__device__ __forceinline__ void load_pieces(u32x4 (&r)[KVTile<D>::KP], const uint16_t* row, int g) {
-  if constexpr (D == 16) {
-    const u32x2 x = *reinterpret_cast<const u32x2_e*>(row + 4 * g);
-    r[0] = u32x4{x.x, x.y, 0u, 0u};
-  } else {
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) r[c] = *reinterpret_cast<const u32x4_e*>(row + 32 * c + 8 * g);
-  }
-}
-
-// Elements (D/16) n.. of a V row.
-template <int D>
-__device__ __forceinline__ void load_v(uint32_t (&r)[KVTile<D>::VD], const uint16_t* row, int n) {
-  const uint16_t* p = row + (D / 16) * n;
-  if constexpr (D == 16) {
-    r[0] = *p;
-  } else if constexpr (D == 32) {
-    typedef uint32_t u32_e __attribute__((aligned(2)));
-    r[0] = *reinterpret_cast<const u32_e*>(p);
-  } else if constexpr (D == 64) {
-    const u32x2 x = *reinterpret_cast<const u32x2_e*>(p);
-    r[0] = x.x;
-    r[1] = x.y;
-  } else {
-#pragma unroll
-    for (int c = 0; c < D / 128; ++c) {
-      const u32x4 x = *reinterpret_cast<const u32x4_e*>(p + 8 * c);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[4 * c + i] = x[i];
-    }
-  }
-}
-
-// Max and sum over the four lane groups g.
-__device__ __forceinline__ float max_g(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float sum_g(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
-
 // What a head's scores are taken against for their probabilities, in log2 units. +inf where nothing has weight
 // (no tokens, or scores of -inf only): the head then gives zeros, and nothing to the weights.
 __device__ __forceinline__ float norm_of(float m, float l) {
   return l == 0.f ? -kMinusInf : m + __builtin_amdgcn_logf(l);
 }
-
-// Scores in log2 units: scale_log2 = scale * log2(e), or with a softcap cap * log2(e).
-struct AttendScale {
-  float scale_log2, cap_scale, cap_log2;
-};
 
 // Tokens [begin, end) of a row of `length` that split `split` of n_split takes: whole 32-token
 // tiles, evenly.

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "cache_kernels.h"
+#include "page_table_kernels.h"
 #include "paged_kv.h"
 #include "pager_core.h"
 #include "pgr_common.h"
@@ -484,6 +485,139 @@ PromptPlan plan_prompt(int64_t batch, int64_t hq, int64_t hkv, int64_t tokens, i
   return p;
 }
 
+// ---- drafted tokens over a cache of pages ------------------------------------------------
+int check_pt_cache(const pgr_pt_cache_t* c) {
+  if (c == nullptr) return set_err(pgr::kErrInvalid, "null cache");
+  const int rc = check_heads(1, c->query_heads, c->kv_heads, c->head_dim, c->dtype);
+  if (rc != pgr::kOk) return rc;
+  const int64_t t = c->page_tokens;
+  if (t != 16 && t != 32 && t != 64 && t != 128 && t != 256)
+    return set_err(pgr::kErrUnsupported, "page_tokens must be 16, 32, 64, 128 or 256");
+  if (c->layers <= 0 || c->layers > 65535 || c->pages <= 0 || c->pages > ((int64_t)1 << 30))
+    return set_err(pgr::kErrInvalid, "layers must be in [1, 65535] and pages in [1, 2^30]");
+  if (!c->keys || !c->values) return set_err(pgr::kErrInvalid, "null cache buffer");
+  if (((uintptr_t)c->keys | (uintptr_t)c->values) % 16 != 0)
+    return set_err(pgr::kErrInvalid, "cache buffers must be 16-byte aligned");
+  return pgr::kOk;
+}
+
+int64_t pt_layer_bytes(const pgr_pt_cache_t* c) { return c->pages * c->kv_heads * c->page_tokens * c->head_dim * 2; }
+
+int check_pt_rows(const pgr_pt_cache_t* c, int64_t batch, int64_t tokens, int64_t width) {
+  if (batch < 0 || tokens < 0 || width < 0) return set_err(pgr::kErrInvalid, "negative dimension");
+  if (batch > 65535 || batch * c->kv_heads > 65535)
+    return set_err(pgr::kErrInvalid, "batch * num_kv_heads must not exceed 65535");
+  if (width > ((int64_t)1 << 30) / c->page_tokens)
+    return set_err(pgr::kErrInvalid, "table width * page_tokens must not exceed 2^30");
+  return pgr::kOk;
+}
+
+int check_pt_call(const pgr_pt_cache_t* c, int64_t layer, const pgr_pt_rows_t* r) {
+  int rc = check_pt_cache(c);
+  if (rc != pgr::kOk) return rc;
+  if (r == nullptr) return set_err(pgr::kErrInvalid, "null rows");
+  rc = check_pt_rows(c, r->batch, r->tokens, r->width);
+  if (rc != pgr::kOk) return rc;
+  if (layer < 0 || layer >= c->layers) return set_err(pgr::kErrInvalid, "layer out of range");
+  if (r->batch > 0 && r->tokens > 0 && (!r->lengths || (r->width > 0 && !r->table)))
+    return set_err(pgr::kErrInvalid, "null table or lengths");
+  return pgr::kOk;
+}
+
+// Whether an operand lies, in whole or in part, in the cache's pages.
+bool in_pages(const pgr_pt_cache_t* c, const Operand& x) {
+  if (x.p == nullptr) return false;
+  const uintptr_t bytes = (uintptr_t)(c->layers * pt_layer_bytes(c)), k = (uintptr_t)c->keys, v = (uintptr_t)c->values;
+  return touches(x, 0, (uintptr_t)x.p, k, k + bytes) || touches(x, 0, (uintptr_t)x.p, v, v + bytes);
+}
+
+Operand table_of(const pgr_pt_rows_t* r) {
+  Operand x = flat(r->width > 0 ? r->table : nullptr, r->width * 4);
+  x.dims = 1;
+  x.size[0] = r->batch;
+  x.stride = &r->table_stride;
+  x.elem = 4;
+  return x;
+}
+
+Operand numbers(const int32_t* p, int64_t n) { return flat(p, n * 4); }
+
+Operand positions_of(const void* p, int is64, const int64_t* stride, int64_t batch, int64_t tokens) {
+  Operand x = flat(p, is64 ? 8 : 4);
+  if (p == nullptr) return x;
+  x.dims = 2;
+  x.size[0] = batch;
+  x.size[1] = tokens;
+  x.stride = stride;
+  x.elem = is64 ? 8 : 4;
+  return x;
+}
+
+pgr::PTPages pages_of(const pgr_pt_cache_t* c, int64_t layer) {
+  pgr::PTPages p;
+  p.keys = static_cast<char*>(c->keys) + layer * pt_layer_bytes(c);
+  p.values = static_cast<char*>(c->values) + layer * pt_layer_bytes(c);
+  p.pages = (int)c->pages;
+  p.hq = (int)c->query_heads;
+  p.hkv = (int)c->kv_heads;
+  while (1 << p.page_shift < (int)c->page_tokens) ++p.page_shift;
+  p.d = (int)c->head_dim;
+  return p;
+}
+
+pgr::PTRows rows_of_call(const pgr_pt_rows_t* r) {
+  pgr::PTRows x;
+  x.table = r->table;
+  x.table_stride = r->table_stride;
+  x.width = (int)r->width;
+  x.lengths = r->lengths;
+  x.counts = r->counts;
+  x.batch = (int)r->batch;
+  x.tokens = (int)r->tokens;
+  return x;
+}
+
+int check_norm(const void* q_weight, const void* k_weight, bool q, bool k, float eps) {
+  if ((q && !q_weight) || (k && !k_weight)) return set_err(pgr::kErrInvalid, "null norm weight");
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return set_err(pgr::kErrInvalid, "eps must be finite and not negative");
+  return pgr::kOk;
+}
+
+// Threads of a launch's first dimension end at 2^32: 64 for a token at most.
+int check_tokens(int64_t batch, int64_t tokens) {
+  if (tokens > ((int64_t)1 << 26) - 4 || batch * tokens > ((int64_t)1 << 26) - 4)
+    return set_err(pgr::kErrInvalid, "batch * tokens must not exceed 2^26 - 4");
+  return pgr::kOk;
+}
+
+struct PTPlan {
+  pgr::PTAttendPlan k;
+  size_t o_pm = 0, o_pl = 0, o_pacc = 0, bytes = 0;
+};
+
+int check_pt_attend(const pgr_pt_cache_t* c, int64_t batch, int64_t tokens) {
+  const int64_t rep = c->query_heads / c->kv_heads;
+  if (tokens > ((int64_t)1 << 20) / rep)
+    return set_err(pgr::kErrInvalid, "tokens * query heads per KV head must not exceed 2^20");
+  if (batch * c->kv_heads * ((tokens * rep + 15) / 16) > (int64_t)1 << 23)
+    return set_err(pgr::kErrInvalid, "batch * tokens * query heads must not exceed 2^27");
+  return pgr::kOk;
+}
+
+PTPlan plan_pt(const pgr_pt_cache_t* c, int64_t batch, int64_t tokens, int64_t width) {
+  PTPlan p;
+  p.k = pgr::pt_attend_plan((int)batch, (int)tokens, (int)c->query_heads, (int)c->kv_heads, width * c->page_tokens,
+                            (int)c->head_dim);
+  if (p.k.n_split == 1) return p;
+  const size_t slots = (size_t)(batch * c->kv_heads) * p.k.blocks * p.k.n_split * p.k.rows;
+  Parts w;
+  p.o_pm = w.take(slots * sizeof(float));
+  p.o_pl = w.take(slots * sizeof(float));
+  p.o_pacc = w.take(slots * (size_t)c->head_dim * sizeof(float));
+  p.bytes = w.bytes;
+  return p;
+}
+
 pgr::PagedKV* kv_of(void* h) { return static_cast<pgr::PagedKV*>(h); }
 
 int kv_rc(pgr::PagedKV* kv, int rc) {
@@ -495,7 +629,7 @@ int kv_rc(pgr::PagedKV* kv, int rc) {
 
 extern "C" {
 
-int pgr_abi_version(void) { return 13; }
+int pgr_abi_version(void) { return 14; }
 
 const char* pgr_last_error(void) { return g_last_error.c_str(); }
 
@@ -1367,6 +1501,266 @@ int pgr_hh_append(const pgr_hh_cache_t* cache, const void* q, const int64_t* q_s
     L.form = rotary_form(inv_freq, rotary_dim, interleaved, factor, 0);
     const hipError_t e = pgr::launch_hh_append(cache->dtype, L, as_stream(stream));
     if (e != hipSuccess) return hip_err(e, "append launch");
+    return pgr::kOk;
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+// ---- drafted tokens over a cache of pages ------------------------------------------------
+int pgr_norm_rotary(const void* q, const int64_t* q_strides, void* q_out, int64_t q_heads, const void* k,
+                    const int64_t* k_strides, void* k_out, int64_t k_heads, const void* q_weight, const void* k_weight,
+                    int weights_f32, float eps, const void* positions, int positions_64bit,
+                    const int64_t* position_strides, const float* inv_freq, int64_t rotary_dim, int64_t batch,
+                    int64_t tokens, int64_t head_dim, int dtype, int interleaved, float factor, void* stream) {
+  try {
+    if (q_heads < 0 || k_heads < 0 || batch < 0 || tokens < 0 || head_dim <= 0)
+      return set_err(pgr::kErrInvalid, "negative or zero dimension");
+    if (dtype != pgr::kF16 && dtype != pgr::kBF16 && dtype != pgr::kF32)
+      return set_err(pgr::kErrInvalid, "dtype must be fp16, bf16 or fp32");
+    int rc = check_rotary(inv_freq, rotary_dim, head_dim, factor);
+    if (rc != pgr::kOk) return rc;
+    if (q_heads > 32767 || k_heads > 32767 || head_dim > 65536 || batch > ((int64_t)1 << 26))
+      return set_err(pgr::kErrInvalid, "shape exceeds the launch limits");
+    rc = check_tokens(batch, tokens);
+    if (rc != pgr::kOk) return rc;
+    if (batch == 0 || tokens == 0 || q_heads + k_heads == 0) return pgr::kOk;
+    if ((q_heads > 0 && (!q || !q_out || !q_strides)) || (k_heads > 0 && (!k || !k_out || !k_strides)))
+      return set_err(pgr::kErrInvalid, "null tensor pointer");
+    if (rotary_dim > 0 && (!positions || !position_strides)) return set_err(pgr::kErrInvalid, "null positions");
+    rc = check_norm(q_weight, k_weight, q_heads > 0, k_heads > 0, eps);
+    if (rc != pgr::kOk) return rc;
+    const int64_t elem = dtype == pgr::kF32 ? 4 : 2, wide = head_dim * (weights_f32 ? 4 : elem);
+    Operand in[6] = {rows_of(q_heads > 0 ? q : nullptr, q_strides, batch, q_heads, tokens, head_dim),
+                     rows_of(k_heads > 0 ? k : nullptr, k_strides, batch, k_heads, tokens, head_dim),
+                     flat(q_heads > 0 ? q_weight : nullptr, wide), flat(k_heads > 0 ? k_weight : nullptr, wide),
+                     positions_of(rotary_dim > 0 ? positions : nullptr, positions_64bit, position_strides, batch, tokens),
+                     flat(rotary_dim > 0 ? inv_freq : nullptr, rotary_dim / 2 * 4)};
+    for (int i = 0; i < 2; ++i) {
+      in[i].row = head_dim * elem;
+      in[i].elem = elem;
+    }
+    const int64_t q_bytes = batch * q_heads * tokens * head_dim * elem, k_bytes = batch * k_heads * tokens * head_dim * elem;
+    for (const Operand& x : in)
+      if ((q_heads > 0 && overlaps(x, q_out, q_bytes)) || (k_heads > 0 && overlaps(x, k_out, k_bytes)))
+        return set_err(pgr::kErrInvalid, "outputs must not overlap the other operands");
+    if (q_heads > 0 && k_heads > 0 && overlaps(flat(q_out, q_bytes), k_out, k_bytes))
+      return set_err(pgr::kErrInvalid, "outputs must not overlap the other operands");
+    pgr::NormRotaryLaunch L;
+    L.x[0] = q;
+    L.x[1] = k;
+    L.y[0] = q_out;
+    L.y[1] = k_out;
+    if (q_heads > 0) L.xs[0] = strides_of(q_strides, 3);
+    if (k_heads > 0) L.xs[1] = strides_of(k_strides, 3);
+    L.heads[0] = (int)q_heads;
+    L.heads[1] = (int)k_heads;
+    L.positions = positions;
+    L.positions64 = positions_64bit != 0;
+    if (position_strides != nullptr) {
+      L.pos_b = position_strides[0];
+      L.pos_t = position_strides[1];
+    }
+    L.form = rotary_form(inv_freq, rotary_dim, interleaved, factor, 0);
+    L.norm.weight[0] = q_weight;
+    L.norm.weight[1] = k_weight;
+    L.norm.weight_f32 = weights_f32 != 0 || dtype == pgr::kF32;
+    L.norm.eps = eps;
+    L.batch = (int)batch;
+    L.tokens = (int)tokens;
+    L.d = (int)head_dim;
+    const hipError_t e = pgr::launch_norm_rotary(dtype, L, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "normed rotary launch");
+    return pgr::kOk;
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+int pgr_pt_append(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_t* rows, const void* q,
+                  const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                  const int64_t* v_strides, void* q_out, const void* positions, int positions_64bit,
+                  const int64_t* position_strides, const int32_t* depths, const float* inv_freq, int64_t rotary_dim,
+                  int interleaved, float factor, const void* q_weight, const void* k_weight, int weights_f32, float eps,
+                  void* stream) {
+  try {
+    int rc = check_pt_call(cache, layer, rows);
+    if (rc != pgr::kOk) return rc;
+    rc = check_rotary(inv_freq, rotary_dim, cache->head_dim, factor);
+    if (rc != pgr::kOk) return rc;
+    const int64_t b = rows->batch, t = rows->tokens, hq = cache->query_heads, hkv = cache->kv_heads, d = cache->head_dim;
+    if (hq + 2 * hkv > 65535) return set_err(pgr::kErrInvalid, "shape exceeds the launch limits");
+    rc = check_tokens(b, t);
+    if (rc != pgr::kOk) return rc;
+    if (b == 0 || t == 0) return pgr::kOk;
+    if (!q || !k || !v || !q_out || !q_strides || !k_strides || !v_strides)
+      return set_err(pgr::kErrInvalid, "null tensor pointer");
+    if (positions != nullptr && !position_strides) return set_err(pgr::kErrInvalid, "null position strides");
+    if (q_weight != nullptr || k_weight != nullptr) {
+      rc = check_norm(q_weight, k_weight, true, true, eps);
+      if (rc != pgr::kOk) return rc;
+    }
+    const int64_t q_bytes = b * hq * t * d * 2, wide = d * (weights_f32 ? 4 : 2);
+    const Operand in[] = {rows_of(q, q_strides, b, hq, t, d),
+                          rows_of(k, k_strides, b, hkv, t, d),
+                          rows_of(v, v_strides, b, hkv, t, d),
+                          positions_of(positions, positions_64bit, position_strides, b, t),
+                          numbers(depths, b * t),
+                          flat(rotary_dim > 0 ? inv_freq : nullptr, rotary_dim / 2 * 4),
+                          flat(q_weight, wide),
+                          flat(k_weight, wide),
+                          table_of(rows),
+                          numbers(rows->lengths, b),
+                          numbers(rows->counts, b)};
+    for (const Operand& x : in) {
+      if (in_pages(cache, x)) return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
+      if (overlaps(x, q_out, q_bytes)) return set_err(pgr::kErrInvalid, "q_out must not overlap the other operands");
+    }
+    if (in_pages(cache, flat(q_out, q_bytes)))
+      return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
+    pgr::NormRotaryLaunch L;
+    L.x[0] = q;
+    L.x[1] = k;
+    L.x[2] = v;
+    L.y[0] = q_out;
+    L.xs[0] = strides_of(q_strides, 3);
+    L.xs[1] = strides_of(k_strides, 3);
+    L.xs[2] = strides_of(v_strides, 3);
+    L.heads[0] = (int)hq;
+    L.heads[1] = (int)hkv;
+    L.positions = positions;
+    L.positions64 = positions_64bit != 0;
+    if (positions != nullptr) {
+      L.pos_b = position_strides[0];
+      L.pos_t = position_strides[1];
+    }
+    L.depths = depths;
+    L.form = rotary_form(inv_freq, rotary_dim, interleaved, factor, 0);
+    L.norm.weight[0] = q_weight;
+    L.norm.weight[1] = k_weight;
+    L.norm.weight_f32 = weights_f32 != 0;
+    L.norm.eps = eps;
+    L.batch = (int)b;
+    L.tokens = (int)t;
+    L.d = (int)d;
+    L.c = pages_of(cache, layer);
+    L.r = rows_of_call(rows);
+    const hipError_t e = pgr::launch_pt_append(cache->dtype, L, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "append launch");
+    return pgr::kOk;
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+size_t pgr_pt_attend_workspace_bytes(const pgr_pt_cache_t* cache, int64_t batch, int64_t tokens, int64_t width) {
+  try {
+    if (check_pt_cache(cache) != pgr::kOk || check_pt_rows(cache, batch, tokens, width) != pgr::kOk ||
+        check_pt_attend(cache, batch, tokens) != pgr::kOk || batch == 0 || tokens == 0)
+      return 0;
+    return plan_pt(cache, batch, tokens, width).bytes;
+  } catch (...) {
+    exception_status();
+    return 0;
+  }
+}
+
+int pgr_pt_attend(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_t* rows, const void* q,
+                  const int64_t* q_strides, void* out, const uint64_t* masks, const int32_t* depths, int64_t window,
+                  float scale, float softcap, void* workspace, size_t workspace_bytes, void* stream) {
+  try {
+    int rc = check_pt_call(cache, layer, rows);
+    if (rc != pgr::kOk) return rc;
+    rc = check_scores(scale, softcap);
+    if (rc != pgr::kOk) return rc;
+    const int64_t b = rows->batch, t = rows->tokens, hq = cache->query_heads, d = cache->head_dim;
+    rc = check_pt_attend(cache, b, t);
+    if (rc != pgr::kOk) return rc;
+    if ((masks == nullptr) != (depths == nullptr)) return set_err(pgr::kErrInvalid, "masks and depths come together");
+    if (masks != nullptr && t > pgr::kMostDrafts)
+      return set_err(pgr::kErrUnsupported, "a tree has up to 64 tokens");
+    if (window < 0) return set_err(pgr::kErrInvalid, "window must not be negative");
+    if (b == 0 || t == 0) return pgr::kOk;
+    if (!q || !q_strides || !out) return set_err(pgr::kErrInvalid, "null tensor pointer");
+    const PTPlan p = plan_pt(cache, b, t, rows->width);
+    if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < p.bytes))
+      return set_err(pgr::kErrCapacity, "workspace too small");
+    if ((uintptr_t)workspace % 16 != 0) return set_err(pgr::kErrInvalid, "workspace must be 16-byte aligned");
+    const int64_t out_bytes = b * t * hq * d * 2;
+    const Operand in[] = {rows_of(q, q_strides, b, hq, t, d), flat(masks, b * t * 8), numbers(depths, b * t),
+                          table_of(rows), numbers(rows->lengths, b), numbers(rows->counts, b)};
+    for (const Operand& x : in) {
+      if (overlaps(x, out, out_bytes)) return set_err(pgr::kErrInvalid, "out must not overlap the other operands");
+      if (p.bytes > 0 && overlaps(x, workspace, (int64_t)p.bytes))
+        return set_err(pgr::kErrInvalid, "the workspace must not overlap the other operands");
+    }
+    if (in_pages(cache, flat(out, out_bytes)) || (p.bytes > 0 && in_pages(cache, flat(workspace, (int64_t)p.bytes))))
+      return set_err(pgr::kErrInvalid, "out and workspace must not lie in the cache's own buffers");
+    if (p.bytes > 0 && overlaps(flat(out, out_bytes), workspace, (int64_t)p.bytes))
+      return set_err(pgr::kErrInvalid, "the workspace must not overlap the other operands");
+    char* w = static_cast<char*>(workspace);
+    pgr::PTAttendLaunch L;
+    L.c = pages_of(cache, layer);
+    L.r = rows_of_call(rows);
+    L.q = q;
+    L.qs = strides_of(q_strides, 3);
+    L.out = out;
+    L.masks = masks;
+    L.depths = depths;
+    // (A window as long as any row is none.)
+    L.window = window > (int64_t)1 << 30 ? 0 : (int)window;
+    L.scale = scale;
+    L.softcap = softcap;
+    L.plan = p.k;
+    if (p.bytes > 0) {
+      L.pm = reinterpret_cast<float*>(w + p.o_pm);
+      L.pl = reinterpret_cast<float*>(w + p.o_pl);
+      L.pacc = reinterpret_cast<float*>(w + p.o_pacc);
+    }
+    const hipError_t e = pgr::launch_pt_attend(cache->dtype, L, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "attend launch");
+    return pgr::kOk;
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+int pgr_pt_keep(const pgr_pt_cache_t* cache, const pgr_pt_rows_t* rows, const int32_t* path, void* stream) {
+  try {
+    int rc = check_pt_call(cache, 0, rows);
+    if (rc != pgr::kOk) return rc;
+    if (rows->tokens > pgr::kMostDrafts) return set_err(pgr::kErrUnsupported, "a path has up to 64 tokens");
+    if (rows->batch == 0 || rows->tokens == 0) return pgr::kOk;
+    if (!path) return set_err(pgr::kErrInvalid, "null tensor pointer");
+    for (const Operand& x : {numbers(path, rows->batch * rows->tokens), table_of(rows), numbers(rows->lengths, rows->batch)})
+      if (in_pages(cache, x)) return set_err(pgr::kErrInvalid, "operands must not lie in the cache's own buffers");
+    pgr::PTKeepLaunch L;
+    L.c = pages_of(cache, 0);
+    L.r = rows_of_call(rows);
+    L.layers = (int)cache->layers;
+    L.path = path;
+    const hipError_t e = pgr::launch_pt_keep(L, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "keep launch");
+    return pgr::kOk;
+  } catch (...) {
+    return exception_status();
+  }
+}
+
+int pgr_draft_tree(const int32_t* parents, int64_t batch, int64_t tokens, uint64_t* masks, int32_t* depths,
+                   void* stream) {
+  try {
+    if (batch < 0 || tokens < 0) return set_err(pgr::kErrInvalid, "negative dimension");
+    if (tokens > pgr::kMostDrafts) return set_err(pgr::kErrUnsupported, "a tree has up to 64 tokens");
+    if (batch > (1 << 24)) return set_err(pgr::kErrInvalid, "batch must not exceed 2^24");
+    if (batch == 0 || tokens == 0) return pgr::kOk;
+    if (!parents || !masks || !depths) return set_err(pgr::kErrInvalid, "null tensor pointer");
+    const Operand x = numbers(parents, batch * tokens);
+    if (overlaps(x, masks, batch * tokens * 8) || overlaps(x, depths, batch * tokens * 4) ||
+        overlaps(flat(depths, batch * tokens * 4), masks, batch * tokens * 8))
+      return set_err(pgr::kErrInvalid, "outputs must not overlap the other operands");
+    const hipError_t e = pgr::launch_draft_tree(parents, (int)batch, (int)tokens, masks, depths, as_stream(stream));
+    if (e != hipSuccess) return hip_err(e, "tree launch");
     return pgr::kOk;
   } catch (...) {
     return exception_status();

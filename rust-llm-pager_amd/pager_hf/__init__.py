@@ -7,9 +7,11 @@ slot pools) and the fused multi-session decoder ``PagedDecoder``. Operator funct
 from .heavy_hitter_cache import HeavyHitterCache
 from .kv_block_store import KVBlockStore, KVBlockStoreStats
 from .kv_pool import NativeKVPool
+from .page_table_cache import DraftTree, PageTableCache, draft_tree
 from .paged_decode import PagedDecoder
 
-__all__ = ["GenerationStats", "HeavyHitterCache", "KVBlockStore", "KVBlockStoreStats", "NativeKVPool", "PagedDecoder", "PagedModel"]
+__all__ = ["DraftTree", "GenerationStats", "HeavyHitterCache", "KVBlockStore", "KVBlockStoreStats", "NativeKVPool",
+           "PageTableCache", "PagedDecoder", "PagedModel", "draft_tree"]
 
 
 def __getattr__(name):

@@ -226,3 +226,81 @@ def rotary_embedding(
             "rotary_embedding",
         )
     return q_out, k_out
+
+
+def _norm_weight(weight: torch.Tensor, name: str, head_dim: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    if tuple(weight.shape) != (head_dim,):
+        raise ValueError(f"{name} must have shape ({head_dim},), got {tuple(weight.shape)}")
+    if weight.dtype not in (dtype, torch.float32):
+        raise TypeError(f"{name} must be {dtype} or torch.float32, got {weight.dtype}")
+    if weight.device != device:
+        raise ValueError(f"tensors on different devices: {device} and {weight.device}")
+    return weight.contiguous()
+
+
+def norm_rotary_embedding(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor | None,
+    *,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    factor: float = 1.0,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """rotary_embedding of q and k whose heads are normed first: x / sqrt(mean(x^2) + eps) * weight, as models with
+    norms of queries and keys (qwen3) have it.
+
+    Shapes, types, pairs and factor as in rotary_embedding; q_weight and k_weight [D] have q's dtype or are float32,
+    both the same (a norm that multiplies by 1 + w takes 1 + w here). Computed in float32 and rounded once, where a
+    norm and a rotation of their own round twice or more. An inv_freq of no elements norms without a turn."""
+    single = q.dim() == 3
+    if q.dim() not in (3, 4):
+        raise ValueError(f"q must be [B, H, T, D] or [B, H, D], got {tuple(q.shape)}")
+    if k is not None and k.dim() != q.dim():
+        raise ValueError(f"k shape {tuple(k.shape)} does not match q shape {tuple(q.shape)}")
+    if single:
+        if positions.dim() != 1:
+            raise ValueError(f"positions must be [B], got {tuple(positions.shape)}")
+        out = norm_rotary_embedding(q.unsqueeze(2), None if k is None else k.unsqueeze(2), positions.unsqueeze(1),
+                                    inv_freq, q_weight, k_weight, eps=eps, interleaved=interleaved, factor=factor)
+        return out[0].squeeze(2), None if k is None else out[1].squeeze(2)
+    _inference_only(q, k, inv_freq, q_weight, k_weight)
+    b, hq, t, d = q.shape
+    if k is not None and (k.shape[0], k.shape[2], k.shape[3]) != (b, t, d):
+        raise ValueError(f"k shape {tuple(k.shape)} does not match q shape {tuple(q.shape)}")
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError("q and k must share one dtype")
+    if (k is None) != (k_weight is None):
+        raise ValueError("k and k_weight come together")
+    if q.dtype not in _CODES:
+        raise NotImplementedError(f"norm_rotary_embedding takes float16, bfloat16 or float32, got {q.dtype}")
+    device = N.require_cuda(q, k)
+    inv_freq = _inv_freq(inv_freq, d, device)
+    positions = _positions(positions, device)
+    if positions.dim() != 2 or positions.shape[0] not in (1, b) or positions.shape[1] != t:
+        raise ValueError(f"positions must be [{b}, {t}] or [1, {t}], got {tuple(positions.shape)}")
+    positions = positions.expand(b, t)
+    q_weight = _norm_weight(q_weight, "q_weight", d, q.dtype, device)
+    if k is not None:
+        k_weight = _norm_weight(k_weight, "k_weight", d, q.dtype, device)
+        if k_weight.dtype != q_weight.dtype:
+            raise TypeError("q_weight and k_weight must share one dtype")
+    q = _dense_last(q)
+    k = _dense_last(k) if k is not None else None
+    q_out = torch.empty((b, hq, t, d), dtype=q.dtype, device=device)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=device) if k is not None else None
+    with _on(device):
+        N.nat.check(
+            N.lib().pgr_norm_rotary(
+                q.data_ptr(), _strides(q, 3), q_out.data_ptr(), hq, N.ptr(k), _strides(k, 3) if k is not None else None,
+                N.ptr(k_out), k.shape[1] if k is not None else 0, q_weight.data_ptr(), N.ptr(k_weight),
+                q_weight.dtype == torch.float32, float(eps), positions.data_ptr(), positions.dtype == torch.int64,
+                _strides(positions, 2), inv_freq.data_ptr(), 2 * inv_freq.numel(), b, t, d, _CODES[q.dtype],
+                bool(interleaved), float(factor), N.stream_of(device),
+            ),
+            "norm_rotary_embedding",
+        )
+    return q_out, k_out
