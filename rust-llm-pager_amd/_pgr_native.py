@@ -201,7 +201,8 @@ SIGNATURES: dict[str, tuple] = {
     "pgr_pt_attend_workspace_bytes": (c_size, [P(PTCache), c_i64, c_i64, c_i64]),
     "pgr_pt_attend": (
         ctypes.c_int,
-        [P(PTCache), c_i64, P(PTRows), c_vp, P(c_i64), c_vp, c_vp, c_vp, c_i64, c_f32, c_f32, c_vp, c_size, c_vp],
+        [P(PTCache), c_i64, P(PTRows), c_vp, P(c_i64), c_vp, c_vp, c_vp, c_i64, c_f32, c_f32, ctypes.c_int,
+         c_vp, c_size, c_vp],
     ),
     "pgr_pt_keep": (ctypes.c_int, [P(PTCache), P(PTRows), c_vp, c_vp]),
     "pgr_draft_tree": (ctypes.c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),

@@ -40,6 +40,7 @@ struct HalfT {
     return __builtin_bit_cast(uint32_t, h);
   }
   static constexpr float kUnit = 0x1p-14f;
+  static constexpr float kSlack = 1.f;  // log2 of what split's weights may be above 1
   static __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
     constexpr float kLower = (1.f - 0x1p-11f) / kUnit;
     const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x * kLower, y * kLower));
@@ -69,6 +70,7 @@ struct Bf16T {
     return __builtin_bit_cast(uint32_t, h);
   }
   static constexpr float kUnit = 1.f;
+  static constexpr float kSlack = 8.f;
   static __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
     constexpr float kLower = 1.f - 0x1p-8f;
     const uint32_t a = __builtin_bit_cast(uint32_t, x * kLower), b = __builtin_bit_cast(uint32_t, y * kLower);

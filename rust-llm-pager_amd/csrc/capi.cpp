@@ -1667,7 +1667,7 @@ size_t pgr_pt_attend_workspace_bytes(const pgr_pt_cache_t* cache, int64_t batch,
 
 int pgr_pt_attend(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_t* rows, const void* q,
                   const int64_t* q_strides, void* out, const uint64_t* masks, const int32_t* depths, int64_t window,
-                  float scale, float softcap, void* workspace, size_t workspace_bytes, void* stream) {
+                  float scale, float softcap, int exact_weights, void* workspace, size_t workspace_bytes, void* stream) {
   try {
     int rc = check_pt_call(cache, layer, rows);
     if (rc != pgr::kOk) return rc;
@@ -1711,6 +1711,7 @@ int pgr_pt_attend(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_
     L.window = window > (int64_t)1 << 30 ? 0 : (int)window;
     L.scale = scale;
     L.softcap = softcap;
+    L.exact = exact_weights != 0;
     L.plan = p.k;
     if (p.bytes > 0) {
       L.pm = reinterpret_cast<float*>(w + p.o_pm);

@@ -53,9 +53,13 @@ hipError_t launch_pt_append(int dtype, const NormRotaryLaunch& p, hipStream_t st
 
 // How an attend call is dealt out.
 struct PTAttendPlan {
+  int waves = 0;    // of a workgroup whose waves hold 32 rows each; 0: one whose waves share its rows
+  int share = 4;    // waves that share their rows (4 or 8)
   int rows = 16;    // rows (new token x query head of a KV head) of a workgroup
   int blocks = 1;   // blocks of rows
   int n_split = 1;  // parts of a block's tokens (1: no merge launch)
+  int tile = 32;    // tokens
+  int least = 4;    // tiles of a part at least
 };
 PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capacity, int d);
 
@@ -69,6 +73,7 @@ struct PTAttendLaunch {
   const int32_t* depths = nullptr;   // with masks
   int window = 0;                    // 0: none
   float scale = 1.f, softcap = 0.f;
+  int exact = 0;  // P as two numbers also where arithmetic bounds
   PTAttendPlan plan;
   float* pm = nullptr;    // [batch, hkv, blocks, n_split, rows]
   float* pl = nullptr;

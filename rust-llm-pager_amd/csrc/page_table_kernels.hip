@@ -36,10 +36,12 @@ __device__ __forceinline__ Span span_of(const PTAttendLaunch& a, int b, int r0, 
   return s;
 }
 
-// Tiles that a split takes of a block's: evenly, a tile for each wave at least.
-__device__ __forceinline__ int tiles_per_split(const Span& s, int n_split, int waves) {
-  const int tiles = (s.end - s.begin + kTile - 1) / kTile;
-  return max((tiles + n_split - 1) / n_split, waves);
+// Tiles of a block's tokens, and those that a split takes of them.
+__device__ __forceinline__ int tiles_of(const PTAttendPlan& p, const Span& s) {
+  return (s.end - s.begin + p.tile - 1) / p.tile;
+}
+__device__ __forceinline__ int tiles_per_split(const PTAttendPlan& p, const Span& s) {
+  return max((tiles_of(p, s) + p.n_split - 1) / p.n_split, p.least);
 }
 
 // Which tokens a row sees.
@@ -68,12 +70,22 @@ __device__ __forceinline__ Row row_of(const PTAttendLaunch& a, const Span& s, in
   return r;
 }
 
-// (Without branches: selects of a few comparisons.)
-__device__ __forceinline__ bool sees(const PTAttendLaunch& a, const Span& s, const Row& r, int c) {
-  const int j = c - s.length;
-  const bool bit = (r.mask >> (j & 63)) & 1, since = c >= r.lo;
-  const bool fresh = a.masks != nullptr ? bit & (j < s.n) : (j <= r.t) & since;
-  return j < 0 ? since : fresh;
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// Bit i: whether the row sees token first + i (of those before its block's end).
+__device__ __forceinline__ uint64_t sees(const PTAttendLaunch& a, const Span& s, const Row& r, int first) {
+  const int at = first - s.length;  // bit 0's number among the new tokens
+  const uint64_t since = ~low_bits(r.lo - first);
+  if (a.masks == nullptr) return low_bits(r.t + 1 - at) & since;
+  const uint64_t fresh = at >= 64 || at <= -64 ? 0ull : at >= 0 ? r.mask >> at : r.mask << -at;
+  return (low_bits(-at) & since) | fresh;
+}
+
+// cap * log2(e) * tanh(x * scale / cap) as 1 - 2 / (1 + e^2y): within 5 half steps of float32 of the cap, where
+// the scores' own products leave no less (a tanh that is exact to small values costs five times as much).
+__device__ __forceinline__ float capped(float x, const AttendScale& sc) {
+  const float e = __builtin_amdgcn_exp2f(x * (sc.cap_scale * (2.f * kLog2e)));
+  return sc.cap_log2 * fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f);
 }
 
 // The block, split, KV head and batch row of a workgroup. Blocks that read the same tokens are neighbours on one
@@ -99,8 +111,16 @@ __device__ __forceinline__ bool work_of(const PTAttendLaunch& a, Work& w) {
 //     S^T[16 tok x 16 rows] = K . Q^T,   O^T[D x 16 rows] += V^T[D x 32 tok] . P^T[32 tok x 16 rows],
 // here for kG groups of 16 rows, which share a tile's K and its transposed V. The waves take tiles in turn and
 // are joined at the end. A half lies in one page (pages are multiples of 16 tokens), whose index is one
-// scalar load, two tiles ahead. P goes into the product with V as two numbers of the cache's type: rounded to
-// one, the output's error is several times what its other roundings explain where sums all but cancel.
+// scalar load, two tiles ahead. P goes into the product with V as two numbers of the cache's type, which costs
+// nothing beside the loads: rounded to one, the output's error is several times what its other roundings explain
+// where sums all but cancel.
+//
+// Bound by HBM, and for a few rows by the two launches' latency. 8 rows x 8192 tokens, 32/8 heads, D 128, one token: 55 us
+// for 268 MB (4.9 TB/s; a copy reaches 5.1), 8 drafted tokens 61; 2 x 65536 tokens: 99 us for 537 MB. Splits for 256
+// workgroups against 512 / 1024: 54.6 / 54.9 / 56.7 us (one token), 61.9 / 65.0 / 72.9 (eight), one row of 28/4 heads
+// 14.4 either way, 16 rows of 4096 tokens, D 64: 19.5 / 21.0 / 21.8. Short rows are finished by one workgroup of
+// eight waves, without a merge: 256 tokens, D 64 6.7 us against 9.4, D 128 8.2 against 10.4; at 512 and 256 tokens
+// (D 128 and 256) the two are even.
 template <class Ty, int D, int kG, int kW>
 __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, AttendScale sc) {
   typedef KVTile<D> T;
@@ -112,7 +132,7 @@ __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, At
   const PTPages& c = a.c;
   const int b = wk.b, h = wk.h, n_rep = c.hq / c.hkv, r0 = wk.block * kRows;
   const Span sp = span_of(a, b, r0, kRows, n_rep);
-  const int per = tiles_per_split(sp, a.plan.n_split, kW);
+  const int per = tiles_per_split(a.plan, sp);
   const int begin = min(sp.begin + wk.split * per * kTile, sp.end), end = min(begin + per * kTile, sp.end);
   // (The merge reads only the splits that hold tokens; a block that is finished here writes its zeros.)
   if (a.plan.n_split > 1 && begin >= end) return;
@@ -224,18 +244,16 @@ __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, At
       float p[8], top = kMinusInf;
       if (sc.cap_log2 > 0.f) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = sc.cap_log2 * tanhf(s[y][i / 4][i & 3] * sc.cap_scale);
+        for (int i = 0; i < 8; ++i) p[i] = capped(s[y][i / 4][i & 3], sc);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = s[y][i / 4][i & 3] * sc.scale_log2;
       }
       if (masked) {
+        const uint32_t here = (there(at.page[0]) ? 0xffffu : 0u) | (there(at.page[1]) ? 0xffff0000u : 0u);
+        const uint32_t seen = (uint32_t)sees(a, sp, row[y], c0 + 4 * g) & (uint32_t)low_bits(end - c0 - 4 * g) & here >> 4 * g;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int tok = c0 + 16 * (i / 4) + 4 * g + (i & 3);
-          const bool seen = (tok < end) & there(at.page[i / 4]) & sees(a, sp, row[y], tok);
-          p[i] = seen ? p[i] : kMinusInf;
-        }
+        for (int i = 0; i < 8; ++i) p[i] = seen >> (16 * (i / 4) + (i & 3)) & 1 ? p[i] : kMinusInf;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = fmaxf(top, p[i]);
@@ -335,37 +353,329 @@ __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, At
   }
 }
 
-// Joins the splits: groups of d / 4 threads take a row each.
-template <class Ty>
-__global__ __launch_bounds__(256) void pt_merge_kernel(PTAttendLaunch a, int waves) {
+// Max and sum over the lanes l and l + 32.
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// ---------------------------------------------------------------------------------------
+// Attention of many rows a KV head (trees of several heads, a prompt's chunks): bound by arithmetic, so each wave
+// holds 32 rows on v_mfma_f32_32x32x16 and all waves fold the same tile of kTok tokens, which passes through LDS
+// once for all of them:
+//     S^T[32 tok x 32 rows] = K . Q^T,   O^T[32 dims x 32 rows] += V^T[32 dims x 16 tok] . P^T[16 tok x 32 rows].
+// Lane (h, n) = (l / 32, l % 32) holds tokens 8 (i / 4) + 4 h + i % 4, i < 16, of row n, which is the P^T operand as it
+// stands; V^T comes from V's rows by the transposing LDS read, four tokens at a time. The 16-byte pieces of a row
+// lie in LDS at their number XORed with bits of the row's, so that neither the 16 rows that an operand of K
+// takes one piece of, nor the four rows of a transposing read, meet in one bank. The next tile's loads are under way
+// in registers while this one is folded.
+//
+// kTwo: P as two numbers, as where the loads bound; here the second product is half as much arithmetic again, so
+// that the caller chooses (P rounded to one number of the cache's type is off by half a step of each weight). A chunk
+// of 2048 tokens over 16384, 32/8 heads, D 128: 664 us with one number (880 TFLOP/s; a library's matrix product
+// reaches 1244), 879 with two; the kernel above took 1265. Trees of 64 tokens over 8 rows of 32768, 28/4: 323 and 405 us
+// (598). Eight waves (one workgroup a CU) against four: 664 and 752 us, 323 and 355; 128 rows, 8 x 8192 tokens:
+// 74 and 76; few workgroups (448 rows, 1000 tokens) 15.4 and 13.5. Up to 32 rows the kernel above is as fast or faster
+// (8 rows x 8192: 61 us; 48 rows here 65, there 80).
+template <int D>
+struct Staged {
+  static constexpr int kPieces = D / 8;  // 16-byte pieces of a token
+  static __device__ __forceinline__ int k_at(int token, int piece) {
+    const int f = kPieces >= 16 ? token & 15 : token / (16 / kPieces) & (kPieces - 1);
+    return token * kPieces + (piece ^ f);
+  }
+  static __device__ __forceinline__ int v_at(int token, int piece) {
+    const int f = kPieces >= 16 ? (token & 3) << 2 : kPieces == 8 ? (token >> 1 & 1) << 2 : 0;
+    return token * kPieces + (piece ^ f);
+  }
+};
+
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+
+template <class Ty, int D, int kW, bool kTwo>
+__global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kernel(PTAttendLaunch a, AttendScale sc) {
+  typedef Staged<D> L;
+  constexpr int kTok = D == 256 ? 32 : 64, kThreads = 64 * kW, kRows = 32 * kW, kHalves = kTok / 32;
+  constexpr int kTilePieces = kTok * L::kPieces, kEach = kTilePieces / kThreads;
+  static_assert(kTilePieces % kThreads == 0 && kThreads % L::kPieces == 0, "whole pieces a thread, in one column");
+  __shared__ u32x4 k_s[2][kTilePieces], v_s[2][kTilePieces];
+  __shared__ uint32_t held_s[2][kTok];  // whether the tile's token is one that the block reads
+  Work wk;
+  if (!work_of(a, wk)) return;
   const PTPages& c = a.c;
-  const int d = c.d, n_rep = c.hq / c.hkv, cols = d / 4, b = blockIdx.z, h = blockIdx.y;
-  const int r = blockIdx.x * (256 / cols) + threadIdx.x / cols, e = threadIdx.x % cols * 4;
-  const int tok = r / n_rep;
+  const int b = wk.b, h_kv = wk.h, n_rep = c.hq / c.hkv;
+  const Span sp = span_of(a, b, wk.block * kRows, kRows, n_rep);
+  const int per = tiles_per_split(a.plan, sp);
+  const int begin = min(sp.begin + wk.split * per * kTok, sp.end), end = min(begin + per * kTok, sp.end);
+  if (a.plan.n_split > 1 && begin >= end) return;
+  const int tiles = (end - begin + kTok - 1) / kTok;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int h = lane >> 5, n = lane & 31;
+  const int32_t* table = a.r.table + b * a.r.table_stride;
+  const int in_page = (1 << c.page_shift) - 1;
+
+  // Loads: thread tid takes piece tid % kPieces of tokens tid / kPieces + i * (kThreads / kPieces).
+  const int piece = tid % L::kPieces, first_token = tid / L::kPieces;
+  constexpr int kApart = kThreads / L::kPieces;
+  const uint16_t* kp = static_cast<const uint16_t*>(c.keys) + ((int64_t)h_kv * D << c.page_shift) + piece * 8;
+  const uint16_t* vp = static_cast<const uint16_t*>(c.values) + ((int64_t)h_kv * D << c.page_shift) + piece * 8;
+  int32_t page[kEach];
+  u32x4 kr[kEach], vr[kEach];
+  uint32_t held = 0;  // bit i: token i of the thread's is read
+  auto pages = [&](int ti) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      page[i] = table[min(begin + ti * kTok + first_token + i * kApart, end - 1) >> c.page_shift];
+  };
+  auto fetch = [&](int ti) {
+    held = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int tok = begin + ti * kTok + first_token + i * kApart;
+      const bool there = page[i] >= 0 && page[i] < c.pages;
+      held |= (there & (tok >= sp.first) & (tok < end)) ? 1u << i : 0u;
+      // (Behind the end: its last token; a page that is not there: the pool's first.)
+      const int64_t at = (((int64_t)(there ? page[i] : 0) * c.hkv << c.page_shift) + (min(tok, end - 1) & in_page)) * D;
+      kr[i] = *reinterpret_cast<const u32x4*>(kp + at);
+      vr[i] = *reinterpret_cast<const u32x4*>(vp + at);
+    }
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int t = first_token + i * kApart;
+      const bool ok = held >> i & 1;
+      k_s[buf][L::k_at(t, piece)] = kr[i];
+      v_s[buf][L::v_at(t, piece)] = ok ? vr[i] : u32x4{0u, 0u, 0u, 0u};  // (NaN times a weight of 0 is NaN)
+      if (piece == 0) held_s[buf][t] = ok;
+    }
+  };
+  if (tiles > 0) {
+    pages(0);
+    fetch(0);
+    pages(min(1, tiles - 1));
+  }
+
+  // The wave's rows.
+  const int r0 = wk.block * kRows + 32 * wave, r = r0 + n, tok = r / n_rep, head = h_kv * n_rep + (r - tok * n_rep);
+  const int t_first = r0 / n_rep, t_last = min((r0 + 31) / n_rep, sp.n - 1);
+  const bool busy = t_first < sp.n;  // uniform
+  const Row row = row_of(a, sp, b, tok);
+  u32x4 q[D / 16];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) q[i] = u32x4{0u, 0u, 0u, 0u};
+  if (tok < sp.n) {
+    const uint16_t* p = static_cast<const uint16_t*>(a.q) + b * a.qs.b + head * a.qs.h + tok * a.qs.t + 8 * h;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) q[i] = *reinterpret_cast<const u32x4_e*>(p + 16 * i);
+  }
+  int lo_most = row.lo;
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) lo_most = max(lo_most, __shfl_xor(lo_most, m));
+  lo_most = __builtin_amdgcn_readfirstlane(lo_most);
+  const int seen_by_all = a.masks != nullptr ? sp.length : sp.length + t_first + 1;
+  const int seen_by_none = a.masks != nullptr ? sp.end : sp.length + t_last + 1;
+
+  if (tiles > 0) put(0);
+  __syncthreads();
+  arrived(q);
+
+  float m_run = kMinusInf, l_run = 0.f;
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
+
+  // The lane's places in a tile: of K piece 2 i + h of token n, of V its part of the transposing reads.
+  int k_at[D / 16], v_at[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) k_at[i] = L::k_at(n, 2 * i + h);
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+    v_at[j] = L::v_at(4 * h + ((lane & 15) >> 2), 4 * j + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) * 8 + 4 * (lane & 1);
+
+  auto fold = [&](int ti, int buf) {
+    const int c0 = begin + ti * kTok;
+    f32x16 s[kHalves];
+#pragma unroll
+    for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[x][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int x = 0; x < kHalves; ++x) s[x] = Ty::mma32(k_s[buf][k_at[i] + 32 * x * L::kPieces], q[i], s[x]);
+    const uint64_t here = __ballot(held_s[buf][lane & (kTok - 1)] != 0);
+    // Uniform: some row of the wave may not see some token of the tile.
+    const bool masked = ~here != 0 || c0 < lo_most || c0 + kTok > seen_by_all;
+    // (Scores stay as the products left them, `unit` of them in log2 units: one multiply-add before the exponential.)
+    float top = kMinusInf, unit = sc.scale_log2;
+    if (sc.cap_log2 > 0.f) {
+      unit = 1.f;
+#pragma unroll
+      for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[x][i] = capped(s[x][i], sc);
+    }
+    if (masked) {
+      const uint64_t seen = sees(a, sp, row, c0 + 4 * h) & here >> 4 * h;
+#pragma unroll
+      for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[x][i] = (uint32_t)(seen >> 32 * x) >> (8 * (i / 4) + i % 4) & 1 ? s[x][i] : kMinusInf;
+    }
+#pragma unroll
+    for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
+    top = max_halves(top) * unit;
+    // The reference of the weights follows the maximum where that is more than kSlack above it: weights are up to
+    // 2^kSlack then, which both parts of P hold.
+    if (__any(top > m_run + Ty::kSlack)) {
+      const float m_new = fmaxf(m_run, top);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == kMinusInf ? 0.f : m_new));
+      l_run *= alpha;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) acc[j] *= alpha;
+      m_run = m_new;
+    }
+    const float ref = m_run == kMinusInf ? 0.f : m_run;  // (scores of -inf weigh nothing, those of NaN stay NaN)
+#pragma unroll
+    for (int x = 0; x < kHalves; ++x) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[x][i] = __builtin_amdgcn_exp2f(fmaf(s[x][i], unit, -ref));
+      float sum[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = (s[x][4 * i] + s[x][4 * i + 1]) + (s[x][4 * i + 2] + s[x][4 * i + 3]);
+      l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        u32x4 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = s[x][8 * y + 2 * i], p1 = s[x][8 * y + 2 * i + 1];
+          if constexpr (kTwo) {
+            uint32_t u, v;
+            Ty::split(p0, p1, u, v);
+            hi[i] = u;
+            lo[i] = v;
+          } else {
+            hi[i] = Ty::pack(p0 * (1.f / Ty::kUnit), p1 * (1.f / Ty::kUnit));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          typedef __attribute__((address_space(3))) i16x4_t Lds;
+          const uint16_t* at = reinterpret_cast<const uint16_t*>(v_s[buf]) + v_at[j] + (32 * x + 16 * y) * D;
+          const i16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)at);
+          const i16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at + 8 * D));
+          const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+          const u32x4 vt = {w0.x, w0.y, w1.x, w1.y};
+          if constexpr (kTwo) acc[j] = Ty::mma32(vt, lo, acc[j]);
+          acc[j] = Ty::mma32(vt, hi, acc[j]);
+        }
+      }
+    }
+  };
+
+  for (int ti = 0; ti < tiles; ++ti) {
+    const int buf = ti & 1;
+    if (ti + 1 < tiles) {
+      fetch(ti + 1);
+      pages(min(ti + 2, tiles - 1));
+    }
+    if (busy && begin + ti * kTok < seen_by_none) fold(ti, buf);
+    if (ti + 1 < tiles) put(buf ^ 1);
+    __syncthreads();
+  }
+
+  const float l = sum_halves(l_run);
   if (tok >= a.r.tokens) return;
+  if (a.plan.n_split == 1) {
+    uint16_t* out = static_cast<uint16_t*>(a.out) + (((int64_t)b * a.r.tokens + tok) * c.hq + head) * D + 4 * h;
+    const bool none = tok >= sp.n || l == 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = Ty::cvt(none ? 0.f : acc[j][4 * i + e] * Ty::kUnit / l);
+        *reinterpret_cast<u32x2_e*>(out + 32 * j + 8 * i) = u32x2{y[0] | y[1] << 16, y[2] | y[3] << 16};
+      }
+    return;
+  }
+  const int64_t part = ((((int64_t)b * c.hkv + h_kv) * a.plan.blocks + wk.block) * a.plan.n_split + wk.split) * kRows +
+                       32 * wave + n;
+  if (h == 0) {
+    a.pm[part] = m_run;
+    a.pl[part] = l;
+  }
+  float* to = a.pacc + part * D + 4 * h;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4*>(to + 32 * j + 8 * i) =
+          f32x4{acc[j][4 * i], acc[j][4 * i + 1], acc[j][4 * i + 2], acc[j][4 * i + 3]} * Ty::kUnit;
+}
+
+// Joins the splits of a row: `groups` groups of d / 4 threads take splits in turn, four dims a thread, under a maximum
+// of their own, and are joined through LDS. Rows and groups fill a workgroup.
+template <class Ty>
+__global__ __launch_bounds__(256) void pt_merge_kernel(PTAttendLaunch a, int groups) {
+  __shared__ float m_s[256], l_s[256];
+  __shared__ f32x4 x_s[256];
+  const PTPages& c = a.c;
+  const int d = c.d, n_rep = c.hq / c.hkv, cols = d / 4, b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+  const int unit = tid / cols, e = (tid - unit * cols) * 4, g = unit % groups;
+  const int r = blockIdx.x * (256 / cols / groups) + unit / groups, tok = r / n_rep;
+  const bool real = tok < a.r.tokens;
   const int block = r / a.plan.rows, in = r - block * a.plan.rows;
   const Span sp = span_of(a, b, block * a.plan.rows, a.plan.rows, n_rep);
-  const int tiles = (sp.end - sp.begin + kTile - 1) / kTile, per = tiles_per_split(sp, a.plan.n_split, waves);
-  const int used = (tiles + per - 1) / per;
+  const int per = tiles_per_split(a.plan, sp), used = real ? (tiles_of(a.plan, sp) + per - 1) / per : 0;
   const int64_t part = (((int64_t)b * c.hkv + h) * a.plan.blocks + block) * a.plan.n_split * a.plan.rows + in;
   float m = kMinusInf, l = 0.f;
-  for (int s = 0; s < used; ++s) m = fmaxf(m, a.pm[part + (int64_t)s * a.plan.rows]);
-  const float ref = m == kMinusInf ? 0.f : m;
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < used; ++s) {
+  for (int s = g; s < used; s += groups) m = fmaxf(m, a.pm[part + (int64_t)s * a.plan.rows]);
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  const float own = m == kMinusInf ? 0.f : m;
+#pragma unroll 4
+  for (int s = g; s < used; s += groups) {
     const int64_t at = part + (int64_t)s * a.plan.rows;
-    const float f = __builtin_amdgcn_exp2f(a.pm[at] - ref);
+    const float f = __builtin_amdgcn_exp2f(a.pm[at] - own);
     l += a.pl[at] * f;
     x += *reinterpret_cast<const f32x4*>(a.pacc + at * d + e) * f;
   }
+  if (groups > 1) {
+    m_s[tid] = m;
+    l_s[tid] = l;
+    x_s[tid] = x;
+    __syncthreads();
+    if (g != 0) return;
+    for (int k = 1; k < groups; ++k) m = fmaxf(m, m_s[tid + k * cols]);
+    const float all = m == kMinusInf ? 0.f : m;
+    l = 0.f;
+    x = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < groups; ++k) {
+      const float f = __builtin_amdgcn_exp2f(m_s[tid + k * cols] - all);
+      l += l_s[tid + k * cols] * f;
+      x += x_s[tid + k * cols] * f;
+    }
+  }
+  if (!real) return;
   const bool none = tok >= sp.n || l == 0.f;
-  uint16_t y[4];
+  uint32_t y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] = Ty::cvt(none ? 0.f : x[i] / l);
   const int64_t head = ((int64_t)b * a.r.tokens + tok) * c.hq + h * n_rep + (r - tok * n_rep);
-  *reinterpret_cast<u32x2_e*>(static_cast<uint16_t*>(a.out) + head * d + e) =
-      u32x2{(uint32_t)y[0] | (uint32_t)y[1] << 16, (uint32_t)y[2] | (uint32_t)y[3] << 16};
+  *reinterpret_cast<u32x2_e*>(static_cast<uint16_t*>(a.out) + head * d + e) = u32x2{y[0] | y[1] << 16, y[2] | y[3] << 16};
 }
 
 // ---------------------------------------------------------------------------------------
@@ -448,34 +758,53 @@ __global__ __launch_bounds__(64) void draft_tree_kernel(const int32_t* parents, 
   }
 }
 
-template <class Ty, int D, int kG>
+template <class Ty, int D>
 hipError_t attend_dim(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
   const int64_t parts = (int64_t)p.r.batch * p.c.hkv * p.plan.n_split;
   const dim3 grid((unsigned)((parts + 7) / 8 * 8 * p.plan.blocks));
-  pt_attend_kernel<Ty, D, kG, 4><<<grid, 256, 0, stream>>>(p, sc);
+  if (p.plan.waves == 0) {
+    if (p.plan.rows == 16 && p.plan.share == 4) pt_attend_kernel<Ty, D, 1, 4><<<grid, 256, 0, stream>>>(p, sc);
+    if constexpr (D < 256) {
+      if (p.plan.rows == 16 && p.plan.share == 8) pt_attend_kernel<Ty, D, 1, 8><<<grid, 512, 0, stream>>>(p, sc);
+      if (p.plan.rows == 32) pt_attend_kernel<Ty, D, 2, 4><<<grid, 256, 0, stream>>>(p, sc);
+    }
+  } else if constexpr (D >= 32) {
+    if (p.plan.waves == 4) {
+      if (p.exact)
+        pt_attend_wide_kernel<Ty, D, 4, true><<<grid, 256, 0, stream>>>(p, sc);
+      else
+        pt_attend_wide_kernel<Ty, D, 4, false><<<grid, 256, 0, stream>>>(p, sc);
+    }
+    if constexpr (D == 64 || D == 128) {
+      if (p.plan.waves == 8) {
+        if (p.exact)
+          pt_attend_wide_kernel<Ty, D, 8, true><<<grid, 512, 0, stream>>>(p, sc);
+        else
+          pt_attend_wide_kernel<Ty, D, 8, false><<<grid, 512, 0, stream>>>(p, sc);
+      }
+    }
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.plan.n_split == 1) return e;
-  const int rows = p.r.tokens * (p.c.hq / p.c.hkv), each = 256 / (D / 4);
+  const int rows = p.r.tokens * (p.c.hq / p.c.hkv);
+  int groups = 1;
+  while (2 * groups <= p.plan.n_split && 2 * groups <= 256 / (D / 4) &&
+         (int64_t)rows * p.c.hkv * p.r.batch * (D / 4) * groups < 256 * 512)
+    groups *= 2;
+  const int each = 256 / (D / 4) / groups;
   const dim3 merge((unsigned)((rows + each - 1) / each), (unsigned)p.c.hkv, (unsigned)p.r.batch);
-  pt_merge_kernel<Ty><<<merge, 256, 0, stream>>>(p, 4);
+  pt_merge_kernel<Ty><<<merge, 256, 0, stream>>>(p, groups);
   return hipGetLastError();
-}
-
-template <class Ty, int D>
-hipError_t attend_rows(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
-  if constexpr (D < 256)
-    if (p.plan.rows == 32) return attend_dim<Ty, D, 2>(p, sc, stream);
-  return attend_dim<Ty, D, 1>(p, sc, stream);
 }
 
 template <class Ty>
 hipError_t attend(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
   switch (p.c.d) {
-    case 16: return attend_rows<Ty, 16>(p, sc, stream);
-    case 32: return attend_rows<Ty, 32>(p, sc, stream);
-    case 64: return attend_rows<Ty, 64>(p, sc, stream);
-    case 128: return attend_rows<Ty, 128>(p, sc, stream);
-    default: return attend_rows<Ty, 256>(p, sc, stream);
+    case 16: return attend_dim<Ty, 16>(p, sc, stream);
+    case 32: return attend_dim<Ty, 32>(p, sc, stream);
+    case 64: return attend_dim<Ty, 64>(p, sc, stream);
+    case 128: return attend_dim<Ty, 128>(p, sc, stream);
+    default: return attend_dim<Ty, 256>(p, sc, stream);
   }
 }
 
@@ -483,12 +812,35 @@ hipError_t attend(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t st
 
 PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capacity, int d) {
   PTAttendPlan p;
-  const int rows = tokens * (hq / hkv);
-  p.rows = rows > 16 && d < 256 ? 32 : 16;
-  p.blocks = (rows + p.rows - 1) / p.rows;
-  const int64_t groups = (int64_t)batch * hkv * p.blocks;
-  const int64_t most = (capacity + 4 * kTile - 1) / (4 * kTile);  // a tile for each wave
-  int64_t n = (1024 + groups - 1) / groups;
+  const int64_t rows = (int64_t)tokens * (hq / hkv), units = (int64_t)batch * hkv;
+  int64_t target = 256;  // workgroups that the card holds at once, or that fill it
+  if (rows > 32 && d >= 32) {
+    p.tile = d == 256 ? 32 : 64;
+    p.least = 2;
+    p.waves = 4;
+    if (rows > 64 && (d == 64 || d == 128) && units * ((rows + 255) / 256) * (capacity / 128) >= 256) p.waves = 8;
+    if (p.waves == 4 && d < 256) target = 512;
+    p.rows = 32 * p.waves;
+  } else {
+    p.rows = rows > 16 && d < 256 ? 32 : 16;
+  }
+  p.blocks = (int)((rows + p.rows - 1) / p.rows);
+  if (p.rows == 16 && capacity * (d < 64 ? 64 : d) <= 1 << 15) {  // one workgroup finishes a row
+    if (d < 256) p.share = p.least = 8;
+    return p;
+  }
+  const int64_t groups = units * p.blocks, most = (capacity + p.least * p.tile - 1) / (p.least * p.tile);
+  int64_t n = target / groups;
+  if (2 * groups > target) {  // whole rounds, as far as a few splits bring them
+    double best = 1e30;
+    for (int k = 1; k <= 4; ++k) {
+      const double cost = (double)((groups * k + target - 1) / target) / k + (k > 1 ? 0.05 + 0.01 * k : 0.);
+      if (cost < best) {
+        best = cost;
+        n = k;
+      }
+    }
+  }
   if (n > most) n = most;
   p.n_split = n < 1 ? 1 : (int)n;
   return p;

@@ -217,7 +217,7 @@ class PageTableCache:
 
     def attend(self, layer: int, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
                counts: torch.Tensor | None = None, tree: DraftTree | None = None, window: int | None = None,
-               softcap: float | None = None, scale: float | None = None) -> torch.Tensor:
+               softcap: float | None = None, scale: float | None = None, exact_weights: bool = False) -> torch.Tensor:
         """Attention of the new tokens' queries q [B, Hq, T, D] (or [B, Hq, D]) over what their rows hold and, among
         the new tokens (appended before, with the same lengths), over those before them and themselves, or those
         that the tree's masks name.
@@ -227,7 +227,11 @@ class PageTableCache:
         in memory: out.transpose(1, 2).reshape(B, T, -1) is the output projection's input and copies nothing.
         Zeros for columns that are not a row's own, for a token that sees nothing and for a head whose scores are all
         -inf. What the pages hold behind a row's new tokens does not matter, nor what they hold before the window of
-        its first new one (nor whether those pages are there)."""
+        its first new one (nor whether those pages are there).
+
+        The probabilities enter the product with V as two numbers of the cache's type, whose rounding does not show;
+        where more than 32 tokens times query heads per KV head make arithmetic the call's bound they are rounded to
+        one, each off by up to half a step of the type, unless ``exact_weights`` (a third more time at such sizes)."""
         _inference_only(q)
         layer = self._layer(layer)
         x = self._new(q, self.num_query_heads, "q")
@@ -244,7 +248,7 @@ class PageTableCache:
                 N.lib().pgr_pt_attend(
                     self._ref, layer, ctypes.byref(rows), x.data_ptr(), _strides(x, 3), out.data_ptr(), N.ptr(masks),
                     N.ptr(depths), int(window or 0), 1.0 / d**0.5 if scale is None else float(scale),
-                    float(softcap or 0.0), N.ptr(ws), nbytes, N.stream_of(self.device),
+                    float(softcap or 0.0), bool(exact_weights), N.ptr(ws), nbytes, N.stream_of(self.device),
                 ),
                 "PageTableCache.attend",
             )

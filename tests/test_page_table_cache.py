@@ -37,7 +37,7 @@ def _append(c=None, layer=0, r=None, q=FAR, k=FAR, v=FAR, q_out=8 << 20, positio
 def _attend(c=None, layer=0, r=None, q=FAR, out=8 << 20, masks=None, depths=None, window=0, scale=1.0, softcap=0.0,
             ws=16 << 20, nbytes=1 << 20, strides=S):
     return nat.load().pgr_pt_attend(c or _cache(), layer, r or _rows(), q, strides, out, masks, depths, window, scale, softcap,
-                                    ws, nbytes, None)
+                                    0, ws, nbytes, None)
 
 
 def _keep(c=None, r=None, path=FAR):

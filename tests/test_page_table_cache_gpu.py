@@ -252,15 +252,17 @@ def test_append_agrees_with_the_operators_apart():
 
 
 # ---- attend --------------------------------------------------------------------------------------
-def _attend_bounds(dtype):
-    """P enters the product with V as two numbers, off by 3 u^2 of it, u half a step; in fp16 under a largest value of
-    2^14, so that half of the smallest subnormal is 2^-39 of it."""
+def _attend_bounds(dtype, two=True):
+    """P enters the product with V as two numbers, off by 3 u^2 of it, u half a step, or rounded to one, off by u; in fp16
+    under a largest value of at least 2^14, so that half of the smallest subnormal is 2^-39 of it."""
     u = STEP[dtype]
-    return dict(step=u, p_step=3 * u * u, p_floor=2.0**-39 if dtype == torch.float16 else 0.0)
+    return dict(step=u, p_step=3 * u * u if two else u, p_floor=2.0**-39 if dtype == torch.float16 else 0.0)
 
 
-def _check_attend(cache, layer, table, lengths, q, out, counts, sees, depth, window, scale, softcap, only=None):
+def _check_attend(cache, layer, table, lengths, q, out, counts, sees, depth, window, scale, softcap, only=None, exact=False):
     b, hq, t, d = q.shape
+    # (As documented: one number where there are more than 32 rows a KV head.)
+    two = exact or t * (hq // cache.num_kv_heads) <= 32
     hkv, page, pages = cache.num_kv_heads, cache.page_tokens, cache.num_pages
     rep, kn, vn, qn = hq // hkv, _np(cache.keys[layer]), _np(cache.values[layer]), _np(q)
     for i, n in enumerate(_clip(counts, b, t)):
@@ -271,7 +273,7 @@ def _check_attend(cache, layer, table, lengths, q, out, counts, sees, depth, win
         for h in range(hkv):
             heads = slice(h * rep, (h + 1) * rep)
             ref, bound = O.attend_row(qn[i, heads], kn[p, h, o], vn[p, h, o], p >= 0, length, n, sees[i], depth[i], window,
-                                      scale, softcap, **_attend_bounds(q.dtype))
+                                      scale, softcap, **_attend_bounds(q.dtype, two))
             rows = slice(0, n) if only is None else [x for x in only if x < n]
             _within(out[i, heads][:, rows], ref[:, rows], bound[:, rows], f"row {i} head {h}")
         assert not out[i, :, n:].any()
@@ -309,12 +311,13 @@ def test_attend(case, kind, dtype):
         tree = draft_tree(_int32(parents))
     before = [cache.keys.clone(), cache.values.clone()]
     scale = 0.3 if kind == "window" else None
+    exact = kind in ("ragged", "tree")
     out = cache.attend(1, q, _int32(table), _int32(lengths), counts=None if counts is None else _int32(counts), tree=tree,
-                       window=window, softcap=softcap, scale=scale)
+                       window=window, softcap=softcap, scale=scale, exact_weights=exact)
     assert out.shape == q.shape and out.transpose(1, 2).is_contiguous()
     for x, y in zip((cache.keys, cache.values), before):
         assert torch.equal(_bits(x), _bits(y))
-    _check_attend(cache, 1, table, lengths, q, out, counts, sees, depth, window, scale or 1.0 / d**0.5, softcap)
+    _check_attend(cache, 1, table, lengths, q, out, counts, sees, depth, window, scale or 1.0 / d**0.5, softcap, exact=exact)
 
 
 @pytest.mark.parametrize("dtype", CACHE_TYPES)
@@ -348,9 +351,9 @@ def test_attend_keeps_more_of_p_than_the_cache_type(t, d, dtype):
     values[1::2] = -values[: 24 + t - 1: 2][: values[1::2].shape[0]]
     cache.values[0][p, :, o] = values.cuda()
     q = (torch.randn(1, 8, t, d, generator=torch.Generator().manual_seed(4)) / 8).to(dtype).cuda()
-    out = cache.attend(0, q, _int32(table), _int32([24]))
+    out = cache.attend(0, q, _int32(table), _int32([24]), exact_weights=True)
     sees, depth = _order(1, t)
-    _check_attend(cache, 0, table, [24], q, out, None, sees, depth, 0, 1.0 / d**0.5, 0.0)
+    _check_attend(cache, 0, table, [24], q, out, None, sees, depth, 0, 1.0 / d**0.5, 0.0, exact=True)
 
 
 @pytest.mark.parametrize("t", [1, 5, 40])
@@ -373,7 +376,7 @@ def test_attend_with_scores_of_infinity_and_nan(t):
     kn, vn, qn = _np(keys[0]), _np(cache.values[0]), _np(q)
     for h in range(2):
         ref, bound = O.attend_row(qn[0, 2 * h: 2 * h + 2], kn[p, h, o], vn[p, h, o], at, 20, t, sees[0], np.arange(t), 0, 0.125,
-                                  0.0, **_attend_bounds(torch.float16))
+                                  0.0, **_attend_bounds(torch.float16, t < 17))
         _within(some[0, 2 * h: 2 * h + 2], ref, bound, "without the token")
     cache.keys.fill_(float("-inf"))
     assert not cache.attend(0, q, tab, ln).any()
