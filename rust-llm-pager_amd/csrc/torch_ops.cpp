@@ -1,6 +1,6 @@
 // Call path of the operator API for plain tensors: the Python functions of
-// pager_hf/streaming_attention.py, pager_hf/rotary.py and pager_hf/heavy_hitter_cache.py hand their
-// arguments to these before anything else.
+// pager_hf/streaming_attention.py, pager_hf/rotary.py, pager_hf/heavy_hitter_cache.py and
+// pager_hf/page_table_cache.py hand their arguments to these before anything else.
 //
 // Each function checks that its arguments are what the kernels take as they are (exact
 // torch.Tensor objects without functorch, functionalization or lazy-bit keys, one GPU, one
@@ -58,6 +58,12 @@ decltype(&pgr_hh_prompt_weights) g_prompt_weights;
 decltype(&pgr_hh_prompt_weights_workspace_bytes) g_prompt_weights_bytes;
 decltype(&pgr_hh_load_prompt) g_load_prompt;
 decltype(&pgr_hh_load_prompt_workspace_bytes) g_load_prompt_bytes;
+decltype(&pgr_norm_rotary) g_norm_rotary;
+decltype(&pgr_pt_append) g_pt_append;
+decltype(&pgr_pt_attend) g_pt_attend;
+decltype(&pgr_pt_attend_workspace_bytes) g_pt_attend_bytes;
+decltype(&pgr_pt_keep) g_pt_keep;
+decltype(&pgr_draft_tree) g_draft_tree;
 PyObject* g_raw_stream;     // torch._C._cuda_getCurrentRawStream
 PyObject* g_out_of_memory;  // torch.OutOfMemoryError
 
@@ -655,6 +661,303 @@ PyObject* py_bind_cache(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+// ---- drafted tokens over a cache of pages ------------------------------------------------
+// Norm weights: [head_dim] of the operands' type or float32. False: not in the form the kernels read.
+bool norm_weight(PyObject* o, const Tensor& like, int64_t head_dim, const Tensor** out) {
+  const Tensor* t = *out = plain(o);
+  return t && t->dim() == 1 && t->size(0) == head_dim && t->device() == like.device() &&
+         (t->scalar_type() == like.scalar_type() || t->scalar_type() == at::kFloat) && !differentiated(*t);
+}
+
+// norm_rotary(q, k or None, positions, inv_freq, q_weight, k_weight or None, eps, interleaved, factor) -> (status, q',
+// k') or None
+PyObject* py_norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 9)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    if (modes_active() || !THPVariable_CheckExact(a[0])) Py_RETURN_NONE;
+    const int64_t dims = THPVariable_Unpack(a[0]).dim();
+    if (dims != 3 && dims != 4) Py_RETURN_NONE;
+    const bool has_k = a[1] != Py_None;
+    const Tensor *q = viewed(a[0], dims), *k = has_k ? viewed(a[1], dims) : nullptr;
+    if (!q || (has_k && !k) || has_k != (a[5] != Py_None) || !THPVariable_CheckExact(a[2])) Py_RETURN_NONE;
+    const c10::Device dev = q->device();
+    const Tensor* pos = &THPVariable_Unpack(a[2]);
+    if (!pos->defined() || !pos->is_cuda() || !plain_keys(*pos) || !whole_numbers(pos, dev)) Py_RETURN_NONE;
+    const int64_t b = q->size(0), hq = q->size(1), t = dims == 4 ? q->size(2) : 1, d = q->size(-1);
+    const int code = dtype_code(q->scalar_type());
+    if (code < 0 || b == 0 || t == 0 || hq == 0 || d == 0 || pos->dim() != dims - 2) Py_RETURN_NONE;
+    if (dims == 4 ? (pos->size(0) != b && pos->size(0) != 1) || pos->size(1) != t : pos->size(0) != b) Py_RETURN_NONE;
+    const int64_t hk = k ? k->size(1) : 0;
+    if (k && (k->scalar_type() != q->scalar_type() || k->device() != dev || k->size(0) != b ||
+              (dims == 4 && k->size(2) != t) || k->size(-1) != d))
+      Py_RETURN_NONE;
+    const Tensor *qw = nullptr, *kw = nullptr;
+    const float* freq = nullptr;
+    int64_t turning = 0;
+    int interleaved = 0;
+    double factor = 0.0, eps = 0.0;
+    if (!norm_weight(a[4], *q, d, &qw) || (k && (!norm_weight(a[5], *q, d, &kw) || kw->scalar_type() != qw->scalar_type())) ||
+        a[3] == Py_None || !frequencies(a[3], dev, d, &freq, &turning) || !PyFloat_CheckExact(a[6]) ||
+        !number(a[6], 0.0, &eps) || !truth(a[7], &interleaved) || !PyFloat_CheckExact(a[8]) || !number(a[8], 1.0, &factor))
+      Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    const auto opt = at::TensorOptions().dtype(q->scalar_type()).device(dev);
+    Tensor qo = at::empty(q->sizes(), opt), ko;
+    if (k) ko = at::empty(k->sizes(), opt);
+    if (!plain_keys(qo)) Py_RETURN_NONE;
+    const int64_t qs[3] = {q->stride(0), q->stride(1), dims == 4 ? q->stride(2) : 0};
+    const int64_t ks[3] = {k ? k->stride(0) : 0, k ? k->stride(1) : 0, k && dims == 4 ? k->stride(2) : 0};
+    const int64_t ps[2] = {dims == 4 && pos->size(0) == 1 ? 0 : pos->stride(0), dims == 4 ? pos->stride(1) : 0};
+    const void *pq = q->const_data_ptr(), *pk = k ? k->const_data_ptr() : nullptr, *pp = pos->const_data_ptr(),
+               *pqw = qw->const_data_ptr(), *pkw = kw ? kw->const_data_ptr() : nullptr;
+    void *pqo = qo.mutable_data_ptr(), *pko = k ? ko.mutable_data_ptr() : nullptr;
+    const int long_pos = pos->scalar_type() == at::kLong, wide = qw->scalar_type() == at::kFloat;
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_norm_rotary(pq, qs, pqo, hq, pk, ks, pko, hk, pqw, pkw, wide, (float)eps, pp, long_pos, ps, freq, turning, b, t, d,
+                       code, interleaved, (float)factor, stream);
+    Py_END_ALLOW_THREADS;
+    if (!k) return Py_BuildValue("(iNO)", rc, THPVariable_Wrap(qo), Py_None);
+    return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(qo), THPVariable_Wrap(ko));
+  });
+}
+
+const Tensor* plain_of(PyObject* o, at::ScalarType type, const c10::Device& dev, at::IntArrayRef shape) {
+  const Tensor* t = plain(o);
+  return t && t->scalar_type() == type && t->device() == dev && t->sizes() == shape ? t : nullptr;
+}
+
+// table [batch, W], lengths [batch] and counts (None or [batch]) of a call.
+bool page_rows(PyObject* table, PyObject* lengths, PyObject* counts, const c10::Device& dev, int64_t b, int64_t t,
+               pgr_pt_rows_t* r) {
+  const Tensor *x = viewed(table, 2), *n = plain_of(lengths, at::kInt, dev, {b});
+  if (!x || !n || x->scalar_type() != at::kInt || x->device() != dev || x->size(0) != b) return false;
+  if (!mask(counts, dev, {b}, &r->counts)) return false;
+  r->table = x->const_data_ptr<int32_t>();
+  r->table_stride = x->stride(0);
+  r->width = x->size(1);
+  r->lengths = n->const_data_ptr<int32_t>();
+  r->batch = b;
+  r->tokens = t;
+  return true;
+}
+
+// tree: None, or (masks int64, depths int32), [batch, tokens] each.
+bool tree_of(PyObject* o, const c10::Device& dev, int64_t b, int64_t t, const uint64_t** masks, const int32_t** depths) {
+  *masks = nullptr;
+  *depths = nullptr;
+  if (o == Py_None) return true;
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2 || t > 64) return false;
+  const Tensor *m = plain_of(PyTuple_GET_ITEM(o, 0), at::kLong, dev, {b, t}),
+               *d = plain_of(PyTuple_GET_ITEM(o, 1), at::kInt, dev, {b, t});
+  if (!m || !d) return false;
+  *masks = reinterpret_cast<const uint64_t*>(m->const_data_ptr<int64_t>());
+  *depths = d->const_data_ptr<int32_t>();
+  return true;
+}
+
+const pgr_pt_cache_t* pages_at(PyObject* o) {
+  return PyLong_CheckExact(o) ? static_cast<const pgr_pt_cache_t*>(PyLong_AsVoidPtr(o)) : nullptr;
+}
+
+// t is a [batch, heads, tokens, head_dim] or [batch, heads, head_dim] operand of the cache on device `index`.
+bool new_tokens(const Tensor* t, const pgr_pt_cache_t* c, int64_t heads, int64_t index) {
+  return t && dtype_code(t->scalar_type()) == c->dtype && t->device().index() == index && t->size(1) == heads &&
+         t->size(-1) == c->head_dim;
+}
+
+// pt_append(cache, device index, layer, q, k, v, table, lengths, inv_freq or None, counts or None, tree or None,
+// positions or None, q_weight or None, k_weight or None, eps, interleaved, factor) -> (status, q') or None
+PyObject* py_pt_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 17)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const pgr_pt_cache_t* c = pages_at(a[0]);
+    int64_t index = 0, layer = 0;
+    if (modes_active() || !c || !integer(a[1], &index) || !integer(a[2], &layer) || layer < 0 || layer >= c->layers ||
+        !THPVariable_CheckExact(a[3]))
+      Py_RETURN_NONE;
+    const int64_t dims = THPVariable_Unpack(a[3]).dim();
+    if (dims != 3 && dims != 4) Py_RETURN_NONE;
+    const Tensor *q = viewed(a[3], dims), *k = viewed(a[4], dims), *v = viewed(a[5], dims);
+    if (!new_tokens(q, c, c->query_heads, index) || !new_tokens(k, c, c->kv_heads, index) ||
+        !new_tokens(v, c, c->kv_heads, index))
+      Py_RETURN_NONE;
+    const c10::Device dev = q->device();
+    const int64_t b = q->size(0), t = dims == 4 ? q->size(2) : 1;
+    for (const Tensor* x : {k, v})
+      if (x->size(0) != b || (dims == 4 && x->size(2) != t)) Py_RETURN_NONE;
+    pgr_pt_rows_t rows;
+    const uint64_t* masks = nullptr;
+    const int32_t* depths = nullptr;
+    const float* freq = nullptr;
+    int64_t turning = 0;
+    int interleaved = 0;
+    double factor = 0.0, eps = 0.0;
+    if (b == 0 || t == 0 || !page_rows(a[6], a[7], a[9], dev, b, t, &rows) || !tree_of(a[10], dev, b, t, &masks, &depths) ||
+        !frequencies(a[8], dev, c->head_dim, &freq, &turning) || !PyFloat_CheckExact(a[14]) || !number(a[14], 0.0, &eps) ||
+        !truth(a[15], &interleaved) || !PyFloat_CheckExact(a[16]) || !number(a[16], 1.0, &factor))
+      Py_RETURN_NONE;
+    const void *pp = nullptr, *pqw = nullptr, *pkw = nullptr;
+    int64_t ps[2] = {0, 0};
+    int long_pos = 0, wide = 0;
+    if (a[11] != Py_None) {
+      if (!THPVariable_CheckExact(a[11])) Py_RETURN_NONE;
+      const Tensor* pos = &THPVariable_Unpack(a[11]);
+      if (!pos->defined() || !pos->is_cuda() || !plain_keys(*pos) || !whole_numbers(pos, dev) || pos->dim() != dims - 2 ||
+          pos->size(0) != b || (dims == 4 && pos->size(1) != t))
+        Py_RETURN_NONE;
+      pp = pos->const_data_ptr();
+      long_pos = pos->scalar_type() == at::kLong;
+      ps[0] = pos->stride(0);
+      ps[1] = dims == 4 ? pos->stride(1) : 0;
+    }
+    if ((a[12] == Py_None) != (a[13] == Py_None)) Py_RETURN_NONE;
+    if (a[12] != Py_None) {
+      const Tensor *qw = nullptr, *kw = nullptr;
+      if (!norm_weight(a[12], *q, c->head_dim, &qw) || !norm_weight(a[13], *q, c->head_dim, &kw) ||
+          qw->scalar_type() != kw->scalar_type())
+        Py_RETURN_NONE;
+      pqw = qw->const_data_ptr();
+      pkw = kw->const_data_ptr();
+      wide = qw->scalar_type() == at::kFloat;
+    }
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    Tensor qo = at::empty(q->sizes(), at::TensorOptions().dtype(q->scalar_type()).device(dev));
+    if (!plain_keys(qo)) Py_RETURN_NONE;
+    int64_t st[3][3];
+    for (int i = 0; i < 3; ++i) {
+      const Tensor* x = i == 0 ? q : i == 1 ? k : v;
+      st[i][0] = x->stride(0);
+      st[i][1] = x->stride(1);
+      st[i][2] = dims == 4 ? x->stride(2) : 0;
+    }
+    const void *pq = q->const_data_ptr(), *pk = k->const_data_ptr(), *pv = v->const_data_ptr();
+    void* pqo = qo.mutable_data_ptr();
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_pt_append(c, layer, &rows, pq, st[0], pk, st[1], pv, st[2], pqo, pp, long_pos, ps, depths, freq, turning,
+                     interleaved, (float)factor, pqw, pkw, wide, (float)eps, stream);
+    Py_END_ALLOW_THREADS;
+    return Py_BuildValue("(iN)", rc, THPVariable_Wrap(qo));
+  });
+}
+
+// pt_attend(cache, device index, layer, q, table, lengths, counts or None, tree or None, window, softcap, scale,
+// exact_weights) -> (status, out) or None
+PyObject* py_pt_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 12)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const pgr_pt_cache_t* c = pages_at(a[0]);
+    int64_t index = 0, layer = 0, window = 0;
+    if (modes_active() || !c || !integer(a[1], &index) || !integer(a[2], &layer) || layer < 0 || layer >= c->layers ||
+        !THPVariable_CheckExact(a[3]))
+      Py_RETURN_NONE;
+    const int64_t dims = THPVariable_Unpack(a[3]).dim();
+    if (dims != 3 && dims != 4) Py_RETURN_NONE;
+    const Tensor* q = viewed(a[3], dims);
+    if (!new_tokens(q, c, c->query_heads, index)) Py_RETURN_NONE;
+    const c10::Device dev = q->device();
+    const int64_t b = q->size(0), t = dims == 4 ? q->size(2) : 1, hq = c->query_heads, d = c->head_dim;
+    pgr_pt_rows_t rows;
+    const uint64_t* masks = nullptr;
+    const int32_t* depths = nullptr;
+    double scale = 0.0, softcap = 0.0;
+    int exact = 0;
+    if (b == 0 || t == 0 || !page_rows(a[4], a[5], a[6], dev, b, t, &rows) || !tree_of(a[7], dev, b, t, &masks, &depths) ||
+        (a[8] != Py_None && !integer(a[8], &window)) || window < 0 || !number(a[9], 0.0, &softcap) ||
+        !number(a[10], 1.0 / std::pow((double)d, 0.5), &scale) || !truth(a[11], &exact))
+      Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    const size_t bytes = g_pt_attend_bytes(c, b, t, rows.width);
+    const auto opt = at::TensorOptions().dtype(q->scalar_type()).device(dev);
+    Tensor out = dims == 4 ? at::empty({b, t, hq, d}, opt) : at::empty({b, hq, d}, opt);
+    if (!plain_keys(out)) Py_RETURN_NONE;
+    c10::DataPtr ws;
+    if (bytes > 0) ws = at::detail::getCUDAHooks().getCUDADeviceAllocator()->allocate(bytes);
+    const int64_t qs[3] = {q->stride(0), q->stride(1), dims == 4 ? q->stride(2) : 0};
+    const void* pq = q->const_data_ptr();
+    void* po = out.mutable_data_ptr();
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_pt_attend(c, layer, &rows, pq, qs, po, masks, depths, window, (float)scale, (float)softcap, exact, ws.get(), bytes,
+                     stream);
+    Py_END_ALLOW_THREADS;
+    return Py_BuildValue("(iN)", rc, THPVariable_Wrap(dims == 4 ? out.transpose(1, 2) : out));
+  });
+}
+
+// pt_keep(cache, device index, table, lengths, path) -> status or None
+PyObject* py_pt_keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 5)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const pgr_pt_cache_t* c = pages_at(a[0]);
+    int64_t index = 0;
+    if (modes_active() || !c || !integer(a[1], &index)) Py_RETURN_NONE;
+    const Tensor* path = plain(a[4]);
+    if (!path || path->scalar_type() != at::kInt || path->device().index() != index || path->dim() != 2) Py_RETURN_NONE;
+    const c10::Device dev = path->device();
+    pgr_pt_rows_t rows;
+    if (path->numel() == 0 || path->size(1) > 64 ||
+        !page_rows(a[2], a[3], Py_None, dev, path->size(0), path->size(1), &rows))
+      Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    const int32_t* p = path->const_data_ptr<int32_t>();
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_pt_keep(c, &rows, p, stream);
+    Py_END_ALLOW_THREADS;
+    return PyLong_FromLong(rc);
+  });
+}
+
+// draft_tree(parents) -> (status, masks, depths) or None
+PyObject* py_draft_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!ready(n, 1)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    if (modes_active()) Py_RETURN_NONE;
+    const Tensor* x = plain(a[0]);
+    if (!x || x->scalar_type() != at::kInt || x->dim() != 2 || x->numel() == 0) Py_RETURN_NONE;
+    const c10::Device dev = x->device();
+    void* stream = nullptr;
+    if (!current_stream(dev, &stream)) return nullptr;
+    const c10::DeviceGuard guard(dev);
+    Tensor masks = at::empty(x->sizes(), at::TensorOptions().dtype(at::kLong).device(dev)),
+           depths = at::empty(x->sizes(), at::TensorOptions().dtype(at::kInt).device(dev));
+    if (!plain_keys(masks)) Py_RETURN_NONE;
+    const int32_t* p = x->const_data_ptr<int32_t>();
+    uint64_t* pm = reinterpret_cast<uint64_t*>(masks.mutable_data_ptr());
+    int32_t* pd = static_cast<int32_t*>(depths.mutable_data_ptr());
+    const int64_t b = x->size(0), t = x->size(1);
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = g_draft_tree(p, b, t, pm, pd, stream);
+    Py_END_ALLOW_THREADS;
+    return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(masks), THPVariable_Wrap(depths));
+  });
+}
+
+// bind_pages(norm_rotary, pt_append, pt_attend, its workspace size, pt_keep, draft_tree: addresses)
+PyObject* py_bind_pages(PyObject*, PyObject* args) {
+  unsigned long long p[6];
+  if (!PyArg_ParseTuple(args, "KKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5])) return nullptr;
+  auto set = [](auto& fn, unsigned long long addr) { fn = reinterpret_cast<std::decay_t<decltype(fn)>>(addr); };
+  set(g_norm_rotary, p[0]);
+  set(g_pt_append, p[1]);
+  set(g_pt_attend, p[2]);
+  set(g_pt_attend_bytes, p[3]);
+  set(g_pt_keep, p[4]);
+  set(g_draft_tree, p[5]);
+  Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, nullptr},
     {"step", (PyCFunction)(void (*)(void))py_step, METH_FASTCALL, nullptr},
@@ -669,6 +972,12 @@ PyMethodDef methods[] = {
     {"attend", (PyCFunction)(void (*)(void))py_attend, METH_FASTCALL, nullptr},
     {"prompt_weights", (PyCFunction)(void (*)(void))py_prompt_weights, METH_FASTCALL, nullptr},
     {"load_prompt", (PyCFunction)(void (*)(void))py_load_prompt, METH_FASTCALL, nullptr},
+    {"bind_pages", py_bind_pages, METH_VARARGS, nullptr},
+    {"norm_rotary", (PyCFunction)(void (*)(void))py_norm_rotary, METH_FASTCALL, nullptr},
+    {"pt_append", (PyCFunction)(void (*)(void))py_pt_append, METH_FASTCALL, nullptr},
+    {"pt_attend", (PyCFunction)(void (*)(void))py_pt_attend, METH_FASTCALL, nullptr},
+    {"pt_keep", (PyCFunction)(void (*)(void))py_pt_keep, METH_FASTCALL, nullptr},
+    {"draft_tree", (PyCFunction)(void (*)(void))py_draft_tree, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

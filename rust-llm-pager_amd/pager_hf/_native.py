@@ -58,6 +58,8 @@ def bind_ops():
     names = ("rotary", "hh_append", "hh_attend", "hh_prompt_weights", "hh_prompt_weights_workspace_bytes",
              "hh_load_prompt", "hh_load_prompt_workspace_bytes")
     _pgr_ops.bind_cache(*(ctypes.cast(getattr(lib(), "pgr_" + n), ctypes.c_void_p).value for n in names))
+    names = ("norm_rotary", "pt_append", "pt_attend", "pt_attend_workspace_bytes", "pt_keep", "draft_tree")
+    _pgr_ops.bind_pages(*(ctypes.cast(getattr(lib(), "pgr_" + n), ctypes.c_void_p).value for n in names))
     return _pgr_ops
 
 

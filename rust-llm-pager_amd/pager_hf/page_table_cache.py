@@ -51,6 +51,10 @@ def draft_tree(parents: torch.Tensor) -> DraftTree:
 
     parents [B, T] int32: each token's parent, an earlier token of its row; anything else (-1) makes it follow
     the held tokens. Made once a step, for all layers."""
+    done = N.ops().draft_tree(parents)
+    if done is not None:
+        N.nat.check(done[0], "draft_tree")
+        return DraftTree(done[1], done[2])
     if parents.dim() != 2:
         raise ValueError(f"parents must be [B, T], got {tuple(parents.shape)}")
     if parents.dtype != torch.int32:
@@ -100,6 +104,7 @@ class PageTableCache:
         self._c = N.nat.PTCache(self._keys.data_ptr(), self._values.data_ptr(), num_layers, num_pages, num_query_heads,
                                 num_kv_heads, page_tokens, head_dim, code)
         self._ref = ctypes.byref(self._c)
+        self._address, self._index, self._ops = ctypes.addressof(self._c), device.index, N.ops()
 
     # What the kernels go by is fixed with the cache: the buffers can be written to, not replaced.
     num_layers = property(lambda self: self._c.layers)
@@ -175,6 +180,11 @@ class PageTableCache:
         With q_weight and k_weight [D] the heads of q and k are normed as norm_rotary_embedding norms them; with
         ``inv_freq`` (rotary.rotary_frequencies) they are turned, at lengths[b] plus the token's depth in the tree
         (its number, without one), or at positions [B, T] ([B] for one token). ``lengths`` stays as it is."""
+        done = self._ops.pt_append(self._address, self._index, layer, q, k, v, table, lengths, inv_freq, counts, tree,
+                                   positions, q_weight, k_weight, eps, interleaved, factor)
+        if done is not None:
+            N.nat.check(done[0], "PageTableCache.append")
+            return done[1]
         _inference_only(q, k, v, inv_freq, q_weight, k_weight)
         layer = self._layer(layer)
         x = self._new(q, self.num_query_heads, "q")
@@ -232,6 +242,11 @@ class PageTableCache:
         The probabilities enter the product with V as two numbers of the cache's type, whose rounding does not show;
         where more than 32 tokens times query heads per KV head make arithmetic the call's bound they are rounded to
         one, each off by up to half a step of the type, unless ``exact_weights`` (a third more time at such sizes)."""
+        done = self._ops.pt_attend(self._address, self._index, layer, q, table, lengths, counts, tree, window, softcap, scale,
+                                   exact_weights)
+        if done is not None:
+            N.nat.check(done[0], "PageTableCache.attend")
+            return done[1]
         _inference_only(q)
         layer = self._layer(layer)
         x = self._new(q, self.num_query_heads, "q")
@@ -260,6 +275,10 @@ class PageTableCache:
         path [B, A] int32, up to 64 new tokens a row; all move at once, from where they were before the call. An
         entry outside [0, 64) leaves token j as it is (-1 behind the last). ``lengths`` stays as it is: the caller
         adds the number of accepted tokens."""
+        done = self._ops.pt_keep(self._address, self._index, table, lengths, path)
+        if done is not None:
+            N.nat.check(done, "PageTableCache.keep")
+            return
         if path.dim() != 2:
             raise ValueError(f"path must be [B, A], got {tuple(path.shape)}")
         b, t = path.shape

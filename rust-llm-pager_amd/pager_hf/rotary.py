@@ -256,6 +256,10 @@ def norm_rotary_embedding(
     Shapes, types, pairs and factor as in rotary_embedding; q_weight and k_weight [D] have q's dtype or are float32,
     both the same (a norm that multiplies by 1 + w takes 1 + w here). Computed in float32 and rounded once, where a
     norm and a rotation of their own round twice or more. An inv_freq of no elements norms without a turn."""
+    done = N.ops().norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, factor)
+    if done is not None:
+        N.nat.check(done[0], "norm_rotary_embedding")
+        return done[1], done[2]
     single = q.dim() == 3
     if q.dim() not in (3, 4):
         raise ValueError(f"q must be [B, H, T, D] or [B, H, D], got {tuple(q.shape)}")

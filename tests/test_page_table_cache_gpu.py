@@ -727,3 +727,75 @@ def test_refusals():
     assert cache.attend(0, q[:, :, :0], table, ln).shape == (1, 4, 0, 64)
     assert cache.append(0, q[:, :, :0], k[:, :, :0], k[:, :, :0], table, ln, inv).shape == (1, 4, 0, 64)
     cache.keep(table, ln, torch.zeros(1, 0, dtype=torch.int32, device="cuda"))
+
+
+def test_both_call_paths_agree(monkeypatch):
+    """Plain tensors go through the native call path, others through Python; either way the same bits."""
+    from pager_hf import _native as N
+
+    ops = N.ops()
+
+    class Counting:
+        def __init__(self):
+            self.taken = 0
+
+        def __getattr__(self, name):
+            def call(*args):
+                got = getattr(ops, name)(*args)
+                self.taken += got is not None
+                return got
+            return call
+
+    class General:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    rng = np.random.default_rng(67)
+    g = torch.Generator().manual_seed(6)
+    inv, _ = rotary_frequencies(64, device="cuda")
+    x = torch.randn(3, 5, 8, 64, generator=g).half().cuda().transpose(1, 2)
+    w = torch.rand(64, generator=g).half().cuda()
+    parents, counts = _int32(_parents(rng, 3, 5)), _int32([5, 2, 0])
+    pos = torch.randint(0, 999, (3, 5), generator=g).cuda()
+    path = _int32([[1, 4, -1], [0, 2, 3], [3, -1, -1]])
+    forms = {  # name: (overrides, whether every call takes the native path)
+        "plain": (dict(), True),
+        "ragged": (dict(counts=counts, window=7, softcap=3.0, scale=0.2, exact=True), True),
+        "positions": (dict(positions=pos, interleaved=True, factor=1.5, weight=w.float()), True),
+        "strided positions": (dict(positions=pos.t().contiguous().t().int()), True),
+        "no norm, no turn": (dict(weight=None, inv=None), True),
+        "strided table": (dict(wide=True), True),
+        "int softcap": (dict(softcap=2), None),
+        "strided counts": (dict(counts=_int32([[5, 0], [2, 0], [1, 0]])[:, 0]), None),
+        "dense last": (dict(x=x.transpose(2, 3).contiguous().transpose(2, 3)), None),
+    }
+    for name, (o, taken) in forms.items():
+        print(f"call path: {name}", flush=True)
+        got = []
+        for path_taken in (Counting(), General()):
+            monkeypatch.setattr(N, "_ops", path_taken)
+            cache, table = _filled(np.random.default_rng(71), 20, 16, 4, 2, 64, torch.float16, [30, 9, 0], 5, garbage=False)
+            table = _int32(table)
+            if o.get("wide"):
+                table = torch.cat([table, table], dim=1)[:, : table.shape[1]]
+            y = o.get("x", x)
+            q, k, v = y[:, :4], y[:, 4:6], y[:, 6:]
+            weight = o.get("weight", w)
+            common = dict(counts=o.get("counts"), tree=draft_tree(parents))
+            turned = cache.append(0, q, k, v, table, _int32([30, 9, 0]), o.get("inv", inv), positions=o.get("positions"),
+                                  q_weight=weight, k_weight=weight, eps=1e-5, interleaved=o.get("interleaved", False),
+                                  factor=o.get("factor", 1.0), **common)
+            out = cache.attend(0, turned, table, _int32([30, 9, 0]), window=o.get("window"), softcap=o.get("softcap"),
+                               scale=o.get("scale"), exact_weights=o.get("exact", False), **common)
+            one = cache.attend(0, turned[:, :, 0], table, _int32([30, 9, 0]))
+            last = cache.append(0, q[:, :, 0], k[:, :, 0], v[:, :, 0], table, _int32([30, 9, 0]), inv)
+            cache.keep(table, _int32([30, 9, 0]), path)
+            n = norm_rotary_embedding(q, k, pos, inv, w, w, eps=1e-5)
+            n1 = norm_rotary_embedding(q[:, :, 0], None, pos[:, 0], inv, w, None)
+            got.append([turned, out, one, last, cache.keys, cache.values, *n, n1[0], common["tree"].masks,
+                        common["tree"].depths])
+            assert out.stride() == got[0][1].stride() and out.transpose(1, 2).is_contiguous()
+            if isinstance(path_taken, Counting) and taken:
+                assert path_taken.taken == 8, (name, path_taken.taken)
+        for a, b in zip(*got):
+            assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b), name
