@@ -495,6 +495,8 @@ int check_pt_cache(const pgr_pt_cache_t* c) {
     return set_err(pgr::kErrUnsupported, "page_tokens must be 16, 32, 64, 128 or 256");
   if (c->layers <= 0 || c->layers > 65535 || c->pages <= 0 || c->pages > ((int64_t)1 << 30))
     return set_err(pgr::kErrInvalid, "layers must be in [1, 65535] and pages in [1, 2^30]");
+  if (c->layers * c->kv_heads > (int64_t)1 << 28)
+    return set_err(pgr::kErrInvalid, "layers * num_kv_heads must not exceed 2^28");
   if (!c->keys || !c->values) return set_err(pgr::kErrInvalid, "null cache buffer");
   if (((uintptr_t)c->keys | (uintptr_t)c->values) % 16 != 0)
     return set_err(pgr::kErrInvalid, "cache buffers must be 16-byte aligned");

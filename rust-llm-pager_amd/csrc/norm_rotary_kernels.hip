@@ -7,7 +7,10 @@
 // Memory-bound: every element is read and written once. A head is held by the lanes of a group, two
 // 16-byte pieces each: the pieces of a pair's halves where the pairs are (i, i + half), pieces a group's
 // width apart otherwise, so that neighbouring lanes read side by side. The mean is summed over the group
-// by lane exchanges; the angles and weights are taken once for all heads a thread walks.
+// by lane exchanges; the angles and weights are taken once for all heads a thread walks, four heads' pieces asked
+// for at a time. 4 x 8191 tokens, 32/8 heads, D 128, bf16: 137 us for 671 MB (4.9 TB/s; a copy reaches 5.1), 145 with
+// one head after the other; the append of as many, up to 3/8 of a row's columns not its own: 154 us for 704 MB, 173
+// where those columns are read all the same.
 #include <hip/hip_runtime.h>
 
 #include "cache_device.h"
@@ -77,7 +80,7 @@ struct Piece {
 template <class Ty, bool kInterleaved, bool kNorm, bool kPages>
 __global__ __launch_bounds__(256) void norm_rotary_kernel(NormRotaryLaunch a, int log_lanes, int per) {
   typedef typename Ty::Raw Raw;
-  constexpr int kV = Piece<Ty>::kV;
+  constexpr int kV = Piece<Ty>::kV, kAhead = 4;
   const int lanes = a.d / (2 * kV);
   const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> log_lanes;
   const int u = threadIdx.x & ((1 << log_lanes) - 1);
@@ -135,70 +138,90 @@ __global__ __launch_bounds__(256) void norm_rotary_kernel(NormRotaryLaunch a, in
       }
     }
     const Raw* x = static_cast<const Raw*>(a.x[s]) + b * a.xs[s].b + t * a.xs[s].t;
-#pragma unroll 4
-    for (int h = from; h < to; ++h) {
-      const Raw* xh = x + h * a.xs[s].h;
-      Piece<Ty> p = __builtin_bit_cast(Piece<Ty>, (u32x4)*reinterpret_cast<const u32x4_e*>(xh + first));
-      Piece<Ty> q = __builtin_bit_cast(Piece<Ty>, (u32x4)*reinterpret_cast<const u32x4_e*>(xh + second));
-      if (s < 2) {
-        float f[kV], g[kV];
-#pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          f[i] = Ty::to_f(p.e[i]);
-          g[i] = Ty::to_f(q.e[i]);
-        }
-        if constexpr (kNorm) {
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < kV; ++i) sum = fmaf(f[i], f[i], fmaf(g[i], g[i], sum));
-          sum = live ? sum : 0.f;
-          for (int m = 1 << log_lanes >> 1; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
-          const float r = 1.f / sqrtf(sum / (float)a.d + a.norm.eps);
-#pragma unroll
-          for (int i = 0; i < kV; ++i) {
-            f[i] = f[i] * r * w[0][i];
-            g[i] = g[i] * r * w[1][i];
-          }
-        }
-        if constexpr (kInterleaved) {
-          if (first_turns) {
-#pragma unroll
-            for (int i = 0; i < kV / 2; ++i) {
-              const float c = f[2 * i], d = f[2 * i + 1];
-              f[2 * i] = turned_x(c, d, cs[i], sn[i]);
-              f[2 * i + 1] = turned_y(c, d, cs[i], sn[i]);
-            }
-          }
-          if (second_turns) {
-#pragma unroll
-            for (int i = 0; i < kV / 2; ++i) {
-              const float c = g[2 * i], d = g[2 * i + 1];
-              g[2 * i] = turned_x(c, d, cs[kV / 2 + i], sn[kV / 2 + i]);
-              g[2 * i + 1] = turned_y(c, d, cs[kV / 2 + i], sn[kV / 2 + i]);
-            }
-          }
-        } else if (first_turns) {
-#pragma unroll
-          for (int i = 0; i < kV; ++i) {
-            const float c = f[i], d = g[i];
-            f[i] = turned_x(c, d, cs[i], sn[i]);
-            g[i] = turned_y(c, d, cs[i], sn[i]);
-          }
-        }
-        if (kNorm || first_turns) {
-#pragma unroll
-          for (int i = 0; i < kV; ++i) p.e[i] = Ty::cvt(f[i]);
-        }
-        if (kNorm || second_turns) {
-#pragma unroll
-          for (int i = 0; i < kV; ++i) q.e[i] = Ty::cvt(g[i]);
+    if (kPages && !k.has) {  // (a token's lanes go together)
+      if (s == 0 && live) {
+        for (int h = from; h < to; ++h) {
+          Raw* y = reinterpret_cast<Raw*>(target<kPages>(a, k, s, b, h, t, (int)sizeof(Raw)));
+          *reinterpret_cast<u32x4_e*>(y + first) = u32x4{0u, 0u, 0u, 0u};
+          *reinterpret_cast<u32x4_e*>(y + second) = u32x4{0u, 0u, 0u, 0u};
         }
       }
-      if (kPages && s == 0 && !k.has) p = q = Piece<Ty>{};
-      Raw* y = reinterpret_cast<Raw*>(target<kPages>(a, k, s, b, h, t, (int)sizeof(Raw)));
-      if (live && y != nullptr) {
-        *reinterpret_cast<u32x4_e*>(y + first) = __builtin_bit_cast(u32x4, p);
-        *reinterpret_cast<u32x4_e*>(y + second) = __builtin_bit_cast(u32x4, q);
+      continue;
+    }
+    for (int h0 = from; h0 < to; h0 += kAhead) {
+      // (Stores keep the compiler from asking for the next heads' pieces before this one's are written.)
+      u32x4 piece[2 * kAhead];
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) {
+        if (h0 + z >= to) break;  // uniform
+        const Raw* xh = x + (h0 + z) * a.xs[s].h;
+        piece[2 * z] = *reinterpret_cast<const u32x4_e*>(xh + first);
+        piece[2 * z + 1] = *reinterpret_cast<const u32x4_e*>(xh + second);
+      }
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) {
+        const int h = h0 + z;
+        if (h >= to) break;  // uniform
+        Piece<Ty> p = __builtin_bit_cast(Piece<Ty>, piece[2 * z]), q = __builtin_bit_cast(Piece<Ty>, piece[2 * z + 1]);
+        if (s < 2) {
+          float f[kV], g[kV];
+#pragma unroll
+          for (int i = 0; i < kV; ++i) {
+            f[i] = Ty::to_f(p.e[i]);
+            g[i] = Ty::to_f(q.e[i]);
+          }
+          if constexpr (kNorm) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < kV; ++i) sum = fmaf(f[i], f[i], fmaf(g[i], g[i], sum));
+            sum = live ? sum : 0.f;
+            for (int m = 1 << log_lanes >> 1; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
+            const float r = 1.f / sqrtf(sum / (float)a.d + a.norm.eps);
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+              f[i] = f[i] * r * w[0][i];
+              g[i] = g[i] * r * w[1][i];
+            }
+          }
+          if constexpr (kInterleaved) {
+            if (first_turns) {
+#pragma unroll
+              for (int i = 0; i < kV / 2; ++i) {
+                const float c = f[2 * i], d = f[2 * i + 1];
+                f[2 * i] = turned_x(c, d, cs[i], sn[i]);
+                f[2 * i + 1] = turned_y(c, d, cs[i], sn[i]);
+              }
+            }
+            if (second_turns) {
+#pragma unroll
+              for (int i = 0; i < kV / 2; ++i) {
+                const float c = g[2 * i], d = g[2 * i + 1];
+                g[2 * i] = turned_x(c, d, cs[kV / 2 + i], sn[kV / 2 + i]);
+                g[2 * i + 1] = turned_y(c, d, cs[kV / 2 + i], sn[kV / 2 + i]);
+              }
+            }
+          } else if (first_turns) {
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+              const float c = f[i], d = g[i];
+              f[i] = turned_x(c, d, cs[i], sn[i]);
+              g[i] = turned_y(c, d, cs[i], sn[i]);
+            }
+          }
+          if (kNorm || first_turns) {
+#pragma unroll
+            for (int i = 0; i < kV; ++i) p.e[i] = Ty::cvt(f[i]);
+          }
+          if (kNorm || second_turns) {
+#pragma unroll
+            for (int i = 0; i < kV; ++i) q.e[i] = Ty::cvt(g[i]);
+          }
+        }
+        Raw* y = reinterpret_cast<Raw*>(target<kPages>(a, k, s, b, h, t, (int)sizeof(Raw)));
+        if (live && y != nullptr) {
+          *reinterpret_cast<u32x4_e*>(y + first) = __builtin_bit_cast(u32x4, p);
+          *reinterpret_cast<u32x4_e*>(y + second) = __builtin_bit_cast(u32x4, q);
+        }
       }
     }
   }

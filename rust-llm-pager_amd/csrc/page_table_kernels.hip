@@ -680,53 +680,67 @@ __global__ __launch_bounds__(256) void pt_merge_kernel(PTAttendLaunch a, int gro
 
 // ---------------------------------------------------------------------------------------
 // The accepted path to the front: token length + j of each row becomes token length + path[j], as all were
-// before the call. A workgroup moves the keys (z even) or the values of one layer, row and KV head, in
-// 16-byte pieces: all of them are read before the first is written. Entries outside [0, 64) move nothing, nor do
-// those that are in their place. Memory-bound, in short pieces.
-constexpr int kKeepMost = kMostDrafts * 32 / 256;  // pieces a thread: 64 tokens of up to 32 pieces
+// before the call. A workgroup finds the moves of one row once and makes them for its share of the row's planes (a
+// plane: one KV head's keys or values in one layer), in 16-byte pieces. A move never reads what another plane's
+// writes, so a workgroup takes as many planes at a time as its registers hold, reads all of their pieces and writes
+// them behind a barrier. Entries outside [0, 64) move nothing, nor do those that are in their place.
+constexpr int kKeepThreads = 512, kKeepEach = 4;  // pieces a thread holds: 64 tokens of up to 32 are one plane's at most
 
-__global__ __launch_bounds__(256) void pt_keep_kernel(PTKeepLaunch a) {
+__global__ __launch_bounds__(kKeepThreads) void pt_keep_kernel(PTKeepLaunch a, int planes, int share) {
   __shared__ int64_t from_s[kMostDrafts], to_s[kMostDrafts];
+  __shared__ int moves_s;
   const PTPages& c = a.c;
-  const int h = blockIdx.x % c.hkv, b = blockIdx.x / c.hkv, tid = threadIdx.x, tokens = a.r.tokens;
-  const int layer = blockIdx.y;
+  const int b = blockIdx.y, tid = threadIdx.x, tokens = a.r.tokens;
+  // A token's element in its plane's first page (head 0 of layer 0), or -1.
   auto cell = [&](int64_t token) {
     const int64_t page = token >> c.page_shift;
     if (page >= a.r.width) return (int64_t)-1;
     const int32_t p = a.r.table[b * a.r.table_stride + page];
     if (p < 0 || p >= c.pages) return (int64_t)-1;
-    return (((int64_t)p * c.hkv + h << c.page_shift) + (token & (((int64_t)1 << c.page_shift) - 1))) * c.d;
+    return (((int64_t)p * c.hkv << c.page_shift) + (token & (((int64_t)1 << c.page_shift) - 1))) * c.d;
   };
-  bool moves = false;
-  if (tid < tokens) {
-    const int64_t length = max(a.r.lengths[b], 0);
-    const int p = a.path[(int64_t)b * tokens + tid];
+  if (tid < 64) {
     int64_t from = -1, to = -1;
-    if (p >= 0 && p < kMostDrafts && p != tid) {
-      from = cell(length + p);
-      to = cell(length + tid);
+    if (tid < tokens) {
+      const int64_t length = max(a.r.lengths[b], 0);
+      const int p = a.path[(int64_t)b * tokens + tid];
+      if (p >= 0 && p < kMostDrafts && p != tid) {
+        from = cell(length + p);
+        to = cell(length + tid);
+      }
     }
-    moves = from >= 0 && to >= 0;
-    from_s[tid] = moves ? from : -1;
-    to_s[tid] = to;
+    const bool moves = from >= 0 && to >= 0;
+    const uint64_t all = __ballot(moves);
+    if (moves) {
+      const int at = __popcll(all & ((1ull << tid) - 1));
+      from_s[at] = from;
+      to_s[at] = to;
+    }
+    if (tid == 0) moves_s = __popcll(all);
   }
-  if (!__syncthreads_or(moves)) return;
-  const int pieces = c.d / 8, n = tokens * pieces;
-  uint16_t* const pool = static_cast<uint16_t*>(blockIdx.z == 0 ? c.keys : c.values) +
-                         (((int64_t)layer * c.pages * c.hkv << c.page_shift) * c.d);
-  u32x4 x[kKeepMost];
-#pragma unroll
-  for (int i = 0; i < kKeepMost; ++i) {
-    const int at = tid + i * 256, j = at / pieces;
-    x[i] = u32x4{0u, 0u, 0u, 0u};
-    if (at < n && from_s[j] >= 0) x[i] = *reinterpret_cast<const u32x4*>(pool + from_s[j] + (at - j * pieces) * 8);
-  }
-  arrived(x);
   __syncthreads();
+  const int pieces = c.d / 8, n = moves_s * pieces;  // of a plane
+  if (n == 0) return;
+  const int held = kKeepThreads * kKeepEach / n;  // planes at a time
+  const int first = blockIdx.x * share, last = min(first + share, planes);
+  const int64_t page = (int64_t)c.d << c.page_shift, layer = page * c.hkv * c.pages;
+  for (int p0 = first; p0 < last; p0 += held) {
+    const int count = min(held, last - p0) * n;
+    u32x4 x[kKeepEach];
+    uint16_t* to[kKeepEach];
 #pragma unroll
-  for (int i = 0; i < kKeepMost; ++i) {
-    const int at = tid + i * 256, j = at / pieces;
-    if (at < n && from_s[j] >= 0) *reinterpret_cast<u32x4*>(pool + to_s[j] + (at - j * pieces) * 8) = x[i];
+    for (int i = 0; i < kKeepEach; ++i) {
+      const int at = min(tid + i * kKeepThreads, count - 1), p = at / n, in = at - p * n, j = in / pieces;
+      const int plane = p0 + p, half = plane >> 1, l = half / c.hkv, h = half - l * c.hkv;
+      uint16_t* const pool = static_cast<uint16_t*>(plane & 1 ? c.values : c.keys) + l * layer + h * page + (in - j * pieces) * 8;
+      to[i] = pool + to_s[j];
+      x[i] = *reinterpret_cast<const u32x4*>(pool + from_s[j]);
+    }
+    arrived(x);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kKeepEach; ++i)
+      if (tid + i * kKeepThreads < count) *reinterpret_cast<u32x4*>(to[i]) = x[i];
   }
 }
 
@@ -855,8 +869,11 @@ hipError_t launch_pt_attend(int dtype, const PTAttendLaunch& p, hipStream_t stre
 }
 
 hipError_t launch_pt_keep(const PTKeepLaunch& p, hipStream_t stream) {
-  const dim3 grid((unsigned)(p.r.batch * p.c.hkv), (unsigned)p.layers, 2);
-  pt_keep_kernel<<<grid, 256, 0, stream>>>(p);
+  const int planes = 2 * p.layers * p.c.hkv;
+  int parts = (2048 + p.r.batch - 1) / p.r.batch;  // about 2048 workgroups
+  if (parts > planes) parts = planes;
+  const int share = (planes + parts - 1) / parts;
+  pt_keep_kernel<<<dim3((unsigned)((planes + share - 1) / share), (unsigned)p.r.batch), kKeepThreads, 0, stream>>>(p, planes, share);
   return hipGetLastError();
 }
 

@@ -94,8 +94,8 @@ class PageTableCache:
             raise NotImplementedError(f"head_dim must be 16, 32, 64, 128 or 256, got {head_dim}")
         if page_tokens not in (16, 32, 64, 128, 256):
             raise NotImplementedError(f"page_tokens must be 16, 32, 64, 128 or 256, got {page_tokens}")
-        if num_pages > 1 << 30 or num_layers > 65535 or num_kv_heads > 65535:
-            raise ValueError("num_pages must not exceed 2^30, num_layers and num_kv_heads 65535")
+        if num_pages > 1 << 30 or num_layers > 65535 or num_kv_heads > 65535 or num_layers * num_kv_heads > 1 << 28:
+            raise ValueError("num_pages must not exceed 2^30, num_layers and num_kv_heads 65535, nor their product 2^28")
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self._dtype, self._device = dtype, device

@@ -48,7 +48,7 @@ BAD_CACHES = [
     (dict(query_heads=3), INV), (dict(query_heads=34), UNS), (dict(head_dim=48), UNS), (dict(dtype=2), UNS),
     (dict(page_tokens=8), UNS), (dict(page_tokens=48), UNS), (dict(page_tokens=512), UNS), (dict(layers=0), INV),
     (dict(pages=0), INV), (dict(pages=(1 << 30) + 1), INV), (dict(layers=65536), INV), (dict(keys=0), INV),
-    (dict(values=(2 << 20) + 8), INV), (dict(kv_heads=0), INV),
+    (dict(values=(2 << 20) + 8), INV), (dict(kv_heads=0), INV), (dict(layers=65535, kv_heads=8192, query_heads=8192), INV),
 ]
 
 
