@@ -76,11 +76,11 @@ struct Piece {
   typename Ty::Raw e[kV];
 };
 
-// kNorm, kPages as the launch asks; 2^log_lanes lanes hold a head, the first d / (2 kV) of them.
-template <class Ty, bool kInterleaved, bool kNorm, bool kPages>
+// kNorm, kPages as the launch asks; kAhead heads are asked for at a time; 2^log_lanes lanes hold a head, the first d / (2 kV) of them.
+template <class Ty, bool kInterleaved, bool kNorm, bool kPages, int kAhead>
 __global__ __launch_bounds__(256) void norm_rotary_kernel(NormRotaryLaunch a, int log_lanes, int per) {
   typedef typename Ty::Raw Raw;
-  constexpr int kV = Piece<Ty>::kV, kAhead = 4;
+  constexpr int kV = Piece<Ty>::kV;
   const int lanes = a.d / (2 * kV);
   const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> log_lanes;
   const int u = threadIdx.x & ((1 << log_lanes) - 1);
@@ -286,7 +286,10 @@ hipError_t pieces(const NormRotaryLaunch& p, hipStream_t stream) {
   if (parts > total) parts = total;
   const int per = (int)((total + parts - 1) / parts);
   const dim3 grid((unsigned)blocks, (unsigned)((total + per - 1) / per));
-  norm_rotary_kernel<Ty, kInterleaved, kNorm, kPages><<<grid, 256, 0, stream>>>(p, log_lanes, per);
+  if (per >= 4)
+    norm_rotary_kernel<Ty, kInterleaved, kNorm, kPages, 4><<<grid, 256, 0, stream>>>(p, log_lanes, per);
+  else  // (a call of few tokens)
+    norm_rotary_kernel<Ty, kInterleaved, kNorm, kPages, 1><<<grid, 256, 0, stream>>>(p, log_lanes, per);
   return hipGetLastError();
 }
 
