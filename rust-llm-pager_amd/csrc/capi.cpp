@@ -594,7 +594,7 @@ int check_tokens(int64_t batch, int64_t tokens) {
 
 struct PTPlan {
   pgr::PTAttendPlan k;
-  size_t o_pm = 0, o_pl = 0, o_pacc = 0, bytes = 0;
+  size_t o_meta = 0, o_pm = 0, o_pl = 0, o_pacc = 0, bytes = 0;
 };
 
 int check_pt_attend(const pgr_pt_cache_t* c, int64_t batch, int64_t tokens) {
@@ -610,9 +610,10 @@ PTPlan plan_pt(const pgr_pt_cache_t* c, int64_t batch, int64_t tokens, int64_t w
   PTPlan p;
   p.k = pgr::pt_attend_plan((int)batch, (int)tokens, (int)c->query_heads, (int)c->kv_heads, width * c->page_tokens,
                             (int)c->head_dim);
-  if (p.k.n_split == 1) return p;
-  const size_t slots = (size_t)(batch * c->kv_heads) * p.k.blocks * p.k.n_split * p.k.rows;
+  if (p.k.slots == 0) return p;
+  const size_t slots = (size_t)c->kv_heads * p.k.blocks * p.k.slots * p.k.rows;
   Parts w;
+  p.o_meta = w.take((size_t)batch * sizeof(int2));
   p.o_pm = w.take(slots * sizeof(float));
   p.o_pl = w.take(slots * sizeof(float));
   p.o_pacc = w.take(slots * (size_t)c->head_dim * sizeof(float));
@@ -1716,6 +1717,7 @@ int pgr_pt_attend(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_
     L.exact = exact_weights != 0;
     L.plan = p.k;
     if (p.bytes > 0) {
+      L.meta = reinterpret_cast<int2*>(w + p.o_meta);
       L.pm = reinterpret_cast<float*>(w + p.o_pm);
       L.pl = reinterpret_cast<float*>(w + p.o_pl);
       L.pacc = reinterpret_cast<float*>(w + p.o_pacc);

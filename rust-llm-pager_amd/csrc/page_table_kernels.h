@@ -57,7 +57,7 @@ struct PTAttendPlan {
   int share = 4;    // waves that share their rows (4 or 8)
   int rows = 16;    // rows (new token x query head of a KV head) of a workgroup
   int blocks = 1;   // blocks of rows
-  int n_split = 1;  // parts of a block's tokens (1: no merge launch)
+  int slots = 0;    // parts that the batch's rows are cut into at most (0: whole rows, no merge launch)
   int tile = 32;    // tokens
   int least = 4;    // tiles of a part at least
 };
@@ -75,7 +75,8 @@ struct PTAttendLaunch {
   float scale = 1.f, softcap = 0.f;
   int exact = 0;  // P as two numbers also where arithmetic bounds
   PTAttendPlan plan;
-  float* pm = nullptr;    // [batch, hkv, blocks, n_split, rows]
+  int2* meta = nullptr;   // [batch]: a row's first part, a part's tiles
+  float* pm = nullptr;    // [hkv, blocks, slots, rows]
   float* pl = nullptr;
   float* pacc = nullptr;  // [..., d]
 };

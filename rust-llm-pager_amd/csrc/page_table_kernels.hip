@@ -36,12 +36,100 @@ __device__ __forceinline__ Span span_of(const PTAttendLaunch& a, int b, int r0, 
   return s;
 }
 
-// Tiles of a block's tokens, and those that a split takes of them.
 __device__ __forceinline__ int tiles_of(const PTAttendPlan& p, const Span& s) {
   return (s.end - s.begin + p.tile - 1) / p.tile;
 }
-__device__ __forceinline__ int tiles_per_split(const PTAttendPlan& p, const Span& s) {
-  return max((tiles_of(p, s) + p.n_split - 1) / p.n_split, p.least);
+
+// Tiles of the longest of a batch row's blocks, at least.
+__device__ __forceinline__ int row_tiles(const PTAttendLaunch& a, int b) {
+  const int capacity = a.r.width << a.c.page_shift;
+  const int length = min(max(a.r.lengths[b], 0), capacity);
+  const int n = min(a.r.counts != nullptr ? min(max(a.r.counts[b], 0), a.r.tokens) : a.r.tokens, capacity - length);
+  // (A window begins up to kTile - 1 tokens early, on a tile's border.)
+  const int held = a.window > 0 ? min(length, a.window + kTile - 1) : length;
+  return n <= 0 ? 0 : (held + n + a.plan.tile - 1) / a.plan.tile;
+}
+
+// The wave's sums up to each lane, by lane shifts within rows of 16 and then across them.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
+// A workgroup's work: a block of rows, a KV head, a batch row and which `per` tiles of the block's.
+struct Work {
+  int block, h, b, split, per;
+};
+
+// The batch's rows are cut into parts of one size, `per` tiles: the least with which there are no more parts than
+// plan.slots, so that long rows have more of them and all workgroups about as much to do (8 rows of 13 drafted tokens
+// over 0 to 8191, D 64, softcapped: 36 us with as many parts for a short row as for a long one). Every wave finds
+// that size and its part by itself; the first workgroup leaves both for the merge. Without splits a part is a row.
+//
+// Blocks that read the same tokens are neighbours on one XCD (workgroups go to the eight XCDs in turn), so that its L2
+// serves all but the first; the longest block is first.
+__device__ __forceinline__ bool work_of(const PTAttendLaunch& a, Work& w) {
+  const unsigned id = blockIdx.x, rest = id >> 3, blocks = a.plan.blocks, hkv = a.c.hkv;
+  const unsigned p = rest / blocks * 8 + (id & 7);
+  w.block = (int)(blocks - 1 - rest % blocks);
+  w.h = (int)(p % hkv);
+  const int part = (int)(p / hkv);
+  w.per = 0;
+  w.split = 0;
+  w.b = part;
+  if (a.plan.slots == 0) return part < a.r.batch;
+  if (part >= a.plan.slots) return false;
+  if (a.r.batch == 1) {
+    w.per = max((row_tiles(a, 0) + a.plan.slots - 1) / a.plan.slots, a.plan.least);
+    w.split = part;
+    w.b = 0;
+    if (id == 0 && threadIdx.x == 0) a.meta[0] = int2{0, w.per};
+    return true;
+  }
+  const int lane = threadIdx.x & 63, mine = lane < a.r.batch ? row_tiles(a, lane) : 0;
+  int all = mine;
+  for (int b = lane + 64; b < a.r.batch; b += 64) all += row_tiles(a, b);
+  int per = max((__builtin_amdgcn_readlane(wave_scan(all), 63) + a.plan.slots - 1) / a.plan.slots, a.plan.least);
+  int upto = 0;  // parts of the first 64 rows up to the lane's
+#pragma unroll 1
+  for (int i = 0;; ++i) {
+    upto = wave_scan((mine + per - 1) / per);
+    int parts = __builtin_amdgcn_readlane(upto, 63);
+    for (int b0 = 64; b0 < a.r.batch; b0 += 64)
+      parts += __builtin_amdgcn_readlane(wave_scan(b0 + lane < a.r.batch ? (row_tiles(a, b0 + lane) + per - 1) / per : 0), 63);
+    if (parts <= a.plan.slots) break;
+    // (There are as many slots as rows, so that one part each ends it.)
+    per = i < 8 ? max(per + 1, (int)min((int64_t)1 << 30, ((int64_t)per * parts + a.plan.slots - 1) / a.plan.slots)) : 1 << 30;
+  }
+  w.per = per;
+  w.b = -1;
+  int before = 0;  // parts of the rows before b0
+  for (int b0 = 0; b0 < a.r.batch; b0 += 64) {
+    const int own = b0 == 0 ? (mine + per - 1) / per
+                            : b0 + lane < a.r.batch ? (row_tiles(a, b0 + lane) + per - 1) / per : 0;
+    const int last = before + (b0 == 0 ? upto : wave_scan(own));  // behind the lane's row
+    if (id == 0 && threadIdx.x < 64 && b0 + lane < a.r.batch) a.meta[b0 + lane] = int2{last - own, per};
+    const uint64_t later = __ballot(last > part);
+    if (w.b < 0 && later != 0) {
+      const int at = __builtin_ctzll(later);
+      w.b = b0 + at;
+      w.split = part - (__builtin_amdgcn_readlane(last, at) - __builtin_amdgcn_readlane(own, at));
+      if (id != 0) break;
+    }
+    before = __builtin_amdgcn_readlane(last, 63);
+  }
+  return w.b >= 0;
+}
+
+// The first row of a part's results: [hkv, blocks, slots, rows], a batch row's parts one after the other.
+__device__ __forceinline__ int64_t slot_of_part(const PTAttendLaunch& a, const Work& w, int rows) {
+  const int part = (int)((blockIdx.x >> 3) / a.plan.blocks * 8 + (blockIdx.x & 7)) / a.c.hkv;
+  return (((int64_t)w.h * a.plan.blocks + w.block) * a.plan.slots + part) * rows;
 }
 
 // Which tokens a row sees.
@@ -88,23 +176,6 @@ __device__ __forceinline__ float capped(float x, const AttendScale& sc) {
   return sc.cap_log2 * fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f);
 }
 
-// The block, split, KV head and batch row of a workgroup. Blocks that read the same tokens are neighbours on one
-// XCD (workgroups go to the eight XCDs in turn), so that its L2 serves all but the first.
-struct Work {
-  int block, split, h, b;
-};
-__device__ __forceinline__ bool work_of(const PTAttendLaunch& a, Work& w) {
-  const unsigned id = blockIdx.x, rest = id >> 3;
-  const unsigned p = rest / a.plan.blocks * 8 + (id & 7);
-  w.block = a.plan.blocks - 1 - (int)(rest % a.plan.blocks);  // the longest first
-  if (p >= (unsigned)(a.r.batch * a.c.hkv * a.plan.n_split)) return false;
-  w.split = (int)(p % a.plan.n_split);
-  const unsigned bh = p / a.plan.n_split;
-  w.h = (int)(bh % a.c.hkv);
-  w.b = (int)(bh / a.c.hkv);
-  return true;
-}
-
 // ---------------------------------------------------------------------------------------
 // Attention of few rows a KV head. As in the bounded cache's attention each wave folds tiles of 32 tokens,
 // two halves of 16, on v_mfma_f32_16x16x32,
@@ -132,10 +203,12 @@ __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, At
   const PTPages& c = a.c;
   const int b = wk.b, h = wk.h, n_rep = c.hq / c.hkv, r0 = wk.block * kRows;
   const Span sp = span_of(a, b, r0, kRows, n_rep);
-  const int per = tiles_per_split(a.plan, sp);
-  const int begin = min(sp.begin + wk.split * per * kTile, sp.end), end = min(begin + per * kTile, sp.end);
-  // (The merge reads only the splits that hold tokens; a block that is finished here writes its zeros.)
-  if (a.plan.n_split > 1 && begin >= end) return;
+  const bool whole = a.plan.slots == 0;
+  // (64 bits: a part's border may lie past any row.)
+  const int begin = whole ? sp.begin : (int)min((int64_t)sp.end, sp.begin + (int64_t)wk.split * wk.per * kTile);
+  const int end = whole ? sp.end : (int)min((int64_t)sp.end, begin + (int64_t)wk.per * kTile);
+  // (The merge reads only the parts that hold tokens; a block that is finished here writes its zeros.)
+  if (!whole && begin >= end) return;
   const int tiles = (end - begin + kTile - 1) / kTile;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
@@ -325,7 +398,7 @@ __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, At
         sm_acc[wave][16 * y + n][(D / 4) * g + (D / 16) * i + j] = acc[y][j][i] * Ty::kUnit;
   }
   __syncthreads();
-  const int64_t part = ((((int64_t)b * c.hkv + h) * a.plan.blocks + wk.block) * a.plan.n_split + wk.split) * kRows;
+  const int64_t part = slot_of_part(a, wk, kRows);
   for (int i = threadIdx.x; i < kRows * D; i += kThreads) {
     const int r = i / D, e = i - r * D, tok = (r0 + r) / n_rep;
     if (tok >= a.r.tokens) break;
@@ -340,7 +413,7 @@ __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, At
       x += sm_acc[w][r][e] * f;
       l += sm_l[w][r] * f;
     }
-    if (a.plan.n_split == 1) {
+    if (whole) {
       const int64_t head = ((int64_t)b * a.r.tokens + tok) * c.hq + h * n_rep + (r0 + r - tok * n_rep);
       static_cast<uint16_t*>(a.out)[head * D + e] = Ty::cvt(tok >= sp.n || l == 0.f ? 0.f : x / l);
     } else {
@@ -409,9 +482,10 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
   const PTPages& c = a.c;
   const int b = wk.b, h_kv = wk.h, n_rep = c.hq / c.hkv;
   const Span sp = span_of(a, b, wk.block * kRows, kRows, n_rep);
-  const int per = tiles_per_split(a.plan, sp);
-  const int begin = min(sp.begin + wk.split * per * kTok, sp.end), end = min(begin + per * kTok, sp.end);
-  if (a.plan.n_split > 1 && begin >= end) return;
+  const bool whole = a.plan.slots == 0;
+  const int begin = whole ? sp.begin : (int)min((int64_t)sp.end, sp.begin + (int64_t)wk.split * wk.per * kTok);
+  const int end = whole ? sp.end : (int)min((int64_t)sp.end, begin + (int64_t)wk.per * kTok);
+  if (!whole && begin >= end) return;
   const int tiles = (end - begin + kTok - 1) / kTok;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int h = lane >> 5, n = lane & 31;
@@ -491,16 +565,15 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
 
-  // The lane's places in a tile: of K piece 2 i + h of token n, of V its part of the transposing reads.
-  int k_at[D / 16], v_at[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) k_at[i] = L::k_at(n, 2 * i + h);
-#pragma unroll
-  for (int j = 0; j < D / 32; ++j)
-    v_at[j] = L::v_at(4 * h + ((lane & 15) >> 2), 4 * j + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) * 8 + 4 * (lane & 1);
+  // The lane's places in a tile: of K piece h of token n (piece 2 i + h: XOR 2 i), of V its part of the transposing reads
+  // of the first 32 dims (j: XOR 32 j elements, where a row is wider than that).
+  const int k_first = L::k_at(n, h);
+  const int v_first = L::v_at(4 * h + ((lane & 15) >> 2), 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) * 8 + 4 * (lane & 1);
 
   auto fold = [&](int ti, int buf) {
     const int c0 = begin + ti * kTok;
+    int k_at = k_first, v_at = v_first;  // (taken apart anew for each tile: a dozen registers less over the loop)
+    asm volatile("" : "+v"(k_at), "+v"(v_at));
     f32x16 s[kHalves];
 #pragma unroll
     for (int x = 0; x < kHalves; ++x)
@@ -509,7 +582,7 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-      for (int x = 0; x < kHalves; ++x) s[x] = Ty::mma32(k_s[buf][k_at[i] + 32 * x * L::kPieces], q[i], s[x]);
+      for (int x = 0; x < kHalves; ++x) s[x] = Ty::mma32(k_s[buf][(k_at ^ 2 * i) + 32 * x * L::kPieces], q[i], s[x]);
     const uint64_t here = __ballot(held_s[buf][lane & (kTok - 1)] != 0);
     // Uniform: some row of the wave may not see some token of the tile.
     const bool masked = ~here != 0 || c0 < lo_most || c0 + kTok > seen_by_all;
@@ -572,7 +645,7 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           typedef __attribute__((address_space(3))) i16x4_t Lds;
-          const uint16_t* at = reinterpret_cast<const uint16_t*>(v_s[buf]) + v_at[j] + (32 * x + 16 * y) * D;
+          const uint16_t* at = reinterpret_cast<const uint16_t*>(v_s[buf]) + (v_at ^ 32 * j) + (32 * x + 16 * y) * D;
           const i16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)at);
           const i16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at + 8 * D));
           const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
@@ -597,7 +670,7 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
 
   const float l = sum_halves(l_run);
   if (tok >= a.r.tokens) return;
-  if (a.plan.n_split == 1) {
+  if (whole) {
     uint16_t* out = static_cast<uint16_t*>(a.out) + (((int64_t)b * a.r.tokens + tok) * c.hq + head) * D + 4 * h;
     const bool none = tok >= sp.n || l == 0.f;
 #pragma unroll
@@ -611,8 +684,7 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
       }
     return;
   }
-  const int64_t part = ((((int64_t)b * c.hkv + h_kv) * a.plan.blocks + wk.block) * a.plan.n_split + wk.split) * kRows +
-                       32 * wave + n;
+  const int64_t part = slot_of_part(a, wk, kRows) + 32 * wave + n;
   if (h == 0) {
     a.pm[part] = m_run;
     a.pl[part] = l;
@@ -626,7 +698,7 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
           f32x4{acc[j][4 * i], acc[j][4 * i + 1], acc[j][4 * i + 2], acc[j][4 * i + 3]} * Ty::kUnit;
 }
 
-// Joins the splits of a row: `groups` groups of d / 4 threads take splits in turn, four dims a thread, under a maximum
+// Joins the parts of a row: `groups` groups of d / 4 threads take parts in turn, four dims a thread, under a maximum
 // of their own, and are joined through LDS. Rows and groups fill a workgroup.
 template <class Ty>
 __global__ __launch_bounds__(256) void pt_merge_kernel(PTAttendLaunch a, int groups) {
@@ -639,19 +711,21 @@ __global__ __launch_bounds__(256) void pt_merge_kernel(PTAttendLaunch a, int gro
   const bool real = tok < a.r.tokens;
   const int block = r / a.plan.rows, in = r - block * a.plan.rows;
   const Span sp = span_of(a, b, block * a.plan.rows, a.plan.rows, n_rep);
-  const int per = tiles_per_split(a.plan, sp), used = real ? (tiles_of(a.plan, sp) + per - 1) / per : 0;
-  const int64_t part = (((int64_t)b * c.hkv + h) * a.plan.blocks + block) * a.plan.n_split * a.plan.rows + in;
+  const int2 meta = a.meta[b];  // the row's first part, a part's tiles
+  const int used = real ? (tiles_of(a.plan, sp) + meta.y - 1) / meta.y : 0;
+  const int64_t part = (((int64_t)h * a.plan.blocks + block) * a.plan.slots + meta.x) * a.plan.rows + in;
   float m = kMinusInf, l = 0.f;
-#pragma unroll 4
-  for (int s = g; s < used; s += groups) m = fmaxf(m, a.pm[part + (int64_t)s * a.plan.rows]);
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  const float own = m == kMinusInf ? 0.f : m;
 #pragma unroll 4
-  for (int s = g; s < used; s += groups) {
+  for (int s = g; s < used; s += groups) {  // (one pass: the loads of several parts are under way together)
     const int64_t at = part + (int64_t)s * a.plan.rows;
-    const float f = __builtin_amdgcn_exp2f(a.pm[at] - own);
-    l += a.pl[at] * f;
-    x += *reinterpret_cast<const f32x4*>(a.pacc + at * d + e) * f;
+    const float ms = a.pm[at], ls = a.pl[at];
+    const f32x4 xs = *reinterpret_cast<const f32x4*>(a.pacc + at * d + e);
+    const float top = fmaxf(m, ms), ref = top == kMinusInf ? 0.f : top;
+    const float f = __builtin_amdgcn_exp2f(m - ref), fs = __builtin_amdgcn_exp2f(ms - ref);
+    l = l * f + ls * fs;
+    x = x * f + xs * fs;
+    m = top;
   }
   if (groups > 1) {
     m_s[tid] = m;
@@ -774,7 +848,7 @@ __global__ __launch_bounds__(64) void draft_tree_kernel(const int32_t* parents, 
 
 template <class Ty, int D>
 hipError_t attend_dim(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
-  const int64_t parts = (int64_t)p.r.batch * p.c.hkv * p.plan.n_split;
+  const int64_t parts = (int64_t)p.c.hkv * (p.plan.slots == 0 ? p.r.batch : p.plan.slots);
   const dim3 grid((unsigned)((parts + 7) / 8 * 8 * p.plan.blocks));
   if (p.plan.waves == 0) {
     if (p.plan.rows == 16 && p.plan.share == 4) pt_attend_kernel<Ty, D, 1, 4><<<grid, 256, 0, stream>>>(p, sc);
@@ -799,10 +873,10 @@ hipError_t attend_dim(const PTAttendLaunch& p, const AttendScale& sc, hipStream_
     }
   }
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.plan.n_split == 1) return e;
+  if (e != hipSuccess || p.plan.slots == 0) return e;
   const int rows = p.r.tokens * (p.c.hq / p.c.hkv);
   int groups = 1;
-  while (2 * groups <= p.plan.n_split && 2 * groups <= 256 / (D / 4) &&
+  while (2 * groups * p.r.batch <= p.plan.slots && 2 * groups <= 256 / (D / 4) &&
          (int64_t)rows * p.c.hkv * p.r.batch * (D / 4) * groups < 256 * 512)
     groups *= 2;
   const int each = 256 / (D / 4) / groups;
@@ -843,6 +917,7 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
     if (d < 256) p.share = p.least = 8;
     return p;
   }
+  // Parts a row on average: as many as fill the card once.
   const int64_t groups = units * p.blocks, most = (capacity + p.least * p.tile - 1) / (p.least * p.tile);
   int64_t n = target / groups;
   if (2 * groups > target) {  // whole rounds, as far as a few splits bring them
@@ -856,7 +931,9 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
     }
   }
   if (n > most) n = most;
-  p.n_split = n < 1 ? 1 : (int)n;
+  if (n <= 1) return p;
+  const int64_t once = target / ((int64_t)hkv * p.blocks);
+  p.slots = (int)(batch > 1 && once > n * batch ? once : n * batch);
   return p;
 }
 

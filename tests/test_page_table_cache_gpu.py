@@ -337,6 +337,42 @@ def test_attend_long_rows(t, dtype):
                       only=sorted({0, t // 3, t - 1}))
 
 
+RAGGED = [
+    # query heads, kv heads, head dim, new tokens, window, lengths
+    (4, 1, 64, 3, 0, [0] * 30 + [3000] + [40] * 38 + [2000]),  # more rows than a wave has lanes, few of them long
+    (4, 2, 128, 1, 0, [7, 0, 5000, 31]),
+    (4, 1, 64, 20, 0, [1] * 129),
+    (4, 1, 32, 30, 700, [2500, 10, 0, 4000, 699, 700, 701]),
+    (8, 1, 128, 40, 0, [6000, 0, 100]),
+    (4, 1, 256, 12, 0, [1500, 3, 1500, 800]),
+    (4, 4, 16, 5, 33, [2000, 1, 31, 32, 33]),
+    (16, 1, 64, 64, 0, [900, 0, 0, 0, 0, 0, 0, 64]),
+]
+
+
+@pytest.mark.parametrize("dtype", CACHE_TYPES)
+@pytest.mark.parametrize("case", RAGGED, ids=[str(c[:5]) for c in RAGGED])
+def test_attend_ragged_batches(case, dtype):
+    """Rows of very different lengths, cut into parts of one size; some of them have no new tokens."""
+    hq, hkv, d, t, window, lengths = case
+    b = len(lengths)
+    rng = np.random.default_rng(83)
+    pages = sum(-(-(n + t) // 32) for n in lengths) + 1
+    cache, table = _filled(rng, pages, 32, hq, hkv, d, dtype, lengths, t)
+    g = torch.Generator().manual_seed(b)
+    q = (torch.randn(b, hq, t, d, generator=g) * 2).to(dtype).cuda()
+    counts = [0 if i % 5 == 4 else t - i % 3 % t for i in range(b)]
+    for sees, depth, tree in ((*_order(b, t), None), (*O.tree(_parents(rng, b, t)), True)):
+        if tree is not None:
+            masks = (sees * (np.uint64(1) << np.arange(t, dtype=np.uint64))).sum(axis=-1, dtype=np.uint64)
+            tree = DraftTree(torch.tensor(masks.view(np.int64), device="cuda"), _int32(depth))
+        out = cache.attend(0, q, _int32(table), _int32(lengths), counts=_int32(counts), tree=tree, window=window)
+        _check_attend(cache, 0, table, lengths, q, out, counts, sees, depth, window, 1.0 / d**0.5, 0.0,
+                      only=sorted({0, t // 2, t - 1}))
+    none = cache.attend(0, q, _int32(table), _int32(lengths), counts=_int32([0] * b), window=window)
+    assert not none.any()
+
+
 @pytest.mark.parametrize("dtype", CACHE_TYPES)
 @pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("t", [1, 5, 40])
