@@ -95,16 +95,33 @@ __device__ __forceinline__ bool work_of(const PTAttendLaunch& a, Work& w) {
   int all = mine;
   for (int b = lane + 64; b < a.r.batch; b += 64) all += row_tiles(a, b);
   int per = max((__builtin_amdgcn_readlane(wave_scan(all), 63) + a.plan.slots - 1) / a.plan.slots, a.plan.least);
-  int upto = 0;  // parts of the first 64 rows up to the lane's
-#pragma unroll 1
-  for (int i = 0;; ++i) {
-    upto = wave_scan((mine + per - 1) / per);
+  // Parts of all rows at `size` tiles a part; upto: of the first 64 rows up to the lane's.
+  int upto = 0;
+  auto parts_at = [&](int size) {
+    upto = wave_scan((mine + size - 1) / size);
     int parts = __builtin_amdgcn_readlane(upto, 63);
     for (int b0 = 64; b0 < a.r.batch; b0 += 64)
-      parts += __builtin_amdgcn_readlane(wave_scan(b0 + lane < a.r.batch ? (row_tiles(a, b0 + lane) + per - 1) / per : 0), 63);
-    if (parts <= a.plan.slots) break;
-    // (There are as many slots as rows, so that one part each ends it.)
-    per = i < 8 ? max(per + 1, (int)min((int64_t)1 << 30, ((int64_t)per * parts + a.plan.slots - 1) / a.plan.slots)) : 1 << 30;
+      parts += __builtin_amdgcn_readlane(wave_scan(b0 + lane < a.r.batch ? (row_tiles(a, b0 + lane) + size - 1) / size : 0), 63);
+    return parts;
+  };
+  int parts = parts_at(per);
+  if (parts > a.plan.slots) {
+    int few = per;  // too small a size; then one that is not (there are as many slots as rows: one part each ends it)
+#pragma unroll 1
+    for (int i = 0; parts > a.plan.slots; ++i) {
+      few = per;
+      per = i < 8 ? max(per + 1, (int)min((int64_t)1 << 30, ((int64_t)per * parts + a.plan.slots - 1) / a.plan.slots)) : 1 << 30;
+      parts = parts_at(per);
+    }
+#pragma unroll 1
+    while (per - few > 1 + (per >> 6)) {  // within a 64th of the least
+      const int size = (few + per) >> 1;
+      if (parts_at(size) > a.plan.slots)
+        few = size;
+      else
+        per = size;
+    }
+    parts_at(per);
   }
   w.per = per;
   w.b = -1;
