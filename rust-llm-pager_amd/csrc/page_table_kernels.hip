@@ -68,7 +68,7 @@ struct Work {
 
 // The batch's rows are cut into parts of one size, `per` tiles: the least with which there are no more parts than
 // plan.slots, so that long rows have more of them and all workgroups about as much to do (8 rows of 13 drafted tokens
-// over 0 to 8191, D 64, softcapped: 36 us with as many parts for a short row as for a long one). Every wave finds
+// over 0 to 8191, D 64, softcapped: 27 us, 36 with as many parts for a short row as for a long one). Every wave finds
 // that size and its part by itself; the first workgroup leaves both for the merge. Without splits a part is a row.
 //
 // Blocks that read the same tokens are neighbours on one XCD (workgroups go to the eight XCDs in turn), so that its L2
@@ -204,11 +204,11 @@ __device__ __forceinline__ float capped(float x, const AttendScale& sc) {
 // where sums all but cancel.
 //
 // Bound by HBM, and for a few rows by the two launches' latency. 8 rows x 8192 tokens, 32/8 heads, D 128, one token: 55 us
-// for 268 MB (4.9 TB/s; a copy reaches 5.1), 8 drafted tokens 61; 2 x 65536 tokens: 99 us for 537 MB. Splits for 256
+// for 268 MB (4.9 TB/s; a copy reaches 5.1), 8 drafted tokens 61; 2 x 65536 tokens: 102 us for 537 MB. Parts for 256
 // workgroups against 512 / 1024: 54.6 / 54.9 / 56.7 us (one token), 61.9 / 65.0 / 72.9 (eight), one row of 28/4 heads
 // 14.4 either way, 16 rows of 4096 tokens, D 64: 19.5 / 21.0 / 21.8. Short rows are finished by one workgroup of
-// eight waves, without a merge: 256 tokens, D 64 6.7 us against 9.4, D 128 8.2 against 10.4; at 512 and 256 tokens
-// (D 128 and 256) the two are even.
+// eight waves, without a merge: 256 tokens, D 64 6.7 us against 9.4, D 128 8.2 against 10.4; at 1000 and 500 tokens
+// (D 64 and 128) the two are even.
 template <class Ty, int D, int kG, int kW>
 __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, AttendScale sc) {
   typedef KVTile<D> T;
@@ -466,11 +466,14 @@ __device__ __forceinline__ float sum_halves(float x) {
 //
 // kTwo: P as two numbers, as where the loads bound; here the second product is half as much arithmetic again, so
 // that the caller chooses (P rounded to one number of the cache's type is off by half a step of each weight). A chunk
-// of 2048 tokens over 16384, 32/8 heads, D 128: 664 us with one number (880 TFLOP/s; a library's matrix product
-// reaches 1244), 879 with two; the kernel above took 1265. Trees of 64 tokens over 8 rows of 32768, 28/4: 323 and 405 us
-// (598). Eight waves (one workgroup a CU) against four: 664 and 752 us, 323 and 355; 128 rows, 8 x 8192 tokens:
-// 74 and 76; few workgroups (448 rows, 1000 tokens) 15.4 and 13.5. Up to 32 rows the kernel above is as fast or faster
-// (8 rows x 8192: 61 us; 48 rows here 65, there 80).
+// of 2048 tokens over 16384, 32/8 heads, D 128: 622 us with one number (939 TFLOP/s; a library's matrix product
+// reaches 1244), 826 with two; the kernel above took 1265. Trees of 64 tokens over 8 rows of 32768, 28/4: 302 and 387 us
+// (598). In the chunk the matrix cores are busy 0.42 of the cycles and the vector units 0.52, one after the other: the
+// two waves of a SIMD go through products and softmax together. Half of the waves half a tile behind the others
+// (676 us), a barrier every second tile (641), raised wave priorities over either product (637 to 653): no better.
+// Eight waves (one workgroup a CU) against four: 664 and 752 us, 323 and 355; 128 rows, 8 x 8192 tokens: 74 and 76; few
+// workgroups (448 rows, 1000 tokens) 15.4 and 13.5. Up to 32 rows the kernel above is as fast or faster (32 rows, 8 x
+// 8192 tokens: 61 us; 48 rows here 65, there 80).
 template <int D>
 struct Staged {
   static constexpr int kPieces = D / 8;  // 16-byte pieces of a token
@@ -774,7 +777,9 @@ __global__ __launch_bounds__(256) void pt_merge_kernel(PTAttendLaunch a, int gro
 // before the call. A workgroup finds the moves of one row once and makes them for its share of the row's planes (a
 // plane: one KV head's keys or values in one layer), in 16-byte pieces. A move never reads what another plane's
 // writes, so a workgroup takes as many planes at a time as its registers hold, reads all of their pieces and writes
-// them behind a barrier. Entries outside [0, 64) move nothing, nor do those that are in their place.
+// them behind a barrier. Entries outside [0, 64) move nothing, nor do those that are in their place. Memory-bound: 1774
+// tokens moved in 64 rows, 8 KV heads, D 128, 32 layers: 101 us for 465 MB (4.6 TB/s); 291 with a workgroup that finds
+// the moves anew for every plane.
 constexpr int kKeepThreads = 512, kKeepEach = 4;  // pieces a thread holds: 64 tokens of up to 32 are one plane's at most
 
 __global__ __launch_bounds__(kKeepThreads) void pt_keep_kernel(PTKeepLaunch a, int planes, int share) {

@@ -12,7 +12,8 @@
 // query (init, fold, finalize; 28/4 heads, D 128, fp16, 64 tokens) 30.6 -> 16.8 us, 4133 tokens
 // the same; the two-pass run of 12 calls (32/4, D 64, batch 4, 8209 tokens) 151 -> 84.6 us.
 // q and k of one token turned (14/2 heads, D 64) 17.9 -> 8.0 us, an append to a full cache of 256 tokens 13.4
-// -> 7.3 us, attention over 256 tokens (28/4, D 128) 10.8 -> 7.1 us.
+// -> 7.3 us, attention over 256 tokens (28/4, D 128) 10.8 -> 7.1 us. One token normed and turned (28/4, D 128) 20.0 ->
+// 8.1 us, appended to pages (14/2, D 64) 19.9 -> 7.6, a path kept (24 layers) 9.8 -> 6.2.
 //
 // libpgr.so's entry points come as addresses (bind), so that the library the Python package has
 // loaded is the one called.
