@@ -648,12 +648,9 @@ def test_captured_steps_replay():
         n = norm_rotary_embedding(q, k, lengths[:, None].expand(2, 7), inv, w, w)
         return out, n[0], n[1]
 
-    stream = torch.cuda.Stream()
-    stream.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(stream):
-        step(caches[0])
-        step(caches[1])
-    torch.cuda.current_stream().wait_stream(stream)
+    for c in caches:
+        step(c)
+    torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         held = step(caches[0])
@@ -680,9 +677,8 @@ def test_the_same_every_time_and_on_two_streams():
     lengths, tree = _int32([4000, 2100, 77]), draft_tree(_int32(_parents(rng, 3, 40)))
     tables = [_int32(t) for _, t in made]
     want = [c.attend(0, q, t, lengths, tree=tree) for (c, _), t in zip(made, tables)]
-    streams = [torch.cuda.Stream() for _ in range(2)]
-    for s in streams:
-        s.wait_stream(torch.cuda.current_stream())
+    streams = [torch.cuda.current_stream(), torch.cuda.Stream()]
+    streams[1].wait_stream(streams[0])
     got = [[], []]
     for _ in range(5):
         for i, s in enumerate(streams):
