@@ -61,15 +61,17 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// A workgroup's work: a block of rows, a KV head, a batch row and which `per` tiles of the block's.
+// A workgroup's work: a block of rows, a KV head, a batch row and which `per` tiles of the block's (whole: all of them).
 struct Work {
   int block, h, b, split, per;
+  bool whole;
 };
 
 // The batch's rows are cut into parts of one size, `per` tiles: the least with which there are no more parts than
 // plan.slots, so that long rows have more of them and all workgroups about as much to do (8 rows of 13 drafted tokens
 // over 0 to 8191, D 64, softcapped: 27 us, 36 with as many parts for a short row as for a long one). Every wave finds
-// that size and its part by itself; the first workgroup leaves both for the merge. Without splits a part is a row.
+// that size and its part by itself; the first workgroup leaves both for the merge. A row of one part is finished by its
+// workgroup; without slots every row is.
 //
 // Blocks that read the same tokens are neighbours on one XCD (workgroups go to the eight XCDs in turn), so that its L2
 // serves all but the first; the longest block is first.
@@ -82,12 +84,15 @@ __device__ __forceinline__ bool work_of(const PTAttendLaunch& a, Work& w) {
   w.per = 0;
   w.split = 0;
   w.b = part;
+  w.whole = true;
   if (a.plan.slots == 0) return part < a.r.batch;
   if (part >= a.plan.slots) return false;
   if (a.r.batch == 1) {
     w.per = max((row_tiles(a, 0) + a.plan.slots - 1) / a.plan.slots, a.plan.least);
     w.split = part;
     w.b = 0;
+    w.whole = row_tiles(a, 0) <= w.per;
+    if (w.whole && part > 0) return false;
     if (id == 0 && threadIdx.x == 0) a.meta[0] = int2{0, w.per};
     return true;
   }
@@ -135,7 +140,9 @@ __device__ __forceinline__ bool work_of(const PTAttendLaunch& a, Work& w) {
     if (w.b < 0 && later != 0) {
       const int at = __builtin_ctzll(later);
       w.b = b0 + at;
-      w.split = part - (__builtin_amdgcn_readlane(last, at) - __builtin_amdgcn_readlane(own, at));
+      const int parts_of_row = __builtin_amdgcn_readlane(own, at);
+      w.split = part - (__builtin_amdgcn_readlane(last, at) - parts_of_row);
+      w.whole = parts_of_row == 1;
       if (id != 0) break;
     }
     before = __builtin_amdgcn_readlane(last, 63);
@@ -220,7 +227,7 @@ __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, At
   const PTPages& c = a.c;
   const int b = wk.b, h = wk.h, n_rep = c.hq / c.hkv, r0 = wk.block * kRows;
   const Span sp = span_of(a, b, r0, kRows, n_rep);
-  const bool whole = a.plan.slots == 0;
+  const bool whole = wk.whole;
   // (64 bits: a part's border may lie past any row.)
   const int begin = whole ? sp.begin : (int)min((int64_t)sp.end, sp.begin + (int64_t)wk.split * wk.per * kTile);
   const int end = whole ? sp.end : (int)min((int64_t)sp.end, begin + (int64_t)wk.per * kTile);
@@ -502,7 +509,7 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
   const PTPages& c = a.c;
   const int b = wk.b, h_kv = wk.h, n_rep = c.hq / c.hkv;
   const Span sp = span_of(a, b, wk.block * kRows, kRows, n_rep);
-  const bool whole = a.plan.slots == 0;
+  const bool whole = wk.whole;
   const int begin = whole ? sp.begin : (int)min((int64_t)sp.end, sp.begin + (int64_t)wk.split * wk.per * kTok);
   const int end = whole ? sp.end : (int)min((int64_t)sp.end, begin + (int64_t)wk.per * kTok);
   if (!whole && begin >= end) return;
@@ -732,6 +739,8 @@ __global__ __launch_bounds__(256) void pt_merge_kernel(PTAttendLaunch a, int gro
   const int block = r / a.plan.rows, in = r - block * a.plan.rows;
   const Span sp = span_of(a, b, block * a.plan.rows, a.plan.rows, n_rep);
   const int2 meta = a.meta[b];  // the row's first part, a part's tiles
+  const int tiles = row_tiles(a, b);
+  if (tiles > 0 && tiles <= meta.y) return;  // (a row of one part is finished by its workgroup)
   const int used = real ? (tiles_of(a.plan, sp) + meta.y - 1) / meta.y : 0;
   const int64_t part = (((int64_t)h * a.plan.blocks + block) * a.plan.slots + meta.x) * a.plan.rows + in;
   float m = kMinusInf, l = 0.f;
@@ -953,9 +962,16 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
     }
   }
   if (n > most) n = most;
-  if (n <= 1) return p;
   const int64_t once = target / ((int64_t)hkv * p.blocks);
-  p.slots = (int)(batch > 1 && once > n * batch ? once : n * batch);
+  if (n > 1) {
+    p.slots = (int)(batch > 1 && once > n * batch ? once : n * batch);
+  } else if (batch > 1 && batch <= 256 && most >= 32) {
+    // The rows fill the card, but one that is much longer than the others would hold the call up: one of 60000 tokens and
+    // 63 of 200 (32/8 heads, D 128) 635 us whole, 78 cut; 64 of 4096 tokens, none of them cut, 184 and 188.
+    // (Not where a row's results are many: it has blocks enough then.)
+    const int64_t slots = batch + (once > 8 ? once : 8), bytes = (int64_t)hkv * p.blocks * p.rows * d * 4;
+    if (slots * bytes <= (int64_t)128 << 20) p.slots = (int)slots;
+  }
   return p;
 }
 

@@ -347,6 +347,10 @@ RAGGED = [
     (4, 1, 256, 12, 0, [1500, 3, 1500, 800]),
     (4, 4, 16, 5, 33, [2000, 1, 31, 32, 33]),
     (16, 1, 64, 64, 0, [900, 0, 0, 0, 0, 0, 0, 64]),
+    # Rows enough to fill the card, of which one is cut and the others are finished by their workgroups.
+    (4, 4, 64, 2, 0, [4500] + [20] * 30 + [0] * 5 + [130] * 34),
+    (16, 1, 64, 20, 0, [50] * 69 + [4200]),
+    (4, 4, 128, 3, 900, [4100, 899, 900, 901] * 17),
 ]
 
 
