@@ -193,11 +193,20 @@ __device__ __forceinline__ uint64_t sees(const PTAttendLaunch& a, const Span& s,
   return (low_bits(-at) & since) | fresh;
 }
 
-// cap * log2(e) * tanh(x * scale / cap) as 1 - 2 / (1 + e^2y): within 5 half steps of float32 of the cap, where
-// the scores' own products leave no less (a tanh that is exact to small values costs five times as much).
+// cap * log2(e) * tanh(y), y = x * scale / cap, as 1 - 2 / (1 + e^2y): within 5 half steps of float32 of the cap, which up to
+// a cap of 64 is 2^-15.7 of a weight at most. Under larger caps (kFar) small y go by the series (the next term is 6e-8
+// of it), so that the error is 3e-6 of the score: in kernels of their own (kFar), since the choice for each score costs 8
+// drafted trees (D 64) 4 of 30 us. tanhf takes three times as much.
+constexpr float kNearCap = 64.f * kLog2e;
+
+template <bool kFar>
 __device__ __forceinline__ float capped(float x, const AttendScale& sc) {
-  const float e = __builtin_amdgcn_exp2f(x * (sc.cap_scale * (2.f * kLog2e)));
-  return sc.cap_log2 * fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f);
+  float t = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (sc.cap_scale * (2.f * kLog2e)))), 1.f);
+  if constexpr (kFar) {
+    const float y = x * sc.cap_scale, y2 = y * y, series = y * fmaf(y2, fmaf(y2, 2.f / 15.f, -1.f / 3.f), 1.f);
+    t = fabsf(y) < 0.1f ? series : t;
+  }
+  return sc.cap_log2 * t;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -216,7 +225,7 @@ __device__ __forceinline__ float capped(float x, const AttendScale& sc) {
 // 14.4 either way, 16 rows of 4096 tokens, D 64: 19.5 / 21.0 / 21.8. Short rows are finished by one workgroup of
 // eight waves, without a merge: 256 tokens, D 64 6.7 us against 9.4, D 128 8.2 against 10.4; at 1000 and 500 tokens
 // (D 64 and 128) the two are even.
-template <class Ty, int D, int kG, int kW>
+template <class Ty, int D, int kG, int kW, bool kFar>
 __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, AttendScale sc) {
   typedef KVTile<D> T;
   constexpr int kThreads = 64 * kW, kRows = 16 * kG;
@@ -339,9 +348,9 @@ __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, At
 #pragma unroll
     for (int y = 0; y < kG; ++y) {
       float p[8], top = kMinusInf;
-      if (sc.cap_log2 > 0.f) {
+      if (kFar || sc.cap_log2 > 0.f) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = capped(s[y][i / 4][i & 3], sc);
+        for (int i = 0; i < 8; ++i) p[i] = capped<kFar>(s[y][i / 4][i & 3], sc);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = s[y][i / 4][i & 3] * sc.scale_log2;
@@ -496,7 +505,7 @@ struct Staged {
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
-template <class Ty, int D, int kW, bool kTwo>
+template <class Ty, int D, int kW, bool kTwo, bool kFar>
 __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kernel(PTAttendLaunch a, AttendScale sc) {
   typedef Staged<D> L;
   constexpr int kTok = D == 256 ? 32 : 64, kThreads = 64 * kW, kRows = 32 * kW, kHalves = kTok / 32;
@@ -615,12 +624,12 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
     const bool masked = ~here != 0 || c0 < lo_most || c0 + kTok > seen_by_all;
     // (Scores stay as the products left them, `unit` of them in log2 units: one multiply-add before the exponential.)
     float top = kMinusInf, unit = sc.scale_log2;
-    if (sc.cap_log2 > 0.f) {
+    if (kFar || sc.cap_log2 > 0.f) {
       unit = 1.f;
 #pragma unroll
       for (int x = 0; x < kHalves; ++x)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[x][i] = capped(s[x][i], sc);
+        for (int i = 0; i < 16; ++i) s[x][i] = capped<kFar>(s[x][i], sc);
     }
     if (masked) {
       const uint64_t seen = sees(a, sp, row, c0 + 4 * h) & here >> 4 * h;
@@ -877,29 +886,29 @@ __global__ __launch_bounds__(64) void draft_tree_kernel(const int32_t* parents, 
   }
 }
 
-template <class Ty, int D>
+template <class Ty, int D, bool kFar>
 hipError_t attend_dim(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
   const int64_t parts = (int64_t)p.c.hkv * (p.plan.slots == 0 ? p.r.batch : p.plan.slots);
   const dim3 grid((unsigned)((parts + 7) / 8 * 8 * p.plan.blocks));
   if (p.plan.waves == 0) {
-    if (p.plan.rows == 16 && p.plan.share == 4) pt_attend_kernel<Ty, D, 1, 4><<<grid, 256, 0, stream>>>(p, sc);
+    if (p.plan.rows == 16 && p.plan.share == 4) pt_attend_kernel<Ty, D, 1, 4, kFar><<<grid, 256, 0, stream>>>(p, sc);
     if constexpr (D < 256) {
-      if (p.plan.rows == 16 && p.plan.share == 8) pt_attend_kernel<Ty, D, 1, 8><<<grid, 512, 0, stream>>>(p, sc);
-      if (p.plan.rows == 32) pt_attend_kernel<Ty, D, 2, 4><<<grid, 256, 0, stream>>>(p, sc);
+      if (p.plan.rows == 16 && p.plan.share == 8) pt_attend_kernel<Ty, D, 1, 8, kFar><<<grid, 512, 0, stream>>>(p, sc);
+      if (p.plan.rows == 32) pt_attend_kernel<Ty, D, 2, 4, kFar><<<grid, 256, 0, stream>>>(p, sc);
     }
   } else if constexpr (D >= 32) {
     if (p.plan.waves == 4) {
       if (p.exact)
-        pt_attend_wide_kernel<Ty, D, 4, true><<<grid, 256, 0, stream>>>(p, sc);
+        pt_attend_wide_kernel<Ty, D, 4, true, kFar><<<grid, 256, 0, stream>>>(p, sc);
       else
-        pt_attend_wide_kernel<Ty, D, 4, false><<<grid, 256, 0, stream>>>(p, sc);
+        pt_attend_wide_kernel<Ty, D, 4, false, kFar><<<grid, 256, 0, stream>>>(p, sc);
     }
     if constexpr (D == 64 || D == 128) {
       if (p.plan.waves == 8) {
         if (p.exact)
-          pt_attend_wide_kernel<Ty, D, 8, true><<<grid, 512, 0, stream>>>(p, sc);
+          pt_attend_wide_kernel<Ty, D, 8, true, kFar><<<grid, 512, 0, stream>>>(p, sc);
         else
-          pt_attend_wide_kernel<Ty, D, 8, false><<<grid, 512, 0, stream>>>(p, sc);
+          pt_attend_wide_kernel<Ty, D, 8, false, kFar><<<grid, 512, 0, stream>>>(p, sc);
       }
     }
   }
@@ -916,14 +925,14 @@ hipError_t attend_dim(const PTAttendLaunch& p, const AttendScale& sc, hipStream_
   return hipGetLastError();
 }
 
-template <class Ty>
+template <class Ty, bool kFar>
 hipError_t attend(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
   switch (p.c.d) {
-    case 16: return attend_dim<Ty, 16>(p, sc, stream);
-    case 32: return attend_dim<Ty, 32>(p, sc, stream);
-    case 64: return attend_dim<Ty, 64>(p, sc, stream);
-    case 128: return attend_dim<Ty, 128>(p, sc, stream);
-    default: return attend_dim<Ty, 256>(p, sc, stream);
+    case 16: return attend_dim<Ty, 16, kFar>(p, sc, stream);
+    case 32: return attend_dim<Ty, 32, kFar>(p, sc, stream);
+    case 64: return attend_dim<Ty, 64, kFar>(p, sc, stream);
+    case 128: return attend_dim<Ty, 128, kFar>(p, sc, stream);
+    default: return attend_dim<Ty, 256, kFar>(p, sc, stream);
   }
 }
 
@@ -980,7 +989,8 @@ hipError_t launch_pt_attend(int dtype, const PTAttendLaunch& p, hipStream_t stre
   sc.scale_log2 = p.scale * kLog2e;
   sc.cap_scale = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
   sc.cap_log2 = p.softcap > 0.f ? p.softcap * kLog2e : 0.f;
-  return dtype == kF16 ? attend<HalfT>(p, sc, stream) : attend<Bf16T>(p, sc, stream);
+  if (sc.cap_log2 > kNearCap) return dtype == kF16 ? attend<HalfT, true>(p, sc, stream) : attend<Bf16T, true>(p, sc, stream);
+  return dtype == kF16 ? attend<HalfT, false>(p, sc, stream) : attend<Bf16T, false>(p, sc, stream);
 }
 
 hipError_t launch_pt_keep(const PTKeepLaunch& p, hipStream_t stream) {

@@ -434,6 +434,42 @@ def test_attend_with_scores_of_infinity_and_nan(t):
         assert torch.equal(out[0, :, : t - 1], plain[0, :, : t - 1])
 
 
+@pytest.mark.parametrize("t", [1, 5, 40])
+def test_a_far_softcap_changes_nothing(t):
+    """c tanh(s / c) differs from s by s^3 / (3 c^2): 2e-7 at c = 1e5 and scores up to 20, less than half a step (2^-24) of
+    the 16 that the scores' terms add up to in magnitude. So the output is within its bound without a cap."""
+    rng = np.random.default_rng(73)
+    cache, table = _filled(rng, 12, 16, 8, 2, 64, torch.float16, [100], t)
+    q = (torch.randn(1, 8, t, 64, generator=torch.Generator().manual_seed(4)) * 2).half().cuda()
+    out = cache.attend(0, q, _int32(table), _int32([100]), softcap=1e5, exact_weights=True)
+    _check_attend(cache, 0, table, [100], q, out, None, *_order(1, t), 0, 1.0 / 64**0.5, 0.0, exact=True)
+
+
+@pytest.mark.parametrize("cap", [0.5, 3.0, 50.0])
+@pytest.mark.parametrize("t", [1, 5, 40])
+def test_softcaps(t, cap):
+    rng = np.random.default_rng(79)
+    cache, table = _filled(rng, 12, 16, 8, 2, 64, torch.float16, [100], t)
+    q = (torch.randn(1, 8, t, 64, generator=torch.Generator().manual_seed(4)) * 4).half().cuda()
+    out = cache.attend(0, q, _int32(table), _int32([100]), softcap=cap, exact_weights=True)
+    _check_attend(cache, 0, table, [100], q, out, None, *_order(1, t), 0, 1.0 / 64**0.5, cap, exact=True)
+
+
+def test_one_token_at_given_positions():
+    rng = np.random.default_rng(89)
+    cache, table = _filled(rng, 9, 16, 4, 2, 64, torch.float16, [3, 40], 1, garbage=False)
+    g = torch.Generator().manual_seed(4)
+    q, k = torch.randn(2, 4, 64, generator=g).half().cuda(), torch.randn(2, 2, 64, generator=g).half().cuda()
+    inv, _ = rotary_frequencies(64, device="cuda")
+    pos = torch.tensor([7, 90000], device="cuda")
+    want = rotary_embedding(q, k, pos, inv)
+    for given in (pos, pos.int(), torch.stack([pos, pos], dim=1)[:, 0]):
+        assert torch.equal(cache.append(0, q, k, k, _int32(table), _int32([3, 40]), inv, positions=given), want[0])
+        for i, n in enumerate([3, 40]):
+            p, o = O.cells(table[i], 16, 9, n, 1)
+            assert torch.equal(cache.keys[0, int(p[0]), :, int(o[0])], want[1][i])
+
+
 def test_masks_that_leave_a_token_nothing():
     rng = np.random.default_rng(37)
     cache, table = _filled(rng, 8, 16, 4, 2, 64, torch.bfloat16, [0, 18], 6)
