@@ -303,9 +303,10 @@ int pgr_pt_append(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_
  * masks lengths[b] + depths[b, t]). Columns that are not new tokens get zeros, as does a head that sees nothing or
  * scores of -inf only. What the cache holds behind a row's new tokens and before all of their windows does not
  * matter; a value that is not finite among those that some token of the call sees may reach all the row's new
- * tokens. The probabilities enter the product with V as two numbers of the cache's dtype, or, where more than 32
- * columns times query heads of a KV head make it arithmetic that bounds the call, rounded to one (off by half a step of
- * each), unless exact_weights. q strides: batch, head, token. tokens * Hq / Hkv <= 2^20. */
+ * tokens. With exact_weights the probabilities enter the product with V as two numbers of the cache's dtype, whose
+ * rounding does not show; without, they may be rounded to one (off by half a step of each), as they are in calls of more
+ * than 32 columns times query heads of a KV head at head dims from 32. q strides: batch, head, token.
+ * tokens * Hq / Hkv <= 2^20. */
 size_t pgr_pt_attend_workspace_bytes(const pgr_pt_cache_t* cache, int64_t batch, int64_t tokens, int64_t width);
 int pgr_pt_attend(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_t* rows, const void* q,
                   const int64_t* q_strides, void* out, const uint64_t* masks, const int32_t* depths, int64_t window,

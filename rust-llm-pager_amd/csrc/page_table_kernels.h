@@ -73,7 +73,7 @@ struct PTAttendLaunch {
   const int32_t* depths = nullptr;   // with masks
   int window = 0;                    // 0: none
   float scale = 1.f, softcap = 0.f;
-  int exact = 0;  // P as two numbers also where arithmetic bounds
+  int exact = 1;  // P as two numbers; 0: one where that is faster
   PTAttendPlan plan;
   int2* meta = nullptr;   // [batch]: a row's first part, a part's tiles
   float* pm = nullptr;    // [hkv, blocks, slots, rows]

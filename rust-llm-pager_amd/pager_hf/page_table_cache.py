@@ -227,7 +227,7 @@ class PageTableCache:
 
     def attend(self, layer: int, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
                counts: torch.Tensor | None = None, tree: DraftTree | None = None, window: int | None = None,
-               softcap: float | None = None, scale: float | None = None, exact_weights: bool = False) -> torch.Tensor:
+               softcap: float | None = None, scale: float | None = None, exact_weights: bool = True) -> torch.Tensor:
         """Attention of the new tokens' queries q [B, Hq, T, D] (or [B, Hq, D]) over what their rows hold and, among
         the new tokens (appended before, with the same lengths), over those before them and themselves, or those
         that the tree's masks name.
@@ -239,9 +239,10 @@ class PageTableCache:
         -inf. What the pages hold behind a row's new tokens does not matter, nor what they hold before the window of
         its first new one (nor whether those pages are there).
 
-        The probabilities enter the product with V as two numbers of the cache's type, whose rounding does not show;
-        where more than 32 tokens times query heads per KV head make arithmetic the call's bound they are rounded to
-        one, each off by up to half a step of the type, unless ``exact_weights`` (a third more time at such sizes)."""
+        The probabilities enter the product with V as two numbers of the cache's type, whose rounding does not show.
+        A caller that may have them rounded to one, each off by up to half a step of the type, says so with
+        ``exact_weights=False``: calls of more than 32 tokens times query heads per KV head then take up to a quarter
+        less time (smaller ones, and all at head dim 16, keep the two, which cost nothing there)."""
         done = self._ops.pt_attend(self._address, self._index, layer, q, table, lengths, counts, tree, window, softcap, scale,
                                    exact_weights)
         if done is not None:
