@@ -286,7 +286,8 @@ typedef struct pgr_pt_rows_s {
 
 /* New tokens into the pages of one layer: k, v [batch, Hkv, tokens, D] and q [batch, Hq, tokens, D] (strides: batch,
  * head, token); with weights q and k are normed as pgr_norm_rotary norms them, with inv_freq turned, at
- * positions (strides: batch, token), or, with positions NULL, at lengths[b] plus depths[b, t] (depths NULL: plus t).
+ * positions (strides: batch, token), or, with positions NULL, at lengths[b] plus depths[b, t] (depths NULL: plus t; a
+ * depth below 0 counts as 0, here and in pgr_pt_attend).
  * q_out [batch, Hq, tokens, D] contiguous receives q, zeros where a token is not new; it must not overlap the other
  * operands. No operand may lie in the cache. Rows that put a token in one and the same place race for it. */
 int pgr_pt_append(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_t* rows, const void* q,

@@ -50,7 +50,7 @@ __device__ __forceinline__ Token token_of(const NormRotaryLaunch& a, int b, int 
   if (!kPages || a.positions != nullptr)
     k.pos = a.form.half > 0 ? load_position(a.positions, a.positions64, b * a.pos_b + t * a.pos_t) : 0;
   else
-    k.pos = length + (a.depths != nullptr ? a.depths[(int64_t)b * a.tokens + t] : t);
+    k.pos = length + (a.depths != nullptr ? max(a.depths[(int64_t)b * a.tokens + t], 0) : t);
   return k;
 }
 

@@ -173,12 +173,13 @@ __device__ __forceinline__ Row row_of(const PTAttendLaunch& a, const Span& s, in
     const int64_t row = (int64_t)b * a.r.tokens;
     r.mask = a.masks[row + at];
     if (s.n < 64) r.mask &= (1ull << s.n) - 1;
-    depth = min(max(a.depths[row + at], 0), kMostDrafts - 1);
+    depth = max(a.depths[row + at], 0);  // (none below 0: what a block reads begins a window before depth 0)
     if (a.window > 0)
       for (int j = 0; j < s.n; ++j)
-        if (min(max(a.depths[row + j], 0), kMostDrafts - 1) <= depth - a.window) r.mask &= ~(1ull << j);
+        if (max(a.depths[row + j], 0) <= depth - a.window) r.mask &= ~(1ull << j);
   }
-  r.lo = a.window > 0 ? s.length + depth - a.window + 1 : 0;
+  // (64 bits, and cut off behind all tokens: a depth may be any number.)
+  r.lo = a.window > 0 ? (int)min((int64_t)s.length + depth - a.window + 1, (int64_t)s.end) : 0;
   return r;
 }
 

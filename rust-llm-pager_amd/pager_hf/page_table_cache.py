@@ -40,7 +40,7 @@ from .rotary import _dense_last, _inference_only, _inv_freq, _norm_weight, _on, 
 
 class DraftTree(NamedTuple):
     """What drafted tokens see of each other: bit j of masks [B, T] int64 is set where the token sees drafted
-    token j; depths [B, T] int32 is what its position lies behind the row's held tokens."""
+    token j; depths [B, T] int32 is what its position lies behind the row's held tokens (below 0 counts as 0)."""
 
     masks: torch.Tensor
     depths: torch.Tensor

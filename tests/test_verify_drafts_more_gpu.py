@@ -8,7 +8,8 @@ import torch
 from oracle import drafted_tokens as O
 from pager_hf import DraftTree
 from pager_hf import _native as N
-from test_verify_drafts_gpu import CACHE_TYPES, _check_attend, _filled, _int32, _order
+from pager_hf.rotary import rotary_frequencies
+from test_verify_drafts_gpu import CACHE_TYPES, STEP, TINY, _check_attend, _filled, _int32, _np, _order, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +51,42 @@ def test_many_rows_keep_the_weights_unless_told_otherwise(d, dtype, path):
     for more, exact in ((dict(), True), (dict(exact_weights=True), True), (dict(exact_weights=False), False)):
         out = cache.attend(0, q, _int32(table), _int32([24]), **more)
         _check_attend(cache, 0, table, [24], q, out, None, *_order(1, t), 0, 1.0 / d**0.5, 0.0, exact=exact)
+
+
+# ---- depths --------------------------------------------------------------------------------------
+DEPTHS = [0, 63, 64, 100, 149, 150, 151, 999, 1 << 20, (1 << 31) - 1, -1, -100]
+
+
+@pytest.mark.parametrize("window", [1, 100, 150, 1 << 30])
+@pytest.mark.parametrize("hq,t", [(4, 12), (16, 12), (8, 60)])
+def test_a_window_goes_by_depths_of_any_size(hq, t, window):
+    """A tree made by hand: its depths are what they say, however large; those below 0 count as 0."""
+    rng = np.random.default_rng(101)
+    lengths = [1000, 20, 0]
+    cache, table = _filled(rng, 40, 32, hq, 2, 64, torch.float16, lengths, t, garbage=False)
+    depth = rng.choice(DEPTHS, (3, t))
+    depth[:, : min(t, 12)] = DEPTHS[: min(t, 12)]
+    sees = rng.random((3, t, t)) < 0.5
+    sees[:, np.arange(t), np.arange(t)] = True
+    q = torch.randn(3, hq, t, 64, generator=torch.Generator().manual_seed(6)).half().cuda()
+    out = cache.attend(0, q, _int32(table), _int32(lengths), tree=_tree_of(sees, depth), window=window)
+    _check_attend(cache, 0, table, lengths, q, out, None, sees, np.maximum(depth, 0), window, 0.125, 0.0, exact=True)
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_goes_by_depths_of_any_size(norm):
+    rng = np.random.default_rng(103)
+    depth = np.array([[0, 63, 64, 1 << 20, -1, -100]])
+    t, dtype = depth.shape[1], torch.float16
+    cache, table = _filled(rng, 4, 16, 4, 2, 64, dtype, [30], t, garbage=False)
+    g = torch.Generator().manual_seed(7)
+    q, k = torch.randn(1, 4, t, 64, generator=g).half().cuda(), torch.randn(1, 2, t, 64, generator=g).half().cuda()
+    inv, _ = rotary_frequencies(64, device="cuda")
+    w = torch.ones(64, device="cuda").half() if norm else None
+    out = cache.append(0, q, k, k, _int32(table), _int32([30]), inv, tree=_tree_of(np.ones((1, t, t), bool), depth), q_weight=w,
+                       k_weight=w)
+    pos = 30 + np.maximum(depth, 0)
+    p, o = (torch.tensor(x, device="cuda") for x in O.cells(table[0], 16, 4, 30, t))
+    for got, x in ((out[0], q), (cache.keys[0][p, :, o].transpose(0, 1), k)):
+        ref, bound = O.norm_rotate(_np(x), None if w is None else _np(w), 1e-6, pos[:, None], _np(inv))
+        _within(got[None], ref, bound + STEP[dtype] * (np.abs(ref) + bound) + TINY[dtype], "turned")
