@@ -751,7 +751,9 @@ __global__ __launch_bounds__(256) void pt_merge_kernel(PTAttendLaunch a, int gro
   const int2 meta = a.meta[b];  // the row's first part, a part's tiles
   const int tiles = row_tiles(a, b);
   if (tiles > 0 && tiles <= meta.y) return;  // (a row of one part is finished by its workgroup)
-  const int used = real ? (tiles_of(a.plan, sp) + meta.y - 1) / meta.y : 0;
+  // (Within the workspace, whatever the lengths have become since.)
+  const int most = max(a.plan.slots - max(meta.x, 0), 0);
+  const int used = real ? min((tiles_of(a.plan, sp) + meta.y - 1) / max(meta.y, 1), most) : 0;
   const int64_t part = (((int64_t)h * a.plan.blocks + block) * a.plan.slots + meta.x) * a.plan.rows + in;
   float m = kMinusInf, l = 0.f;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
@@ -958,6 +960,9 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
     if (d < 256) p.share = p.least = 8;
     return p;
   }
+  // The device adds the batch's tiles up in 32 bits: beyond, rows are left whole (2^35 tokens; such a table is
+  // one that rows share).
+  if (batch * ((capacity + p.tile - 1) / p.tile) >= (int64_t)1 << 30) return p;
   // Parts a row on average: as many as fill the card once.
   const int64_t groups = units * p.blocks, most = (capacity + p.least * p.tile - 1) / (p.least * p.tile);
   int64_t n = target / groups;

@@ -1,0 +1,29 @@
+"""How attend calls over pages are dealt out, by the workspace they ask for (CPU)."""
+from __future__ import annotations
+
+import pytest
+
+import _pgr_native as nat
+
+
+def _cache(query_heads=4, kv_heads=2, head_dim=32, page_tokens=16):
+    return nat.PTCache(keys=1 << 20, values=2 << 20, layers=1, pages=4, query_heads=query_heads, kv_heads=kv_heads,
+                       page_tokens=page_tokens, head_dim=head_dim, dtype=1)
+
+
+def _bytes(batch, tokens, capacity, **geometry):
+    c = _cache(**geometry)
+    return nat.load().pgr_pt_attend_workspace_bytes(c, batch, tokens, -(-capacity // c.page_tokens))
+
+
+MOST = 1 << 30  # tokens of a row
+
+
+@pytest.mark.parametrize("batch,tokens,capacity,cut", [
+    (1, 1, MOST, True), (31, 1, MOST, True), (32, 1, MOST, False), (64, 1, MOST, False), (256, 1, MOST, False),
+    (65535, 1, MOST, False), (64, 64, MOST, False), (128, 64, MOST, False), (64, 1, MOST >> 1, False), (64, 1, MOST >> 2, True),
+])
+def test_rows_whose_tiles_pass_32_bits_stay_whole(batch, tokens, capacity, cut):
+    """The rows' tiles (32 tokens; 64 with more than 32 rows a KV head) are added up in 32 bits on the device, so a batch
+    of 2^30 of them or more is not cut into parts. (Rows may share a table's row, so such a call can be made.)"""
+    assert (_bytes(batch, tokens, capacity, query_heads=4, kv_heads=1) > 0) == cut
