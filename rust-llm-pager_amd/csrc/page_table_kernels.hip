@@ -960,6 +960,11 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
     if (d < 256) p.share = p.least = 8;
     return p;
   }
+  // Every wave walks the batch to find its part, 64 rows at a time and several times over, and there are as many parts as
+  // rows or more: above 256 rows that costs what it gains. One token, 16/1 heads, D 32, rows of 0 to 4096 tokens, cut
+  // and whole: 300 rows 35 and 25 us, 700 89 and 37, 1025 166 and 50, 4097 1729 and 202; 8/1, D 128, all of 4095 tokens: 300
+  // rows 127 and 137, 700 287 and 248.
+  if (batch > 256) return p;
   // The device adds the batch's tiles up in 32 bits: beyond, rows are left whole (2^35 tokens; such a table is
   // one that rows share).
   if (batch * ((capacity + p.tile - 1) / p.tile) >= (int64_t)1 << 30) return p;
@@ -980,7 +985,7 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
   const int64_t once = target / ((int64_t)hkv * p.blocks);
   if (n > 1) {
     p.slots = (int)(batch > 1 && once > n * batch ? once : n * batch);
-  } else if (batch > 1 && batch <= 256 && most >= 32) {
+  } else if (batch > 1 && most >= 32) {
     // The rows fill the card, but one that is much longer than the others would hold the call up: one of 60000 tokens and
     // 63 of 200 (32/8 heads, D 128) 635 us whole, 78 cut; 64 of 4096 tokens, none of them cut, 184 and 188.
     // (Not where a row's results are many: it has blocks enough then.)

@@ -27,3 +27,14 @@ def test_rows_whose_tiles_pass_32_bits_stay_whole(batch, tokens, capacity, cut):
     """The rows' tiles (32 tokens; 64 with more than 32 rows a KV head) are added up in 32 bits on the device, so a batch
     of 2^30 of them or more is not cut into parts. (Rows may share a table's row, so such a call can be made.)"""
     assert (_bytes(batch, tokens, capacity, query_heads=4, kv_heads=1) > 0) == cut
+
+
+@pytest.mark.parametrize("geometry", [dict(query_heads=16, kv_heads=1, head_dim=32), dict(query_heads=8, kv_heads=1, head_dim=128),
+                                      dict(query_heads=32, kv_heads=8, head_dim=128), dict(query_heads=8, kv_heads=2, head_dim=256)],
+                         ids=str)
+@pytest.mark.parametrize("tokens", [1, 5, 64])
+def test_large_batches_stay_whole(tokens, geometry):
+    """Finding a part walks the batch, in every workgroup: not above 256 rows."""
+    for batch in (257, 300, 520, 1025, 4097, 7000):
+        assert _bytes(batch, tokens, 4096, **geometry) == 0, batch
+    assert _bytes(2, tokens, 4096, **geometry) > 0

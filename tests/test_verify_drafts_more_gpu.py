@@ -90,3 +90,19 @@ def test_append_goes_by_depths_of_any_size(norm):
     for got, x in ((out[0], q), (cache.keys[0][p, :, o].transpose(0, 1), k)):
         ref, bound = O.norm_rotate(_np(x), None if w is None else _np(w), 1e-6, pos[:, None], _np(inv))
         _within(got[None], ref, bound + STEP[dtype] * (np.abs(ref) + bound) + TINY[dtype], "turned")
+
+
+# ---- batches -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("window", [0, 70])
+def test_attend_over_more_than_a_thousand_rows(window):
+    """One KV head, ragged rows, one of them long."""
+    rng = np.random.default_rng(107)
+    b, t, dtype = 1100, 2, torch.float16
+    lengths = [int(x) for x in rng.integers(0, 40, b)]
+    lengths[700] = 4000
+    pages = sum(-(-(n + t) // 32) for n in lengths) + 1
+    cache, table = _filled(rng, pages, 32, 16, 1, 32, dtype, lengths, t)
+    counts = [i % 4 for i in range(b)]  # 3: all of them
+    q = torch.randn(b, 16, t, 32, generator=torch.Generator().manual_seed(6)).to(dtype).cuda()
+    out = cache.attend(0, q, _int32(table), _int32(lengths), counts=_int32(counts), window=window)
+    _check_attend(cache, 0, table, lengths, q, out, counts, *_order(b, t), window, 1.0 / 32**0.5, 0.0, exact=True)
