@@ -971,10 +971,28 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
   // Parts a row on average: as many as fill the card once.
   const int64_t groups = units * p.blocks, most = (capacity + p.least * p.tile - 1) / (p.least * p.tile);
   int64_t n = target / groups;
-  if (2 * groups > target) {  // whole rounds, as far as a few splits bring them
+  if (2 * groups > target) {
+    // The blocks all but fill the card, or more: cut where whole rounds of workgroups come nearer by more than the parts
+    // cost. The unit is a round of the longest block. Blocks of a prompt's tokens shorten from the last to the first, the
+    // longest start first: they end after their mean work and the shortest block, or after whole rounds. A part's results
+    // are written and read once more, which takes as long as two tokens for each of its rows, and 300 tokens at most (where
+    // arithmetic bounds a token takes longer). 256 MiB of them at most: a token more must not ask for gigabytes.
+    // Whole, in 2 and in 4 parts (P as one number): a prompt of 8193 tokens, 32/8 heads, D 128, 619, 720 and 777 us (8192: 665,
+    // 740, 780), one of 2100 over 16384 1101, 853, 736; 9 rows of 130 over 900, 32/4, D 64, 31, 49, 52; 65 rows of one
+    // token over 4096, 32/8, 222, 209, 208.
+    const double round = (double)groups / target, last = tokens < capacity ? 1. - tokens / (double)capacity : 0.,
+                 mean = 0.5 * (1. + last);
+    const double each = 2. * rows / p.blocks < 300. ? 2. * rows / p.blocks : 300.;
     double best = 1e30;
     for (int k = 1; k <= 4; ++k) {
-      const double cost = (double)((groups * k + target - 1) / target) / k + (k > 1 ? 0.05 + 0.01 * k : 0.);
+      const double whole = (double)((groups * k + target - 1) / target) / k;
+      const double even = round * mean + (k == 1 ? last : 1. / k);
+      double cost = even < whole ? even : whole;
+      if (cost < 1. / k) cost = 1. / k;
+      if (k > 1) {
+        if (groups * k * p.rows * (d + 2) * 4 > (int64_t)256 << 20) break;
+        cost += 0.05 + 0.01 * k + k * round * each / (capacity * mean);
+      }
       if (cost < best) {
         best = cost;
         n = k;

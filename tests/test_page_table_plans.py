@@ -38,3 +38,38 @@ def test_large_batches_stay_whole(tokens, geometry):
     for batch in (257, 300, 520, 1025, 4097, 7000):
         assert _bytes(batch, tokens, 4096, **geometry) == 0, batch
     assert _bytes(2, tokens, 4096, **geometry) > 0
+
+
+GEOMETRIES = [(32, 8, 128), (28, 4, 128), (14, 2, 64), (16, 1, 32), (16, 16, 64), (8, 1, 256), (4, 2, 16)]
+SIZES = sorted({max(1, (1 << k) + i) for k in range(0, 18) for i in (-1, 0, 1)})
+
+
+@pytest.mark.parametrize("geometry", GEOMETRIES, ids=str)
+def test_the_workspace_is_bounded_whatever_the_batch_and_the_prompt(geometry):
+    """256 MiB of parts at most (and 1 KiB a buffer for its alignment, and the batch's own table of parts)."""
+    hq, hkv, d = geometry
+    for batch in (1, 2, 3, 31, 64, 65, 128, 255, 256, 257, 300, 2049):
+        for tokens in SIZES:
+            if tokens * (hq // hkv) > 1 << 20 or batch * hkv * tokens * (hq // hkv) > 1 << 27:
+                continue
+            for held in (0, 1000, 32768, 1 << 20):
+                n = _bytes(batch, tokens, tokens + held, query_heads=hq, kv_heads=hkv, head_dim=d)
+                assert n <= (256 << 20) + 4096 + 8 * batch, (batch, tokens, held, n)
+
+
+@pytest.mark.parametrize("batch,tokens,held,geometry", [
+    (1, 8192, 0, (32, 8, 128)), (1, 8193, 0, (32, 8, 128)), (1, 16385, 0, (32, 8, 128)), (1, 2049, 0, (32, 8, 128)),
+    (1, 65537, 0, (32, 8, 128)), (9, 130, 900, (32, 4, 64)), (130, 40, 500, (8, 2, 128)),
+])
+def test_calls_whose_parts_cost_more_than_they_bring_stay_whole(batch, tokens, held, geometry):
+    hq, hkv, d = geometry
+    assert _bytes(batch, tokens, tokens + held, query_heads=hq, kv_heads=hkv, head_dim=d) == 0
+
+
+@pytest.mark.parametrize("batch,tokens,held,geometry", [
+    (1, 2100, 16384, (32, 8, 128)), (65, 1, 4096, (32, 8, 128)), (33, 64, 4096, (32, 8, 128)), (65, 5, 4000, (28, 4, 128)),
+    (1, 1, 1000, (14, 2, 64)), (8, 64, 32768, (28, 4, 128)), (8, 13, 8191, (32, 4, 64)),
+])
+def test_calls_that_parts_make_faster_are_cut(batch, tokens, held, geometry):
+    hq, hkv, d = geometry
+    assert _bytes(batch, tokens, tokens + held, query_heads=hq, kv_heads=hkv, head_dim=d) > 0

@@ -9,7 +9,7 @@ from oracle import drafted_tokens as O
 from pager_hf import DraftTree
 from pager_hf import _native as N
 from pager_hf.rotary import rotary_frequencies
-from test_verify_drafts_gpu import CACHE_TYPES, STEP, TINY, _check_attend, _filled, _int32, _np, _order, _within
+from test_verify_drafts_gpu import CACHE_TYPES, STEP, TINY, _attend_bounds, _check_attend, _filled, _int32, _np, _order, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,21 @@ def test_attend_over_more_than_a_thousand_rows(window):
     q = torch.randn(b, 16, t, 32, generator=torch.Generator().manual_seed(6)).to(dtype).cuda()
     out = cache.attend(0, q, _int32(table), _int32(lengths), counts=_int32(counts), window=window)
     _check_attend(cache, 0, table, lengths, q, out, counts, *_order(b, t), window, 1.0 / 32**0.5, 0.0, exact=True)
+
+
+@pytest.mark.parametrize("tokens", [2048, 2049])
+def test_prompts_of_one_token_more(tokens):
+    """A prompt into an empty cache whose blocks of rows just fill the card, and one token more."""
+    rng = np.random.default_rng(109)
+    cache, table = _filled(rng, 70, 32, 32, 8, 64, torch.bfloat16, [0], tokens)
+    q = torch.randn(1, 32, tokens, 64, generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+    out = cache.attend(0, q, _int32(table), _int32([0]))
+    sees, depth = _order(1, tokens)
+    kn, vn, qn = (x[0].double() for x in (cache.keys, cache.values, q))
+    p, o = (torch.tensor(x, device="cuda") for x in O.cells(table[0], 32, 70, 0, tokens))
+    for at in (0, 1, 63, 64, 65, 1000, 2046, tokens - 1):
+        for h in (0, 7):
+            ref, bound = O.attend_row(_np(qn[4 * h: 4 * h + 4, at: at + 1]), _np(kn[p, h, o][: at + 1]), _np(vn[p, h, o][: at + 1]),
+                                      np.ones(at + 1, bool), at, 1, sees[0, :1, :1], depth[0, :1], 0, 0.125, 0.0,
+                                      **_attend_bounds(torch.bfloat16))
+            _within(out[0, 4 * h: 4 * h + 4, at: at + 1], ref, bound, f"token {at} head {h}")
