@@ -194,20 +194,40 @@ __device__ __forceinline__ uint64_t sees(const PTAttendLaunch& a, const Span& s,
   return (low_bits(-at) & since) | fresh;
 }
 
-// cap * log2(e) * tanh(y), y = x * scale / cap, as 1 - 2 / (1 + e^2y): within 5 half steps of float32 of the cap, which up to
-// a cap of 64 is 2^-15.7 of a weight at most. Under larger caps (kFar) small y go by the series (the next term is 6e-8
-// of it), so that the error is 3e-6 of the score: in kernels of their own (kFar), since the choice for each score costs 8
-// drafted trees (D 64) 4 of 30 us. tanhf takes three times as much.
-constexpr float kNearCap = 64.f * kLog2e;
+// Scores x to cap * log2(e) * tanh(y), y = x * scale / cap, by z = 2 log2(e) y (x * cap_scale here): 1 - 2 / (1 + 2^z), whose error
+// is that of numbers about 1, and below kNear (y below 0.6) z times a polynomial in z^2, whose error goes by the score. The
+// polynomial is fitted to an even relative error of 2^-23.5; with float32's roundings it is within 4 half steps of the
+// score, the other within 5 of the score and 3 of the cap (a unit in the last place each for the exponential and the
+// reciprocal counted in). Caps lie far above most scores, and where all of a wave's are near, the polynomial takes no
+// longer than the exponential would: 13 drafted tokens over 8 x 8191, 32/4 heads, D 64, 37 us without a cap, 41 with the
+// exponential alone, 43 so, and 50 under a cap of 5 that many scores pass; a chunk of 2048 tokens over 16384, 32/8,
+// D 128, 830, 980, 984 and 1202.
+constexpr float kNear = 1.73f;
 
-template <bool kFar>
-__device__ __forceinline__ float capped(float x, const AttendScale& sc) {
-  float t = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (sc.cap_scale * (2.f * kLog2e)))), 1.f);
-  if constexpr (kFar) {
-    const float y = x * sc.cap_scale, y2 = y * y, series = y * fmaf(y2, fmaf(y2, 2.f / 15.f, -1.f / 3.f), 1.f);
-    t = fabsf(y) < 0.1f ? series : t;
+__device__ __forceinline__ float capped_near(float z) {
+  const float z2 = z * z;
+  return z * fmaf(z2, fmaf(z2, fmaf(z2, fmaf(z2, 1.1262515e-06f, -3.135718e-05f), 0.000665667001f), -0.013875721f), 0.346573591f);
+}
+
+template <int N, class V>
+__device__ __forceinline__ void capped(V& s, const AttendScale& sc) {
+  float most = 0.f;
+  float near[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s[i] *= sc.cap_scale;
+    near[i] = capped_near(s[i]);
+    most = fmaxf(most, fabsf(s[i]));
   }
-  return sc.cap_log2 * t;
+  if (__any(most >= kNear)) {  // (NaN is NaN either way)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[i])), 1.f);
+      near[i] = fabsf(s[i]) >= kNear ? far : near[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = sc.cap_log2 * near[i];
 }
 
 // ---------------------------------------------------------------------------------------
@@ -226,7 +246,7 @@ __device__ __forceinline__ float capped(float x, const AttendScale& sc) {
 // 14.4 either way, 16 rows of 4096 tokens, D 64: 19.5 / 21.0 / 21.8. Short rows are finished by one workgroup of
 // eight waves, without a merge: 256 tokens, D 64 6.7 us against 9.4, D 128 8.2 against 10.4; at 1000 and 500 tokens
 // (D 64 and 128) the two are even.
-template <class Ty, int D, int kG, int kW, bool kFar>
+template <class Ty, int D, int kG, int kW>
 __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, AttendScale sc) {
   typedef KVTile<D> T;
   constexpr int kThreads = 64 * kW, kRows = 16 * kG;
@@ -349,12 +369,13 @@ __global__ __launch_bounds__(64 * kW) void pt_attend_kernel(PTAttendLaunch a, At
 #pragma unroll
     for (int y = 0; y < kG; ++y) {
       float p[8], top = kMinusInf;
-      if (kFar || sc.cap_log2 > 0.f) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = capped<kFar>(s[y][i / 4][i & 3], sc);
+      for (int i = 0; i < 8; ++i) p[i] = s[y][i / 4][i & 3];
+      if (sc.cap_log2 > 0.f) {
+        capped<8>(p, sc);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = s[y][i / 4][i & 3] * sc.scale_log2;
+        for (int i = 0; i < 8; ++i) p[i] *= sc.scale_log2;
       }
       if (masked) {
         const uint32_t here = (there(at.page[0]) ? 0xffffu : 0u) | (there(at.page[1]) ? 0xffff0000u : 0u);
@@ -506,7 +527,7 @@ struct Staged {
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
-template <class Ty, int D, int kW, bool kTwo, bool kFar>
+template <class Ty, int D, int kW, bool kTwo>
 __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kernel(PTAttendLaunch a, AttendScale sc) {
   typedef Staged<D> L;
   constexpr int kTok = D == 256 ? 32 : 64, kThreads = 64 * kW, kRows = 32 * kW, kHalves = kTok / 32;
@@ -625,12 +646,10 @@ __global__ __launch_bounds__(64 * kW, D == 256 ? 1 : 2) void pt_attend_wide_kern
     const bool masked = ~here != 0 || c0 < lo_most || c0 + kTok > seen_by_all;
     // (Scores stay as the products left them, `unit` of them in log2 units: one multiply-add before the exponential.)
     float top = kMinusInf, unit = sc.scale_log2;
-    if (kFar || sc.cap_log2 > 0.f) {
+    if (sc.cap_log2 > 0.f) {
       unit = 1.f;
 #pragma unroll
-      for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[x][i] = capped<kFar>(s[x][i], sc);
+      for (int x = 0; x < kHalves; ++x) capped<16>(s[x], sc);
     }
     if (masked) {
       const uint64_t seen = sees(a, sp, row, c0 + 4 * h) & here >> 4 * h;
@@ -889,29 +908,29 @@ __global__ __launch_bounds__(64) void draft_tree_kernel(const int32_t* parents, 
   }
 }
 
-template <class Ty, int D, bool kFar>
+template <class Ty, int D>
 hipError_t attend_dim(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
   const int64_t parts = (int64_t)p.c.hkv * (p.plan.slots == 0 ? p.r.batch : p.plan.slots);
   const dim3 grid((unsigned)((parts + 7) / 8 * 8 * p.plan.blocks));
   if (p.plan.waves == 0) {
-    if (p.plan.rows == 16 && p.plan.share == 4) pt_attend_kernel<Ty, D, 1, 4, kFar><<<grid, 256, 0, stream>>>(p, sc);
+    if (p.plan.rows == 16 && p.plan.share == 4) pt_attend_kernel<Ty, D, 1, 4><<<grid, 256, 0, stream>>>(p, sc);
     if constexpr (D < 256) {
-      if (p.plan.rows == 16 && p.plan.share == 8) pt_attend_kernel<Ty, D, 1, 8, kFar><<<grid, 512, 0, stream>>>(p, sc);
-      if (p.plan.rows == 32) pt_attend_kernel<Ty, D, 2, 4, kFar><<<grid, 256, 0, stream>>>(p, sc);
+      if (p.plan.rows == 16 && p.plan.share == 8) pt_attend_kernel<Ty, D, 1, 8><<<grid, 512, 0, stream>>>(p, sc);
+      if (p.plan.rows == 32) pt_attend_kernel<Ty, D, 2, 4><<<grid, 256, 0, stream>>>(p, sc);
     }
   } else if constexpr (D >= 32) {
     if (p.plan.waves == 4) {
       if (p.exact)
-        pt_attend_wide_kernel<Ty, D, 4, true, kFar><<<grid, 256, 0, stream>>>(p, sc);
+        pt_attend_wide_kernel<Ty, D, 4, true><<<grid, 256, 0, stream>>>(p, sc);
       else
-        pt_attend_wide_kernel<Ty, D, 4, false, kFar><<<grid, 256, 0, stream>>>(p, sc);
+        pt_attend_wide_kernel<Ty, D, 4, false><<<grid, 256, 0, stream>>>(p, sc);
     }
     if constexpr (D == 64 || D == 128) {
       if (p.plan.waves == 8) {
         if (p.exact)
-          pt_attend_wide_kernel<Ty, D, 8, true, kFar><<<grid, 512, 0, stream>>>(p, sc);
+          pt_attend_wide_kernel<Ty, D, 8, true><<<grid, 512, 0, stream>>>(p, sc);
         else
-          pt_attend_wide_kernel<Ty, D, 8, false, kFar><<<grid, 512, 0, stream>>>(p, sc);
+          pt_attend_wide_kernel<Ty, D, 8, false><<<grid, 512, 0, stream>>>(p, sc);
       }
     }
   }
@@ -928,14 +947,14 @@ hipError_t attend_dim(const PTAttendLaunch& p, const AttendScale& sc, hipStream_
   return hipGetLastError();
 }
 
-template <class Ty, bool kFar>
+template <class Ty>
 hipError_t attend(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
   switch (p.c.d) {
-    case 16: return attend_dim<Ty, 16, kFar>(p, sc, stream);
-    case 32: return attend_dim<Ty, 32, kFar>(p, sc, stream);
-    case 64: return attend_dim<Ty, 64, kFar>(p, sc, stream);
-    case 128: return attend_dim<Ty, 128, kFar>(p, sc, stream);
-    default: return attend_dim<Ty, 256, kFar>(p, sc, stream);
+    case 16: return attend_dim<Ty, 16>(p, sc, stream);
+    case 32: return attend_dim<Ty, 32>(p, sc, stream);
+    case 64: return attend_dim<Ty, 64>(p, sc, stream);
+    case 128: return attend_dim<Ty, 128>(p, sc, stream);
+    default: return attend_dim<Ty, 256>(p, sc, stream);
   }
 }
 
@@ -1015,11 +1034,11 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
 
 hipError_t launch_pt_attend(int dtype, const PTAttendLaunch& p, hipStream_t stream) {
   AttendScale sc;
-  sc.scale_log2 = p.scale * kLog2e;
-  sc.cap_scale = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
-  sc.cap_log2 = p.softcap > 0.f ? p.softcap * kLog2e : 0.f;
-  if (sc.cap_log2 > kNearCap) return dtype == kF16 ? attend<HalfT, true>(p, sc, stream) : attend<Bf16T, true>(p, sc, stream);
-  return dtype == kF16 ? attend<HalfT, false>(p, sc, stream) : attend<Bf16T, false>(p, sc, stream);
+  constexpr double kLog2 = 1.4426950408889634;  // (of e; each factor rounded once)
+  sc.scale_log2 = (float)(p.scale * kLog2);
+  sc.cap_scale = p.softcap > 0.f ? (float)(p.scale / (double)p.softcap * (2. * kLog2)) : 0.f;
+  sc.cap_log2 = p.softcap > 0.f ? (float)(p.softcap * kLog2) : 0.f;
+  return dtype == kF16 ? attend<HalfT>(p, sc, stream) : attend<Bf16T>(p, sc, stream);
 }
 
 hipError_t launch_pt_keep(const PTKeepLaunch& p, hipStream_t stream) {

@@ -124,3 +124,82 @@ def test_prompts_of_one_token_more(tokens):
                                       np.ones(at + 1, bool), at, 1, sees[0, :1, :1], depth[0, :1], 0, 0.125, 0.0,
                                       **_attend_bounds(torch.bfloat16))
             _within(out[0, 4 * h: 4 * h + 4, at: at + 1], ref, bound, f"token {at} head {h}")
+
+
+# ---- softcaps ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", CACHE_TYPES)
+@pytest.mark.parametrize("cap", [0.75, 20.0, 60.0, 64.0, 5000.0])
+@pytest.mark.parametrize("t", [3, 60])
+def test_a_softcap_is_as_near_as_the_score_not_as_the_cap(t, cap, dtype):
+    """Two tokens whose weighted values all but cancel, scores of at most 2. Queries and keys of one component: the
+    product is exact (8 + 8 bits in bf16, 11 + 2 in fp16). A score then has: the scale's quotient, its product with the cap's
+    reciprocal and the last product with a constant of its own, half a step each, which tanh passes on no larger
+    than relative to itself, and tanh's own 6; 4 for the softmax's difference and exponential, of a score of 2 at
+    most. Two scores: twice that. The sums and quotient: 8 more."""
+    rng = np.random.default_rng(113)
+    cache, table = _filled(rng, 8, 16, 8, 2, 64, dtype, [2], t, garbage=False)
+    p, o = (torch.tensor(x, device="cuda") for x in O.cells(table[0], 16, 8, 0, 2))
+    keys = torch.zeros(2, 2, 64)
+    keys[0, :, 0], keys[1, :, 0] = 1.0, 1.0 + 2.0**-6
+    cache.keys[0][p, :, o] = keys.to(dtype).cuda()
+    values = torch.ones(2, 2, 64)
+    values[1] = -(1.0 + torch.linspace(-0.04, 0.04, 64)).to(dtype).float()
+    cache.values[0][p, :, o] = values.to(dtype).cuda()
+    q = torch.zeros(1, 8, t, 64)
+    q[..., 0] = torch.rand(1, 8, t, generator=torch.Generator().manual_seed(5)) * 3.9 - 1.95
+    q = q.to(dtype).cuda()
+    none = _tree_of(np.zeros((1, t, t), bool), np.zeros((1, t), np.int64))  # (the new tokens see the held two alone)
+    out = cache.attend(0, q, _int32(table), _int32([2]), tree=none, softcap=cap, scale=1.0)
+    s = _np(q)[0, :, :, :1] * np.array([1.0, 1.0 + 2.0**-6])
+    y = cap * np.tanh(s / cap)
+    w = np.exp(y - y.max(-1, keepdims=True))
+    w /= w.sum(-1, keepdims=True)
+    v = _np(values)[:, 0]
+    ref = w @ v
+    bounds = _attend_bounds(dtype)
+    rel = 2 * 14 * 2.0**-24 * np.abs(y).max(-1, keepdims=True) + 8 * 2.0**-24 + bounds["p_step"]
+    bound = (w * rel) @ np.abs(v) + bounds["p_floor"] * 2
+    bound = bound + STEP[dtype] * (np.abs(ref) + bound) + TINY[dtype]
+    _within(out[0], ref, bound, f"cap {cap}")
+
+
+@pytest.mark.parametrize("dtype", CACHE_TYPES)
+@pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("cap", [65.0, 200.0])
+def test_softcaps_above_64(cap, d, dtype):
+    """Scores on both sides of the cap's straight part; a row cut into parts and joined, short rows, many rows."""
+    for lengths, hq, t, width in (([3000], 4, 1, 0), ([3000], 16, 9, 0), ([90, 3], 8, 5, 0), ([260], 8, 30, 4000)):
+        rng = np.random.default_rng(127)
+        pages = sum(-(-(n + t) // 16) for n in lengths) + 3
+        cache, table = _filled(rng, pages, 16, hq, 1, d, dtype, lengths, t, spare=2 + width)
+        b = len(lengths)
+        q = (torch.randn(b, hq, t, d, generator=torch.Generator().manual_seed(4)) * 8).to(dtype).cuda()
+        out = cache.attend(0, q, _int32(table), _int32(lengths), softcap=cap, scale=8.0 / d**0.5)
+        _check_attend(cache, 0, table, lengths, q, out, None, *_order(b, t), 0, 8.0 / d**0.5, cap, exact=True)
+
+
+def test_a_softcap_passes_infinities_and_nan_on():
+    """Scores of both infinities are the cap's two ends; a score of NaN stays with its token and head."""
+    for t in (1, 40):
+        cache, table = _filled(np.random.default_rng(131), 8, 16, 4, 1, 64, torch.float16, [20], t, garbage=False)
+        p, o = O.cells(table[0], 16, 8, 0, 20 + t)
+        q = torch.rand(1, 4, t, 64, generator=torch.Generator().manual_seed(6)).half().cuda() + 0.1
+        cache.keys[0, int(p[3]), :, int(o[3])] = float("inf")
+        cache.keys[0, int(p[4]), :, int(o[4])] = float("-inf")
+        out = cache.attend(0, q, _int32(table), _int32([20]), softcap=20.0)
+        kn, vn, qn = _np(cache.keys[0]), _np(cache.values[0]), _np(q)
+        kn[p[3], :, o[3]], kn[p[4], :, o[4]] = 1e9, -1e9  # (as good as infinite under the cap)
+        ref, _ = O.attend_row(qn[0], kn[p, 0, o], vn[p, 0, o], np.ones(20 + t, bool), 20, t, _order(1, t)[0][0], np.arange(t), 0,
+                              0.125, 20.0, **_attend_bounds(torch.float16))
+        # (Two scores off by the product's roundings and by 10 half steps of the cap; sums and the exponent; P; the output.)
+        plain = [i for i in range(20 + t) if i not in (3, 4)]
+        size = (np.abs(qn[0]) @ np.abs(kn[p, 0, o][plain]).T).max() * 0.125
+        off = (2 * (64 + 4) * size + 2 * 10 * 20.0 + 20 + t + 16 + 4 * 40.0) * 2.0**-24 + 3 * STEP[torch.float16] ** 2
+        bound = off * np.abs(vn[p, 0, o]).max()
+        _within(out[0], ref, bound + STEP[torch.float16] * (np.abs(ref) + bound) + TINY[torch.float16], "ends")
+        bad = q.clone()
+        bad[0, 2, t - 1, 5] = float("nan")
+        got = cache.attend(0, bad, _int32(table), _int32([20]), softcap=20.0)
+        assert torch.isnan(got[0, 2, t - 1]).all()
+        got[0, 2, t - 1] = out[0, 2, t - 1]
+        assert torch.equal(got, out)
