@@ -161,13 +161,15 @@ class PageTableCache:
                             tokens)
         return rows, (table, lengths, counts)
 
-    def _tree(self, tree: DraftTree | None, batch: int, tokens: int):
+    def _tree(self, tree: DraftTree | tuple[torch.Tensor, torch.Tensor] | None, batch: int, tokens: int):
         if tree is None:
             return None, None
         if tokens > 64:
             raise NotImplementedError(f"a tree has up to 64 tokens, got {tokens}")
-        return (self._numbers(tree.masks, "tree.masks", (batch, tokens), torch.int64),
-                self._numbers(tree.depths, "tree.depths", (batch, tokens)))
+        if not isinstance(tree, tuple) or len(tree) != 2:
+            raise TypeError(f"tree must be a DraftTree or a pair (masks, depths), got {type(tree).__name__}")
+        return (self._numbers(tree[0], "tree.masks", (batch, tokens), torch.int64),
+                self._numbers(tree[1], "tree.depths", (batch, tokens)))
 
     def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
                lengths: torch.Tensor, inv_freq: torch.Tensor | None = None, *, counts: torch.Tensor | None = None,

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import drafted_tokens as O
-from pager_hf import DraftTree
+from pager_hf import DraftTree, draft_tree
 from pager_hf import _native as N
 from pager_hf.rotary import rotary_frequencies
 from test_verify_drafts_gpu import CACHE_TYPES, STEP, TINY, _attend_bounds, _check_attend, _filled, _int32, _np, _order, _within
@@ -203,3 +203,21 @@ def test_a_softcap_passes_infinities_and_nan_on():
         assert torch.isnan(got[0, 2, t - 1]).all()
         got[0, 2, t - 1] = out[0, 2, t - 1]
         assert torch.equal(got, out)
+
+
+# ---- forms of a call -----------------------------------------------------------------------------
+def test_a_tree_may_be_a_plain_pair(path):
+    cache, table = _filled(np.random.default_rng(137), 8, 16, 4, 2, 64, torch.float16, [20], 5, garbage=False)
+    q = torch.randn(1, 4, 5, 64, generator=torch.Generator().manual_seed(6)).half().cuda()
+    tree = draft_tree(_int32([[-1, 0, 0, 1, 3]]))
+    inv, _ = rotary_frequencies(64, device="cuda")
+    tab, ln = _int32(table), _int32([20])
+    want = cache.append(0, q, q[:, :2], q[:, 2:], tab, ln, inv, tree=tree)
+    assert torch.equal(cache.append(0, q, q[:, :2], q[:, 2:], tab, ln, inv, tree=(tree.masks, tree.depths)), want)
+    want = cache.attend(0, q, tab, ln, tree=tree)
+    assert torch.equal(cache.attend(0, q, tab, ln, tree=(tree.masks, tree.depths)), want)
+    for bad in ((tree.masks,), (tree.masks, tree.depths, tree.depths), tree.masks, 3):
+        with pytest.raises(TypeError, match="tree"):
+            cache.attend(0, q, tab, ln, tree=bad)
+        with pytest.raises(TypeError, match="tree"):
+            cache.append(0, q, q[:, :2], q[:, 2:], tab, ln, inv, tree=bad)
