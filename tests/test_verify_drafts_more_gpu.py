@@ -8,7 +8,7 @@ import torch
 from oracle import drafted_tokens as O
 from pager_hf import DraftTree, draft_tree
 from pager_hf import _native as N
-from pager_hf.rotary import rotary_frequencies
+from pager_hf.rotary import norm_rotary_embedding, rotary_frequencies
 from test_verify_drafts_gpu import CACHE_TYPES, STEP, TINY, _attend_bounds, _check_attend, _filled, _int32, _np, _order, _within
 
 pytestmark = pytest.mark.gpu
@@ -221,3 +221,39 @@ def test_a_tree_may_be_a_plain_pair(path):
             cache.attend(0, q, tab, ln, tree=bad)
         with pytest.raises(TypeError, match="tree"):
             cache.append(0, q, q[:, :2], q[:, 2:], tab, ln, inv, tree=bad)
+
+
+# ---- the norm ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(STEP))
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,r", [(64, 64), (128, 32), (16, 8), (96, 24), (80, 20)])
+def test_normed_heads_are_of_unit_size(d, r, interleaved, dtype):
+    """Unit weights and no eps: a turn changes no length, so the root mean square is 1 to the output's rounding (and d + 30
+    half steps of float32)."""
+    x = (torch.randn(2, 3, 7, d, generator=torch.Generator().manual_seed(8)) * 5).to(dtype).cuda()
+    inv, _ = rotary_frequencies(r, device="cuda")
+    pos = torch.arange(7, device="cuda").repeat(2, 1) * 1000
+    w = torch.ones(d, device="cuda").to(dtype)
+    y, _ = norm_rotary_embedding(x, None, pos, inv, w, None, eps=0.0, interleaved=interleaved)
+    rms = np.sqrt((_np(y) ** 2).mean(-1))
+    assert np.all(np.abs(rms - 1) <= STEP[dtype] + (d + 30) * 2.0**-24)
+
+
+@pytest.mark.parametrize("dtype", list(STEP))
+@pytest.mark.parametrize("r", [0, 64])
+def test_a_head_with_an_infinite_element(r, dtype):
+    """Its root mean square is infinite: that element (and the one that it turns with) is NaN, as inf * 0 is, the others are
+    zeros; other heads do not see it."""
+    x = torch.randn(1, 2, 3, 64, generator=torch.Generator().manual_seed(8)).to(dtype).cuda()
+    w = torch.ones(64, device="cuda").to(dtype)
+    inv = rotary_frequencies(64, device="cuda")[0] if r else torch.empty(0, device="cuda")
+    pos = torch.arange(5, 8, device="cuda")[None]
+    want, _ = norm_rotary_embedding(x, None, pos, inv, w, None)
+    x[0, 1, 2, 7] = float("inf")
+    y, _ = norm_rotary_embedding(x, None, pos, inv, w, None)
+    bad = [7, 39] if r else [7]
+    assert torch.isnan(y[0, 1, 2, bad]).all()
+    y[0, 1, 2, bad] = 0.0
+    assert not y[0, 1, 2].any()
+    y[0, 1, 2] = want[0, 1, 2]
+    assert torch.equal(y, want)
