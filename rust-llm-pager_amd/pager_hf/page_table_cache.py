@@ -265,7 +265,7 @@ class PageTableCache:
             N.nat.check(
                 N.lib().pgr_pt_attend(
                     self._ref, layer, ctypes.byref(rows), x.data_ptr(), _strides(x, 3), out.data_ptr(), N.ptr(masks),
-                    N.ptr(depths), int(window or 0), 1.0 / d**0.5 if scale is None else float(scale),
+                    N.ptr(depths), min(int(window or 0), 1 << 31), 1.0 / d**0.5 if scale is None else float(scale),
                     float(softcap or 0.0), bool(exact_weights), N.ptr(ws), nbytes, N.stream_of(self.device),
                 ),
                 "PageTableCache.attend",

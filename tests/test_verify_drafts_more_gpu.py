@@ -223,6 +223,14 @@ def test_a_tree_may_be_a_plain_pair(path):
             cache.append(0, q, q[:, :2], q[:, 2:], tab, ln, inv, tree=bad)
 
 
+def test_a_window_of_any_number(path):
+    cache, table = _filled(np.random.default_rng(139), 8, 16, 4, 2, 64, torch.float16, [50], 2, garbage=False)
+    q = torch.randn(1, 4, 2, 64, generator=torch.Generator().manual_seed(6)).half().cuda()
+    want = cache.attend(0, q, _int32(table), _int32([50]))
+    for window in (1 << 30, 1 << 31, (1 << 32) + 1, (1 << 63) - 1, 1 << 63, (1 << 64) + 1):
+        assert torch.equal(cache.attend(0, q, _int32(table), _int32([50]), window=window), want), window
+
+
 # ---- the norm ------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", list(STEP))
 @pytest.mark.parametrize("interleaved", [False, True])
