@@ -228,7 +228,8 @@ __global__ __launch_bounds__(256) void norm_rotary_kernel(NormRotaryLaunch a, in
 }
 
 // Heads that are no whole number of 16-byte pieces, or whose rotary part is none: a wave per head, element by
-// element, read twice.
+// element, read twice, with angles of its own. Simple, and far from what the bytes would take: 8 x 8191 tokens, 32/8 heads,
+// bf16, D 16 of which 8 turn 1274 us (39 where all turn), 4 x 4096 tokens, D 96 of which 24 turn 362 (49 at a copy's rate).
 template <class Ty, bool kPages>
 __global__ __launch_bounds__(256) void norm_rotary_any_kernel(NormRotaryLaunch a, int64_t n, int total) {
   typedef typename Ty::Raw Raw;

@@ -239,7 +239,8 @@ class PageTableCache:
         in memory: out.transpose(1, 2).reshape(B, T, -1) is the output projection's input and copies nothing.
         Zeros for columns that are not a row's own, for a token that sees nothing and for a head whose scores are all
         -inf. What the pages hold behind a row's new tokens does not matter, nor what they hold before the window of
-        its first new one (nor whether those pages are there).
+        its first new one (nor whether those pages are there). A value in V that is not finite, of a token that some new
+        token of the row sees, may reach all of the row's new tokens.
 
         The probabilities enter the product with V as two numbers of the cache's type, whose rounding does not show.
         A caller that may have them rounded to one, each off by up to half a step of the type, says so with
