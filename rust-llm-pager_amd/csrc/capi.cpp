@@ -594,7 +594,7 @@ int check_tokens(int64_t batch, int64_t tokens) {
 
 struct PTPlan {
   pgr::PTAttendPlan k;
-  size_t o_meta = 0, o_pm = 0, o_pl = 0, o_pacc = 0, bytes = 0;
+  size_t o_meta = 0, o_parts = 0, o_pm = 0, o_pl = 0, o_pacc = 0, bytes = 0;
 };
 
 int check_pt_attend(const pgr_pt_cache_t* c, int64_t batch, int64_t tokens) {
@@ -614,6 +614,7 @@ PTPlan plan_pt(const pgr_pt_cache_t* c, int64_t batch, int64_t tokens, int64_t w
   const size_t slots = (size_t)c->kv_heads * p.k.blocks * p.k.slots * p.k.rows;
   Parts w;
   p.o_meta = w.take((size_t)batch * sizeof(int2));
+  if (p.k.listed) p.o_parts = w.take((size_t)p.k.slots * sizeof(int2));
   p.o_pm = w.take(slots * sizeof(float));
   p.o_pl = w.take(slots * sizeof(float));
   p.o_pacc = w.take(slots * (size_t)c->head_dim * sizeof(float));
@@ -1718,6 +1719,7 @@ int pgr_pt_attend(const pgr_pt_cache_t* cache, int64_t layer, const pgr_pt_rows_
     L.plan = p.k;
     if (p.bytes > 0) {
       L.meta = reinterpret_cast<int2*>(w + p.o_meta);
+      if (p.k.listed) L.parts = reinterpret_cast<int2*>(w + p.o_parts);
       L.pm = reinterpret_cast<float*>(w + p.o_pm);
       L.pl = reinterpret_cast<float*>(w + p.o_pl);
       L.pacc = reinterpret_cast<float*>(w + p.o_pacc);

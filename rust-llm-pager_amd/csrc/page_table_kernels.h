@@ -60,6 +60,7 @@ struct PTAttendPlan {
   int slots = 0;    // parts that the batch's rows are cut into at most (0: whole rows, no merge launch)
   int tile = 32;    // tokens
   int least = 4;    // tiles of a part at least
+  bool listed = false;  // a launch of its own finds the parts
 };
 PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capacity, int d);
 
@@ -76,6 +77,7 @@ struct PTAttendLaunch {
   int exact = 1;  // P as two numbers; 0: one where that is faster
   PTAttendPlan plan;
   int2* meta = nullptr;   // [batch]: a row's first part, a part's tiles
+  int2* parts = nullptr;  // plan.listed: [slots]: a part's batch row (-1: no part) and its number in the row
   float* pm = nullptr;    // [hkv, blocks, slots, rows]
   float* pl = nullptr;
   float* pacc = nullptr;  // [..., d]
@@ -95,5 +97,7 @@ hipError_t launch_draft_tree(const int32_t* parents, int batch, int tokens, uint
 
 // New tokens of a row that a tree's masks cover, and tokens of a path.
 constexpr int kMostDrafts = 64;
+// Rows of a batch whose parts are listed.
+constexpr int kMostListed = 8192;
 
 }  // namespace pgr

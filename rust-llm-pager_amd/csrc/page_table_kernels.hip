@@ -70,8 +70,8 @@ struct Work {
 // The batch's rows are cut into parts of one size, `per` tiles: the least with which there are no more parts than
 // plan.slots, so that long rows have more of them and all workgroups about as much to do (8 rows of 13 drafted tokens
 // over 0 to 8191, D 64, softcapped: 27 us, 36 with as many parts for a short row as for a long one). Every wave finds
-// that size and its part by itself; the first workgroup leaves both for the merge. A row of one part is finished by its
-// workgroup; without slots every row is.
+// that size and its part by itself; the first workgroup leaves both for the merge. (In large batches a launch before this
+// one has listed the parts.) A row of one part is finished by its workgroup; without slots every row is.
 //
 // Blocks that read the same tokens are neighbours on one XCD (workgroups go to the eight XCDs in turn), so that its L2
 // serves all but the first; the longest block is first.
@@ -87,6 +87,15 @@ __device__ __forceinline__ bool work_of(const PTAttendLaunch& a, Work& w) {
   w.whole = true;
   if (a.plan.slots == 0) return part < a.r.batch;
   if (part >= a.plan.slots) return false;
+  if (a.parts != nullptr) {
+    const int2 listed = a.parts[part];
+    if (listed.x < 0) return false;
+    w.b = listed.x;
+    w.split = listed.y;
+    w.per = a.meta[w.b].y;
+    w.whole = row_tiles(a, w.b) <= w.per;
+    return true;
+  }
   if (a.r.batch == 1) {
     w.per = max((row_tiles(a, 0) + a.plan.slots - 1) / a.plan.slots, a.plan.least);
     w.split = part;
@@ -148,6 +157,60 @@ __device__ __forceinline__ bool work_of(const PTAttendLaunch& a, Work& w) {
     before = __builtin_amdgcn_readlane(last, 63);
   }
   return w.b >= 0;
+}
+
+// The parts of a large batch, listed once: the size of a part as above, each row's first part and each part's row. One
+// workgroup, a thread for so many rows that follow each other. Any size from total / (slots - batch) on leaves no more than
+// `slots` parts, since a row has at most one that is not full; a dozen sums over the batch find the least. Latency alone.
+constexpr int kListThreads = 1024;
+
+__global__ __launch_bounds__(kListThreads) void pt_list_kernel(PTAttendLaunch a) {
+  __shared__ int tiles_s[kMostListed];
+  __shared__ int wave_s[kListThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, batch = a.r.batch, slots = a.plan.slots;
+  const int each = (batch + kListThreads - 1) / kListThreads, first = min(tid * each, batch), last = min(first + each, batch);
+  // Sum over the threads; `before`: over those before this one.
+  auto sum = [&](int x, int& before) {
+    const int upto = wave_scan(x);
+    __syncthreads();
+    if (lane == 63) wave_s[wave] = upto;
+    __syncthreads();
+    int all = 0;
+    before = upto - x;
+    for (int w = 0; w < kListThreads / 64; ++w) {
+      before += w < wave ? wave_s[w] : 0;
+      all += wave_s[w];
+    }
+    return all;
+  };
+  int mine = 0, before;
+  for (int b = first; b < last; ++b) {
+    tiles_s[b] = row_tiles(a, b);
+    mine += tiles_s[b];
+  }
+  const int total = sum(mine, before);
+  auto own_at = [&](int size) {
+    int parts = 0;
+    for (int b = first; b < last; ++b) parts += (tiles_s[b] + size - 1) / size;
+    return parts;
+  };
+  int few = max((total + slots - 1) / slots, a.plan.least) - 1, per = max((total - 1) / (slots - batch) + 1, few + 1);
+#pragma unroll 1
+  while (per - few > 1 + (per >> 6)) {  // few: too small, or not tried; per: not too small
+    const int size = (few + per) >> 1;
+    if (sum(own_at(size), before) > slots)
+      few = size;
+    else
+      per = size;
+  }
+  const int all = sum(own_at(per), before);
+  for (int b = first; b < last; ++b) {
+    const int n = (tiles_s[b] + per - 1) / per;
+    a.meta[b] = int2{before, per};
+    for (int i = 0; i < n; ++i) a.parts[before + i] = int2{b, i};
+    before += n;
+  }
+  for (int i = all + tid; i < slots; i += kListThreads) a.parts[i] = int2{-1, 0};
 }
 
 // The first row of a part's results: [hkv, blocks, slots, rows], a batch row's parts one after the other.
@@ -912,6 +975,11 @@ template <class Ty, int D>
 hipError_t attend_dim(const PTAttendLaunch& p, const AttendScale& sc, hipStream_t stream) {
   const int64_t parts = (int64_t)p.c.hkv * (p.plan.slots == 0 ? p.r.batch : p.plan.slots);
   const dim3 grid((unsigned)((parts + 7) / 8 * 8 * p.plan.blocks));
+  if (p.plan.listed) {
+    pt_list_kernel<<<1, kListThreads, 0, stream>>>(p);
+    const hipError_t listed = hipGetLastError();
+    if (listed != hipSuccess) return listed;
+  }
   if (p.plan.waves == 0) {
     if (p.plan.rows == 16 && p.plan.share == 4) pt_attend_kernel<Ty, D, 1, 4><<<grid, 256, 0, stream>>>(p, sc);
     if constexpr (D < 256) {
@@ -979,16 +1047,27 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
     if (d < 256) p.share = p.least = 8;
     return p;
   }
-  // Every wave walks the batch to find its part, 64 rows at a time and several times over, and there are as many parts as
-  // rows or more: above 256 rows that costs what it gains. One token, 16/1 heads, D 32, rows of 0 to 4096 tokens, cut
-  // and whole: 300 rows 35 and 25 us, 700 89 and 37, 1025 166 and 50, 4097 1729 and 202; 8/1, D 128, all of 4095 tokens: 300
-  // rows 127 and 137, 700 287 and 248.
-  if (batch > 256) return p;
   // The device adds the batch's tiles up in 32 bits: beyond, rows are left whole (2^35 tokens; such a table is
   // one that rows share).
   if (batch * ((capacity + p.tile - 1) / p.tile) >= (int64_t)1 << 30) return p;
+  const int64_t groups = units * p.blocks, most = (capacity + p.least * p.tile - 1) / (p.least * p.tile),
+                once = target / ((int64_t)hkv * p.blocks);
+  // Places for a part of each row and for those of long rows. (None where a row's results are many: it has blocks enough
+  // then.)
+  const int64_t places = batch + (once > 8 ? once : 8);
+  const bool few = places * hkv * p.blocks * p.rows * d * 4 <= (int64_t)128 << 20;
+  if (batch > 256) {
+    // Parts that every workgroup finds by walking the batch cost more than they gain here (one token, 16/1 heads, D 32, rows
+    // of 0 to 4096 tokens, walked and whole: 300 rows 35 and 25 us, 1025 166 and 50, 4097 1729 and 202), so they are
+    // listed once, by a launch of their own, and only where a row can be so long that it would hold the call up: one of
+    // 60000 tokens among 299 of 200, 32/8 heads, D 128, 653 us whole, 167 walked, 110 listed; among 999 708, 1049, 222. Rows
+    // alike under such a table pay for the launches: 300 of 1000 tokens 218 us whole, 245 walked, 232 listed; 16/1 heads,
+    // D 32, 12, 25 and 20.
+    p.listed = few && batch <= kMostListed && most >= 64;
+    if (p.listed) p.slots = (int)places;
+    return p;
+  }
   // Parts a row on average: as many as fill the card once.
-  const int64_t groups = units * p.blocks, most = (capacity + p.least * p.tile - 1) / (p.least * p.tile);
   int64_t n = target / groups;
   if (2 * groups > target) {
     // The blocks all but fill the card, or more: cut where whole rounds of workgroups come nearer by more than the parts
@@ -1019,15 +1098,12 @@ PTAttendPlan pt_attend_plan(int batch, int tokens, int hq, int hkv, int64_t capa
     }
   }
   if (n > most) n = most;
-  const int64_t once = target / ((int64_t)hkv * p.blocks);
   if (n > 1) {
     p.slots = (int)(batch > 1 && once > n * batch ? once : n * batch);
   } else if (batch > 1 && most >= 32) {
     // The rows fill the card, but one that is much longer than the others would hold the call up: one of 60000 tokens and
     // 63 of 200 (32/8 heads, D 128) 635 us whole, 78 cut; 64 of 4096 tokens, none of them cut, 184 and 188.
-    // (Not where a row's results are many: it has blocks enough then.)
-    const int64_t slots = batch + (once > 8 ? once : 8), bytes = (int64_t)hkv * p.blocks * p.rows * d * 4;
-    if (slots * bytes <= (int64_t)128 << 20) p.slots = (int)slots;
+    if (few) p.slots = (int)places;
   }
   return p;
 }

@@ -40,6 +40,13 @@ def test_large_batches_stay_whole(tokens, geometry):
     assert _bytes(2, tokens, 4096, **geometry) > 0
 
 
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_large_batches_with_room_for_long_rows_are_cut(tokens):
+    for batch in (257, 300, 1000, 2000):
+        assert _bytes(batch, tokens, 32768, query_heads=16, kv_heads=1, head_dim=32) > 0
+    assert _bytes(8193, tokens, 32768, query_heads=16, kv_heads=1, head_dim=32) == 0
+
+
 GEOMETRIES = [(32, 8, 128), (28, 4, 128), (14, 2, 64), (16, 1, 32), (16, 16, 64), (8, 1, 256), (4, 2, 16)]
 SIZES = sorted({max(1, (1 << k) + i) for k in range(0, 18) for i in (-1, 0, 1)})
 

@@ -108,6 +108,59 @@ def test_attend_over_more_than_a_thousand_rows(window):
     _check_attend(cache, 0, table, lengths, q, out, counts, *_order(b, t), window, 1.0 / 32**0.5, 0.0, exact=True)
 
 
+LARGE = [
+    # batch, query heads, kv heads, head dim, new tokens, window, long rows
+    (300, 8, 2, 64, 1, 0, {100: 5000}), (1100, 16, 1, 32, 2, 0, {0: 2100, 700: 4000, 1099: 900}), (257, 16, 1, 64, 20, 0, {256: 3000}),
+    (300, 8, 1, 256, 2, 0, {7: 1500}), (400, 4, 4, 128, 3, 500, {5: 2000, 6: 2000, 398: 700}), (2100, 4, 2, 16, 1, 0, {2099: 3000}),
+    (1025, 2, 1, 64, 40, 0, {1024: 1300}),
+]
+
+
+@pytest.mark.parametrize("dtype", CACHE_TYPES)
+@pytest.mark.parametrize("case", LARGE, ids=[str(c[:6]) for c in LARGE])
+def test_long_rows_of_large_batches_are_cut(case, dtype):
+    """Parts are listed by a launch of their own: rows of one part, of many and of none."""
+    b, hq, hkv, d, t, window, longer = case
+    rng = np.random.default_rng(109)
+    lengths = [0 if i % 9 == 3 else int(x) for i, x in enumerate(rng.integers(0, 30, b))]
+    for i, n in longer.items():
+        lengths[i] = n
+    pages = sum(-(-(n + t) // 32) for n in lengths) + 1
+    cache, table = _filled(rng, pages, 32, hq, hkv, d, dtype, lengths, t, spare=520)
+    assert N.lib().pgr_pt_attend_workspace_bytes(cache._ref, b, t, table.shape[1]) > 0
+    counts = [t if i in longer else i % (t + 1) for i in range(b)]
+    q = torch.randn(b, hq, t, d, generator=torch.Generator().manual_seed(6)).to(dtype).cuda()
+    for _ in range(2):
+        out = cache.attend(0, q, _int32(table), _int32(lengths), counts=_int32(counts), window=window)
+        _check_attend(cache, 0, table, lengths, q, out, counts, *_order(b, t), window, 1.0 / d**0.5, 0.0, exact=True,
+                      only=sorted({0, t // 2, t - 1}))
+    assert not cache.attend(0, q, _int32(table), _int32(lengths), counts=_int32([0] * b), window=window).any()
+
+
+def test_a_captured_call_of_a_large_batch_replays():
+    """The parts are listed anew from the lengths of each replay."""
+    rng = np.random.default_rng(149)
+    b, most = 300, 2500
+    cache, _ = _filled(rng, 80, 32, 8, 1, 64, torch.float16, [most], 3, garbage=False)
+    table = _int32(np.concatenate([rng.permutation(79), np.full(500, -1)])[None]).expand(b, -1)  # (rows that share their pages)
+    q = torch.randn(b, 8, 3, 64, generator=torch.Generator().manual_seed(6)).half().cuda()
+    lengths = _int32([5] * b)
+    cache.attend(0, q, table, lengths)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = cache.attend(0, q, table, lengths)
+    for i in range(4):
+        now = rng.integers(0, 40, b)
+        now[rng.integers(0, b, i)] = rng.integers(1000, most, i)
+        lengths.copy_(_int32(now))
+        want = cache.attend(0, q, table, lengths)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want)
+        torch.randn(1000, device="cuda").sort()  # eager work between the replays
+
+
 @pytest.mark.parametrize("tokens", [2048, 2049])
 def test_prompts_of_one_token_more(tokens):
     """A prompt into an empty cache whose blocks of rows just fill the card, and one token more."""
