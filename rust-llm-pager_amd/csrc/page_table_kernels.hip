@@ -5,6 +5,9 @@
 // a page that is not there: its tokens are not seen. So no value in them can lead an access astray.
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
+#include <cmath>
+
 #include "cache_device.h"
 #include "page_table_kernels.h"
 
@@ -1112,8 +1115,11 @@ hipError_t launch_pt_attend(int dtype, const PTAttendLaunch& p, hipStream_t stre
   AttendScale sc;
   constexpr double kLog2 = 1.4426950408889634;  // (of e; each factor rounded once)
   sc.scale_log2 = (float)(p.scale * kLog2);
-  sc.cap_scale = p.softcap > 0.f ? (float)(p.scale / (double)p.softcap * (2. * kLog2)) : 0.f;
-  sc.cap_log2 = p.softcap > 0.f ? (float)(p.softcap * kLog2) : 0.f;
+  // (Scores are far below 2^88, so that a cap of 2^96 changes none of them by half a step, and larger ones pass float32's range
+  // here; under the smallest caps the quotient must not, since 0 times infinity is NaN.)
+  const bool capped = p.softcap > 0.f && p.softcap < 0x1p96f;
+  sc.cap_scale = capped ? (float)std::fmin(p.scale / (double)p.softcap * (2. * kLog2), (double)FLT_MAX) : 0.f;
+  sc.cap_log2 = capped ? (float)(p.softcap * kLog2) : 0.f;
   return dtype == kF16 ? attend<HalfT>(p, sc, stream) : attend<Bf16T>(p, sc, stream);
 }
 

@@ -231,6 +231,21 @@ def test_softcaps_above_64(cap, d, dtype):
         _check_attend(cache, 0, table, lengths, q, out, None, *_order(b, t), 0, 8.0 / d**0.5, cap, exact=True)
 
 
+@pytest.mark.parametrize("t", [1, 40])
+def test_softcaps_at_the_ends_of_float32(t):
+    """The largest change nothing; under the smallest all scores are alike, those of a key of zeros too."""
+    cache, table = _filled(np.random.default_rng(151), 8, 16, 4, 1, 64, torch.float16, [20], t, garbage=False)
+    p, o = O.cells(table[0], 16, 8, 0, 20 + t)
+    cache.keys[0, int(p[3]), :, int(o[3])] = 0.0
+    q = torch.randn(1, 4, t, 64, generator=torch.Generator().manual_seed(6)).half().cuda()
+    want = cache.attend(0, q, _int32(table), _int32([20]))
+    for cap in (3.4e38, 2.0**127, 2.0**100):
+        assert torch.equal(cache.attend(0, q, _int32(table), _int32([20]), softcap=cap), want)
+    for cap in (1e-40, 2.0**-149, 1e-37, 1e-30):
+        out = cache.attend(0, q, _int32(table), _int32([20]), softcap=cap)
+        _check_attend(cache, 0, table, [20], q, out, None, *_order(1, t), 0, 0.125, cap, exact=True)
+
+
 def test_a_softcap_passes_infinities_and_nan_on():
     """Scores of both infinities are the cap's two ends; a score of NaN stays with its token and head."""
     for t in (1, 40):
