@@ -572,12 +572,12 @@ __device__ __forceinline__ float sum_halves(float x) {
 // P is off by half a step of each weight: in bf16 the output is then 0.0023 of its norm from 64 bits, 0.0017 with two): here
 // the second product is half as much arithmetic again. A chunk of 2048 tokens over 16384, 32/8 heads, D 128: 826 us with
 // two numbers, 622 with one (939 TFLOP/s; a library's matrix product reaches 1244); the kernel above took 1265. Trees of
-// 64 tokens over 8 rows of 32768, 28/4: 387 and 302 us (598). The figures below are with one number. In the chunk the matrix cores are busy 0.42 of the cycles and the vector units 0.52, one after the other: the
-// two waves of a SIMD go through products and softmax together. Half of the waves half a tile behind the others
-// (676 us), a barrier every second tile (641), raised wave priorities over either product (637 to 653): no better.
-// Eight waves (one workgroup a CU) against four: 664 and 752 us, 323 and 355; 128 rows, 8 x 8192 tokens: 74 and 76; few
-// workgroups (448 rows, 1000 tokens) 15.4 and 13.5. Up to 32 rows the kernel above is as fast or faster (32 rows, 8 x
-// 8192 tokens: 61 us; 48 rows here 65, there 80).
+// 64 tokens over 8 rows of 32768, 28/4: 387 and 302 us (598). In the chunk the matrix cores are busy 0.50 of the cycles and
+// the vector units 0.57 (0.42 and 0.52 with one number), one after the other: the two waves of a SIMD go through products
+// and softmax together. With one number: half of the waves half a tile behind the others (676 us), a barrier every second
+// tile (641), raised wave priorities over either product (637 to 653): no better. Eight waves (one workgroup a CU) against
+// four: 664 and 752 us, 323 and 355; 128 rows, 8 x 8192 tokens: 74 and 76; few workgroups (448 rows, 1000 tokens) 15.4 and
+// 13.5. Up to 32 rows the kernel above is as fast or faster (32 rows, 8 x 8192 tokens: 61 us; 48 rows here 65, there 80).
 template <int D>
 struct Staged {
   static constexpr int kPieces = D / 8;  // 16-byte pieces of a token
